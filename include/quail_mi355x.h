@@ -256,6 +256,52 @@ int qx_kv_scatter(const void* k, int64_t k_ld, const void* v, int64_t v_ld, void
                   void* v_pool, const int64_t* src, const int64_t* dst, int64_t count,
                   int64_t row_elems, int v_to_f16, hipStream_t stream);
 
+/*
+ * An arena that keeps K and V in 8 bits (no counterpart in the reference,
+ * whose pools are bf16): k_pool and v_pool hold e4m3 codes, rows of HK*D
+ * bytes, and scales one byte for K and one for V per (page of 16 rows, KV
+ * head), at scales[(page*HK + head)*2 + (0 for K, 1 for V)]: an E8M0 byte b
+ * in [1, 247] that stands for 2^(b - 127). A row's value is code * 2^(b - 127).
+ *
+ * Both calls write whole page items. items (device): 5 int32 per item,
+ * {destination page, source page, keep, row0, count}, keep + count <= 16: the
+ * page's rows [0, keep) are the source page's (mostly the destination itself;
+ * another for a copied partial page), the next `count` are the fresh rows
+ * row0, row0 + 1, ...; rows past them stay as they are. The scale's byte is
+ * the least b with max |fresh| <= 448 * 2^(b - 127) (infinities count as the
+ * largest float, NaN not at all), or with keep > 0 the larger of that and
+ * the source page's; kept codes then move by that power of two, exactly
+ * unless they become subnormal. A call writes each destination page once,
+ * and no item's source is another item's destination.
+ *
+ * qx_qk_norm_rope_kv8: rows of the qkv projection, as in
+ * qx_qk_norm_rope_kv: K through its norm and RoPE in fp32 and from there to
+ * its code in one rounding, V as it is; with q_out the items' rows of q as
+ * qx_qk_norm_rope writes them. qx_kv8_write: K and V rows (bf16, HK*D
+ * values, k_ld and v_ld apart) as they are.
+ */
+int qx_qk_norm_rope_kv8(const void* qkv, int64_t qkv_ld, void* q_out, int64_t q_ld, void* k_pool,
+                        void* v_pool, void* scales, const int* items, int64_t n_items,
+                        const void* cos_sin, int cs_is_f32, const int64_t* positions,
+                        const void* q_w, const void* k_w, int64_t HQ, int64_t HK, int64_t D,
+                        float eps, hipStream_t stream);
+int qx_kv8_write(const void* k, int64_t k_ld, const void* v, int64_t v_ld, void* k_pool,
+                 void* v_pool, void* scales, const int* items, int64_t n_items, int64_t HK,
+                 int64_t D, hipStream_t stream);
+
+/*
+ * Pages src[i] -> dst[i] (HOST arrays, read before the call returns) of
+ * every pool of an arena: n_pools pools of page_bytes a page, pool_stride
+ * bytes apart from `pools`, and with n_scale_pools > 0 the scales' pages the
+ * same way. Every page's source is read as it was before the call: a page
+ * that is a destination twice, or a source and a destination, is refused
+ * (-1), and so is an id outside [0, num_pages).
+ */
+int qx_copy_pages(void* pools, int64_t n_pools, int64_t pool_stride, int64_t page_bytes,
+                  void* scales, int64_t n_scale_pools, int64_t scale_stride, int64_t scale_bytes,
+                  const int* src, const int* dst, int64_t count, int64_t num_pages,
+                  hipStream_t stream);
+
 /* out[i] = table[ids[i]] (bf16 rows). Replaces vLLM embed_tokens (qwen3.py:123). */
 int qx_embed(const void* table, int64_t t_ld, const int64_t* ids, void* out, int64_t o_ld,
              int64_t n, int64_t H, hipStream_t stream);
@@ -382,6 +428,27 @@ int qx_attention_lse_tiled(const void* q, int64_t q_ld, const int64_t* q_index, 
                            hipStream_t stream);
 
 /*
+ * qx_paged_attention and qx_attention_lse over an 8-bit arena's pages (codes
+ * and scales as qx_kv8_write lays them out): rows query rows in seqs
+ * sequences, each through its row of the block table; q_index as in
+ * qx_attention_lse. Exactly one of out_bf16 (rows of o_ld elements) and
+ * out_fp8 (D == 128; out_scales[h*os_ld + row]); lse (may be NULL) as in
+ * qx_attention_lse; a row that sees no key gets 0 and -inf. max_q and
+ * max_used bound the sequences' rows and keys. workspace:
+ * qx_paged_attention8_workspace bytes of the caller's, 16-byte aligned (NULL
+ * where that is 0), used by this call alone until the stream has passed it.
+ */
+int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used,
+                                      int64_t HQ, int64_t HK, int64_t D);
+int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
+                        const void* v_pool, const void* scales, const int* cu_q, const int* used,
+                        const int* table, int64_t table_ld, int64_t seqs, int64_t rows,
+                        int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
+                        int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
+                        int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
+                        void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * Replaces Engine.merge_attn_quant / the merge_attn_quant Triton kernel
  * (attention.py:902-948, QUANT on, UE8M0 off): for row t with
  * source[t] >= 0, w = bf16(sigmoid(lb[h*lb_ld + source[t]] - la[h*la_ld + t])),
@@ -466,6 +533,10 @@ int qx_prefix_tree(const int64_t* tokens, const int64_t* offsets, int64_t n,
  *   priority is tokens per page the key alone holds. victim = {found, key,
  *   pages it alone held, tokens}; the victim stays resident.
  * qx_pages_free_list: the free stack, bottom first.
+ * qx_pages_compact: the keys' pages take the lowest ids (*n pages move,
+ *   src[i] -> dst[i]; the caller copies them, no dst is a src) and the free
+ *   stack hands out the rest in rising order; -1 while a key is pinned or a
+ *   pack's temporary key lives. No counterpart in the reference.
  */
 int qx_pages_create(int64_t num_pages, int64_t page_tokens, void** pool);
 int qx_pages_destroy(void* pool);
@@ -485,6 +556,7 @@ int qx_pages_pin(void* pool, int64_t key);
 int qx_pages_retain(void* pool, int64_t key, int has_priority, double priority);
 int qx_pages_pop_victim(void* pool, const int64_t* keep, int64_t n_keep, int64_t* victim);
 int qx_pages_free_list(void* pool, int32_t* pages, int64_t cap, int64_t* n);
+int qx_pages_compact(void* pool, int32_t* src, int32_t* dst, int64_t cap, int64_t* n);
 
 /*
  * Host function (no device work): one pack of the unified causal path.

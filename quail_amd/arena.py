@@ -11,12 +11,22 @@ HBM layout: one allocation split [k0, v0, k1, v1, ...]; each pool is
 (num_pages * page_tokens, num_kv_heads, head_dim) bf16, so page p holds pool
 rows p*T .. p*T + T - 1 and a KV row is num_kv_heads * head_dim contiguous
 bf16 (2 KiB for Qwen3-4B). At 16 tokens a page is 32 KiB per layer and pool.
+
+With dtype=torch.float8_e4m3fn K and V are kept in 8 bits instead (half the
+bytes a token takes and a reader moves): each pool holds e4m3 codes, and
+`scales` one E8M0 byte b (2^(b - 127)) for K and one for V per (layer, page,
+KV head), (num_layers, num_pages, num_kv_heads, 2).
 """
+
+import ctypes
 
 import numpy as np
 import torch
 
+from quail_amd import _lib
 from quail_amd.pages import PageArena
+
+FP8 = torch.float8_e4m3fn
 
 
 class _Claim:
@@ -34,8 +44,16 @@ class _Claim:
 
 class KVArena:
     def __init__(self, num_layers: int, num_pages: int, page_tokens: int, num_kv_heads: int,
-                 d_head: int, dtype=torch.bfloat16, device="cuda", v_dtype=torch.float16):
-        if dtype != torch.bfloat16 or v_dtype not in (torch.bfloat16, torch.float16):
+                 d_head: int, dtype=torch.bfloat16, device="cuda", v_dtype=None):
+        if v_dtype is None:
+            v_dtype = FP8 if dtype == FP8 else torch.float16
+        if dtype == FP8:
+            if v_dtype != FP8:
+                raise ValueError("8-bit pages hold K and V in e4m3")
+            if page_tokens != 16 or d_head not in (64, 128):
+                raise ValueError(f"8-bit pages have 16 rows of head_dim 64 or 128, not "
+                                 f"{page_tokens} of {d_head}")
+        elif dtype != torch.bfloat16 or v_dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("K pages are bf16; V pages bf16 or fp16")
         self.torch = torch
         self.dtype = dtype
@@ -64,7 +82,17 @@ class KVArena:
         # when written, and the PV product then keeps 11 bits of each
         # probability instead of 8)
         self.v = [p.view(self.v_dtype).view(rows, heads, dim) for p in parts[1::2]]
+        self.storage = storage
+        self.scales = None
+        if self.eight_bit:
+            self.scales = torch.full((self.num_layers, num_pages, heads, 2), 127,
+                                     dtype=torch.uint8, device=self.device)
         self._claims = {}
+
+    @property
+    def eight_bit(self) -> bool:
+        """Whether K and V are e4m3 codes with a scale per (page, KV head)."""
+        return self.dtype == FP8
 
     # ---- sizes -------------------------------------------------------------
 
@@ -206,6 +234,83 @@ class KVArena:
         pages = self.alloc(key, tokens, base_tokens=0)
         return None if pages is None else (key, pages)
 
+    # ---- copies, forks and compaction ----------------------------------------------
+
+    def copy_pages(self, src, dst) -> None:
+        """Pages src[i] -> dst[i] in every layer, K and V (and their scales),
+        on the current stream. Page ids are host values; each destination is
+        named once and is no source (ValueError otherwise)."""
+        src, dst = list(src), list(dst)
+        if len(src) != len(dst):
+            raise ValueError(f"{len(src)} source pages for {len(dst)} destinations")
+        if not self.storage.is_cuda:
+            raise ValueError("page copies run on the GPU; this arena is on the CPU")
+        from quail_amd.engine import _stream
+        ids = ctypes.c_int32 * max(1, len(src))
+        heads, dim = self.kv_shape
+        size = self.storage.element_size()
+        page = self.page_tokens * heads * dim * size
+        pool = self.num_pages * page
+        scales = (None, 0, 0, 0)
+        if self.eight_bit:
+            scales = (self.scales.data_ptr(), self.num_layers, 2 * heads * self.num_pages, 2 * heads)
+        try:
+            with torch.cuda.device(self.storage.device):
+                _lib.call("qx_copy_pages", self.storage.data_ptr(), 2 * self.num_layers, pool, page,
+                          *scales, ids(*src), ids(*dst), len(src), self.num_pages, _stream())
+        except _lib.QxError as err:
+            if "hipError" in str(err):
+                raise
+            raise ValueError(str(err)) from err
+
+    def fork(self, key, children, tokens=None, capacity_tokens=None):
+        """New keys that continue the first `tokens` tokens of a resident key
+        (all of them by default), each in pages of its own from there: they
+        read the key's full pages as borrowed ones, and its partial last page
+        is copied (current stream) into the first page of each. Returns the
+        children's own pages, or None with nothing changed when the free list
+        is short (evict retained keys first)."""
+        acct = self.accounting
+        children = list(children)
+        if len(set(children)) != len(children):
+            raise ValueError("a fork names each child once")
+        held = acct.key_tokens(key)
+        tokens = held if tokens is None else tokens
+        capacity = tokens if capacity_tokens is None else capacity_tokens
+        if not 0 <= tokens <= held:
+            raise ValueError(f"fork of {tokens} tokens from a key that holds {held}")
+        if capacity < tokens:
+            raise ValueError(f"capacity of {capacity} tokens for a fork of {tokens}")
+        for child in children:
+            if acct.is_resident(child):
+                raise KeyError(f"{child!r} already resident")
+        full, rest = divmod(tokens, self.page_tokens)
+        shared = acct.shared_pages(key, full * self.page_tokens)
+        table = acct.table_pages(key)
+        if len(shared) != full or len(table) < acct.pages_needed(tokens):
+            raise ValueError("the key's leading pages were dropped")
+        need = acct.pages_needed(capacity) - full
+        if need * len(children) > acct.free_pages:
+            return None
+        pages = [acct.alloc(child, tokens, capacity, borrowed=shared) for child in children]
+        if rest and children:
+            self.copy_pages([table[full]] * len(children), [own[0] for own in pages])
+        return pages
+
+    def compact(self) -> int:
+        """Move the resident keys' pages to the lowest ids (current stream),
+        so that the pages past them are free in one run; returns the pages
+        moved. Between stages only: ValueError while a key is pinned, held or
+        being read, or a pack's temporary pages live."""
+        if self._claims:
+            raise ValueError("keys are held for borrowers or being read")
+        if not self.storage.is_cuda:
+            raise ValueError("page copies run on the GPU; this arena is on the CPU")
+        src, dst = self.accounting.compact()
+        if src:
+            self.copy_pages(src, dst)
+        return len(src)
+
     def free_key(self, key) -> int:
         """Free a key's pages, or once its holds and reads are over (a key
         queued borrowers will read, or that an admission reads, waits for
@@ -289,6 +394,11 @@ class KVArena:
     def layer_kv(self, layer: int):
         """Flat K and V pools of one layer: (rows, num_kv_heads, head_dim)."""
         return self.k[layer], self.v[layer]
+
+    def layer_scales(self, layer: int):
+        """The E8M0 bytes of one layer of an 8-bit arena: (num_pages,
+        num_kv_heads, 2), K's and V's."""
+        return self.scales[layer]
 
     def paged_kv(self, layer: int):
         heads, dim = self.kv_shape

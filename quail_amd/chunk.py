@@ -233,6 +233,8 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
         # the scatter source is the pack's rows in order: row i's KV goes to
         # dst[i], which lets qk_norm_rope write it in place
         rows_in_order=bool(src.size == n_tok and np.array_equal(src, np.arange(n_tok))))
+    if getattr(arena, "eight_bit", False):
+        unified["page_writes"] = page_writes(src, dst, unified["tail_src"], unified["tail_dst"])
     meta = dict(layer=0, unified=unified, cu_a=cu_a,
                 max_a=int(np.diff(cu_a).max()) if len(cu_a) > 1 else 0,
                 final_query=_final_query(cu_q, used, table, final))
@@ -470,6 +472,8 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
     meta = dict(layer=0, unified=None, kv_src=kv_src, kv_dst=kv_dst, row_pool_dst=row_pool_dst,
                 reads=reads,
                 segments=segments, cu_a=cu_a_arr, max_a=segments["max_q"])
+    if getattr(arena, "eight_bit", False):
+        meta["page_writes"] = () if kv_src is None else page_writes(kv_src, kv_dst)
     if timing is not None:
         timing["pack_py"] = timing.get("pack_py", 0.0) + (t1 - t0)
         timing["pack_reads"] = timing.get("pack_reads", 0.0) + (time.perf_counter() - t1)
@@ -519,6 +523,76 @@ def _final_query(cu_q, used, table, final):
                 max_used=int(visible.max()), causal=True)
 
 
+PAGE_ROWS = 16
+
+
+def page_writes(src, dst, tail_src=None, tail_dst=None):
+    """The page items of a pack's KV writes to an 8-bit arena, whose scale
+    covers a page: pack row src[i] goes to pool row dst[i], after pool rows
+    tail_src were copied to tail_dst (a partial page's rows into another's
+    same slots). Returns a tuple of (n, 5) int32 arrays, (destination page,
+    source page, kept rows, first pack row, rows), to be written one after
+    the other: the writes of each page in order, copied pages last.
+
+    Rows of one page form runs of consecutive pack rows in consecutive slots;
+    a run keeps the slots before it. A run that starts at or before the slot
+    where an earlier run of the page ended would drop that run: ValueError."""
+    src, dst = np.asarray(src, dtype=np.int64), np.asarray(dst, dtype=np.int64)
+    live = dst >= 0
+    src, dst = src[live], dst[live]
+    if not len(dst):
+        return ()
+    page = dst // PAGE_ROWS
+    first = np.ones(len(dst), dtype=bool)
+    first[1:] = (np.diff(dst) != 1) | (np.diff(src) != 1) | (np.diff(page) != 0)
+    at = np.flatnonzero(first)
+    count = np.diff(np.append(at, len(dst)))
+    page, keep, row0 = page[at], dst[at] % PAGE_ROWS, src[at]
+    # the run's place among its page's runs
+    order = np.argsort(page, kind="stable")
+    sorted_page = page[order]
+    new = np.ones(len(order), dtype=bool)
+    new[1:] = np.diff(sorted_page) != 0
+    same = ~new[1:]
+    ends = (keep + count)[order]
+    if (keep[order][1:][same] < ends[:-1][same]).any():
+        raise ValueError("a page's rows must be written in rising order")
+    place = np.arange(len(order)) - np.maximum.accumulate(np.where(new, np.arange(len(order)), 0))
+    phase = np.empty(len(order), dtype=np.int64)
+    phase[order] = place
+    source = page.copy()
+    if tail_src is not None and len(tail_src):
+        tail_src, tail_dst = np.asarray(tail_src), np.asarray(tail_dst)
+        if (tail_src % PAGE_ROWS != tail_dst % PAGE_ROWS).any():
+            raise ValueError("a copied page's rows keep their slots")
+        pages, where, rows = np.unique(tail_dst // PAGE_ROWS, return_index=True,
+                                       return_counts=True)
+        pos = np.searchsorted(pages, page)
+        hit = (pos < len(pages)) & (pages[np.minimum(pos, len(pages) - 1)] == page)
+        if hit.sum() != len(pages) or phase[hit].any() or (rows[pos[hit]] != keep[hit]).any():
+            raise ValueError("a copied page takes one run of the pack's rows, behind its own")
+        source[hit] = tail_src[where[pos[hit]]] // PAGE_ROWS
+        phase[hit] = phase.max() + 1    # once every source page is whole
+    items = np.stack([page, source, keep, row0, count], 1).astype(np.int32)
+    return tuple(np.ascontiguousarray(items[phase == p]) for p in np.unique(phase))
+
+
+def attention_plan(cu_q, used, table, *, heads, causal=True):
+    """The tables of a paged attention call over sequences a caller lays out
+    itself (Engine.read_pages): sequence s has query rows cu_q[s] .. cu_q[s+1]
+    and keys [0, used[s]) through table[s]. cu_q, used and table are int32
+    tensors on the device; heads = (HQ, HK, D)."""
+    host = dict(cu_q=cu_q.cpu().numpy(), used=used.cpu().numpy(), causal=causal)
+    tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
+                  max_q=int(np.diff(host["cu_q"]).max(initial=0)),
+                  max_used=int(host["used"].max(initial=0)))
+    work, n_work, rows = _work_list(host, heads, choose_rows=True)
+    if n_work:
+        import torch
+        tables.update(work=torch.from_numpy(work).to(cu_q.device), n_work=n_work, work_rows=rows)
+    return tables
+
+
 # ---- staging ----------------------------------------------------------------
 
 STAGING_DEPTH = 4
@@ -558,6 +632,12 @@ class InputStaging:
         return dev[:count].view(src.shape)
 
 
+def _upload_items(phases, staging):
+    import torch
+    return tuple(staging.copy(f"page_writes_{i}", items, torch.int32)
+                 for i, items in enumerate(phases))
+
+
 def upload(chunk: Chunk, staging: InputStaging) -> Chunk:
     """Move a packed chunk's index arrays to the device (int64 ids/rows, int32 tables)."""
     import torch
@@ -574,6 +654,8 @@ def upload(chunk: Chunk, staging: InputStaging) -> Chunk:
     if u["tail_src"] is not None:
         dev["tail_src"] = staging.copy("tail_src", u["tail_src"], torch.int64)
         dev["tail_dst"] = staging.copy("tail_dst", u["tail_dst"], torch.int64)
+    if u.get("page_writes") is not None:
+        dev["page_writes"] = _upload_items(u["page_writes"], staging)
     dev["used"] = staging.copy("unified_lengths", u["used"], torch.int32)
     dev["cu_q"] = staging.copy("unified_cu_q", u["cu_q"], torch.int32)
     dev["table"] = staging.copy("block_table", u["table"], torch.int32)
@@ -603,6 +685,8 @@ def _upload_tree(chunk: Chunk, staging: InputStaging) -> Chunk:
     if meta["kv_src"] is not None:
         meta["kv_src"] = staging.copy("kv_src", meta["kv_src"], torch.int64)
         meta["kv_dst"] = staging.copy("kv_dst", meta["kv_dst"], torch.int64)
+    if meta.get("page_writes") is not None:
+        meta["page_writes"] = _upload_items(meta["page_writes"], staging)
     if meta.get("row_pool_dst") is not None:
         chunk.host["row_pool_dst"] = meta["row_pool_dst"]
         meta["row_pool_dst"] = staging.copy("row_pool_dst", meta["row_pool_dst"], torch.int64)

@@ -1,0 +1,487 @@
+// Paged varlen GQA attention over an arena that keeps K and V in 8 bits.
+//
+//   o_i = sum_j softmax_j(scale * q_i . k_j) v_j
+//   k_j = kc_j * 2^(bk - 127),  v_j = vc_j * 2^(bv - 127)
+//
+// with e4m3 codes kc, vc and one E8M0 byte for K and one for V per (page,
+// KV head) at scales[(page * HK + head) * 2 + (0, 1)]. Sequences, block
+// table, causal alignment and GQA are those of paged_attention_kernel
+// (attention.hip). Codes are exact in bf16, so both products run on the bf16
+// matrix cores over the codes themselves: K's scale multiplies a page's 16
+// scores and V's its 16 probabilities, both in fp32 (a power of two each).
+// P is rounded to bf16 (2^-9 of a weight, about what the bf16 output rounds
+// by); scores, maxima, sums and outputs stay in fp32.
+#include <algorithm>
+
+#include "qx_common.h"
+#include "qx_status.h"
+
+namespace qx {
+namespace {
+
+constexpr int kPage = 16;  // tokens per arena page
+constexpr int kMaxKeys = 2560 * kPage;  // per sequence, as the 16-bit call takes
+constexpr int kMaxChunk = 8192;         // keys per split: 512 pages' ids and scales in LDS
+typedef __attribute__((address_space(3))) v2i lds_v2i;
+
+struct Attn8Args {
+  const uint16_t* q;
+  int64_t q_ld;
+  const int64_t* q_index;
+  const uint8_t *kp, *vp;
+  const uint16_t* scales;  // (pages, HK) pairs of bytes
+  const int *cu_q, *used, *table;
+  int64_t table_ld;
+  int max_used, HQ, HK, causal;
+  float scale_log2;
+  uint16_t* out16;
+  uint8_t* out8;
+  int64_t o_ld;
+  float* oscales;
+  int64_t os_ld;
+  float* lse;
+  int64_t lse_ld;
+  // splits: keys per split, and the partial results of `splits` of them
+  int chunk, splits;
+  int64_t rows;
+  float *part_o, *part_ml;
+};
+
+// 2^(b - 127) of an E8M0 byte b >= 1
+__device__ __forceinline__ float e8m0(int b) { return __uint_as_float((uint32_t)b << 23); }
+
+// 8 codes -> 8 bf16 (exact)
+__device__ __forceinline__ v8bf codes_bf16(uint32_t lo, uint32_t hi) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// One row of one head, 8 consecutive columns on each of its D / 8 lanes: the
+// bf16 row, or (D = 128) its e4m3 codes and their scale, from the values
+// rounded to bf16 as the separate quantization would see them.
+template <int D>
+__device__ __forceinline__ void store_row(const Attn8Args& p, int64_t row, int head, int j,
+                                          const float (&y)[8]) {
+  if (p.out8) {
+    if constexpr (D == 128) {
+      float v[8], amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = round_bf16(y[k]);
+        amax = fmaxf(amax, fabsf(v[k]));
+      }
+      const float s = fp8_scale(group_max<16>(amax));
+      const float r = recip(s);
+      *reinterpret_cast<uint2*>(p.out8 + row * p.o_ld + head * D + 8 * j) = make_uint2(
+          pack4_fp8(div_by(v[0], s, r), div_by(v[1], s, r), div_by(v[2], s, r), div_by(v[3], s, r)),
+          pack4_fp8(div_by(v[4], s, r), div_by(v[5], s, r), div_by(v[6], s, r), div_by(v[7], s, r)));
+      if (j == 0) p.oscales[(int64_t)head * p.os_ld + row] = s;
+    }
+    return;
+  }
+  *reinterpret_cast<uint4*>(p.out16 + row * p.o_ld + head * D + 8 * j) =
+      make_uint4(pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3]), pack2_bf16(y[4], y[5]),
+                 pack2_bf16(y[6], y[7]));
+}
+
+// Few query rows over long caches. The workgroup's 16 * NB columns are
+// (row, head of the KV head's group) pairs of one sequence; its 4 waves take
+// turns at steps of 32 keys (two pages) of the split [split * chunk, ...):
+// each wave moves its own K and V rows HBM -> LDS (a ring of kRing steps, no
+// barrier in the loop) and keeps its own softmax state; the four are joined
+// at the end, and splits by split_merge_kernel.
+//
+// S^T = K Q^T by 16x16x32 MFMAs: lane l holds column l % 16 and, of each
+// page, keys 4 (l / 16) + 0..3. P^T is then the PV product's B operand as it
+// stands when its 32 k slots are numbered (l / 16) * 8 + page * 4 + r, and
+// V^T in that order comes from the row-major codes by ds_read_b64_tr_b8.
+// Both tiles are XOR-swizzled by 16-byte chunks: the rows that one LDS read
+// touches land in different banks.
+constexpr int kRing = 2;
+
+template <int D, int NB>
+__global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
+  constexpr int CH = D / 16;              // 16-byte chunks per code row
+  constexpr int NC = D / 32;              // MFMA k-steps over the head dim
+  constexpr int ND = D / 16;              // 16-row d blocks of O^T
+  constexpr int TILE = 32 * D;            // bytes of one step's K (or V)
+  constexpr int LOADS = TILE / 1024;      // direct loads per tile
+  constexpr int KPL = 1024 / D;           // keys per direct load
+  constexpr int COLS = 16 * NB;
+  constexpr int LDS_RING = 4 * kRing * 2 * TILE;
+  constexpr int LDS_JOIN = 4 * COLS * D * 4 + 4 * COLS * 8;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS_RING > LDS_JOIN ? LDS_RING : LDS_JOIN];
+  __shared__ int pages[kMaxChunk / kPage];
+  __shared__ uint16_t bytes[kMaxChunk / kPage];
+
+  const int s = blockIdx.z;
+  const int G = p.HQ / p.HK;
+  const int kvh = blockIdx.y % p.HK;
+  const int cgroup = blockIdx.y / p.HK;
+  const int q0 = p.cu_q[s], q_len = p.cu_q[s + 1] - q0;
+  const int used = min(p.used[s], p.max_used);
+  const int cols = q_len * G;
+  if (cgroup * COLS >= cols) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, g4 = lane >> 4;
+
+  // keys [k0, k1) of this split that the last column of the group sees
+  const int last_col = min(cgroup * COLS + COLS, cols) - 1;
+  const int seen_end = p.causal ? min(used, used - q_len + last_col / G + 1) : used;
+  const int k0 = blockIdx.x * p.chunk;
+  const int k1 = min(seen_end, k0 + p.chunk);
+  const int npages = k1 > k0 ? (k1 - k0 + kPage - 1) / kPage : 0;
+  const int* trow = p.table + (int64_t)s * p.table_ld + k0 / kPage;
+  for (int i = tid; i < npages; i += 256) {
+    const int page = trow[i];
+    pages[i] = page;
+    bytes[i] = p.scales[(int64_t)page * p.HK + kvh];
+  }
+
+  // this lane's columns: their rows, heads, Q fragments and visible keys
+  v8bf qf[NB][NC];
+  int lim[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int c = cgroup * COLS + n * 16 + c16;
+    const int cc = min(c, cols - 1);
+    const int r = cc / G, head = kvh * G + cc % G;
+    const int64_t row = p.q_index ? p.q_index[q0 + r] : (int64_t)(q0 + r);
+    const uint16_t* q = p.q + row * p.q_ld + (int64_t)head * D;
+    lim[n] = c < cols ? (p.causal ? min(used, used - q_len + r + 1) : used) : 0;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      qf[n][k] = *reinterpret_cast<const v8bf*>(q + (k >> 1) * (D == 128 ? 64 : 0) + g4 * 16 +
+                                                (k & 1) * 8);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) asm volatile("" ::"v"(qf[n][k]));
+  }
+  __syncthreads();
+
+  const int64_t kv_row = (int64_t)p.HK * D;
+  const uint8_t* kbase = p.kp + kvh * D;
+  const uint8_t* vbase = p.vp + kvh * D;
+  uint8_t* ring = lds + wave * (kRing * 2 * TILE);
+  auto kswz = [](int key) { return D == 128 ? (key >> 1) & 7 : (key >> 2) & 3; };
+  auto vswz = [](int key) {
+    return D == 128 ? ((key >> 1) & 3) | ((key >> 2) & 4) : ((key >> 2) & 1) | ((key >> 3) & 2);
+  };
+  // step t of this wave: keys [k0 + 32 (4 t + wave), + 32); lanes past the
+  // split's last key read that key again
+  const int nsteps = (npages * kPage + 31) / 32;
+  const int mine = nsteps > wave ? (nsteps - wave + 3) / 4 : 0;
+  auto issue = [&](int t) {
+    const int key0 = 32 * (4 * t + wave);
+    uint8_t* at = ring + (t % kRing) * (2 * TILE);
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int in_step = i * KPL + lane / CH;
+        const int key = min(key0 + in_step, k1 - k0 - 1);
+        const int chunk = (lane % CH) ^ (v ? vswz(in_step) : kswz(in_step));
+        const int64_t row = (int64_t)pages[key / kPage] * kPage + key % kPage;
+        lds_dma16((v ? vbase : kbase) + row * kv_row + chunk * 16, at + v * TILE + i * 1024);
+      }
+  };
+
+  v4f o[NB][ND];
+  float m[NB], l[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // nothing of the above in flight beside the ring's loads
+  if (mine > 0) issue(0);
+  for (int t = 0; t < mine; ++t) {
+    // this wave's reads of the slot that step t + 1 refills have returned
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    if (t + 1 < mine) {
+      issue(t + 1);
+      wait_vmcnt<2 * LOADS>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    asm volatile("" ::: "memory");
+    const uint8_t* kt = ring + (t % kRing) * (2 * TILE);
+    const uint8_t* vt = kt + TILE;
+    const int key0 = 32 * (4 * t + wave);
+    const int pg = key0 / kPage;
+    const int b0 = bytes[pg], b1 = bytes[min(pg + 1, npages - 1)];
+    const float ks[2] = {e8m0(b0 & 255) * p.scale_log2, e8m0(b1 & 255) * p.scale_log2};
+    const float vs[2] = {e8m0(b0 >> 8), e8m0(b1 >> 8)};
+
+    v4f sc[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sc[n][0] = sc[n][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int pgi = 0; pgi < 2; ++pgi) {
+      const int key = pgi * 16 + c16;
+#pragma unroll
+      for (int k2 = 0; k2 < NC / 2; ++k2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(
+            kt + key * D + ((k2 * 4 + g4) ^ kswz(key)) * 16);
+        const v8bf lo = codes_bf16(w.x, w.y), hi = codes_bf16(w.z, w.w);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          sc[n][pgi] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qf[n][2 * k2], sc[n][pgi], 0, 0, 0);
+          sc[n][pgi] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qf[n][2 * k2 + 1], sc[n][pgi], 0, 0, 0);
+        }
+      }
+    }
+    v8bf pf[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int room = lim[n] - k0 - key0 - g4 * 4;  // key pgi * 16 + r of this lane is below it
+      float z[8], top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z[e] = (e >> 2) * 16 + (e & 3) < room ? sc[n][e >> 2][e & 3] * ks[e >> 2] : -INFINITY;
+        top = fmaxf(top, z[e]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float m_new = fmaxf(m[n], top);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m[n] - m_use);
+      m[n] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float pe = __builtin_amdgcn_exp2f(z[e] - m_use);
+        sum += pe;
+        pf[n][e] = (__bf16)(pe * vs[e >> 2]);
+      }
+      l[n] = l[n] * alpha + sum;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][d][e] *= alpha;
+    }
+    const int x = lane & 15;
+    const int vkey = (x >> 3) * 16 + g4 * 4 + ((x >> 1) & 3);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (lds_v2i*)(vt + vkey * D + ((d ^ vswz(vkey)) * 16) + (x & 1) * 8));
+      const v8bf vf = codes_bf16(w[0], w[1]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[n][d], 0, 0, 0);
+    }
+  }
+  __syncthreads();  // every wave is past its ring
+
+  // join the waves: o of (column, d = 16 blk + 4 g4 + e) as [wave][column][d]
+  float* jo = reinterpret_cast<float*>(lds);
+  float* jml = jo + 4 * COLS * D;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    l[n] += __shfl_xor(l[n], 16, 64);
+    l[n] += __shfl_xor(l[n], 32, 64);
+    float* at = jo + (wave * COLS + n * 16 + c16) * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<v4f*>(at + ((d * 4 + g4) ^ (c16 & 7)) * 4) = o[n][d];
+    if (g4 == 0) {
+      jml[(wave * COLS + n * 16 + c16) * 2] = m[n];
+      jml[(wave * COLS + n * 16 + c16) * 2 + 1] = l[n];
+    }
+  }
+  __syncthreads();
+  constexpr int LPC = D / 8;  // lanes per column, 8 values each
+  for (int cc = tid / LPC; cc < COLS; cc += 256 / LPC) {
+    const int c = cgroup * COLS + cc;
+    const int j = tid % LPC;
+    if (c >= cols) continue;  // whole columns leave together
+    float mm = -INFINITY, ll = 0.f, y[8] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jml[(w * COLS + cc) * 2]);
+    const float m_use = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(jml[(w * COLS + cc) * 2] - m_use);
+      ll += jml[(w * COLS + cc) * 2 + 1] * f;
+      const float* at = jo + (w * COLS + cc) * D;
+      const v4f a = *reinterpret_cast<const v4f*>(at + ((2 * j) ^ (cc & 7)) * 4);
+      const v4f b = *reinterpret_cast<const v4f*>(at + ((2 * j + 1) ^ (cc & 7)) * 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        y[k] += a[k] * f;
+        y[4 + k] += b[k] * f;
+      }
+    }
+    const int64_t row = q0 + c / G;
+    const int head = kvh * G + c % G;
+    if (p.splits > 1) {
+      const int64_t at = ((int64_t)blockIdx.x * p.rows + row) * p.HQ + head;
+      if (j == 0) {
+        p.part_ml[2 * at] = mm;
+        p.part_ml[2 * at + 1] = ll;
+      }
+      if (mm != -INFINITY) {
+        *reinterpret_cast<v4f*>(p.part_o + at * D + 8 * j) = v4f{y[0], y[1], y[2], y[3]};
+        *reinterpret_cast<v4f*>(p.part_o + at * D + 8 * j + 4) = v4f{y[4], y[5], y[6], y[7]};
+      }
+      continue;
+    }
+    const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] *= inv;
+    store_row<D>(p, row, head, j, y);
+    if (p.lse && j == 0)
+      p.lse[(int64_t)head * p.lse_ld + row] =
+          ll > 0.f ? (__log2f(ll) + m_use) * 0.6931471805599453f : -INFINITY;
+  }
+}
+
+// Join the splits of each (row, head): D / 8 lanes per pair.
+template <int D>
+__global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p, int64_t pairs) {
+  constexpr int LPC = D / 8;
+  const int64_t pair = (int64_t)blockIdx.x * (256 / LPC) + threadIdx.x / LPC;
+  const int j = threadIdx.x % LPC;
+  if (pair >= pairs) return;
+  const int64_t row = pair / p.HQ;
+  const int head = (int)(pair % p.HQ);
+  const int64_t step = p.rows * p.HQ;
+  float mm = -INFINITY;
+  for (int i = 0; i < p.splits; ++i) mm = fmaxf(mm, p.part_ml[2 * (i * step + pair)]);
+  const float m_use = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f, y[8] = {};
+  for (int i = 0; i < p.splits; ++i) {
+    const float mi = p.part_ml[2 * (i * step + pair)];
+    if (mi == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(mi - m_use);
+    ll += p.part_ml[2 * (i * step + pair) + 1] * f;
+    const float* at = p.part_o + (i * step + pair) * D + 8 * j;
+    const v4f a = *reinterpret_cast<const v4f*>(at), b = *reinterpret_cast<const v4f*>(at + 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      y[k] += a[k] * f;
+      y[4 + k] += b[k] * f;
+    }
+  }
+  const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y[k] *= inv;
+  store_row<D>(p, row, head, j, y);
+  if (p.lse && j == 0)
+    p.lse[(int64_t)head * p.lse_ld + row] =
+        ll > 0.f ? (__log2f(ll) + m_use) * 0.6931471805599453f : -INFINITY;
+}
+
+// Column blocks of a workgroup: two of 16 where a sequence's (row, head)
+// pairs pass one.
+inline int few_blocks(int64_t max_q, int64_t G) { return max_q * G > 16 ? 2 : 1; }
+
+// Keys per split of a call (a multiple of 128: the four waves' steps).
+int64_t split_chunk(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HK, int64_t G) {
+  const int64_t cols = 16 * few_blocks(max_q, G);
+  const int64_t groups = std::max<int64_t>(1, seqs * HK * ((max_q * G + cols - 1) / cols));
+  const int64_t want = std::max<int64_t>(1, 1024 / groups);
+  int64_t chunk = (max_used + want - 1) / want;
+  chunk = std::max<int64_t>(chunk, 256);
+  return std::min<int64_t>((chunk + 127) / 128 * 128, kMaxChunk);
+}
+
+int64_t split_count(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HK, int64_t G) {
+  const int64_t chunk = split_chunk(seqs, max_q, max_used, HK, G);
+  return std::max<int64_t>(1, (max_used + chunk - 1) / chunk);
+}
+
+template <int D, int NB>
+void few_launch(const Attn8Args& a, int64_t seqs, int64_t max_q, hipStream_t stream) {
+  const int G = a.HQ / a.HK;
+  const int64_t groups = (max_q * G + 16 * NB - 1) / (16 * NB);
+  hipLaunchKernelGGL((attention8_few_kernel<D, NB>),
+                     dim3((unsigned)a.splits, (unsigned)(a.HK * groups), (unsigned)seqs), dim3(256),
+                     0, stream, a);
+}
+
+}  // namespace
+}  // namespace qx
+
+using namespace qx;
+
+extern "C" {
+
+int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used,
+                                      int64_t HQ, int64_t HK, int64_t D) {
+  QX_CHECK(seqs >= 0 && rows >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 &&
+               HQ % HK == 0 && (D == 64 || D == 128),
+           "attention8_workspace: arguments");
+  const int64_t splits = split_count(seqs, max_q, max_used, HK, HQ / HK);
+  return splits > 1 ? splits * rows * HQ * (D + 2) * 4 : 0;
+}
+
+int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
+                        const void* v_pool, const void* scales, const int* cu_q, const int* used,
+                        const int* table, int64_t table_ld, int64_t seqs, int64_t rows,
+                        int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
+                        int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
+                        int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
+                        void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  QX_CHECK(q && k_pool && v_pool && scales && cu_q && used && table, "attention8: null pointer");
+  QX_CHECK((out_bf16 != nullptr) != (out_fp8 != nullptr), "attention8: one output, bf16 or e4m3");
+  QX_CHECK(D == 64 || D == 128, "attention8: head_dim %lld", (long long)D);
+  QX_CHECK(HQ > 0 && HK > 0 && HQ % HK == 0, "attention8: heads %lld/%lld", (long long)HQ,
+           (long long)HK);
+  QX_CHECK(page == kPage, "attention8: page of %lld tokens (the arena uses 16)", (long long)page);
+  QX_CHECK(seqs >= 0 && rows >= 0 && max_q >= 0 && max_used >= 0 && max_used <= kMaxKeys,
+           "attention8: %lld sequences, %lld rows, max_q %lld, max_used %lld (at most %d)",
+           (long long)seqs, (long long)rows, (long long)max_q, (long long)max_used, kMaxKeys);
+  QX_CHECK(!out_fp8 || (D == 128 && out_scales && os_ld >= rows && o_ld % 8 == 0),
+           "attention8: the e4m3 output needs D = 128, its scales and o_ld %% 8 == 0");
+  QX_CHECK(q_ld % 8 == 0 && o_ld % 8 == 0 && (!lse || lse_ld >= rows), "attention8: strides");
+  QX_CHECK((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out_bf16) & 15) == 0 &&
+               ((uintptr_t)out_fp8 & 7) == 0 && ((uintptr_t)scales & 1) == 0,
+           "attention8: alignment");
+  QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
+  if (seqs == 0 || max_q == 0 || rows == 0) return QX_OK;
+  const int64_t G = HQ / HK;
+  const int nb = few_blocks(max_q, G);
+  QX_CHECK(HK * ((max_q * G + 16 * nb - 1) / (16 * nb)) < 65536, "attention8: %lld rows a sequence",
+           (long long)max_q);
+  const int64_t need = qx_paged_attention8_workspace(seqs, rows, max_q, max_used, HQ, HK, D);
+  QX_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+           "attention8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+           (long long)need);
+  Attn8Args a{(const uint16_t*)q, q_ld, q_index, (const uint8_t*)k_pool, (const uint8_t*)v_pool,
+              (const uint16_t*)scales, cu_q, used, table, table_ld, (int)max_used, (int)HQ, (int)HK,
+              causal, scale * 1.4426950408889634f, (uint16_t*)out_bf16, (uint8_t*)out_fp8, o_ld,
+              out_scales, os_ld, lse, lse_ld};
+  a.chunk = (int)split_chunk(seqs, max_q, max_used, HK, G);
+  a.splits = (int)split_count(seqs, max_q, max_used, HK, G);
+  a.rows = rows;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o + (int64_t)a.splits * rows * HQ * D;
+  if (D == 128) {
+    if (nb == 1) few_launch<128, 1>(a, seqs, max_q, stream);
+    else few_launch<128, 2>(a, seqs, max_q, stream);
+  } else {
+    if (nb == 1) few_launch<64, 1>(a, seqs, max_q, stream);
+    else few_launch<64, 2>(a, seqs, max_q, stream);
+  }
+  if (a.splits > 1) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    const int64_t pairs = rows * HQ;
+    const int per = D == 128 ? 16 : 32;
+    const dim3 grid((unsigned)((pairs + per - 1) / per));
+    if (D == 128)
+      hipLaunchKernelGGL(split_merge_kernel<128>, grid, dim3(256), 0, stream, a, pairs);
+    else
+      hipLaunchKernelGGL(split_merge_kernel<64>, grid, dim3(256), 0, stream, a, pairs);
+  }
+  QX_LAUNCH_STATUS();
+}
+
+}  // extern "C"

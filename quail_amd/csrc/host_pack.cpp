@@ -425,6 +425,54 @@ int qx_pages_free_list(void* pool, int32_t* pages, int64_t cap, int64_t* n) {
   return QX_OK;
 }
 
+// Give the resident keys' pages the lowest ids: every page in use past the
+// first `live` ids (live = pages in use) takes the next free one below, both
+// in rising order. src[i] -> dst[i] are the moves (the caller copies the
+// pages); the free stack is left as a new pool's would be past `live`.
+// Refused while a key is pinned or a pack's temporary key lives: admitted
+// documents' and packs' block tables name the pages as they are.
+static int pages_compact(PagePool* p, int32_t* src, int32_t* dst, int64_t cap, int64_t* n) {
+  QX_CHECK(p && n, "pages_compact: null pointer");
+  for (auto& kv : p->keys)
+    QX_CHECK(!kv.second.pinned && kv.first >= 0,
+             "pages_compact: a pinned key or a pack's temporary pages are in use");
+  const int64_t live = p->num_pages - (int64_t)p->free.size();
+  std::vector<int32_t> to(p->num_pages, -1), from, into;
+  int32_t gap = 0;
+  for (int64_t page = live; page < p->num_pages; ++page) {
+    if (p->holds[page] == 0) continue;
+    while (p->holds[gap] != 0) ++gap;
+    to[page] = gap;
+    from.push_back((int32_t)page);
+    into.push_back(gap++);
+  }
+  QX_CHECK((int64_t)from.size() <= cap && (from.empty() || (src && dst)),
+           "pages_compact: %zu moves, room for %lld", from.size(), (long long)cap);
+  for (size_t i = 0; i < from.size(); ++i) {
+    src[i] = from[i];
+    dst[i] = into[i];
+    p->holds[into[i]] = p->holds[from[i]];
+    p->holds[from[i]] = 0;
+  }
+  for (auto& kv : p->keys)
+    for (auto* pages : {&kv.second.borrowed, &kv.second.owned})
+      for (int32_t& page : *pages)
+        if (to[page] >= 0) page = to[page];
+  for (int64_t i = 0; i < (int64_t)p->free.size(); ++i)
+    p->free[i] = (int32_t)(p->num_pages - 1 - i);
+  *n = (int64_t)from.size();
+  return QX_OK;
+}
+
+int qx_pages_compact(void* pool, int32_t* src, int32_t* dst, int64_t cap, int64_t* n) {
+  try {
+    return pages_compact(pool_of(pool), src, dst, cap, n);
+  } catch (const std::bad_alloc&) {
+    qx::set_error("pages_compact: out of host memory");
+    return QX_EINVAL;
+  }
+}
+
 // groups: 8 int64 per group {key, fresh, f, start, prefix tokens, suffixes,
 // suffix tokens kept in the key's pages, every suffix row answers};
 // prefix_ids: the fresh groups' prefixes, concatenated; suffix_lens and

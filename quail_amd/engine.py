@@ -491,7 +491,8 @@ class Engine:
         pack's meta carrying `row_pool_dst` (pool row
         per pack row, -1 for none), the same pass also writes the pack's KV
         into the arena pages of meta's layer (the kv_src -> kv_dst writes,
-        attention.py:1405)."""
+        attention.py:1405); an 8-bit arena's pages by meta's `page_writes`
+        (call A then reads the rows as they are, V in bf16)."""
         n = qkv.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if qkv.shape[1] < (hq + 2 * hk) * d:
@@ -507,7 +508,11 @@ class Engine:
             raise ValueError("identity must be arange(n) int64")
         cache = self._rope_cache()
         pools, dst2 = (None, None), None
-        if meta is not None and meta.get("row_pool_dst") is not None:
+        eight_bit = self._eight_bit()
+        if eight_bit and meta is not None and meta.get("page_writes") is not None:
+            self._write_pages(qkv, positions, attn, meta["page_writes"], meta["layer"])
+            meta["kv_fresh_layer"] = meta["layer"]
+        elif meta is not None and meta.get("row_pool_dst") is not None:
             dst2 = meta["row_pool_dst"]
             if dst2.shape[0] != n:
                 raise ValueError(f"row_pool_dst has {dst2.shape[0]} rows, qkv {n}")
@@ -528,15 +533,22 @@ class Engine:
         pages of meta's layer (pool row meta["unified"]["row_dst"][i]; the
         fresh-row write of write_kv, attention.py:1178-1191, in the same pass
         over qkv). Returns q; this layer's write_kv then copies only the
-        retained tails."""
+        retained tails. An 8-bit arena's pages are written by the page items
+        meta["unified"]["page_writes"], which hold every row once and the
+        retained tails too."""
         n = qkv.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if qkv.shape[1] < (hq + 2 * hk) * d:
             raise ValueError(f"qkv width {qkv.shape[1]} < {(hq + 2 * hk) * d}")
+        layer = meta["layer"]
+        if self._eight_bit():
+            q = torch.empty((n, hq * d), dtype=torch.bfloat16, device=qkv.device)
+            self._write_pages(qkv, positions, attn, meta["unified"]["page_writes"], layer, q)
+            meta["kv_fresh_layer"] = layer
+            return q
         dst = meta["unified"]["row_dst"]
         if dst.shape[0] != n:
             raise ValueError(f"row_dst has {dst.shape[0]} rows, qkv {n}")
-        layer = meta["layer"]
         k_pool, v_pool = self.arena.layer_kv(layer)
         self._check_pools(k_pool, v_pool)
         q = torch.empty((n, hq * d), dtype=torch.bfloat16, device=qkv.device)
@@ -554,7 +566,11 @@ class Engine:
         its V go into the arena pages of meta's layer, and q stays as the
         projection left it; this layer's paged attention then normalizes and
         rotates q as it loads it (qx_paged_attention_qnorm), with the same
-        arithmetic (bit for bit). Returns the raw q columns of qkv (a view)."""
+        arithmetic (bit for bit). Returns the raw q columns of qkv (a view).
+        The attention of an 8-bit arena takes q normed and rotated: there
+        this is qk_norm_rope_kv."""
+        if self._eight_bit():
+            return self.qk_norm_rope_kv(qkv, positions, attn, meta)
         n = qkv.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if d != GROUP or qkv.shape[1] < (hq + 2 * hk) * d:
@@ -586,12 +602,58 @@ class Engine:
             raise ValueError(f"V pool dtype {v_pool.dtype}: V pages are bf16 or fp16")
 
     def _v_dtype(self):
-        return self.arena.layer_kv(0)[1].dtype
+        """The type of contiguous V rows beside the arena's pages (call A)."""
+        return torch.bfloat16 if self._eight_bit() else self.arena.layer_kv(0)[1].dtype
+
+    def _eight_bit(self):
+        return getattr(self.arena, "eight_bit", False)
+
+    def _pools8(self, layer):
+        """The pointers of a layer's K codes, V codes and scales."""
+        k_pool, v_pool = self.arena.layer_kv(layer)
+        return _ptr(k_pool), _ptr(v_pool), _ptr(self.arena.layer_scales(layer))
+
+    def _write_pages(self, qkv, positions, attn, phases, layer, q=None):
+        """K (normed and rotated) and V of the page items' qkv rows into an
+        8-bit arena's pages, phase by phase, and their rows of q into `q`."""
+        hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
+        if qkv.shape[1] < (hq + 2 * hk) * d:
+            raise ValueError(f"qkv width {qkv.shape[1]} < {(hq + 2 * hk) * d}")
+        if positions.shape[0] != qkv.shape[0]:
+            raise ValueError(f"{positions.shape[0]} positions for {qkv.shape[0]} rows")
+        cache = self._rope_cache()
+        for items in phases:
+            self._check_items(items)
+            _lib.call("qx_qk_norm_rope_kv8", _ptr(qkv), qkv.stride(0), _ptr(q),
+                      0 if q is None else q.stride(0), *self._pools8(layer), _ptr(items),
+                      items.shape[0], _ptr(cache), int(cache.dtype == torch.float32),
+                      _ptr(positions), _ptr(attn.q_norm.weight), _ptr(attn.k_norm.weight), hq, hk,
+                      d, float(attn.q_norm.variance_epsilon), _stream())
+
+    def _write_page_rows(self, k3, v3, phases, layer):
+        """The same from K and V rows as they are (bf16)."""
+        for t in (k3, v3):
+            if t.dtype != torch.bfloat16:
+                raise ValueError(f"KV rows of {t.dtype}: 8-bit pages are written from bf16 rows")
+        for items in phases:
+            self._check_items(items)
+            _lib.call("qx_kv8_write", _ptr(k3), k3.stride(0), _ptr(v3), v3.stride(0),
+                      *self._pools8(layer), _ptr(items), items.shape[0], self.num_kv_heads,
+                      self.head_dim, _stream())
+
+    @staticmethod
+    def _check_items(items):
+        if items.dtype != torch.int32 or items.dim() != 2 or items.shape[1] != 5 or \
+                not items.is_contiguous():
+            raise ValueError("page items are contiguous (n, 5) int32")
 
     def kv_row_scatter(self, k3, v3, src, dst, layer):
         """Scatter KV rows into the layer's arena pages; dst < 0 is padding.
         bf16 V rows going to an fp16 V pool are converted (saturated at
         +-65504); rows already of the pool's type (the tail copy) are copied."""
+        if self._eight_bit():
+            raise ValueError("8-bit pages are written by page items (quail_amd.chunk.page_writes), "
+                             "not row by row")
         count = src.shape[0]
         row = self.num_kv_heads * self.head_dim
         k_pool, v_pool = self.arena.layer_kv(layer)
@@ -617,6 +679,13 @@ class Engine:
             return
         # qk_norm_rope_kv already wrote this layer's fresh rows
         fresh = meta.pop("kv_fresh_layer", None) != layer
+        if self._eight_bit():
+            if fresh and pool["page_writes"]:
+                if k3 is None:
+                    raise ValueError(f"layer {layer}: no K/V rows and none written by "
+                                     "qk_norm_rope_kv")
+                self._write_page_rows(k3, v3, pool["page_writes"], layer)
+            return
         if fresh and pool["src"].numel():
             if k3 is None:
                 raise ValueError(f"layer {layer}: no K/V rows and none written by "
@@ -668,8 +737,8 @@ class Engine:
         layer = meta["layer"]
         dev = q3.device
         written = meta.pop("kv_fresh_layer", None) == layer   # by qk_norm_rope_rows
-        if meta.get("kv_src") is not None and meta["kv_src"].numel() and not written:
-            self.kv_row_scatter(k3, v3, meta["kv_src"], meta["kv_dst"], layer)
+        if not written:
+            self._write_tree_kv(k3, v3, meta, layer)
         # call A reads the pack's own K and V rows contiguous (as
         # qk_norm_rope_rows gives them, else one identity scatter)
         row = hk * d
@@ -700,8 +769,11 @@ class Engine:
         k_pool, v_pool = self.arena.layer_kv(layer)
         out_b = torch.empty((nb, hq * d), dtype=torch.bfloat16, device=dev)
         lse_b = torch.empty((hq, max(nb, 1)), dtype=torch.float32, device=dev)
-        self._lse_call(q3, reads["rows"], k_pool, v_pool, reads, reads["table"], None, scale,
-                       out_b, lse_b)
+        if self._eight_bit():
+            self._attend8(q3, reads, layer, scale, q_index=reads["rows"], out=out_b, lse=lse_b)
+        else:
+            self._lse_call(q3, reads["rows"], k_pool, v_pool, reads, reads["table"], None, scale,
+                           out_b, lse_b)
         if reads.get("nodes") is not None:
             self._call_c(q3, k_rows, v_rows, reads["nodes"], scale, out_b, lse_b)
         args = (_ptr(out_a), out_a.stride(0), _ptr(out_b), out_b.stride(0), _ptr(lse_a),
@@ -720,6 +792,13 @@ class Engine:
             self.quant(merged, output=(o_q, o_s))
         meta["layer"] += 1
         return o_q, o_s
+
+    def _write_tree_kv(self, k3, v3, meta, layer):
+        """A tree pack's KV writes (attention.py:1405) from its K and V rows."""
+        if self._eight_bit():
+            self._write_page_rows(k3, v3, meta["page_writes"], layer)
+        elif meta.get("kv_src") is not None and meta["kv_src"].numel():
+            self.kv_row_scatter(k3, v3, meta["kv_src"], meta["kv_dst"], layer)
 
     def _call_c(self, q3, k_rows, v_rows, nodes, scale, out_b, lse_b):
         """Call C (attention.py:1424-1434): label-path rows over the rows
@@ -765,6 +844,51 @@ class Engine:
                   lse.stride(0), _ptr(work), n_work, rows, int(v.dtype == torch.bfloat16),
                   _stream())
 
+    def _attend8(self, q3, tables, layer, scale, *, q_index=None, out=None, quant=None, lse=None):
+        """One qx_paged_attention8 call over `tables`: bf16 rows into `out`, or
+        the o_proj input into quant = (e4m3 rows, scales), and each row's
+        log-sum-exp into `lse`."""
+        hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
+        n = q3.shape[0] if q_index is None else q_index.shape[0]
+        table, seqs = tables["table"], tables["used"].shape[0]
+        max_q, max_used = int(tables["max_q"]), int(tables["max_used"])
+        size = _lib.count("qx_paged_attention8_workspace", seqs, n, max_q, max_used, hq, hk, d)
+        work = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
+        o8, s8 = (None, None) if quant is None else quant
+        o = out if quant is None else o8
+        _lib.call("qx_paged_attention8", _ptr(q3), q3.stride(0), _ptr(q_index),
+                  *self._pools8(layer), _ptr(tables["cu_q"]), _ptr(tables["used"]), _ptr(table),
+                  table.stride(0), seqs, n, max_q, max_used, hq, hk, d, self.arena.page_tokens,
+                  float(scale), int(tables.get("causal", True)), _ptr(out), _ptr(o8), o.stride(0),
+                  _ptr(s8), 0 if s8 is None else self._scale_ld(s8), _ptr(lse),
+                  0 if lse is None else lse.stride(0), _ptr(work), size, _stream())
+
+    def read_pages(self, q3, tables, layer, *, softmax_scale=None):
+        """Attention of q3's rows (n, HQ, D), normed and rotated, over pages
+        the arena holds: `tables` as quail_amd.chunk.attention_plan or a
+        pack's reads give them (cu_q, used, table, max_q, max_used, causal).
+        Returns (bf16 rows (n, HQ*D), log-sum-exps (HQ, n) fp32); a row that
+        sees no key gets 0 and -inf."""
+        n, hq, d = q3.shape
+        if (hq, d) != (self.num_q_heads, self.head_dim) or q3.dtype != torch.bfloat16:
+            raise ValueError(f"query rows of {tuple(q3.shape)} {q3.dtype} for "
+                             f"{self.num_q_heads} heads of {self.head_dim} in bf16")
+        if q3.stride(2) != 1 or (hq > 1 and q3.stride(1) != d):
+            raise ValueError("a query row's heads are contiguous")
+        scale = d ** -0.5 if softmax_scale is None else softmax_scale
+        out = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
+        lse = torch.empty((hq, n), dtype=torch.float32, device=q3.device)
+        if not n:
+            return out, lse
+        if self._eight_bit():
+            self._attend8(q3, tables, layer, scale, out=out, lse=lse)
+        else:
+            k_pool, v_pool = self.arena.layer_kv(layer)
+            self._check_pools(k_pool, v_pool)
+            self._lse_call(q3, None, k_pool, v_pool, tables, tables["table"], None, float(scale),
+                           out, lse)
+        return out, lse
+
     def attention_unified(self, q3, k3, v3, meta, *, softmax_scale=None, output=None):
         """Write the chunk's KV to its pages, then one paged causal call with
         the o_proj input quantization fused (attention.py:1477-1573)."""
@@ -784,9 +908,8 @@ class Engine:
         meta = chunk.meta
         if chunk.attention_mode == "tree":
             layer = meta["layer"]
-            written = meta.pop("kv_fresh_layer", None) == layer
-            if meta.get("kv_src") is not None and meta["kv_src"].numel() and not written:
-                self.kv_row_scatter(k3, v3, meta["kv_src"], meta["kv_dst"], layer)
+            if meta.pop("kv_fresh_layer", None) != layer:
+                self._write_tree_kv(k3, v3, meta, layer)
         else:
             self.write_kv(k3, v3, meta)
         meta.pop("q_norm_on_load", None)
@@ -821,9 +944,6 @@ class Engine:
         qkv projection, normalized and rotated as the kernel loads it."""
         n = q3.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
-        k_pool, v_pool = self.arena.layer_kv(layer)
-        self._check_pools(k_pool, v_pool)
-        v_bf16 = int(v_pool.dtype == torch.bfloat16)
         scale = d ** -0.5 if softmax_scale is None else softmax_scale
         table = tables["table"]
         if output is not None:
@@ -831,6 +951,17 @@ class Engine:
         else:
             o_q = torch.empty((n, hq * d), dtype=self.fp8, device=q3.device)
             o_s = self._col_major_scales(n, hq * d, q3.device)
+        if self._eight_bit():
+            if d == GROUP:
+                self._attend8(q3, tables, layer, scale, quant=(o_q, o_s))
+            else:
+                o = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
+                self._attend8(q3, tables, layer, scale, out=o)
+                self.quant(o, output=(o_q, o_s))
+            return o_q, o_s
+        k_pool, v_pool = self.arena.layer_kv(layer)
+        self._check_pools(k_pool, v_pool)
+        v_bf16 = int(v_pool.dtype == torch.bfloat16)
         seqs = tables["used"].shape[0]
         q_ld = q3.stride(0)
         args = (_ptr(k_pool), _ptr(v_pool), _ptr(tables["cu_q"]), _ptr(tables["used"]),
@@ -870,6 +1001,8 @@ class Engine:
         n = q3.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         unified = meta["unified"]
+        if self._eight_bit():
+            return self.read_pages(q3, unified, layer)[0]
         k_pool, v_pool = self.arena.layer_kv(layer)
         o = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
         table = unified["table"]

@@ -254,6 +254,15 @@ class PageArena:
             left -= take
         return rows
 
+    def compact(self):
+        """Give the resident keys' pages the lowest ids: (moved pages, their
+        new ids). ValueError while a key is pinned or a pack's temporary pages
+        live. The caller copies the pages before anything reads them."""
+        moved = (ctypes.c_int32 * max(1, self.num_pages))()
+        _pages_call("qx_pages_compact", self.handle, moved, self._buf, self.num_pages,
+                    ctypes.byref(self._out))
+        return moved[:self._out.value], self._buf[:self._out.value]
+
     # ---- pins and retention ------------------------------------------------
 
     def pin(self, key) -> None:
