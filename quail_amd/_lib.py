@@ -54,7 +54,8 @@ SIGNATURES = {
     "qx_paged_attention8_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64],
     "qx_paged_attention8": [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _i64, _p, _i64, _p, _i64,
-                            _p, _i64, _p],
+                            _p, _i64, _p, _i64, _p],
+    "qx_paged_attention8_work": [_p, _p, _i64, _i64, _i64, _i32, _p, _i64],
     "qx_copy_pages": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p],
     "qx_pages_compact": [_p, _p, _p, _i64, _p],
     "qx_embed": [_p, _i64, _p, _p, _i64, _i64, _i64, _p],
@@ -103,7 +104,8 @@ SIGNATURES = {
 # entry points returning a count (>= 0) or -1 instead of a status
 RETURNS_COUNT = {"qx_paged_attention_work", "qx_paged_attention_tile_rows",
                  "qx_paged_attention_max_keys", "qx_vocab_logprobs_workspace",
-                 "qx_vocab_logprobs_noalloc_max_bytes", "qx_paged_attention8_workspace"}
+                 "qx_vocab_logprobs_noalloc_max_bytes", "qx_paged_attention8_workspace",
+                 "qx_paged_attention8_work"}
 
 
 class QxUnavailable(RuntimeError):

@@ -242,7 +242,8 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
         for tables in (unified, meta["final_query"]):
             if tables is not None:
                 tables["work"], tables["n_work"], tables["work_rows"] = _work_list(
-                    tables, attention_heads, choose_rows=True)
+                    tables, attention_heads, choose_rows=True,
+                    eight_bit=getattr(arena, "eight_bit", False))
     if timing is not None:
         timing["pack_py"] = timing.get("pack_py", 0.0) + (t1 - t0)
         timing["pack_unified"] = timing.get("pack_unified", 0.0) + (time.perf_counter() - t1)
@@ -464,8 +465,10 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
     if attention_heads is not None:
         for tables in (segments, reads, reads and reads.get("nodes")):
             if tables:
+                # call B alone reads the arena's pages
                 tables["work"], tables["n_work"], tables["work_rows"] = _work_list(
-                    tables, attention_heads, choose_rows=True)
+                    tables, attention_heads, choose_rows=True,
+                    eight_bit=tables is reads and getattr(arena, "eight_bit", False))
     ids = _cat(id_parts)
     positions = _cat(pos_parts)
     final = _cat(finals)
@@ -484,11 +487,12 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
                  host_ids=ids, host_positions=positions)
 
 
-def _work_list(tables, heads, choose_rows=False):
+def _work_list(tables, heads, choose_rows=False, eight_bit=False):
     """(work pairs, count, query rows per item) of a paged call over `tables`
     (host arrays). choose_rows: the tile height qx_paged_attention_tile_rows
     picks for these sequences (the call must then pass it); otherwise the
-    default (0)."""
+    default (0). eight_bit: for a call over an 8-bit arena's pages (its tiles
+    have one height)."""
     from quail_amd import _lib
     hq, hk, d = heads
     cu_q = np.ascontiguousarray(tables["cu_q"], dtype=np.int32)
@@ -496,6 +500,12 @@ def _work_list(tables, heads, choose_rows=False):
     seqs = len(used)
     causal = int(tables.get("causal", True))
     rows = 0
+    if eight_bit:
+        cap = int(cu_q[-1]) + seqs if seqs else 1
+        work = np.zeros(2 * max(cap, 1), dtype=np.int32)
+        n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
+                       hk, causal, work.ctypes.data, cap)
+        return work[:2 * n], n, 0
     if choose_rows:
         rows = _lib.count("qx_paged_attention_tile_rows", cu_q.ctypes.data, used.ctypes.data,
                           seqs, hq, hk, d, causal)
@@ -577,16 +587,17 @@ def page_writes(src, dst, tail_src=None, tail_dst=None):
     return tuple(np.ascontiguousarray(items[phase == p]) for p in np.unique(phase))
 
 
-def attention_plan(cu_q, used, table, *, heads, causal=True):
+def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
     """The tables of a paged attention call over sequences a caller lays out
     itself (Engine.read_pages): sequence s has query rows cu_q[s] .. cu_q[s+1]
     and keys [0, used[s]) through table[s]. cu_q, used and table are int32
-    tensors on the device; heads = (HQ, HK, D)."""
+    tensors on the device; heads = (HQ, HK, D); eight_bit: whether the arena
+    that is read keeps 8-bit pages."""
     host = dict(cu_q=cu_q.cpu().numpy(), used=used.cpu().numpy(), causal=causal)
     tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),
                   max_used=int(host["used"].max(initial=0)))
-    work, n_work, rows = _work_list(host, heads, choose_rows=True)
+    work, n_work, rows = _work_list(host, heads, choose_rows=True, eight_bit=eight_bit)
     if n_work:
         import torch
         tables.update(work=torch.from_numpy(work).to(cu_q.device), n_work=n_work, work_rows=rows)

@@ -12,9 +12,11 @@
 // P is rounded to bf16 (2^-9 of a weight, about what the bf16 output rounds
 // by); scores, maxima, sums and outputs stay in fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "qx_common.h"
 #include "qx_status.h"
+#include "work_list.h"
 
 namespace qx {
 namespace {
@@ -342,6 +344,338 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
   }
 }
 
+// Many query rows. A workgroup is 4 waves: QSUB 32-row query tiles of one
+// sequence x HPB heads that share a KV head, one wave per (tile, head); keys
+// come in 64-key tiles (four pages, one per wave to move), software
+// pipelined with one barrier a step. A page's codes travel HBM -> registers,
+// become bf16, scaled (exact), once per workgroup, and lie in LDS as the
+// 16-bit kernel's tiles do, so that both products run on the bf16 matrix
+// cores. (Scores from the codes themselves on the FP8 cores, with q as the
+// sum of two e4m3 numbers, take the same matrix time and no conversion, but
+// those cores drop what lies 2^-12 below the largest product of a sum.)
+constexpr int kBK = 64;
+// a row's reference max moves when a tile raises its max by more than this
+// many powers of two (probabilities then stay below 2^8)
+constexpr float kLazyLog2 = 8.0f;
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+template <int D, int HPB, int QSUB>
+__global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, const int* work,
+                                                                 int zgroups, int seqs) {
+  static_assert(HPB * QSUB == 4, "four waves");
+  constexpr int BQ = 32 * QSUB;
+  constexpr int NC = D / 16;       // MFMA k-steps of S
+  constexpr int NDS = D / 32;      // 32-row d tiles of O^T
+  constexpr int VROW = 2 * D;      // bytes of a bf16 V row in LDS
+  constexpr int CH = D / 16;       // 16-byte chunks of a code row
+  constexpr int KPL = 1024 / D;    // keys per direct load
+  constexpr int LOADS = 16 / KPL;  // loads of a page's 16 rows
+  __shared__ __attribute__((aligned(1024))) uint8_t k_lds[2][kBK * VROW];
+  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[2][kBK * VROW];
+  __shared__ int pages[kMaxKeys / kPage];
+  __shared__ uint16_t bytes[kMaxKeys / kPage];
+
+  int s, qt, zg;
+  if (work) {
+    const int item = blockIdx.x / zgroups;
+    zg = blockIdx.x % zgroups;
+    s = work[2 * item];
+    qt = work[2 * item + 1];
+  } else {
+    s = blockIdx.y;
+    qt = gridDim.x - 1 - blockIdx.x;
+    zg = blockIdx.z;
+  }
+  const int sc = min(max(s, 0), seqs - 1);
+  const int q0 = p.cu_q[sc], q_len = p.cu_q[sc + 1] - q0;
+  const int used = min(p.used[sc], p.max_used);
+  if (s < 0 || s >= seqs || qt < 0 || qt * BQ >= q_len) return;
+  const int G = p.HQ / p.HK;
+  const int per_kv = G / HPB;
+  const int kvh = zg / per_kv;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = kvh * G + (zg % per_kv) * HPB + wave % HPB;
+  const int qsub = wave / HPB;
+  const int half = lane >> 5, col = lane & 31;
+
+  const int off = p.causal ? used - q_len : 0;
+  const int wave_row0 = qt * BQ + qsub * 32;
+  const int r = wave_row0 + col;
+  const bool r_ok = r < q_len;
+  const int block_last = min(qt * BQ + BQ, q_len) - 1;
+  const int kv_end = max(0, p.causal ? min(used, off + block_last + 1) : used);
+  const int ntiles = (kv_end + kBK - 1) / kBK;
+  const int npages = (kv_end + kPage - 1) / kPage;
+  const int lim = p.causal ? min(off + r + 1, used) : used;  // keys < lim are visible
+  const int lim_min = p.causal ? min(off + wave_row0 + 1, used) : used;
+  const bool rows_full = wave_row0 + 32 <= q_len;
+
+  // the sequence's pages and this KV head's scale bytes
+  const int* trow = p.table + (int64_t)s * p.table_ld;
+  for (int i = tid; i < npages; i += 256) {
+    const int page = trow[i];
+    pages[i] = page;
+    bytes[i] = p.scales[(int64_t)page * p.HK + kvh];
+  }
+  // Q^T fragments (B operand): lane holds row `col`, d = c * 16 + half * 8 .. + 8
+  v8bf qf[NC];
+  {
+    const int rr = r_ok ? r : q_len - 1;
+    const int64_t row = p.q_index ? p.q_index[q0 + rr] : (int64_t)(q0 + rr);
+    const uint16_t* q = p.q + row * p.q_ld + (int64_t)head * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qf[c] = *reinterpret_cast<const v8bf*>(q + c * 16 + half * 8);
+  }
+  __syncthreads();
+
+  const int64_t kv_row = (int64_t)p.HK * D;
+  const uint8_t* kbase = p.kp + kvh * D;
+  const uint8_t* vbase = p.vp + kvh * D;
+  // 16-byte chunk swizzles of the bf16 rows, as the 16-bit kernel's
+  auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
+  auto vswz = [](int key) { return D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; };
+  // this wave's page of a tile: lane's 16 codes of row j * KPL + lane / CH
+  const int row0 = lane / CH, chunk = lane % CH;
+  uint4 kreg[LOADS], vreg[LOADS];
+  // rows past the last key re-read it
+  auto load = [&](int t, const uint8_t* base, uint4 (&reg)[LOADS]) {
+    const int first = t * kBK + wave * kPage;
+    const int slot = min(first, kv_end - 1) / kPage;
+    const int left = kv_end - 1 - slot * kPage;  // the last row of this page to read
+    const int64_t page = __builtin_amdgcn_readfirstlane(pages[slot]);
+    const uint8_t* at = base + page * kPage * kv_row + chunk * 16;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      reg[j] = *reinterpret_cast<const uint4*>(at + (uint32_t)(min(row0 + j * KPL, left) * (int)kv_row));
+  };
+  auto store = [&](int t, uint8_t* tile, const uint4 (&reg)[LOADS], bool v) {
+    const int slot = min(t * (kBK / kPage) + wave, npages - 1);
+    const int pair = __builtin_amdgcn_readfirstlane(bytes[slot]);
+    const float scale = e8m0(v ? pair >> 8 : pair & 255);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int key = wave * kPage + row0 + j * KPL;
+      const uint32_t w[4] = {reg[j].x, reg[j].y, reg[j].z, reg[j].w};
+      uint32_t b[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
+        b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true));
+      }
+      const int z = v ? vswz(key) : kswz(key);
+      *reinterpret_cast<uint4*>(tile + key * VROW + ((2 * chunk) ^ z) * 16) = make_uint4(b[0], b[1], b[2], b[3]);
+      *reinterpret_cast<uint4*>(tile + key * VROW + ((2 * chunk + 1) ^ z) * 16) = make_uint4(b[4], b[5], b[6], b[7]);
+    }
+  };
+  // K fragment (A operand of S^T): key `col` (+ 32), d chunk 2c + half
+  int k_off[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) k_off[c] = col * VROW + (((2 * c + half) ^ kswz(col)) * 16);
+  // V^T fragment by transposing reads: lane 16 g + x reads 4 halfwords of key
+  // 4 * half + x / 4 (+ 8) at column 16 (g & 1) + 4 (x & 3) of a 32-d tile
+  int v_off[NDS];
+  {
+    const int x = lane & 15;
+    const int key = 4 * half + (x >> 2);
+    const int c = 2 * ((lane >> 4) & 1) + ((x & 3) >> 1);
+#pragma unroll
+    for (int d = 0; d < NDS; ++d)
+      v_off[d] = key * VROW + (((d * 4 + c) ^ vswz(key)) * 16) + 8 * (x & 1);
+  }
+
+  v16f o[NDS];
+#pragma unroll
+  for (int d = 0; d < NDS; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  auto read_k = [&](const uint8_t* kl, int c, v8bf (&f)[2]) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      f[ks] = *reinterpret_cast<const v8bf*>(kl + ks * 32 * VROW + k_off[c]);
+  };
+  auto read_v = [&](const uint8_t* vl, int kc, int d) -> v8bf {
+    const uint8_t* at = vl + ((kc >> 1) * 32 + (kc & 1) * 16) * VROW + v_off[d];
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * VROW));
+    const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(v8bf, both);
+  };
+  auto mask_tile = [&](int t, v16f (&sacc)[2]) {
+    const int t0 = t * kBK;
+    if (t0 + kBK <= lim_min && rows_full) return;  // every row of the wave sees it whole
+    const int room = r_ok ? lim - t0 - half * 4 : -1;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sacc[ks][i] = ks * 32 + (i >> 2) * 8 + (i & 3) < room ? sacc[ks][i] : -INFINITY;
+  };
+  auto rescale = [&](const v16f (&sacc)[2], float& alpha, float& m_use) {
+    float part[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      part[g] = sacc[g >> 1][(g & 1) * 8];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) part[g] = fmaxf(part[g], sacc[g >> 1][(g & 1) * 8 + i]);
+    }
+    const float tmax = max_halves(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+    const float m_cand = fmaxf(m_run, tmax);
+    const bool move = (m_cand - m_run) * p.scale_log2 > kLazyLog2;
+    alpha = move ? __builtin_amdgcn_exp2f((m_run - m_cand) * p.scale_log2) : 1.0f;
+    m_run = move ? m_cand : m_run;
+    m_use = m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+      for (int d = 0; d < NDS; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+    }
+  };
+  auto step_end = [&]() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    lds_barrier();
+  };
+  // Step t: softmax and PV of tile t beside S of tile t + 1. Tiles reach LDS
+  // a step before their use: K of tile t + 2 and V of tile t + 1 are stored
+  // from the registers that step t - 1 loaded, and the next ones load.
+  // The exponentials run between the S MFMAs, two behind each, in an order
+  // that sched_barrier keeps.
+  auto step = [&](const int t, const int cur, v16f (&s_cur)[2], v16f (&s_next)[2], auto last_c) {
+    constexpr bool LAST = decltype(last_c)::value;
+    if (!LAST) {
+      store(t + 1, &v_lds[cur ^ 1][0], vreg, true);
+      if (t + 2 < ntiles) {
+        store(t + 2, &k_lds[cur][0], kreg, false);
+        load(t + 2, vbase, vreg);
+        if (t + 3 < ntiles) load(t + 3, kbase, kreg);
+      }
+    }
+    const uint8_t* kl = &k_lds[cur ^ 1][0];
+    const uint8_t* vl = &v_lds[cur][0];
+    constexpr int kAhead = 3;
+    v8bf kf[NC][2];
+    if (!LAST) {
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) read_k(kl, c, kf[c]);
+    }
+    mask_tile(t, s_cur);
+    float alpha, m_use;
+    rescale(s_cur, alpha, m_use);
+    float psum = 0.f;
+    v8bf pf[4], vf[4][NDS];
+    constexpr int PER = 16 / NC;  // scores behind each MFMA
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (!LAST) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (ks == 0 && c + kAhead < NC) read_k(kl, c + kAhead, kf[c + kAhead]);
+        }
+        if (c == NC - 1) {  // V of the first 16 keys
+#pragma unroll
+          for (int d = ks * (NDS / 2); d < (ks + 1) * (NDS / 2); ++d) vf[0][d] = read_v(vl, 0, d);
+        }
+        if (!LAST)
+          s_next[ks] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[c][ks], qf[c], c == 0 ? v16f{} : s_next[ks], 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          const int i = (c * 2 + ks) * PER + u;
+          const float pv = __builtin_amdgcn_exp2f(fmaf(s_cur[i >> 4][i & 15], p.scale_log2, -m_use));
+          psum += pv;
+          pf[i >> 3][i & 7] = (__bf16)pv;
+        }
+      }
+    if (!LAST) __builtin_amdgcn_sched_barrier(0);
+    l_run = l_run * alpha + sum_halves(psum);
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int d = 0; d < NDS; ++d) {
+        if (kc < 3) vf[kc + 1][d] = read_v(vl, kc + 1, d);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[kc][d], pf[kc], o[d], 0, 0, 0);
+        if (!LAST) __builtin_amdgcn_sched_barrier(0);
+      }
+    step_end();
+  };
+
+  v16f sa[2], sb[2];
+  if (ntiles > 0) {
+    load(0, kbase, kreg);
+    load(0, vbase, vreg);
+    store(0, &k_lds[0][0], kreg, false);
+    if (ntiles > 1) load(1, kbase, kreg);
+    store(0, &v_lds[0][0], vreg, true);
+    if (ntiles > 1) {
+      load(1, vbase, vreg);
+      store(1, &k_lds[1][0], kreg, false);
+      if (ntiles > 2) load(2, kbase, kreg);
+    }
+    step_end();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      v8bf kf[2];
+      read_k(&k_lds[0][0], c, kf);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        sa[ks] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[c], c == 0 ? v16f{} : sa[ks], 0, 0, 0);
+    }
+    step_end();
+    int t = 0;
+    for (; t + 2 < ntiles; t += 2) {
+      step(t, 0, sa, sb, std::false_type{});
+      step(t + 1, 1, sb, sa, std::false_type{});
+    }
+    if (t + 1 < ntiles) {
+      step(t, 0, sa, sb, std::false_type{});
+      step(t + 1, 1, sb, sa, std::true_type{});
+    } else {
+      step(t, 0, sa, sb, std::true_type{});
+    }
+  }
+
+  // epilogue: lane holds row `col`, d = dt * 32 + (i / 4) * 8 + half * 4 + i % 4;
+  // the wave's rows go out through LDS so that a store writes whole rows,
+  // 16-byte chunks XOR-swizzled by the row
+  const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+  if (p.lse && r_ok && half == 0) {
+    const float m_use = m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
+    p.lse[(int64_t)head * p.lse_ld + q0 + r] =
+        l_run > 0.f ? (__log2f(l_run) + m_use) * 0.6931471805599453f : -INFINITY;
+  }
+  uint8_t* stage = &v_lds[0][0] + wave * 32 * VROW;
+  static_assert(4 * 32 * VROW <= sizeof(v_lds), "epilogue staging");
+  constexpr int OCH = VROW / 16;
+#pragma unroll
+  for (int d = 0; d < NDS; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int at = 2 * (d * 32 + g * 8 + half * 4);
+      *reinterpret_cast<uint2*>(stage + col * VROW + (((at >> 4) ^ (col % OCH)) << 4) + (at & 15)) =
+          make_uint2(pack2_bf16(o[d][g * 4] * inv, o[d][g * 4 + 1] * inv),
+                     pack2_bf16(o[d][g * 4 + 2] * inv, o[d][g * 4 + 3] * inv));
+    }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  constexpr int LPC = D / 8, RPP = 64 / LPC;
+  const int rows_here = min(32, q_len - wave_row0);
+#pragma unroll
+  for (int pass = 0; pass < 32 / RPP; ++pass) {
+    const int rr = pass * RPP + lane / LPC, j = lane % LPC;
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * VROW + ((j ^ (rr % OCH)) << 4));
+    if (rr < rows_here) {  // whole rows
+      const float y[8] = {lo_bf16(w.x), hi_bf16(w.x), lo_bf16(w.y), hi_bf16(w.y),
+                          lo_bf16(w.z), hi_bf16(w.z), lo_bf16(w.w), hi_bf16(w.w)};
+      store_row<D>(p, q0 + wave_row0 + rr, head, j, y);
+    }
+  }
+}
+
 // Join the splits of each (row, head): D / 8 lanes per pair.
 template <int D>
 __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p, int64_t pairs) {
@@ -397,6 +731,29 @@ int64_t split_count(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HK, i
   return std::max<int64_t>(1, (max_used + chunk - 1) / chunk);
 }
 
+// Heads per workgroup of the tile kernel, and its query rows.
+inline int tile_heads(int64_t G) { return G % 4 == 0 ? 4 : (G % 2 == 0 ? 2 : 1); }
+inline int tile_height(int64_t G) { return 32 * (4 / tile_heads(G)); }
+
+// The few-row kernel up to two column blocks.
+inline bool few_rows(int64_t max_q, int64_t G) { return max_q * G <= 32; }
+
+template <int D>
+void tile_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t seqs, int64_t max_q,
+                 hipStream_t stream) {
+  const int G = a.HQ / a.HK, hpb = tile_heads(G), rows = tile_height(G);
+  const int zgroups = a.HQ / hpb;
+  const dim3 grid = work ? dim3((unsigned)(n_work * zgroups))
+                         : dim3((unsigned)((max_q + rows - 1) / rows), (unsigned)seqs,
+                                (unsigned)zgroups);
+  if (hpb == 4)
+    hipLaunchKernelGGL((attention8_tile_kernel<D, 4, 1>), grid, dim3(256), 0, stream, a, work, zgroups, (int)seqs);
+  else if (hpb == 2)
+    hipLaunchKernelGGL((attention8_tile_kernel<D, 2, 2>), grid, dim3(256), 0, stream, a, work, zgroups, (int)seqs);
+  else
+    hipLaunchKernelGGL((attention8_tile_kernel<D, 1, 4>), grid, dim3(256), 0, stream, a, work, zgroups, (int)seqs);
+}
+
 template <int D, int NB>
 void few_launch(const Attn8Args& a, int64_t seqs, int64_t max_q, hipStream_t stream) {
   const int G = a.HQ / a.HK;
@@ -418,8 +775,16 @@ int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q,
   QX_CHECK(seqs >= 0 && rows >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 &&
                HQ % HK == 0 && (D == 64 || D == 128),
            "attention8_workspace: arguments");
+  if (!few_rows(max_q, HQ / HK)) return 0;
   const int64_t splits = split_count(seqs, max_q, max_used, HK, HQ / HK);
   return splits > 1 ? splits * rows * HQ * (D + 2) * 4 : 0;
+}
+
+int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                                 int64_t HK, int causal, int* work, int64_t capacity) {
+  QX_CHECK(cu_q && used && work && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
+           "attention8_work: arguments");
+  return attention_work_list(cu_q, used, seqs, tile_height(HQ / HK), causal, work, capacity);
 }
 
 int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
@@ -428,7 +793,8 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
                         int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
                         int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
                         int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
-                        void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+                        const int* work, int64_t n_work, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream) {
   QX_CHECK(q && k_pool && v_pool && scales && cu_q && used && table, "attention8: null pointer");
   QX_CHECK((out_bf16 != nullptr) != (out_fp8 != nullptr), "attention8: one output, bf16 or e4m3");
   QX_CHECK(D == 64 || D == 128, "attention8: head_dim %lld", (long long)D);
@@ -445,6 +811,7 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
                ((uintptr_t)out_fp8 & 7) == 0 && ((uintptr_t)scales & 1) == 0,
            "attention8: alignment");
   QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
+  QX_CHECK(!work || (n_work >= 0 && n_work * HQ < (1LL << 24)), "attention8: work items");
   if (seqs == 0 || max_q == 0 || rows == 0) return QX_OK;
   const int64_t G = HQ / HK;
   const int nb = few_blocks(max_q, G);
@@ -458,6 +825,12 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
               (const uint16_t*)scales, cu_q, used, table, table_ld, (int)max_used, (int)HQ, (int)HK,
               causal, scale * 1.4426950408889634f, (uint16_t*)out_bf16, (uint8_t*)out_fp8, o_ld,
               out_scales, os_ld, lse, lse_ld};
+  if (!few_rows(max_q, G)) {
+    if (work && n_work == 0) return QX_OK;
+    if (D == 128) tile_launch<128>(a, work, n_work, seqs, max_q, stream);
+    else tile_launch<64>(a, work, n_work, seqs, max_q, stream);
+    QX_LAUNCH_STATUS();
+  }
   a.chunk = (int)split_chunk(seqs, max_q, max_used, HK, G);
   a.splits = (int)split_count(seqs, max_q, max_used, HK, G);
   a.rows = rows;

@@ -854,6 +854,11 @@ class Engine:
         max_q, max_used = int(tables["max_q"]), int(tables["max_used"])
         size = _lib.count("qx_paged_attention8_workspace", seqs, n, max_q, max_used, hq, hk, d)
         work = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
+        # the list of the call's query tiles, when the plan or pack carries one
+        items = tables.get("work")
+        if not torch.is_tensor(items):
+            items = None
+        n_items = int(tables.get("n_work", 0)) if items is not None else 0
         o8, s8 = (None, None) if quant is None else quant
         o = out if quant is None else o8
         _lib.call("qx_paged_attention8", _ptr(q3), q3.stride(0), _ptr(q_index),
@@ -861,7 +866,8 @@ class Engine:
                   table.stride(0), seqs, n, max_q, max_used, hq, hk, d, self.arena.page_tokens,
                   float(scale), int(tables.get("causal", True)), _ptr(out), _ptr(o8), o.stride(0),
                   _ptr(s8), 0 if s8 is None else self._scale_ld(s8), _ptr(lse),
-                  0 if lse is None else lse.stride(0), _ptr(work), size, _stream())
+                  0 if lse is None else lse.stride(0), _ptr(items), n_items, _ptr(work), size,
+                  _stream())
 
     def read_pages(self, q3, tables, layer, *, softmax_scale=None):
         """Attention of q3's rows (n, HQ, D), normed and rotated, over pages

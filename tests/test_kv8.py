@@ -221,12 +221,12 @@ def test_entry_points_refuse_bad_arguments():
     def attend(**kw):
         a = dict(q=16, q_ld=4096, k=16, v=16, s=16, cu=16, used=16, table=16, tld=8, seqs=1, rows=1,
                  mq=1, mu=64, hq=32, hk=8, d=128, page=16, out=16, out8=None, o_ld=4096, os=None,
-                 os_ld=0, lse=None, lse_ld=0, ws=None, wsb=0)
+                 os_ld=0, lse=None, lse_ld=0, work=None, n_work=0, ws=None, wsb=0)
         a.update(kw)
         _lib.call("qx_paged_attention8", a["q"], a["q_ld"], None, a["k"], a["v"], a["s"], a["cu"],
                   a["used"], a["table"], a["tld"], a["seqs"], a["rows"], a["mq"], a["mu"], a["hq"],
                   a["hk"], a["d"], a["page"], 0.1, 1, a["out"], a["out8"], a["o_ld"], a["os"],
-                  a["os_ld"], a["lse"], a["lse_ld"], a["ws"], a["wsb"], None)
+                  a["os_ld"], a["lse"], a["lse_ld"], a["work"], a["n_work"], a["ws"], a["wsb"], None)
 
     for kw, match in ((dict(q=None), "null"), (dict(table=None), "null"), (dict(out=None), "output"),
                       (dict(out8=16), "output"), (dict(d=96), "head_dim"), (dict(hk=5), "heads"),
@@ -236,7 +236,8 @@ def test_entry_points_refuse_bad_arguments():
                       (dict(q_ld=4095), "strides"), (dict(lse=16, lse_ld=0), "strides"),
                       (dict(q=18), "alignment"), (dict(k=17), "alignment"),
                       (dict(seqs=65536), "grid"), (dict(mu=40000), "workspace"),
-                      (dict(mu=40000, ws=16, wsb=100), "workspace")):
+                      (dict(mu=40000, ws=16, wsb=100), "workspace"),
+                      (dict(work=16, n_work=-1), "work"), (dict(work=16, n_work=1 << 24), "work")):
         with pytest.raises(_lib.QxError, match=match):
             attend(**kw)
     assert _lib.count("qx_paged_attention8_workspace", 1, 1, 1, 40000, 32, 8, 128) > 0
