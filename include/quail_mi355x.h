@@ -434,24 +434,34 @@ int qx_attention_lse_tiled(const void* q, int64_t q_ld, const int64_t* q_index, 
  * qx_attention_lse. Exactly one of out_bf16 (rows of o_ld elements) and
  * out_fp8 (D == 128; out_scales[h*os_ld + row]); lse (may be NULL) as in
  * qx_attention_lse; a row that sees no key gets 0 and -inf. max_q and
- * max_used bound the sequences' rows and keys. work/n_work: the list that the
- * host function qx_paged_attention8_work makes (qx_paged_attention_work's, for
- * this call's tiles), or NULL/0; calls of few rows a sequence do not read it. workspace:
- * qx_paged_attention8_workspace bytes of the caller's, 16-byte aligned (NULL
- * where that is 0), used by this call alone until the stream has passed it.
+max_used bound the sequences' rows and keys.
+ *
+ * work, n_work, unit: the items of the call, or NULL, 0, 0. The host functions
+ * qx_paged_attention8_unit and _work make them from host copies of cu_q and
+ * used: unit > 0 where every sequence has few rows (the items are (sequence,
+ * i) for its keys [i * unit, (i + 1) * unit), whose results a second launch
+ * joins), 0 where the items are query tiles as qx_paged_attention_work's;
+ * _work returns their number (<= capacity) or -1.
+ * workspace: qx_paged_attention8_workspace bytes of the caller's (has_work:
+ * whether the call gets a list), 16-byte aligned (NULL where that is 0), used
+ * by this call alone until the stream has passed it.
  */
+int64_t qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                                 int64_t HK);
+int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                                 int64_t HK, int causal, int64_t unit, int* work,
+                                 int64_t capacity);
 int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used,
-                                      int64_t HQ, int64_t HK, int64_t D);
+                                      int64_t HQ, int64_t HK, int64_t D, int has_work,
+                                      int64_t unit);
 int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
                         const void* v_pool, const void* scales, const int* cu_q, const int* used,
                         const int* table, int64_t table_ld, int64_t seqs, int64_t rows,
                         int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
                         int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
                         int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
-                        const int* work, int64_t n_work, void* workspace, int64_t workspace_bytes,
-                        hipStream_t stream);
-int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
-                                 int64_t HK, int causal, int* work, int64_t capacity);
+                        const int* work, int64_t n_work, int64_t unit, void* workspace,
+                        int64_t workspace_bytes, hipStream_t stream);
 
 /*
  * Replaces Engine.merge_attn_quant / the merge_attn_quant Triton kernel

@@ -491,8 +491,8 @@ def _work_list(tables, heads, choose_rows=False, eight_bit=False):
     """(work pairs, count, query rows per item) of a paged call over `tables`
     (host arrays). choose_rows: the tile height qx_paged_attention_tile_rows
     picks for these sequences (the call must then pass it); otherwise the
-    default (0). eight_bit: for a call over an 8-bit arena's pages (its tiles
-    have one height)."""
+    default (0). eight_bit: for a call over an 8-bit arena's pages (the third value
+    is then the keys per item, 0 for query tiles)."""
     from quail_amd import _lib
     hq, hk, d = heads
     cu_q = np.ascontiguousarray(tables["cu_q"], dtype=np.int32)
@@ -501,11 +501,14 @@ def _work_list(tables, heads, choose_rows=False, eight_bit=False):
     causal = int(tables.get("causal", True))
     rows = 0
     if eight_bit:
-        cap = int(cu_q[-1]) + seqs if seqs else 1
+        unit = _lib.count("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
+                          hk)
+        cap = (int(cu_q[-1]) + seqs if not unit else
+               seqs + int(np.maximum(used, 0).sum()) // unit) if seqs else 1
         work = np.zeros(2 * max(cap, 1), dtype=np.int32)
         n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
-                       hk, causal, work.ctypes.data, cap)
-        return work[:2 * n], n, 0
+                       hk, causal, unit, work.ctypes.data, cap)
+        return work[:2 * n], n, unit
     if choose_rows:
         rows = _lib.count("qx_paged_attention_tile_rows", cu_q.ctypes.data, used.ctypes.data,
                           seqs, hq, hk, d, causal)
@@ -593,7 +596,17 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
     and keys [0, used[s]) through table[s]. cu_q, used and table are int32
     tensors on the device; heads = (HQ, HK, D); eight_bit: whether the arena
     that is read keeps 8-bit pages."""
+    for name, t, dims in (("cu_q", cu_q, 1), ("used", used, 1), ("table", table, 2)):
+        if str(t.dtype) != "torch.int32" or t.dim() != dims or t.stride(dims - 1) != 1:
+            raise ValueError(f"{name}: int32 of {dims} dimension(s), rows contiguous")
     host = dict(cu_q=cu_q.cpu().numpy(), used=used.cpu().numpy(), causal=causal)
+    if not len(host["cu_q"]) == len(host["used"]) + 1 == table.shape[0] + 1:
+        raise ValueError(f"{len(host['used'])} sequences, {len(host['cu_q'])} bounds, "
+                         f"{table.shape[0]} table rows")
+    if host["cu_q"][0] != 0 or (np.diff(host["cu_q"]) < 0).any() or (host["used"] < 0).any():
+        raise ValueError("cu_q rises from 0 and used is not negative")
+    if host["used"].max(initial=0) > table.shape[1] * PAGE_ROWS:
+        raise ValueError(f"{host['used'].max()} keys in {table.shape[1]} pages")
     tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),
                   max_used=int(host["used"].max(initial=0)))

@@ -12,7 +12,10 @@
 // P is rounded to bf16 (2^-9 of a weight, about what the bf16 output rounds
 // by); scores, maxima, sums and outputs stay in fp32.
 #include <algorithm>
+#include <new>
 #include <type_traits>
+#include <utility>
+#include <vector>
 
 #include "qx_common.h"
 #include "qx_status.h"
@@ -23,7 +26,7 @@ namespace {
 
 constexpr int kPage = 16;  // tokens per arena page
 constexpr int kMaxKeys = 2560 * kPage;  // per sequence, as the 16-bit call takes
-constexpr int kMaxChunk = 8192;         // keys per split: 512 pages' ids and scales in LDS
+constexpr int kMaxChunk = 2048;         // keys per split
 typedef __attribute__((address_space(3))) v2i lds_v2i;
 
 struct Attn8Args {
@@ -105,7 +108,9 @@ __device__ __forceinline__ void store_row(const Attn8Args& p, int64_t row, int h
 constexpr int kRing = 2;
 
 template <int D, int NB>
-__global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
+__global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, const int* work,
+                                                                int seqs) {
+  static_assert(kMaxChunk / kPage <= 256, "a page id for each thread");
   constexpr int CH = D / 16;              // 16-byte chunks per code row
   constexpr int NC = D / 32;              // MFMA k-steps over the head dim
   constexpr int ND = D / 16;              // 16-row d blocks of O^T
@@ -119,49 +124,38 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
   __shared__ int pages[kMaxChunk / kPage];
   __shared__ uint16_t bytes[kMaxChunk / kPage];
 
-  const int s = blockIdx.z;
+  // The block table's entries come in one round of loads with the sequence's
+  // bounds (rows hold max_used keys' entries; those past the sequence's own
+  // are not used), and the scales in one with q and the first step's K and V.
+  int s, split;
+  if (work) {
+    s = work[2 * blockIdx.x];
+    split = work[2 * blockIdx.x + 1];
+    if (s < 0 || s >= seqs || split < 0 || split >= p.splits) return;  // not an item of this call
+  } else {
+    s = blockIdx.z;
+    split = blockIdx.x;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int k0 = split * p.chunk;
+  const int* trow = p.table + (int64_t)s * p.table_ld;
+  const int page = trow[min(k0 / kPage + tid, max((p.max_used - 1) / kPage, 0))];
   const int G = p.HQ / p.HK;
   const int kvh = blockIdx.y % p.HK;
   const int cgroup = blockIdx.y / p.HK;
   const int q0 = p.cu_q[s], q_len = p.cu_q[s + 1] - q0;
   const int used = min(p.used[s], p.max_used);
   const int cols = q_len * G;
-  if (cgroup * COLS >= cols) return;
-  const int tid = threadIdx.x, lane = tid & 63;
+  if (cgroup * COLS >= cols || (split && k0 >= used)) return;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g4 = lane >> 4;
 
   // keys [k0, k1) of this split that the last column of the group sees
   const int last_col = min(cgroup * COLS + COLS, cols) - 1;
   const int seen_end = p.causal ? min(used, used - q_len + last_col / G + 1) : used;
-  const int k0 = blockIdx.x * p.chunk;
   const int k1 = min(seen_end, k0 + p.chunk);
   const int npages = k1 > k0 ? (k1 - k0 + kPage - 1) / kPage : 0;
-  const int* trow = p.table + (int64_t)s * p.table_ld + k0 / kPage;
-  for (int i = tid; i < npages; i += 256) {
-    const int page = trow[i];
-    pages[i] = page;
-    bytes[i] = p.scales[(int64_t)page * p.HK + kvh];
-  }
-
-  // this lane's columns: their rows, heads, Q fragments and visible keys
-  v8bf qf[NB][NC];
-  int lim[NB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int c = cgroup * COLS + n * 16 + c16;
-    const int cc = min(c, cols - 1);
-    const int r = cc / G, head = kvh * G + cc % G;
-    const int64_t row = p.q_index ? p.q_index[q0 + r] : (int64_t)(q0 + r);
-    const uint16_t* q = p.q + row * p.q_ld + (int64_t)head * D;
-    lim[n] = c < cols ? (p.causal ? min(used, used - q_len + r + 1) : used) : 0;
-#pragma unroll
-    for (int k = 0; k < NC; ++k)
-      qf[n][k] = *reinterpret_cast<const v8bf*>(q + (k >> 1) * (D == 128 ? 64 : 0) + g4 * 16 +
-                                                (k & 1) * 8);
-#pragma unroll
-    for (int k = 0; k < NC; ++k) asm volatile("" ::"v"(qf[n][k]));
-  }
+  if (tid < npages) pages[tid] = page;
   __syncthreads();
 
   const int64_t kv_row = (int64_t)p.HK * D;
@@ -190,6 +184,27 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
         lds_dma16((v ? vbase : kbase) + row * kv_row + chunk * 16, at + v * TILE + i * 1024);
       }
   };
+  if (mine > 0) issue(0);
+  if (tid < npages) bytes[tid] = p.scales[(int64_t)page * p.HK + kvh];
+
+  // this lane's columns: their rows, heads, Q fragments and visible keys
+  v8bf qf[NB][NC];
+  int lim[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int c = cgroup * COLS + n * 16 + c16;
+    const int cc = min(c, cols - 1);
+    const int r = cc / G, head = kvh * G + cc % G;
+    const int64_t row = p.q_index ? p.q_index[q0 + r] : (int64_t)(q0 + r);
+    const uint16_t* q = p.q + row * p.q_ld + (int64_t)head * D;
+    lim[n] = c < cols ? (p.causal ? min(used, used - q_len + r + 1) : used) : 0;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      qf[n][k] = *reinterpret_cast<const v8bf*>(q + (k >> 1) * (D == 128 ? 64 : 0) + g4 * 16 +
+                                                (k & 1) * 8);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) asm volatile("" ::"v"(qf[n][k]));
+  }
 
   v4f o[NB][ND];
   float m[NB], l[NB];
@@ -200,8 +215,7 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  __builtin_amdgcn_s_waitcnt(0);  // nothing of the above in flight beside the ring's loads
-  if (mine > 0) issue(0);
+  __syncthreads();  // bytes, and nothing in flight beside the ring's loads
   for (int t = 0; t < mine; ++t) {
     // this wave's reads of the slot that step t + 1 refills have returned
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
@@ -323,7 +337,7 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p) {
     const int64_t row = q0 + c / G;
     const int head = kvh * G + c % G;
     if (p.splits > 1) {
-      const int64_t at = ((int64_t)blockIdx.x * p.rows + row) * p.HQ + head;
+      const int64_t at = ((int64_t)split * p.rows + row) * p.HQ + head;
       if (j == 0) {
         p.part_ml[2 * at] = mm;
         p.part_ml[2 * at + 1] = ll;
@@ -676,59 +690,128 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   }
 }
 
-// Join the splits of each (row, head): D / 8 lanes per pair.
-template <int D>
-__global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p, int64_t pairs) {
-  constexpr int LPC = D / 8;
-  const int64_t pair = (int64_t)blockIdx.x * (256 / LPC) + threadIdx.x / LPC;
-  const int j = threadIdx.x % LPC;
-  if (pair >= pairs) return;
-  const int64_t row = pair / p.HQ;
-  const int head = (int)(pair % p.HQ);
+// Join the splits of each (row, head), WAVES waves per pair: a lane weighs
+// one split (in every wave alike), and each group of 16 lanes adds up every
+// (4 WAVES)-th split's output. A split without a key has weight 0 and an
+// output that nobody wrote: it is read and not used.
+template <int D, int WAVES>
+__global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
+  constexpr int PER = D / 16;  // columns per lane
+  constexpr int GROUPS = 4 * WAVES;
+  __shared__ v4f part[WAVES > 1 ? GROUPS * D / 4 : 1];
+  const int wave = threadIdx.x >> 6;
+  const int in_seq = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const int s = blockIdx.y;
+  const int q0 = p.cu_q[s], q_len = p.cu_q[s + 1] - q0;
+  const int used = min(p.used[s], p.max_used);
+  if (in_seq >= q_len * p.HQ) return;
+  const int splits = max(1, (used + p.chunk - 1) / p.chunk);
+  const int64_t row = q0 + in_seq / p.HQ;
+  const int head = in_seq % p.HQ;
+  const int64_t pair = row * p.HQ + head;
+  const int lane = threadIdx.x & 63, j = lane & 15;
+  const int g = (WAVES == 1 ? 0 : 4 * wave) + (lane >> 4);
   const int64_t step = p.rows * p.HQ;
-  float mm = -INFINITY;
-  for (int i = 0; i < p.splits; ++i) mm = fmaxf(mm, p.part_ml[2 * (i * step + pair)]);
-  const float m_use = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, y[8] = {};
-  for (int i = 0; i < p.splits; ++i) {
-    const float mi = p.part_ml[2 * (i * step + pair)];
-    if (mi == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(mi - m_use);
-    ll += p.part_ml[2 * (i * step + pair) + 1] * f;
-    const float* at = p.part_o + (i * step + pair) * D + 8 * j;
-    const v4f a = *reinterpret_cast<const v4f*>(at), b = *reinterpret_cast<const v4f*>(at + 4);
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + pair;
+  const float* po = p.part_o + pair * D + PER * j;
+  float mm = -INFINITY, ll = 0.f, y[PER] = {};
+  for (int first = 0; first < splits; first += 64) {
+    const bool live = first + lane < splits;
+    const float2 mine = live ? ml[(first + lane) * step] : make_float2(-INFINITY, 0.f);
+    const float top = fmaxf(mm, group_max<64>(mine.x));
+    const float top_use = top == -INFINITY ? 0.f : top;
+    const float w = __builtin_amdgcn_exp2f(mine.x - top_use);
+    const float keep = __builtin_amdgcn_exp2f(mm - top_use);
+    ll = ll * keep + group_sum<64>(mine.y * w);
+    mm = top;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      y[k] += a[k] * f;
-      y[4 + k] += b[k] * f;
+    for (int k = 0; k < PER; ++k) y[k] *= keep;
+    const int n = min(64, splits - first);
+    constexpr int UNROLL = 4;
+    for (int i = g; i < n; i += UNROLL * GROUPS) {
+      v4f a[UNROLL][PER / 4];
+      float wi[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int at = i + u * GROUPS;
+        wi[u] = __shfl(w, min(at, 63), 64);
+        if (at >= n) wi[u] = 0.f;
+#pragma unroll
+        for (int k = 0; k < PER / 4; ++k)
+          a[u][k] = *reinterpret_cast<const v4f*>(po + (first + min(at, n - 1)) * step * D + 4 * k);
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          y[k] = wi[u] != 0.f ? fmaf(a[u][k >> 2][k & 3], wi[u], y[k]) : y[k];
     }
+  }
+  if constexpr (WAVES > 1) {
+#pragma unroll
+    for (int k = 0; k < PER / 4; ++k)
+      part[g * (D / 4) + j * (PER / 4) + k] = v4f{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]};
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) y[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i)
+#pragma unroll
+      for (int k = 0; k < PER / 4; ++k) {
+        const v4f a = part[(i * 4 + (lane >> 4)) * (D / 4) + j * (PER / 4) + k];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[4 * k + e] += a[e];
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    y[k] += __shfl_xor(y[k], 16, 64);
+    y[k] += __shfl_xor(y[k], 32, 64);
   }
   const float inv = ll > 0.f ? 1.0f / ll : 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) y[k] *= inv;
-  store_row<D>(p, row, head, j, y);
-  if (p.lse && j == 0)
+  for (int k = 0; k < PER; ++k) y[k] *= inv;
+  // D / 8 lanes store 8 columns each
+  if constexpr (PER == 4) {
+    float z[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      z[k] = y[k];
+      z[4 + k] = __shfl(y[k], lane + 1, 64);
+    }
+    if (lane < 16 && !(j & 1)) store_row<D>(p, row, head, j >> 1, z);
+  } else {
+    if (lane < 16) store_row<D>(p, row, head, j, y);
+  }
+  if (p.lse && lane == 0)
     p.lse[(int64_t)head * p.lse_ld + row] =
-        ll > 0.f ? (__log2f(ll) + m_use) * 0.6931471805599453f : -INFINITY;
+        ll > 0.f ? (__log2f(ll) + mm) * 0.6931471805599453f : -INFINITY;
 }
 
 // Column blocks of a workgroup: two of 16 where a sequence's (row, head)
 // pairs pass one.
 inline int few_blocks(int64_t max_q, int64_t G) { return max_q * G > 16 ? 2 : 1; }
 
-// Keys per split of a call (a multiple of 128: the four waves' steps).
-int64_t split_chunk(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HK, int64_t G) {
+// Keys per split (a multiple of 128: the four waves' steps) of sequences
+// whose longest has max_used keys and which hold `keys` keys in all. A step
+// of 128 keys takes a workgroup about 1 us where few run (memory latency),
+// joining splits 3 us and a launch, so
+//   - sequences of up to 768 keys are not split (1 of 300 keys: 6.9 us, in
+//     two 9.1; 1 of 1000: 11.9 us whole, 9.5 in splits of 256);
+//   - calls that one round of workgroups covers take about 256 of them (1
+//     sequence of 40,000 keys: 21.3 us in 1280s, 23.9 in 640s, 26.7 in 384s;
+//     16 of ~1000: 18 us, 17.3, 19.5);
+//   - larger ones at least 1024 for an even end, of up to 2048 keys (16 of
+//     ~9000 keys: 70.3 us in 1280s, 76.7 in 2048s; 200 of ~1900 keys: 150 us
+//     in 1024s as in 2048s, 144 in 4096s; of ~350: 38.4 whole, 46 split).
+int64_t split_chunk(int64_t keys, int64_t max_q, int64_t max_used, int64_t HK,
+                    int64_t G) {
   const int64_t cols = 16 * few_blocks(max_q, G);
-  const int64_t groups = std::max<int64_t>(1, seqs * HK * ((max_q * G + cols - 1) / cols));
-  const int64_t want = std::max<int64_t>(1, 1024 / groups);
-  int64_t chunk = (max_used + want - 1) / want;
-  chunk = std::max<int64_t>(chunk, 256);
-  return std::min<int64_t>((chunk + 127) / 128 * 128, kMaxChunk);
-}
-
-int64_t split_count(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HK, int64_t G) {
-  const int64_t chunk = split_chunk(seqs, max_q, max_used, HK, G);
-  return std::max<int64_t>(1, (max_used + chunk - 1) / chunk);
+  const int64_t total = keys * HK * ((max_q * G + cols - 1) / cols);  // keys of all workgroups
+  int64_t chunk = std::max(std::min<int64_t>(total / 256, 1280), std::min<int64_t>(total / 1024, 2048));
+  chunk = max_used <= 768 ? max_used : std::max<int64_t>(256, std::min(chunk, max_used));
+  return std::max<int64_t>(128, (chunk + 127) / 128 * 128);
 }
 
 // Heads per workgroup of the tile kernel, and its query rows.
@@ -755,12 +838,27 @@ void tile_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t se
 }
 
 template <int D, int NB>
-void few_launch(const Attn8Args& a, int64_t seqs, int64_t max_q, hipStream_t stream) {
+void few_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t seqs, int64_t max_q,
+                hipStream_t stream) {
   const int G = a.HQ / a.HK;
   const int64_t groups = (max_q * G + 16 * NB - 1) / (16 * NB);
-  hipLaunchKernelGGL((attention8_few_kernel<D, NB>),
-                     dim3((unsigned)a.splits, (unsigned)(a.HK * groups), (unsigned)seqs), dim3(256),
-                     0, stream, a);
+  const dim3 grid(work ? (unsigned)n_work : (unsigned)a.splits, (unsigned)(a.HK * groups),
+                  work ? 1u : (unsigned)seqs);
+  hipLaunchKernelGGL((attention8_few_kernel<D, NB>), grid, dim3(256), 0, stream, a, work,
+                     (int)seqs);
+  if (a.splits > 16)
+    hipLaunchKernelGGL((split_merge_kernel<D, 4>), dim3((unsigned)(max_q * a.HQ), (unsigned)seqs),
+                       dim3(256), 0, stream, a);
+  else if (a.splits > 1)
+    hipLaunchKernelGGL((split_merge_kernel<D, 1>),
+                       dim3((unsigned)((max_q * a.HQ + 3) / 4), (unsigned)seqs), dim3(256), 0,
+                       stream, a);
+}
+
+// Keys per work item of a call (0: the items are query tiles).
+int64_t call_unit(int64_t keys, int64_t max_q, int64_t max_used, int64_t HK,
+                  int64_t G) {
+  return few_rows(max_q, G) ? split_chunk(keys, max_q, max_used, HK, G) : 0;
 }
 
 }  // namespace
@@ -770,21 +868,63 @@ using namespace qx;
 
 extern "C" {
 
-int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used,
-                                      int64_t HQ, int64_t HK, int64_t D) {
-  QX_CHECK(seqs >= 0 && rows >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 &&
-               HQ % HK == 0 && (D == 64 || D == 128),
-           "attention8_workspace: arguments");
-  if (!few_rows(max_q, HQ / HK)) return 0;
-  const int64_t splits = split_count(seqs, max_q, max_used, HK, HQ / HK);
-  return splits > 1 ? splits * rows * HQ * (D + 2) * 4 : 0;
+int64_t qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                                 int64_t HK) {
+  QX_CHECK(cu_q && used && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
+           "attention8_unit: arguments");
+  int64_t max_q = 0, max_used = 0, keys = 0;
+  for (int64_t s = 0; s < seqs; ++s) {
+    max_q = std::max<int64_t>(max_q, cu_q[s + 1] - cu_q[s]);
+    max_used = std::max<int64_t>(max_used, used[s]);
+    keys += std::max(used[s], 0);
+  }
+  return call_unit(keys, max_q, max_used, HK, HQ / HK);
+}
+
+static int64_t few_work_list(const int* cu_q, const int* used, int64_t seqs, int64_t unit,
+                             int* work, int64_t capacity) {
+  // whole splits first, then the rest, longest first
+  std::vector<std::pair<int, std::pair<int, int>>> items;
+  for (int64_t s = 0; s < seqs; ++s) {
+    if (cu_q[s + 1] == cu_q[s]) continue;
+    for (int64_t i = 0, k0 = 0; i == 0 || k0 < used[s]; ++i, k0 += unit)
+      items.push_back({(int)std::min<int64_t>(unit, used[s] - k0), {(int)s, (int)i}});
+  }
+  QX_CHECK((int64_t)items.size() <= capacity, "attention8_work: %zu items, room for %lld",
+           items.size(), (long long)capacity);
+  std::stable_sort(items.begin(), items.end(),
+                   [](const auto& a, const auto& b) { return a.first > b.first; });
+  for (size_t i = 0; i < items.size(); ++i) {
+    work[2 * i] = items[i].second.first;
+    work[2 * i + 1] = items[i].second.second;
+  }
+  return (int64_t)items.size();
 }
 
 int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
-                                 int64_t HK, int causal, int* work, int64_t capacity) {
-  QX_CHECK(cu_q && used && work && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
+                                 int64_t HK, int causal, int64_t unit, int* work,
+                                 int64_t capacity) {
+  QX_CHECK(cu_q && used && work && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0 && unit >= 0,
            "attention8_work: arguments");
-  return attention_work_list(cu_q, used, seqs, tile_height(HQ / HK), causal, work, capacity);
+  try {
+    return unit ? few_work_list(cu_q, used, seqs, unit, work, capacity)
+                : attention_work_list(cu_q, used, seqs, tile_height(HQ / HK), causal, work,
+                                      capacity);
+  } catch (const std::bad_alloc&) {
+    set_error("attention8_work: out of host memory");
+    return QX_EINVAL;
+  }
+}
+
+int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used,
+                                      int64_t HQ, int64_t HK, int64_t D, int has_work,
+                                      int64_t unit) {
+  QX_CHECK(seqs >= 0 && rows >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 &&
+               HQ % HK == 0 && (D == 64 || D == 128) && unit >= 0,
+           "attention8_workspace: arguments");
+  if (!has_work) unit = call_unit(seqs * max_used, max_q, max_used, HK, HQ / HK);
+  const int64_t splits = unit ? (max_used + unit - 1) / unit : 0;
+  return splits > 1 ? splits * rows * HQ * (D + 2) * 4 : 0;
 }
 
 int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
@@ -793,8 +933,8 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
                         int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
                         int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
                         int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
-                        const int* work, int64_t n_work, void* workspace, int64_t workspace_bytes,
-                        hipStream_t stream) {
+                        const int* work, int64_t n_work, int64_t unit, void* workspace,
+                        int64_t workspace_bytes, hipStream_t stream) {
   QX_CHECK(q && k_pool && v_pool && scales && cu_q && used && table, "attention8: null pointer");
   QX_CHECK((out_bf16 != nullptr) != (out_fp8 != nullptr), "attention8: one output, bf16 or e4m3");
   QX_CHECK(D == 64 || D == 128, "attention8: head_dim %lld", (long long)D);
@@ -812,12 +952,15 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
            "attention8: alignment");
   QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
   QX_CHECK(!work || (n_work >= 0 && n_work * HQ < (1LL << 24)), "attention8: work items");
-  if (seqs == 0 || max_q == 0 || rows == 0) return QX_OK;
+  QX_CHECK(unit >= 0 && unit % 128 == 0 && unit <= kMaxChunk && (work || !unit),
+           "attention8: work items of %lld keys", (long long)unit);
+  if (seqs == 0 || max_q == 0 || rows == 0 || (work && n_work == 0)) return QX_OK;
   const int64_t G = HQ / HK;
   const int nb = few_blocks(max_q, G);
   QX_CHECK(HK * ((max_q * G + 16 * nb - 1) / (16 * nb)) < 65536, "attention8: %lld rows a sequence",
            (long long)max_q);
-  const int64_t need = qx_paged_attention8_workspace(seqs, rows, max_q, max_used, HQ, HK, D);
+  const int64_t need =
+      qx_paged_attention8_workspace(seqs, rows, max_q, max_used, HQ, HK, D, work != nullptr, unit);
   QX_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
            "attention8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
            (long long)need);
@@ -825,34 +968,23 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
               (const uint16_t*)scales, cu_q, used, table, table_ld, (int)max_used, (int)HQ, (int)HK,
               causal, scale * 1.4426950408889634f, (uint16_t*)out_bf16, (uint8_t*)out_fp8, o_ld,
               out_scales, os_ld, lse, lse_ld};
-  if (!few_rows(max_q, G)) {
-    if (work && n_work == 0) return QX_OK;
+  if (!work) unit = call_unit(seqs * max_used, max_q, max_used, HK, G);
+  if (!unit) {
     if (D == 128) tile_launch<128>(a, work, n_work, seqs, max_q, stream);
     else tile_launch<64>(a, work, n_work, seqs, max_q, stream);
     QX_LAUNCH_STATUS();
   }
-  a.chunk = (int)split_chunk(seqs, max_q, max_used, HK, G);
-  a.splits = (int)split_count(seqs, max_q, max_used, HK, G);
+  a.chunk = (int)unit;
+  a.splits = (int)std::max<int64_t>(1, (max_used + unit - 1) / unit);
   a.rows = rows;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + (int64_t)a.splits * rows * HQ * D;
   if (D == 128) {
-    if (nb == 1) few_launch<128, 1>(a, seqs, max_q, stream);
-    else few_launch<128, 2>(a, seqs, max_q, stream);
+    if (nb == 1) few_launch<128, 1>(a, work, n_work, seqs, max_q, stream);
+    else few_launch<128, 2>(a, work, n_work, seqs, max_q, stream);
   } else {
-    if (nb == 1) few_launch<64, 1>(a, seqs, max_q, stream);
-    else few_launch<64, 2>(a, seqs, max_q, stream);
-  }
-  if (a.splits > 1) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-    const int64_t pairs = rows * HQ;
-    const int per = D == 128 ? 16 : 32;
-    const dim3 grid((unsigned)((pairs + per - 1) / per));
-    if (D == 128)
-      hipLaunchKernelGGL(split_merge_kernel<128>, grid, dim3(256), 0, stream, a, pairs);
-    else
-      hipLaunchKernelGGL(split_merge_kernel<64>, grid, dim3(256), 0, stream, a, pairs);
+    if (nb == 1) few_launch<64, 1>(a, work, n_work, seqs, max_q, stream);
+    else few_launch<64, 2>(a, work, n_work, seqs, max_q, stream);
   }
   QX_LAUNCH_STATUS();
 }

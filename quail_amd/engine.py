@@ -238,6 +238,11 @@ def _swiglu_launches(n: int, k: int, m: int) -> tuple:
     return ((m, config),)
 
 
+@functools.lru_cache(maxsize=4096)
+def _attention8_workspace(*sizes):
+    return _lib.count("qx_paged_attention8_workspace", *sizes)
+
+
 class Engine:
     """Kernels, quantization and paged attention over the KV arena.
 
@@ -852,13 +857,15 @@ class Engine:
         n = q3.shape[0] if q_index is None else q_index.shape[0]
         table, seqs = tables["table"], tables["used"].shape[0]
         max_q, max_used = int(tables["max_q"]), int(tables["max_used"])
-        size = _lib.count("qx_paged_attention8_workspace", seqs, n, max_q, max_used, hq, hk, d)
-        work = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
-        # the list of the call's query tiles, when the plan or pack carries one
-        items = tables.get("work")
-        if not torch.is_tensor(items):
-            items = None
-        n_items = int(tables.get("n_work", 0)) if items is not None else 0
+        # the call's items and their keys, when the plan or pack carries them
+        work = tables.get("work")
+        if not torch.is_tensor(work):
+            work = None
+        n_work = int(tables.get("n_work", 0)) if work is not None else 0
+        unit = int(tables.get("work_rows", 0)) if work is not None else 0
+        size = _attention8_workspace(seqs, n, max_q, max_used, hq, hk, d, int(work is not None),
+                                     unit)
+        space = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
         o8, s8 = (None, None) if quant is None else quant
         o = out if quant is None else o8
         _lib.call("qx_paged_attention8", _ptr(q3), q3.stride(0), _ptr(q_index),
@@ -866,7 +873,7 @@ class Engine:
                   table.stride(0), seqs, n, max_q, max_used, hq, hk, d, self.arena.page_tokens,
                   float(scale), int(tables.get("causal", True)), _ptr(out), _ptr(o8), o.stride(0),
                   _ptr(s8), 0 if s8 is None else self._scale_ld(s8), _ptr(lse),
-                  0 if lse is None else lse.stride(0), _ptr(items), n_items, _ptr(work), size,
+                  0 if lse is None else lse.stride(0), _ptr(work), n_work, unit, _ptr(space), size,
                   _stream())
 
     def read_pages(self, q3, tables, layer, *, softmax_scale=None):
@@ -881,6 +888,9 @@ class Engine:
                              f"{self.num_q_heads} heads of {self.head_dim} in bf16")
         if q3.stride(2) != 1 or (hq > 1 and q3.stride(1) != d):
             raise ValueError("a query row's heads are contiguous")
+        rows = int(tables["cu_q"].shape[0]) - 1
+        if rows != tables["used"].shape[0]:
+            raise ValueError(f"{rows} query ranges for {tables['used'].shape[0]} sequences")
         scale = d ** -0.5 if softmax_scale is None else softmax_scale
         out = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
         lse = torch.empty((hq, n), dtype=torch.float32, device=q3.device)

@@ -109,6 +109,33 @@ def test_packs_page_items_write_what_their_scatter_writes(seed):
     assert "page_writes" not in pack_chunk(plain, groups).meta["unified"]
 
 
+def test_attention_items_cover_every_key_of_few_row_calls_and_every_tile_of_others():
+    def items(q_lens, used, hq=32, hk=8, causal=1):
+        cu_q = np.concatenate([[0], np.cumsum(q_lens)]).astype(np.int32)
+        used = np.asarray(used, dtype=np.int32)
+        unit = _lib.count("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data,
+                          len(used), hq, hk)
+        work = np.zeros(2 * 4096, dtype=np.int32)
+        n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, len(used),
+                       hq, hk, causal, unit, work.ctypes.data, 4096)
+        with pytest.raises(_lib.QxError, match="room|capacity"):
+            _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, len(used),
+                       hq, hk, causal, unit, work.ctypes.data, n - 1)
+        return unit, [tuple(work[2 * i:2 * i + 2]) for i in range(n)]
+
+    used = [300, 0, 8192, 5, 40000]
+    unit, got = items([1, 2, 3, 0, 1], used)
+    assert unit and unit % 128 == 0
+    want = [(s, i) for s, u in enumerate(used) if s != 3 for i in range(max(1, -(-u // unit)))]
+    assert sorted(got) == sorted(want)
+    load = [min(unit, used[s] - i * unit) for s, i in got]
+    assert load == sorted(load, reverse=True)
+    unit, got = items([100, 1, 33], [150, 40, 33])
+    assert unit == 0 and sorted(got) == [(0, 0), (0, 1), (0, 2), (0, 3), (1, 0), (2, 0), (2, 1)]
+    unit, got = items([100, 1], [150, 40], hq=16)       # two heads a KV head: 64 rows
+    assert unit == 0 and sorted(got) == [(0, 0), (0, 1), (1, 0)]
+
+
 def test_scale_bytes_and_codes_of_the_oracle():
     assert [ref.scale_byte(a) for a in (0.0, 448.0, 448.1, 1.75, 1.76, 3.5e-38)] == \
         [1, 127, 128, 119, 120, 1]
@@ -221,12 +248,14 @@ def test_entry_points_refuse_bad_arguments():
     def attend(**kw):
         a = dict(q=16, q_ld=4096, k=16, v=16, s=16, cu=16, used=16, table=16, tld=8, seqs=1, rows=1,
                  mq=1, mu=64, hq=32, hk=8, d=128, page=16, out=16, out8=None, o_ld=4096, os=None,
-                 os_ld=0, lse=None, lse_ld=0, work=None, n_work=0, ws=None, wsb=0)
+                 os_ld=0, lse=None, lse_ld=0, work=None, n_work=0, unit=0, ws=None,
+                 wsb=0)
         a.update(kw)
         _lib.call("qx_paged_attention8", a["q"], a["q_ld"], None, a["k"], a["v"], a["s"], a["cu"],
                   a["used"], a["table"], a["tld"], a["seqs"], a["rows"], a["mq"], a["mu"], a["hq"],
                   a["hk"], a["d"], a["page"], 0.1, 1, a["out"], a["out8"], a["o_ld"], a["os"],
-                  a["os_ld"], a["lse"], a["lse_ld"], a["work"], a["n_work"], a["ws"], a["wsb"], None)
+                  a["os_ld"], a["lse"], a["lse_ld"], a["work"], a["n_work"], a["unit"], a["ws"],
+                  a["wsb"], None)
 
     for kw, match in ((dict(q=None), "null"), (dict(table=None), "null"), (dict(out=None), "output"),
                       (dict(out8=16), "output"), (dict(d=96), "head_dim"), (dict(hk=5), "heads"),
@@ -237,11 +266,17 @@ def test_entry_points_refuse_bad_arguments():
                       (dict(q=18), "alignment"), (dict(k=17), "alignment"),
                       (dict(seqs=65536), "grid"), (dict(mu=40000), "workspace"),
                       (dict(mu=40000, ws=16, wsb=100), "workspace"),
-                      (dict(work=16, n_work=-1), "work"), (dict(work=16, n_work=1 << 24), "work")):
+                      (dict(work=16, n_work=-1), "work"), (dict(work=16, n_work=1 << 24), "work"),
+                      (dict(unit=128), "items"), (dict(work=16, n_work=1, unit=100), "items"),
+                      (dict(work=16, n_work=1, unit=8192), "items"),
+                      (dict(work=16, n_work=1, unit=128, mu=256), "workspace")):
         with pytest.raises(_lib.QxError, match=match):
             attend(**kw)
-    assert _lib.count("qx_paged_attention8_workspace", 1, 1, 1, 40000, 32, 8, 128) > 0
-    assert _lib.count("qx_paged_attention8_workspace", 1, 1, 1, 64, 32, 8, 128) == 0
+    space = lambda *a: _lib.count("qx_paged_attention8_workspace", 1, 1, *a)  # noqa: E731
+    assert space(1, 40000, 32, 8, 128, 0, 0) > 0
+    assert space(1, 64, 32, 8, 128, 0, 0) == 0
+    assert space(1, 512, 32, 8, 128, 1, 128) == 4 * 32 * 130 * 4
+    assert space(1000, 40000, 32, 8, 128, 1, 0) == 0
     attend(seqs=0)
     attend(rows=0)
 
