@@ -253,3 +253,48 @@ def test_copy_pages_is_exact_in_every_layer(dtype, layers, hk, d, pages, moved):
     assert torch.equal(raw, want.view(-1))
     if scales is not None:
         assert torch.equal(arena.scales, scales)
+
+
+def engine_arena(pages, hk=8, d=128, layers=1, dtype=FP8):
+    return KVArena(layers, pages, PAGE, hk, d, dtype=dtype)
+
+
+@pytest.mark.parametrize("attention_mode", ["unified", "tree"])
+@pytest.mark.parametrize("kind", ["one question", "questions"])
+def test_stage_runs_on_an_8_bit_arena(attention_mode, kind):
+    """A whole stage of the small model (head_dim 64): documents behind a
+    shared prefix, packed, borrowed and read through 8-bit pages. Its margins
+    differ from a bf16 arena's by the codes' roundings (2^-4 of a value each,
+    many of either sign): within 0.5 of margins that spread over several."""
+    from quail_amd import readout as ro
+    from quail_amd.executor import StageRun
+    from quail_amd.model import CONFIGS, build_synthetic, retain_answer_head
+    from quail_amd.qwen3 import Qwen3Pipeline
+    from quail_amd.workload import make_workload
+
+    wl = make_workload("tiny", seed=0)
+    model = build_synthetic(CONFIGS["tiny"], seed=0, device="cuda", gen_device="cpu",
+                            norm_init="random")
+    cfg = model.config
+    rng = np.random.default_rng(1)
+    prefixes, suffixes = wl.groups_input()
+    if kind == "questions":
+        suffixes = [[rng.integers(0, 4096, int(n)) for n in rng.integers(2, 9, 3)]
+                    for _ in prefixes]
+    got = {}
+    for dtype in (torch.bfloat16, FP8):
+        arena = KVArena(cfg.layers, 3 * wl.chunk_budget // PAGE + 64, PAGE, cfg.kv_heads,
+                        cfg.head_dim, dtype=dtype)
+        retain_answer_head(model, wl.label_ids[:2])
+        rows = ro.AnswerRows(model, [wl.label_ids[0]], [wl.label_ids[1]])
+        run = StageRun(Qwen3Pipeline(model, arena), arena, ro.AsyncMargins(rows), prefixes,
+                       suffixes, wl.chunk_budget // 4, attention_mode=attention_mode)
+        results = run.run()
+        torch.cuda.synchronize()
+        assert run.stats["chunks"] > 1
+        flat = [m for r in results for m in (r if isinstance(r, list) else [r])]
+        got[dtype] = np.array([y - n for y, n in flat])
+    off = np.abs(got[FP8] - got[torch.bfloat16])
+    print("margins", got[torch.bfloat16].std(), "off", off.max(), np.sqrt((off ** 2).mean()))
+    assert np.isfinite(got[FP8]).all()
+    assert off.max() < 0.5 and off.max() > 0
