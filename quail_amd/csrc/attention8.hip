@@ -64,6 +64,24 @@ __device__ __forceinline__ v8bf codes_bf16(uint32_t lo, uint32_t hi) {
   return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Four codes: which are NaN (0x7f or 0xff), as the bytes' top bits. A key
+// that some rows of a tile see and others do not has weight 0 for the others,
+// and 0 * NaN would be theirs too: in tiles that a mask cuts, V's NaN codes
+// go into the products as 0, and the rows that see them get their NaN at the
+// end.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t without(uint32_t w, uint32_t nans) {
+  return w & ~((nans >> 7) * 0xffu);
+}
+
+// ln(sum exp) of a row from its sum against 2^m; -inf without a key, NaN for
+// a NaN sum
+__device__ __forceinline__ float row_lse(float sum, float m) {
+  return sum == 0.f ? -INFINITY : (__log2f(sum) + m) * 0.6931471805599453f;
+}
+
 // One row of one head, 8 consecutive columns on each of its D / 8 lanes: the
 // bf16 row, or (D = 128) its e4m3 codes and their scale, from the values
 // rounded to bf16 as the separate quantization would see them.
@@ -216,6 +234,10 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
     for (int d = 0; d < ND; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
   }
   __syncthreads();  // bytes, and nothing in flight beside the ring's loads
+  // from this key of the split on, some column sees less than the last one
+  const int cut = p.causal && q_len > 1
+                      ? min(used, used - q_len + cgroup * COLS / G + 1) - k0 : INT32_MAX;
+  uint32_t nans = 0;
   for (int t = 0; t < mine; ++t) {
     // this wave's reads of the slot that step t + 1 refills have returned
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
@@ -285,12 +307,34 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
     const int vkey = (x >> 3) * 16 + g4 * 4 + ((x >> 1) & 3);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
           (lds_v2i*)(vt + vkey * D + ((d ^ vswz(vkey)) * 16) + (x & 1) * 8));
+      if (key0 + 32 > cut) {
+        const uint32_t n0 = nan_codes(w[0]), n1 = nan_codes(w[1]);
+        w = v2i{(int)without(w[0], n0), (int)without(w[1], n1)};
+        nans |= n0 | n1;
+      }
       const v8bf vf = codes_bf16(w[0], w[1]);
 #pragma unroll
       for (int n = 0; n < NB; ++n)
         o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[n][d], 0, 0, 0);
+    }
+  }
+  if (__builtin_amdgcn_ballot_w64(nans != 0)) {  // rare: this wave's keys in the cut, again
+    for (int t = 0; t < mine; ++t) {
+      const int key0 = 32 * (4 * t + wave);
+      for (int key = max(key0, cut); key < min(key0 + 32, k1 - k0); ++key) {
+        const uint8_t* v = vbase + ((int64_t)pages[key / kPage] * kPage + key % kPage) * kv_row;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const uint32_t n = nan_codes(*reinterpret_cast<const uint32_t*>(v + d * 16 + g4 * 4));
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k0 + key < lim[b] && (n >> (8 * e + 7) & 1)) o[b][d][e] = __builtin_nanf("");
+        }
+      }
     }
   }
   __syncthreads();  // every wave is past its ring
@@ -348,13 +392,13 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
       }
       continue;
     }
-    const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+    const float inv = ll == 0.f ? 0.f : 1.0f / ll;
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] *= inv;
     store_row<D>(p, row, head, j, y);
     if (p.lse && j == 0)
       p.lse[(int64_t)head * p.lse_ld + row] =
-          ll > 0.f ? (__log2f(ll) + m_use) * 0.6931471805599453f : -INFINITY;
+          row_lse(ll, m_use);
   }
 }
 
@@ -389,6 +433,7 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   __shared__ __attribute__((aligned(1024))) uint8_t v_lds[2][kBK * VROW];
   __shared__ int pages[kMaxKeys / kPage];
   __shared__ uint16_t bytes[kMaxKeys / kPage];
+  __shared__ int nans;
 
   int s, qt, zg;
   if (work) {
@@ -425,6 +470,9 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   const int lim = p.causal ? min(off + r + 1, used) : used;  // keys < lim are visible
   const int lim_min = p.causal ? min(off + wave_row0 + 1, used) : used;
   const bool rows_full = wave_row0 + 32 <= q_len;
+  // tiles from this one on hold keys that some row of the workgroup sees and
+  // another does not
+  const int cut = p.causal ? max(0, min(used, off + qt * BQ + 1)) / kBK : INT32_MAX;
 
   // the sequence's pages and this KV head's scale bytes
   const int* trow = p.table + (int64_t)s * p.table_ld;
@@ -433,6 +481,7 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
     pages[i] = page;
     bytes[i] = p.scales[(int64_t)page * p.HK + kvh];
   }
+  if (tid == 0) nans = 0;
   // Q^T fragments (B operand): lane holds row `col`, d = c * 16 + half * 8 .. + 8
   v8bf qf[NC];
   {
@@ -471,7 +520,15 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int key = wave * kPage + row0 + j * KPL;
-      const uint32_t w[4] = {reg[j].x, reg[j].y, reg[j].z, reg[j].w};
+      uint32_t w[4] = {reg[j].x, reg[j].y, reg[j].z, reg[j].w};
+      if (v && t >= cut) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t n = nan_codes(w[i]);
+          if (n) nans = 1;
+          w[i] = without(w[i], n);
+        }
+      }
       uint32_t b[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -652,14 +709,29 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
     }
   }
 
+  if (ntiles > cut && nans) {  // rare: the keys of the cut tiles, again
+    for (int key = cut * kBK; key < kv_end; ++key) {
+      const uint8_t* v = vbase + ((int64_t)pages[key / kPage] * kPage + key % kPage) * kv_row;
+#pragma unroll
+      for (int d = 0; d < NDS; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t n = nan_codes(*reinterpret_cast<const uint32_t*>(v + d * 32 + g * 8 + half * 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key < lim && (n >> (8 * e + 7) & 1)) o[d][g * 4 + e] = __builtin_nanf("");
+        }
+    }
+  }
+
   // epilogue: lane holds row `col`, d = dt * 32 + (i / 4) * 8 + half * 4 + i % 4;
   // the wave's rows go out through LDS so that a store writes whole rows,
   // 16-byte chunks XOR-swizzled by the row
-  const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+  const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
   if (p.lse && r_ok && half == 0) {
     const float m_use = m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
     p.lse[(int64_t)head * p.lse_ld + q0 + r] =
-        l_run > 0.f ? (__log2f(l_run) + m_use) * 0.6931471805599453f : -INFINITY;
+        row_lse(l_run, m_use);
   }
   uint8_t* stage = &v_lds[0][0] + wave * 32 * VROW;
   static_assert(4 * 32 * VROW <= sizeof(v_lds), "epilogue staging");
@@ -769,7 +841,7 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
     y[k] += __shfl_xor(y[k], 16, 64);
     y[k] += __shfl_xor(y[k], 32, 64);
   }
-  const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
 #pragma unroll
   for (int k = 0; k < PER; ++k) y[k] *= inv;
   // D / 8 lanes store 8 columns each
@@ -786,7 +858,7 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
   }
   if (p.lse && lane == 0)
     p.lse[(int64_t)head * p.lse_ld + row] =
-        ll > 0.f ? (__log2f(ll) + mm) * 0.6931471805599453f : -INFINITY;
+        row_lse(ll, mm);
 }
 
 // Column blocks of a workgroup: two of 16 where a sequence's (row, head)

@@ -255,6 +255,46 @@ def test_copy_pages_is_exact_in_every_layer(dtype, layers, hk, d, pages, moved):
         assert torch.equal(arena.scales, scales)
 
 
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (24, 8, 64), (8, 8, 128)])
+@pytest.mark.parametrize("q_len,used", [(5, 40), (40, 40), (70, 300), (33, 64)])
+def test_nan_keys_and_values_reach_only_the_rows_that_see_them(hq, hk, d, q_len, used):
+    """NaN codes in K and V of one late token: rows before it are as they are
+    without it, bit for bit; rows that see it are NaN (V: in its columns)."""
+    from quail_amd.chunk import attention_plan
+    g = torch.Generator().manual_seed(5)
+    pages = -(-used // PAGE) + 1
+    arena = KVArena(1, pages, PAGE, hk, d, dtype=FP8)
+    fill(arena, g)
+    cu_q, u, table = sequences(g, (q_len,), (used,), pages)
+    plan = attention_plan(*(torch.from_numpy(a).to(DEV) for a in (cu_q, u, table)),
+                          heads=(hq, hk, d))
+    q = torch.randn(q_len, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    eng = engine_of(arena, hq)
+    clean, clean_lse = eng.read_pages(q, plan, 0)
+    at = used - 3                                   # seen by the last 3 rows
+    row = int(table[0, at // PAGE]) * PAGE + at % PAGE
+    k, v = arena.layer_kv(0)
+    keep = v.view(torch.uint8)[row].clone()
+    v.view(torch.uint8)[row, 0, 5] = 0x7f
+    v.view(torch.uint8)[row, hk - 1, d - 1] = 0xff
+    out, lse = eng.read_pages(q, plan, 0)
+    group = hq // hk
+    want = clean.view(q_len, hq, d).clone()
+    want[-3:, :group, 5] = float("nan")
+    want[-3:, -group:, d - 1] = float("nan")
+    got = out.view(q_len, hq, d)
+    assert bool(((got == want) | (torch.isnan(got) & torch.isnan(want))).all())
+    assert torch.equal(lse, clean_lse)
+    v.view(torch.uint8)[row] = keep
+    k.view(torch.uint8)[row, 0, 7] = 0x7f
+    out, lse = eng.read_pages(q, plan, 0)
+    got = out.view(q_len, hq, d)
+    assert torch.equal(got[:-3], clean.view(q_len, hq, d)[:-3])
+    assert torch.equal(got[:, group:], clean.view(q_len, hq, d)[:, group:])
+    assert bool(torch.isnan(got[-3:, :group]).all() and torch.isnan(lse[:group, -3:]).all())
+    assert torch.equal(lse[:, :-3], clean_lse[:, :-3])
+
+
 def engine_arena(pages, hk=8, d=128, layers=1, dtype=FP8):
     return KVArena(layers, pages, PAGE, hk, d, dtype=dtype)
 
