@@ -438,16 +438,16 @@ max_used bound the sequences' rows and keys.
  *
  * work, n_work, unit: the items of the call, or NULL, 0, 0. The host functions
  * qx_paged_attention8_unit and _work make them from host copies of cu_q and
- * used: unit > 0 where every sequence has few rows (the items are (sequence,
- * i) for its keys [i * unit, (i + 1) * unit), whose results a second launch
- * joins), 0 where the items are query tiles as qx_paged_attention_work's;
- * _work returns their number (<= capacity) or -1.
+ * used: *unit > 0 where every sequence has few rows (items are (sequence, i),
+ * its keys [i * unit, (i + 1) * unit)), else items are (sequence, query tile |
+ * i << 16), whole tiles (0) or their keys in splits of -unit; a second launch
+ * joins the splits. _work returns the items' number (<= capacity) or -1.
  * workspace: qx_paged_attention8_workspace bytes of the caller's (has_work:
  * whether the call gets a list), 16-byte aligned (NULL where that is 0), used
  * by this call alone until the stream has passed it.
  */
-int64_t qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
-                                 int64_t HK);
+int qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                             int64_t HK, int causal, int64_t* unit);
 int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
                                  int64_t HK, int causal, int64_t unit, int* work,
                                  int64_t capacity);

@@ -52,7 +52,7 @@ SIGNATURES = {
                             _i64, _i64, _f32, _p],
     "qx_kv8_write": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p],
     "qx_paged_attention8_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i64],
-    "qx_paged_attention8_unit": [_p, _p, _i64, _i64, _i64],
+    "qx_paged_attention8_unit": [_p, _p, _i64, _i64, _i64, _i32, _p],
     "qx_paged_attention8": [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _i64, _p, _i64, _p, _i64,
                             _p, _i64, _i64, _p, _i64, _p],
@@ -106,7 +106,7 @@ SIGNATURES = {
 RETURNS_COUNT = {"qx_paged_attention_work", "qx_paged_attention_tile_rows",
                  "qx_paged_attention_max_keys", "qx_vocab_logprobs_workspace",
                  "qx_vocab_logprobs_noalloc_max_bytes", "qx_paged_attention8_workspace",
-                 "qx_paged_attention8_work", "qx_paged_attention8_unit"}
+                 "qx_paged_attention8_work"}
 
 
 class QxUnavailable(RuntimeError):

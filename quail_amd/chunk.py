@@ -501,10 +501,13 @@ def _work_list(tables, heads, choose_rows=False, eight_bit=False):
     causal = int(tables.get("causal", True))
     rows = 0
     if eight_bit:
-        unit = _lib.count("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
-                          hk)
-        cap = (int(cu_q[-1]) + seqs if not unit else
-               seqs + int(np.maximum(used, 0).sum()) // unit) if seqs else 1
+        found = ctypes.c_int64()
+        _lib.call("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data, seqs, hq, hk,
+                  causal, ctypes.byref(found))
+        unit = found.value
+        tiles = 1 if unit > 0 else -(-np.diff(cu_q) // 32)
+        parts = 1 if not unit else np.maximum(-(-used // abs(unit)), 1)
+        cap = int((np.ones(seqs, dtype=np.int64) * tiles * parts).sum())
         work = np.zeros(2 * max(cap, 1), dtype=np.int32)
         n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
                        hk, causal, unit, work.ctypes.data, cap)

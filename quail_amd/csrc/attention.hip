@@ -37,10 +37,10 @@
 // unrounded fp32 P.
 #include <algorithm>
 #include <type_traits>
+#include <vector>
 
 #include "qx_common.h"
 #include "qx_status.h"
-#include "work_list.h"
 
 namespace qx {
 namespace {
@@ -1233,7 +1233,29 @@ int64_t qx_paged_attention_work(const int* cu_q, const int* used, int64_t seqs, 
                   (long long)D, (long long)G);
     return QX_EINVAL;
   }
-  return qx::attention_work_list(cu_q, used, seqs, bq, causal, work, capacity);
+  struct Item { int64_t load; int s, qt; };
+  std::vector<Item> items;
+  for (int64_t s = 0; s < seqs; ++s) {
+    const int q_len = cu_q[s + 1] - cu_q[s];
+    const int u = used[s];
+    for (int qt = 0; qt * bq < q_len; ++qt) {
+      const int last = std::min(qt * bq + bq, q_len) - 1;
+      const int keys = causal ? std::min(u, u - q_len + last + 1) : u;
+      items.push_back({(int64_t)keys, (int)s, qt});
+    }
+  }
+  if ((int64_t)items.size() > capacity) {
+    qx::set_error("attention_work: %zu items exceed the capacity %lld", items.size(),
+                  (long long)capacity);
+    return QX_EINVAL;
+  }
+  std::stable_sort(items.begin(), items.end(),
+                   [](const Item& a, const Item& b) { return a.load > b.load; });
+  for (size_t i = 0; i < items.size(); ++i) {
+    work[2 * i] = items[i].s;
+    work[2 * i + 1] = items[i].qt;
+  }
+  return (int64_t)items.size();
 }
 
 }  // extern "C"

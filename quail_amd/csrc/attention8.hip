@@ -19,7 +19,6 @@
 
 #include "qx_common.h"
 #include "qx_status.h"
-#include "work_list.h"
 
 namespace qx {
 namespace {
@@ -46,8 +45,9 @@ struct Attn8Args {
   int64_t os_ld;
   float* lse;
   int64_t lse_ld;
-  // splits: keys per split, and the partial results of `splits` of them
-  int chunk, splits;
+  // keys per split (0: whole sequences), the most splits of a sequence, the
+  // query rows of a tile (0: few rows), and the splits' partial results
+  int chunk, splits, tile_rows;
   int64_t rows;
   float *part_o, *part_ml;
 };
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
     }
     const int64_t row = q0 + c / G;
     const int head = kvh * G + c % G;
-    if (p.splits > 1) {
+    if (used > p.chunk) {
       const int64_t at = ((int64_t)split * p.rows + row) * p.HQ + head;
       if (j == 0) {
         p.part_ml[2 * at] = mm;
@@ -412,6 +412,14 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
 // sum of two e4m3 numbers, take the same matrix time and no conversion, but
 // those cores drop what lies 2^-12 below the largest product of a sum.)
 constexpr int kBK = 64;
+
+// the keys that the last row of a query tile sees, which the tile visits
+__host__ __device__ inline int tile_keys(int used, int q_len, int qt, int rows, int causal) {
+  const int last = (qt * rows + rows < q_len ? qt * rows + rows : q_len) - 1;
+  const int keys = causal ? used - q_len + last + 1 : used;
+  return keys < 0 ? 0 : keys < used ? keys : used;
+}
+
 // a row's reference max moves when a tile raises its max by more than this
 // many powers of two (probabilities then stay below 2^8)
 constexpr float kLazyLog2 = 8.0f;
@@ -435,62 +443,58 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   __shared__ uint16_t bytes[kMaxKeys / kPage];
   __shared__ int nans;
 
-  int s, qt, zg;
+  int s, qt, zg, split = 0;
   if (work) {
     const int item = blockIdx.x / zgroups;
     zg = blockIdx.x % zgroups;
     s = work[2 * item];
-    qt = work[2 * item + 1];
+    qt = work[2 * item + 1] & 0xffff;
+    split = work[2 * item + 1] >> 16;
   } else {
     s = blockIdx.y;
     qt = gridDim.x - 1 - blockIdx.x;
     zg = blockIdx.z;
   }
+  // The sequence's bounds and its pages' ids in one round of loads (rows of
+  // the block table hold max_used keys' entries; those past the sequence's
+  // own are not used); K, V, q and the scales in the next.
+  const int tid = threadIdx.x, lane = tid & 63;
   const int sc = min(max(s, 0), seqs - 1);
+  const int k0 = split * p.chunk;
+  const int last_entry = max((p.max_used - 1) / kPage, 0);
+  const int* trow = p.table + (int64_t)sc * p.table_ld;
+  const int page = trow[min(k0 / kPage + tid, last_entry)];
   const int q0 = p.cu_q[sc], q_len = p.cu_q[sc + 1] - q0;
   const int used = min(p.used[sc], p.max_used);
-  if (s < 0 || s >= seqs || qt < 0 || qt * BQ >= q_len) return;
+  if (s < 0 || s >= seqs || split < 0 || (split && split >= p.splits) || qt * BQ >= q_len) return;
   const int G = p.HQ / p.HK;
   const int per_kv = G / HPB;
   const int kvh = zg / per_kv;
-  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = kvh * G + (zg % per_kv) * HPB + wave % HPB;
   const int qsub = wave / HPB;
   const int half = lane >> 5, col = lane & 31;
 
+  // keys count from the split's first one
   const int off = p.causal ? used - q_len : 0;
   const int wave_row0 = qt * BQ + qsub * 32;
   const int r = wave_row0 + col;
   const bool r_ok = r < q_len;
-  const int block_last = min(qt * BQ + BQ, q_len) - 1;
-  const int kv_end = max(0, p.causal ? min(used, off + block_last + 1) : used);
+  const int block_end = tile_keys(used, q_len, qt, BQ, p.causal);
+  const bool whole = p.chunk == 0 || block_end <= p.chunk;
+  const int kv_end = max(0, whole ? block_end : min(block_end - k0, p.chunk));
   const int ntiles = (kv_end + kBK - 1) / kBK;
   const int npages = (kv_end + kPage - 1) / kPage;
-  const int lim = p.causal ? min(off + r + 1, used) : used;  // keys < lim are visible
-  const int lim_min = p.causal ? min(off + wave_row0 + 1, used) : used;
+  const int lim = (p.causal ? min(off + r + 1, used) : used) - k0;  // keys < lim are visible
+  const int lim_min = (p.causal ? min(off + wave_row0 + 1, used) : used) - k0;
   const bool rows_full = wave_row0 + 32 <= q_len;
   // tiles from this one on hold keys that some row of the workgroup sees and
   // another does not
-  const int cut = p.causal ? max(0, min(used, off + qt * BQ + 1)) / kBK : INT32_MAX;
+  const int cut = p.causal ? max(0, min(used, off + qt * BQ + 1) - k0) / kBK : INT32_MAX;
 
-  // the sequence's pages and this KV head's scale bytes
-  const int* trow = p.table + (int64_t)s * p.table_ld;
-  for (int i = tid; i < npages; i += 256) {
-    const int page = trow[i];
-    pages[i] = page;
-    bytes[i] = p.scales[(int64_t)page * p.HK + kvh];
-  }
+  if (tid < npages) pages[tid] = page;
+  for (int i = tid + 256; i < npages; i += 256) pages[i] = trow[k0 / kPage + i];
   if (tid == 0) nans = 0;
-  // Q^T fragments (B operand): lane holds row `col`, d = c * 16 + half * 8 .. + 8
-  v8bf qf[NC];
-  {
-    const int rr = r_ok ? r : q_len - 1;
-    const int64_t row = p.q_index ? p.q_index[q0 + rr] : (int64_t)(q0 + rr);
-    const uint16_t* q = p.q + row * p.q_ld + (int64_t)head * D;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) qf[c] = *reinterpret_cast<const v8bf*>(q + c * 16 + half * 8);
-  }
   __syncthreads();
 
   const int64_t kv_row = (int64_t)p.HK * D;
@@ -499,6 +503,8 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   // 16-byte chunk swizzles of the bf16 rows, as the 16-bit kernel's
   auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
   auto vswz = [](int key) { return D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; };
+  // Q^T fragments (B operand): lane holds row `col`, d = c * 16 + half * 8 .. + 8
+  v8bf qf[NC];
   // this wave's page of a tile: lane's 16 codes of row j * KPL + lane / CH
   const int row0 = lane / CH, chunk = lane % CH;
   uint4 kreg[LOADS], vreg[LOADS];
@@ -676,14 +682,24 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 
   v16f sa[2], sb[2];
   if (ntiles > 0) {
+    uint4 k1[LOADS];
     load(0, kbase, kreg);
     load(0, vbase, vreg);
+    if (ntiles > 1) load(1, kbase, k1);
+    for (int i = tid; i < npages; i += 256) bytes[i] = p.scales[(int64_t)pages[i] * p.HK + kvh];
+    {
+      const int rr = r_ok ? r : q_len - 1;
+      const int64_t row = p.q_index ? p.q_index[q0 + rr] : (int64_t)(q0 + rr);
+      const uint16_t* q = p.q + row * p.q_ld + (int64_t)head * D;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) qf[c] = *reinterpret_cast<const v8bf*>(q + c * 16 + half * 8);
+    }
+    __syncthreads();
     store(0, &k_lds[0][0], kreg, false);
-    if (ntiles > 1) load(1, kbase, kreg);
     store(0, &v_lds[0][0], vreg, true);
     if (ntiles > 1) {
+      store(1, &k_lds[1][0], k1, false);
       load(1, vbase, vreg);
-      store(1, &k_lds[1][0], kreg, false);
       if (ntiles > 2) load(2, kbase, kreg);
     }
     step_end();
@@ -727,6 +743,22 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   // epilogue: lane holds row `col`, d = dt * 32 + (i / 4) * 8 + half * 4 + i % 4;
   // the wave's rows go out through LDS so that a store writes whole rows,
   // 16-byte chunks XOR-swizzled by the row
+  if (!whole) {  // a split: its state as it stands
+    const int64_t at = ((int64_t)split * p.rows + q0 + r) * p.HQ + head;
+    if (r_ok) {
+#pragma unroll
+      for (int d = 0; d < NDS; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<v4f*>(p.part_o + at * D + d * 32 + g * 8 + half * 4) =
+              v4f{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      if (half == 0) {
+        p.part_ml[2 * at] = m_run * p.scale_log2;
+        p.part_ml[2 * at + 1] = l_run;
+      }
+    }
+    return;
+  }
   const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
   if (p.lse && r_ok && half == 0) {
     const float m_use = m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
@@ -777,7 +809,11 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
   const int q0 = p.cu_q[s], q_len = p.cu_q[s + 1] - q0;
   const int used = min(p.used[s], p.max_used);
   if (in_seq >= q_len * p.HQ) return;
-  const int splits = max(1, (used + p.chunk - 1) / p.chunk);
+  const int keys = p.tile_rows
+                       ? tile_keys(used, q_len, in_seq / p.HQ / p.tile_rows, p.tile_rows, p.causal)
+                       : used;
+  if (keys <= p.chunk) return;  // not split: its rows went out whole
+  const int splits = (keys + p.chunk - 1) / p.chunk;
   const int64_t row = q0 + in_seq / p.HQ;
   const int head = in_seq % p.HQ;
   const int64_t pair = row * p.HQ + head;
@@ -894,6 +930,17 @@ inline int tile_height(int64_t G) { return 32 * (4 / tile_heads(G)); }
 inline bool few_rows(int64_t max_q, int64_t G) { return max_q * G <= 32; }
 
 template <int D>
+void merge_launch(const Attn8Args& a, int64_t seqs, int64_t max_q, hipStream_t stream) {
+  if (a.splits > 16)
+    hipLaunchKernelGGL((split_merge_kernel<D, 4>), dim3((unsigned)(max_q * a.HQ), (unsigned)seqs),
+                       dim3(256), 0, stream, a);
+  else if (a.splits > 1)
+    hipLaunchKernelGGL((split_merge_kernel<D, 1>),
+                       dim3((unsigned)((max_q * a.HQ + 3) / 4), (unsigned)seqs), dim3(256), 0,
+                       stream, a);
+}
+
+template <int D>
 void tile_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t seqs, int64_t max_q,
                  hipStream_t stream) {
   const int G = a.HQ / a.HK, hpb = tile_heads(G), rows = tile_height(G);
@@ -901,12 +948,14 @@ void tile_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t se
   const dim3 grid = work ? dim3((unsigned)(n_work * zgroups))
                          : dim3((unsigned)((max_q + rows - 1) / rows), (unsigned)seqs,
                                 (unsigned)zgroups);
-  if (hpb == 4)
-    hipLaunchKernelGGL((attention8_tile_kernel<D, 4, 1>), grid, dim3(256), 0, stream, a, work, zgroups, (int)seqs);
-  else if (hpb == 2)
-    hipLaunchKernelGGL((attention8_tile_kernel<D, 2, 2>), grid, dim3(256), 0, stream, a, work, zgroups, (int)seqs);
-  else
-    hipLaunchKernelGGL((attention8_tile_kernel<D, 1, 4>), grid, dim3(256), 0, stream, a, work, zgroups, (int)seqs);
+#define QX_TILE(H, Q)                                                                          \
+  hipLaunchKernelGGL((attention8_tile_kernel<D, H, Q>), grid, dim3(256), 0, stream, a, work,   \
+                     zgroups, (int)seqs)
+  if (hpb == 4) QX_TILE(4, 1);
+  else if (hpb == 2) QX_TILE(2, 2);
+  else QX_TILE(1, 4);
+#undef QX_TILE
+  merge_launch<D>(a, seqs, max_q, stream);
 }
 
 template <int D, int NB>
@@ -918,18 +967,38 @@ void few_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t seq
                   work ? 1u : (unsigned)seqs);
   hipLaunchKernelGGL((attention8_few_kernel<D, NB>), grid, dim3(256), 0, stream, a, work,
                      (int)seqs);
-  if (a.splits > 16)
-    hipLaunchKernelGGL((split_merge_kernel<D, 4>), dim3((unsigned)(max_q * a.HQ), (unsigned)seqs),
-                       dim3(256), 0, stream, a);
-  else if (a.splits > 1)
-    hipLaunchKernelGGL((split_merge_kernel<D, 1>),
-                       dim3((unsigned)((max_q * a.HQ + 3) / 4), (unsigned)seqs), dim3(256), 0,
-                       stream, a);
+  merge_launch<D>(a, seqs, max_q, stream);
 }
 
-// Keys per work item of a call (0: the items are query tiles).
-int64_t call_unit(int64_t keys, int64_t max_q, int64_t max_used, int64_t HK,
-                  int64_t G) {
+// What a call's work items are: keys per split of the few-row kernel (> 0),
+// query tiles (0), or query tiles in splits of that many keys (< 0).
+int64_t list_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ, int64_t HK,
+                  int causal) {
+  const int64_t G = HQ / HK;
+  int64_t max_q = 0, max_used = 0, keys = 0;
+  for (int64_t s = 0; s < seqs; ++s) {
+    max_q = std::max<int64_t>(max_q, cu_q[s + 1] - cu_q[s]);
+    max_used = std::max<int64_t>(max_used, used[s]);
+    keys += std::max(used[s], 0);
+  }
+  if (few_rows(max_q, G)) return split_chunk(keys, max_q, max_used, HK, G);
+  // 64-key steps of all workgroups, and of the longest one
+  const int rows = tile_height(G);
+  int64_t steps = 0, longest = 0;
+  for (int64_t s = 0; s < seqs; ++s)
+    for (int qt = 0; (int64_t)qt * rows < cu_q[s + 1] - cu_q[s]; ++qt) {
+      const int64_t n = (tile_keys(used[s], cu_q[s + 1] - cu_q[s], qt, rows, causal) + kBK - 1) / kBK;
+      steps += n;
+      longest = std::max(longest, n);
+    }
+  steps *= HQ / tile_heads(G);
+  const int64_t even = std::max<int64_t>(4, (steps + 511) / 512);  // of each workgroup at a time
+  if (longest <= even + 6 || longest * 4 <= even * 5) return 0;
+  return -kBK * even;
+}
+
+// The same of a call without a list: whole query tiles where rows are many.
+int64_t call_unit(int64_t keys, int64_t max_q, int64_t max_used, int64_t HK, int64_t G) {
   return few_rows(max_q, G) ? split_chunk(keys, max_q, max_used, HK, G) : 0;
 }
 
@@ -941,34 +1010,35 @@ using namespace qx;
 extern "C" {
 
 int64_t qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
-                                 int64_t HK) {
-  QX_CHECK(cu_q && used && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
+                                 int64_t HK, int causal, int64_t* unit) {
+  QX_CHECK(cu_q && used && unit && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
            "attention8_unit: arguments");
-  int64_t max_q = 0, max_used = 0, keys = 0;
-  for (int64_t s = 0; s < seqs; ++s) {
-    max_q = std::max<int64_t>(max_q, cu_q[s + 1] - cu_q[s]);
-    max_used = std::max<int64_t>(max_used, used[s]);
-    keys += std::max(used[s], 0);
-  }
-  return call_unit(keys, max_q, max_used, HK, HQ / HK);
+  *unit = list_unit(cu_q, used, seqs, HQ, HK, causal);
+  return QX_OK;
 }
 
-static int64_t few_work_list(const int* cu_q, const int* used, int64_t seqs, int64_t unit,
-                             int* work, int64_t capacity) {
-  // whole splits first, then the rest, longest first
-  std::vector<std::pair<int, std::pair<int, int>>> items;
+// Items of (sequence, part), heaviest first; rows 0: parts are splits of
+// `unit` keys, else part = query tile | split << 16 (unit 0: no splits).
+static int64_t work_list(const int* cu_q, const int* used, int64_t seqs, int rows, int causal,
+                         int64_t unit, int* work, int64_t capacity) {
+  struct Item { int64_t load; int s, part; };
+  std::vector<Item> items;
   for (int64_t s = 0; s < seqs; ++s) {
-    if (cu_q[s + 1] == cu_q[s]) continue;
-    for (int64_t i = 0, k0 = 0; i == 0 || k0 < used[s]; ++i, k0 += unit)
-      items.push_back({(int)std::min<int64_t>(unit, used[s] - k0), {(int)s, (int)i}});
+    const int q_len = cu_q[s + 1] - cu_q[s];
+    for (int qt = 0; rows ? qt * rows < q_len : qt < 1 && q_len > 0; ++qt) {
+      const int64_t keys = rows ? tile_keys(used[s], q_len, qt, rows, causal) : used[s];
+      const int64_t part = unit ? unit : std::max<int64_t>(keys, 1);
+      for (int64_t i = 0, k0 = 0; i == 0 || k0 < keys; ++i, k0 += part)
+        items.push_back({std::min(part, keys - k0), (int)s, rows ? (int)(qt | i << 16) : (int)i});
+    }
   }
   QX_CHECK((int64_t)items.size() <= capacity, "attention8_work: %zu items, room for %lld",
            items.size(), (long long)capacity);
   std::stable_sort(items.begin(), items.end(),
-                   [](const auto& a, const auto& b) { return a.first > b.first; });
+                   [](const Item& a, const Item& b) { return a.load > b.load; });
   for (size_t i = 0; i < items.size(); ++i) {
-    work[2 * i] = items[i].second.first;
-    work[2 * i + 1] = items[i].second.second;
+    work[2 * i] = items[i].s;
+    work[2 * i + 1] = items[i].part;
   }
   return (int64_t)items.size();
 }
@@ -976,12 +1046,14 @@ static int64_t few_work_list(const int* cu_q, const int* used, int64_t seqs, int
 int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
                                  int64_t HK, int causal, int64_t unit, int* work,
                                  int64_t capacity) {
-  QX_CHECK(cu_q && used && work && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0 && unit >= 0,
+  QX_CHECK(cu_q && used && work && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
            "attention8_work: arguments");
+  const int rows = unit > 0 ? 0 : tile_height(HQ / HK);
+  for (int64_t s = 0; s < seqs; ++s)
+    QX_CHECK((cu_q[s + 1] - cu_q[s]) / 32 < 65536, "attention8_work: a sequence of %d rows",
+             cu_q[s + 1] - cu_q[s]);
   try {
-    return unit ? few_work_list(cu_q, used, seqs, unit, work, capacity)
-                : attention_work_list(cu_q, used, seqs, tile_height(HQ / HK), causal, work,
-                                      capacity);
+    return work_list(cu_q, used, seqs, rows, causal, unit < 0 ? -unit : unit, work, capacity);
   } catch (const std::bad_alloc&) {
     set_error("attention8_work: out of host memory");
     return QX_EINVAL;
@@ -992,9 +1064,10 @@ int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q,
                                       int64_t HQ, int64_t HK, int64_t D, int has_work,
                                       int64_t unit) {
   QX_CHECK(seqs >= 0 && rows >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 &&
-               HQ % HK == 0 && (D == 64 || D == 128) && unit >= 0,
+               HQ % HK == 0 && (D == 64 || D == 128),
            "attention8_workspace: arguments");
   if (!has_work) unit = call_unit(seqs * max_used, max_q, max_used, HK, HQ / HK);
+  if (unit < 0) unit = -unit;
   const int64_t splits = unit ? (max_used + unit - 1) / unit : 0;
   return splits > 1 ? splits * rows * HQ * (D + 2) * 4 : 0;
 }
@@ -1024,7 +1097,8 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
            "attention8: alignment");
   QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
   QX_CHECK(!work || (n_work >= 0 && n_work * HQ < (1LL << 24)), "attention8: work items");
-  QX_CHECK(unit >= 0 && unit % 128 == 0 && unit <= kMaxChunk && (work || !unit),
+  QX_CHECK((work || !unit) && (unit <= 0 ? unit % kBK == 0 && unit >= -kMaxKeys
+                                         : unit % 128 == 0 && unit <= kMaxChunk),
            "attention8: work items of %lld keys", (long long)unit);
   if (seqs == 0 || max_q == 0 || rows == 0 || (work && n_work == 0)) return QX_OK;
   const int64_t G = HQ / HK;
@@ -1041,17 +1115,16 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
               causal, scale * 1.4426950408889634f, (uint16_t*)out_bf16, (uint8_t*)out_fp8, o_ld,
               out_scales, os_ld, lse, lse_ld};
   if (!work) unit = call_unit(seqs * max_used, max_q, max_used, HK, G);
-  if (!unit) {
-    if (D == 128) tile_launch<128>(a, work, n_work, seqs, max_q, stream);
-    else tile_launch<64>(a, work, n_work, seqs, max_q, stream);
-    QX_LAUNCH_STATUS();
-  }
-  a.chunk = (int)unit;
-  a.splits = (int)std::max<int64_t>(1, (max_used + unit - 1) / unit);
+  a.chunk = (int)(unit < 0 ? -unit : unit);
+  a.splits = unit ? (int)std::max<int64_t>(1, (max_used + a.chunk - 1) / a.chunk) : 1;
+  a.tile_rows = unit > 0 ? 0 : tile_height(G);
   a.rows = rows;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + (int64_t)a.splits * rows * HQ * D;
-  if (D == 128) {
+  if (unit <= 0) {
+    if (D == 128) tile_launch<128>(a, work, n_work, seqs, max_q, stream);
+    else tile_launch<64>(a, work, n_work, seqs, max_q, stream);
+  } else if (D == 128) {
     if (nb == 1) few_launch<128, 1>(a, work, n_work, seqs, max_q, stream);
     else few_launch<128, 2>(a, work, n_work, seqs, max_q, stream);
   } else {

@@ -123,6 +123,8 @@ CASES = [
     ((21, 33, 64, 100), (70, 33, 700, 101), True),
     ((2, 1), (5000, 9000), False),                  # split over the keys
     ((130, 3), (130, 1), True),
+    ((40, 21, 70), (9000, 100, 1500), True),        # tiles split over the keys
+    ((33, 9), (6000, 640), False),
 ]
 
 

@@ -109,31 +109,53 @@ def test_packs_page_items_write_what_their_scatter_writes(seed):
     assert "page_writes" not in pack_chunk(plain, groups).meta["unified"]
 
 
-def test_attention_items_cover_every_key_of_few_row_calls_and_every_tile_of_others():
+def test_attention_items_cover_every_key_of_every_tile():
+    import ctypes
+
     def items(q_lens, used, hq=32, hk=8, causal=1):
         cu_q = np.concatenate([[0], np.cumsum(q_lens)]).astype(np.int32)
         used = np.asarray(used, dtype=np.int32)
-        unit = _lib.count("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data,
-                          len(used), hq, hk)
-        work = np.zeros(2 * 4096, dtype=np.int32)
-        n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, len(used),
-                       hq, hk, causal, unit, work.ctypes.data, 4096)
-        with pytest.raises(_lib.QxError, match="room|capacity"):
-            _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, len(used),
-                       hq, hk, causal, unit, work.ctypes.data, n - 1)
-        return unit, [tuple(work[2 * i:2 * i + 2]) for i in range(n)]
+        unit = ctypes.c_int64()
+        _lib.call("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data, len(used), hq, hk,
+                  causal, ctypes.byref(unit))
+        work = np.zeros(2 * 8192, dtype=np.int32)
 
+        def fill(cap):
+            return _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data,
+                              len(used), hq, hk, causal, unit.value, work.ctypes.data, cap)
+        n = fill(8192)
+        with pytest.raises(_lib.QxError, match="room"):
+            fill(n - 1)
+        return unit.value, [(int(s), int(p) & 0xffff, int(p) >> 16)
+                            for s, p in work[:2 * n].reshape(-1, 2)]
+
+    # few rows a sequence: splits of their keys
     used = [300, 0, 8192, 5, 40000]
     unit, got = items([1, 2, 3, 0, 1], used)
     assert unit and unit % 128 == 0
-    want = [(s, i) for s, u in enumerate(used) if s != 3 for i in range(max(1, -(-u // unit)))]
-    assert sorted(got) == sorted(want)
-    load = [min(unit, used[s] - i * unit) for s, i in got]
+    assert sorted(got) == [(s, i, 0) for s, u in enumerate(used) if s != 3
+                           for i in range(max(1, -(-u // unit)))]
+    load = [min(unit, used[s] - i * unit) for s, i, _ in got]
     assert load == sorted(load, reverse=True)
+    # whole query tiles
     unit, got = items([100, 1, 33], [150, 40, 33])
-    assert unit == 0 and sorted(got) == [(0, 0), (0, 1), (0, 2), (0, 3), (1, 0), (2, 0), (2, 1)]
+    assert unit == 0
+    assert sorted(got) == [(s, t, 0) for s, t in ((0, 0), (0, 1), (0, 2), (0, 3), (1, 0), (2, 0),
+                                                  (2, 1))]
     unit, got = items([100, 1], [150, 40], hq=16)       # two heads a KV head: 64 rows
-    assert unit == 0 and sorted(got) == [(0, 0), (0, 1), (1, 0)]
+    assert unit == 0 and sorted(got) == [(0, 0, 0), (0, 1, 0), (1, 0, 0)]
+    # tiles whose keys are split: one long sequence among short ones
+    q_lens, used = [40, 21, 21, 0], [20000, 900, 70, 10]
+    unit, got = items(q_lens, used)
+    assert unit < 0 and unit % 64 == 0
+    want = []
+    for s, (q, u) in enumerate(zip(q_lens, used)):
+        for t in range(-(-q // 32)):
+            keys = u - q + min(32 * t + 32, q)
+            want += [(s, t, i) for i in range(-(-keys // -unit))]
+    assert sorted(got) == sorted(want)
+    # many rows of equal length: nothing to even out
+    assert items([8000, 8000], [8100, 8100])[0] == 0
 
 
 def test_scale_bytes_and_codes_of_the_oracle():
@@ -269,6 +291,8 @@ def test_entry_points_refuse_bad_arguments():
                       (dict(work=16, n_work=-1), "work"), (dict(work=16, n_work=1 << 24), "work"),
                       (dict(unit=128), "items"), (dict(work=16, n_work=1, unit=100), "items"),
                       (dict(work=16, n_work=1, unit=8192), "items"),
+                      (dict(work=16, n_work=1, unit=-100), "items"),
+                      (dict(work=16, n_work=1, unit=-64, mu=256), "workspace"),
                       (dict(work=16, n_work=1, unit=128, mu=256), "workspace")):
         with pytest.raises(_lib.QxError, match=match):
             attend(**kw)
