@@ -487,7 +487,6 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   const int npages = (kv_end + kPage - 1) / kPage;
   const int lim = (p.causal ? min(off + r + 1, used) : used) - k0;  // keys < lim are visible
   const int lim_min = (p.causal ? min(off + wave_row0 + 1, used) : used) - k0;
-  const bool rows_full = wave_row0 + 32 <= q_len;
   // tiles from this one on hold keys that some row of the workgroup sees and
   // another does not
   const int cut = p.causal ? max(0, min(used, off + qt * BQ + 1) - k0) / kBK : INT32_MAX;
@@ -508,59 +507,68 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   // this wave's page of a tile: lane's 16 codes of row j * KPL + lane / CH
   const int row0 = lane / CH, chunk = lane % CH;
   uint4 kreg[LOADS], vreg[LOADS];
-  // rows past the last key re-read it
+  // this wave's page of tile t (the last one past the keys' end), and the
+  // lane's bytes in it: rows past the last key read that one again
+  auto slot_of = [&](int t) { return min(t * kBK + wave * kPage, kv_end - 1) / kPage; };
+  auto place = [&](int t, int j) -> uint32_t {
+    const int left = kv_end - 1 - slot_of(t) * kPage;
+    return (uint32_t)(min(row0 + j * KPL, left) * (int)kv_row + chunk * 16);
+  };
   auto load = [&](int t, const uint8_t* base, uint4 (&reg)[LOADS]) {
-    const int first = t * kBK + wave * kPage;
-    const int slot = min(first, kv_end - 1) / kPage;
-    const int left = kv_end - 1 - slot * kPage;  // the last row of this page to read
-    const int64_t page = __builtin_amdgcn_readfirstlane(pages[slot]);
-    const uint8_t* at = base + page * kPage * kv_row + chunk * 16;
+    const int64_t page = __builtin_amdgcn_readfirstlane(pages[slot_of(t)]);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
-      reg[j] = *reinterpret_cast<const uint4*>(at + (uint32_t)(min(row0 + j * KPL, left) * (int)kv_row));
+      reg[j] = *reinterpret_cast<const uint4*>(base + page * kPage * kv_row + place(t, j));
   };
-  auto store = [&](int t, uint8_t* tile, const uint4 (&reg)[LOADS], bool v) {
+  // the scale of this wave's page of a tile
+  auto scale_of = [&](int t, bool v) -> float {
     const int slot = min(t * (kBK / kPage) + wave, npages - 1);
     const int pair = __builtin_amdgcn_readfirstlane(bytes[slot]);
-    const float scale = e8m0(v ? pair >> 8 : pair & 255);
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int key = wave * kPage + row0 + j * KPL;
-      uint32_t w[4] = {reg[j].x, reg[j].y, reg[j].z, reg[j].w};
-      if (v && t >= cut) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t n = nan_codes(w[i]);
-          if (n) nans = 1;
-          w[i] = without(w[i], n);
-        }
-      }
-      uint32_t b[8];
+    return e8m0(v ? pair >> 8 : pair & 255);
+  };
+  // where this lane's 16 codes of row row0 + j KPL go, as bf16: st_k ^ 128 j
+  // (st_v) past j KPL rows, and their second half at that ^ 16
+  const int st_row = (wave * kPage + row0) * VROW;
+  const int st_k = st_row + (((2 * chunk) ^ kswz(row0)) * 16);
+  const int st_v = st_row + (((2 * chunk) ^ vswz(row0)) * 16);
+  auto store = [&](uint8_t* tile, uint4 reg, int j, int at, float scale, bool v, bool check) {
+    uint32_t w[4] = {reg.x, reg.y, reg.z, reg.w};
+    if (check) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
-        b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true));
+        const uint32_t n = nan_codes(w[i]);
+        if (n) nans = 1;
+        w[i] = without(w[i], n);
       }
-      const int z = v ? vswz(key) : kswz(key);
-      *reinterpret_cast<uint4*>(tile + key * VROW + ((2 * chunk) ^ z) * 16) = make_uint4(b[0], b[1], b[2], b[3]);
-      *reinterpret_cast<uint4*>(tile + key * VROW + ((2 * chunk + 1) ^ z) * 16) = make_uint4(b[4], b[5], b[6], b[7]);
     }
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false));
+      b[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true));
+    }
+    uint8_t* to = tile + j * KPL * VROW + (v ? at : at ^ (128 * j));
+    *reinterpret_cast<uint4*>(to) = make_uint4(b[0], b[1], b[2], b[3]);
+    *reinterpret_cast<uint4*>(tile + j * KPL * VROW + ((v ? at : at ^ (128 * j)) ^ 16)) = make_uint4(b[4], b[5], b[6], b[7]);
   };
-  // K fragment (A operand of S^T): key `col` (+ 32), d chunk 2c + half
-  int k_off[NC];
+  auto store_all = [&](int t, uint8_t* tile, const uint4 (&reg)[LOADS], bool v) {
+    const float scale = scale_of(t, v);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) k_off[c] = col * VROW + (((2 * c + half) ^ kswz(col)) * 16);
+    for (int j = 0; j < LOADS; ++j) store(tile, reg[j], j, v ? st_v : st_k, scale, v, v && t >= cut);
+  };
+  // a whole tile's rows: this wave's page, and each lane's place in it
+  uint32_t in_page[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) in_page[j] = (uint32_t)((row0 + j * KPL) * (int)kv_row + chunk * 16);
+  // K fragment (A operand of S^T): key `col` (+ 32), d chunk 2c + half, at
+  // k_base ^ 32 c (the swizzle moves chunks within the row)
+  const int k_base = col * VROW + ((half ^ kswz(col)) * 16);
   // V^T fragment by transposing reads: lane 16 g + x reads 4 halfwords of key
-  // 4 * half + x / 4 (+ 8) at column 16 (g & 1) + 4 (x & 3) of a 32-d tile
-  int v_off[NDS];
-  {
-    const int x = lane & 15;
-    const int key = 4 * half + (x >> 2);
-    const int c = 2 * ((lane >> 4) & 1) + ((x & 3) >> 1);
-#pragma unroll
-    for (int d = 0; d < NDS; ++d)
-      v_off[d] = key * VROW + (((d * 4 + c) ^ vswz(key)) * 16) + 8 * (x & 1);
-  }
+  // 4 * half + x / 4 (+ 8) at column 16 (g & 1) + 4 (x & 3) of a 32-d tile,
+  // d tile d at v_base ^ 64 d
+  const int v_key = 4 * half + ((lane & 15) >> 2);
+  const int v_base = v_key * VROW +
+                     (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz(v_key)) * 16) + 8 * (lane & 1);
 
   v16f o[NDS];
 #pragma unroll
@@ -569,13 +577,13 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
 
-  auto read_k = [&](const uint8_t* kl, int c, v8bf (&f)[2]) {
+  auto read_k = [&](const uint8_t* kl, int kb, int c, v8bf (&f)[2]) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
-      f[ks] = *reinterpret_cast<const v8bf*>(kl + ks * 32 * VROW + k_off[c]);
+      f[ks] = *reinterpret_cast<const v8bf*>(kl + ks * 32 * VROW + (kb ^ (32 * c)));
   };
-  auto read_v = [&](const uint8_t* vl, int kc, int d) -> v8bf {
-    const uint8_t* at = vl + ((kc >> 1) * 32 + (kc & 1) * 16) * VROW + v_off[d];
+  auto read_v = [&](const uint8_t* vl, int vb, int kc, int d) -> v8bf {
+    const uint8_t* at = vl + ((kc >> 1) * 32 + (kc & 1) * 16) * VROW + (vb ^ (64 * d));
     const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
     const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * VROW));
     const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -583,8 +591,8 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   };
   auto mask_tile = [&](int t, v16f (&sacc)[2]) {
     const int t0 = t * kBK;
-    if (t0 + kBK <= lim_min && rows_full) return;  // every row of the wave sees it whole
-    const int room = r_ok ? lim - t0 - half * 4 : -1;
+    if (t0 + kBK <= lim_min) return;  // every row of the wave sees it whole
+    const int room = lim - t0 - half * 4;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -618,28 +626,29 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   };
   // Step t: softmax and PV of tile t beside S of tile t + 1. Tiles reach LDS
   // a step before their use: K of tile t + 2 and V of tile t + 1 are stored
-  // from the registers that step t - 1 loaded, and the next ones load.
-  // The exponentials run between the S MFMAs, two behind each, in an order
-  // that sched_barrier keeps.
-  auto step = [&](const int t, const int cur, v16f (&s_cur)[2], v16f (&s_next)[2], auto last_c) {
-    constexpr bool LAST = decltype(last_c)::value;
-    if (!LAST) {
-      store(t + 1, &v_lds[cur ^ 1][0], vreg, true);
-      if (t + 2 < ntiles) {
-        store(t + 2, &k_lds[cur][0], kreg, false);
-        load(t + 2, vbase, vreg);
-        if (t + 3 < ntiles) load(t + 3, kbase, kreg);
-      }
-    }
+  // from the registers that step t - 1 loaded, and the next ones load. The
+  // exponentials run between the S MFMAs, two behind each, the conversions
+  // and stores between the PV MFMAs, in an order that sched_barrier keeps.
+  // FAST: no row's mask reaches tiles t and t + 1, and tiles up to t + 3 are
+  // whole.
+  enum { kFast, kNext, kLast };
+  auto step = [&](const int t, const int cur, v16f (&s_cur)[2], v16f (&s_next)[2], auto kind_c) {
+    constexpr int KIND = decltype(kind_c)::value;
+    constexpr bool LAST = KIND == kLast, FAST = KIND == kFast;
     const uint8_t* kl = &k_lds[cur ^ 1][0];
     const uint8_t* vl = &v_lds[cur][0];
-    constexpr int kAhead = 3;
+    // recomputed here rather than kept across the loop
+    const int kb = opaque(k_base), vb = opaque(v_base);
+    const int sk = opaque(st_k), sv = opaque(st_v);
+    constexpr int kAhead = 1;  // chunks of K read before their MFMAs: more were as fast, and took registers
     v8bf kf[NC][2];
+    int page_v = 0, page_k = 0;
+    float scale_k = 1.f, scale_v = 1.f;
     if (!LAST) {
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c) read_k(kl, c, kf[c]);
+      for (int c = 0; c < kAhead; ++c) read_k(kl, kb, c, kf[c]);
     }
-    mask_tile(t, s_cur);
+    if (!FAST) mask_tile(t, s_cur);
     float alpha, m_use;
     rescale(s_cur, alpha, m_use);
     float psum = 0.f;
@@ -651,11 +660,19 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
       for (int ks = 0; ks < 2; ++ks) {
         if (!LAST) {
           __builtin_amdgcn_sched_barrier(0);
-          if (ks == 0 && c + kAhead < NC) read_k(kl, c + kAhead, kf[c + kAhead]);
+          if (ks == 0 && c + kAhead < NC) read_k(kl, kb, c + kAhead, kf[c + kAhead]);
+          if (c == 0 && ks == 1) {
+            page_v = pages[FAST ? (t + 2) * (kBK / kPage) + wave : slot_of(t + 2)];
+            page_k = pages[FAST ? (t + 3) * (kBK / kPage) + wave : slot_of(t + 3)];
+          }
+          if (c == 1 && ks == 1) {
+            scale_v = scale_of(t + 1, true);
+            scale_k = scale_of(t + 2, false);
+          }
         }
         if (c == NC - 1) {  // V of the first 16 keys
 #pragma unroll
-          for (int d = ks * (NDS / 2); d < (ks + 1) * (NDS / 2); ++d) vf[0][d] = read_v(vl, 0, d);
+          for (int d = ks * (NDS / 2); d < (ks + 1) * (NDS / 2); ++d) vf[0][d] = read_v(vl, vb, 0, d);
         }
         if (!LAST)
           s_next[ks] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[c][ks], qf[c], c == 0 ? v16f{} : s_next[ks], 0, 0, 0);
@@ -669,18 +686,36 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
       }
     if (!LAST) __builtin_amdgcn_sched_barrier(0);
     l_run = l_run * alpha + sum_halves(psum);
+    constexpr int SLOTS = 4 * NDS;  // MFMAs of PV; 2 LOADS stores go behind every few
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc)
 #pragma unroll
       for (int d = 0; d < NDS; ++d) {
-        if (kc < 3) vf[kc + 1][d] = read_v(vl, kc + 1, d);
+        if (kc < 3) vf[kc + 1][d] = read_v(vl, vb, kc + 1, d);
         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[kc][d], pf[kc], o[d], 0, 0, 0);
-        if (!LAST) __builtin_amdgcn_sched_barrier(0);
+        if (!LAST) {
+          const int slot = kc * NDS + d;
+          if (slot % (SLOTS / (2 * LOADS)) == 0) {
+            const int u = slot / (SLOTS / (2 * LOADS)), j = u % LOADS;
+            if (u < LOADS)
+              store(&v_lds[cur ^ 1][0], vreg[j], j, sv, scale_v, true, !FAST && t + 1 >= cut);
+            else if (FAST || t + 2 < ntiles)
+              store(&k_lds[cur][0], kreg[j], j, sk, scale_k, false, false);
+            // the register's next load
+            if (FAST || t + (u < LOADS ? 2 : 3) < ntiles)
+              (u < LOADS ? vreg : kreg)[j] = *reinterpret_cast<const uint4*>(
+                  (u < LOADS ? vbase : kbase) +
+                  (int64_t)__builtin_amdgcn_readfirstlane(u < LOADS ? page_v : page_k) * kPage * kv_row +
+                  (FAST ? in_page[j] : place(t + (u < LOADS ? 2 : 3), j)));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     step_end();
   };
 
   v16f sa[2], sb[2];
+  int checked = cut;  // the first tile whose NaN codes were left out
   if (ntiles > 0) {
     uint4 k1[LOADS];
     load(0, kbase, kreg);
@@ -695,10 +730,10 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
       for (int c = 0; c < NC; ++c) qf[c] = *reinterpret_cast<const v8bf*>(q + c * 16 + half * 8);
     }
     __syncthreads();
-    store(0, &k_lds[0][0], kreg, false);
-    store(0, &v_lds[0][0], vreg, true);
+    store_all(0, &k_lds[0][0], kreg, false);
+    store_all(0, &v_lds[0][0], vreg, true);
     if (ntiles > 1) {
-      store(1, &k_lds[1][0], k1, false);
+      store_all(1, &k_lds[1][0], k1, false);
       load(1, vbase, vreg);
       if (ntiles > 2) load(2, kbase, kreg);
     }
@@ -706,27 +741,32 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       v8bf kf[2];
-      read_k(&k_lds[0][0], c, kf);
+      read_k(&k_lds[0][0], k_base, c, kf);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
         sa[ks] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qf[c], c == 0 ? v16f{} : sa[ks], 0, 0, 0);
     }
     step_end();
     int t = 0;
+    const int whole_tiles = kv_end / kBK;
+    for (; t + 4 < whole_tiles && t + 2 < cut; t += 2) {
+      step(t, 0, sa, sb, std::integral_constant<int, kFast>{});
+      step(t + 1, 1, sb, sa, std::integral_constant<int, kFast>{});
+    }
     for (; t + 2 < ntiles; t += 2) {
-      step(t, 0, sa, sb, std::false_type{});
-      step(t + 1, 1, sb, sa, std::false_type{});
+      step(t, 0, sa, sb, std::integral_constant<int, kNext>{});
+      step(t + 1, 1, sb, sa, std::integral_constant<int, kNext>{});
     }
     if (t + 1 < ntiles) {
-      step(t, 0, sa, sb, std::false_type{});
-      step(t + 1, 1, sb, sa, std::true_type{});
+      step(t, 0, sa, sb, std::integral_constant<int, kNext>{});
+      step(t + 1, 1, sb, sa, std::integral_constant<int, kLast>{});
     } else {
-      step(t, 0, sa, sb, std::true_type{});
+      step(t, 0, sa, sb, std::integral_constant<int, kLast>{});
     }
   }
 
-  if (ntiles > cut && nans) {  // rare: the keys of the cut tiles, again
-    for (int key = cut * kBK; key < kv_end; ++key) {
+  if (nans) {  // rare: the keys of the tiles looked at, again
+    for (int key = checked * kBK; key < kv_end; ++key) {
       const uint8_t* v = vbase + ((int64_t)pages[key / kPage] * kPage + key % kPage) * kv_row;
 #pragma unroll
       for (int d = 0; d < NDS; ++d)
@@ -982,7 +1022,15 @@ int64_t list_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ, in
     keys += std::max(used[s], 0);
   }
   if (few_rows(max_q, G)) return split_chunk(keys, max_q, max_used, HK, G);
-  // 64-key steps of all workgroups, and of the longest one
+  // 64-key steps of all workgroups, and of the longest one. A step takes about
+  // 1.6 us in a workgroup alone on its CU, 2.1 beside another; joining splits a
+  // launch and the traffic of their rows. Split
+  //   - into 256 workgroups of equal steps, where the longest has 6 more (21
+  //     rows on one document of 8000 tokens: 156 us whole, 25; on 8 of ~900:
+  //     34, 21; 100 on 8 of ~8000: 228, 142);
+  //   - into 512 where it has 24 more and a quarter more (12 rows on 60
+  //     documents of ~4000: 203, 192); not for less (21 rows on 60 of ~900, 33
+  //     steps against 15: 56 us whole, 74; one document's 2000 rows: 60, 87).
   const int rows = tile_height(G);
   int64_t steps = 0, longest = 0;
   for (int64_t s = 0; s < seqs; ++s)
@@ -992,9 +1040,11 @@ int64_t list_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ, in
       longest = std::max(longest, n);
     }
   steps *= HQ / tile_heads(G);
-  const int64_t even = std::max<int64_t>(4, (steps + 511) / 512);  // of each workgroup at a time
-  if (longest <= even + 6 || longest * 4 <= even * 5) return 0;
-  return -kBK * even;
+  const int64_t one = std::max<int64_t>(4, (steps + 255) / 256);
+  if (longest > one + 6) return -kBK * one;
+  const int64_t two = std::max<int64_t>(4, (steps + 511) / 512);
+  if (longest > two + 24 && longest * 4 > two * 5) return -kBK * two;
+  return 0;
 }
 
 // The same of a call without a list: whole query tiles where rows are many.
