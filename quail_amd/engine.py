@@ -624,8 +624,12 @@ class Engine:
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if qkv.shape[1] < (hq + 2 * hk) * d:
             raise ValueError(f"qkv width {qkv.shape[1]} < {(hq + 2 * hk) * d}")
-        if positions.shape[0] != qkv.shape[0]:
-            raise ValueError(f"{positions.shape[0]} positions for {qkv.shape[0]} rows")
+        if positions.shape != (qkv.shape[0],) or positions.dtype != torch.int64 or \
+                not positions.is_contiguous():
+            raise ValueError(f"positions: {qkv.shape[0]} contiguous int64, not "
+                             f"{tuple(positions.shape)} {positions.dtype}")
+        if qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1:
+            raise ValueError(f"qkv rows are contiguous bf16, not {qkv.dtype}")
         cache = self._rope_cache()
         for items in phases:
             self._check_items(items)
