@@ -233,7 +233,8 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
         # the scatter source is the pack's rows in order: row i's KV goes to
         # dst[i], which lets qk_norm_rope write it in place
         rows_in_order=bool(src.size == n_tok and np.array_equal(src, np.arange(n_tok))))
-    if getattr(arena, "eight_bit", False):
+    eight_bit = getattr(arena, "eight_bit", False)
+    if eight_bit:
         unified["page_writes"] = page_writes(src, dst, unified["tail_src"], unified["tail_dst"])
     meta = dict(layer=0, unified=unified, cu_a=cu_a,
                 max_a=int(np.diff(cu_a).max()) if len(cu_a) > 1 else 0,
@@ -241,9 +242,9 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
     if attention_heads is not None:
         for tables in (unified, meta["final_query"]):
             if tables is not None:
-                tables["work"], tables["n_work"], tables["work_rows"] = _work_list(
-                    tables, attention_heads, choose_rows=True,
-                    eight_bit=getattr(arena, "eight_bit", False))
+                tables["work"], tables["n_work"], tables["work_rows"] = (
+                    _work_list8(tables, attention_heads) if eight_bit else
+                    _work_list(tables, attention_heads, choose_rows=True))
     if timing is not None:
         timing["pack_py"] = timing.get("pack_py", 0.0) + (t1 - t0)
         timing["pack_unified"] = timing.get("pack_unified", 0.0) + (time.perf_counter() - t1)
@@ -462,20 +463,21 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
     segments = dict(cu_q=cu_a_arr, used=np.diff(cu_a_arr).astype(np.int32),
                     max_q=int(np.diff(cu_a_arr).max()) if len(cu_a) > 1 else 0, causal=True)
     segments["max_used"] = segments["max_q"]
+    eight_bit = getattr(arena, "eight_bit", False)
     if attention_heads is not None:
         for tables in (segments, reads, reads and reads.get("nodes")):
             if tables:
                 # call B alone reads the arena's pages
-                tables["work"], tables["n_work"], tables["work_rows"] = _work_list(
-                    tables, attention_heads, choose_rows=True,
-                    eight_bit=tables is reads and getattr(arena, "eight_bit", False))
+                tables["work"], tables["n_work"], tables["work_rows"] = (
+                    _work_list8(tables, attention_heads) if eight_bit and tables is reads else
+                    _work_list(tables, attention_heads, choose_rows=True))
     ids = _cat(id_parts)
     positions = _cat(pos_parts)
     final = _cat(finals)
     meta = dict(layer=0, unified=None, kv_src=kv_src, kv_dst=kv_dst, row_pool_dst=row_pool_dst,
                 reads=reads,
                 segments=segments, cu_a=cu_a_arr, max_a=segments["max_q"])
-    if getattr(arena, "eight_bit", False):
+    if eight_bit:
         meta["page_writes"] = () if kv_src is None else page_writes(kv_src, kv_dst)
     if timing is not None:
         timing["pack_py"] = timing.get("pack_py", 0.0) + (t1 - t0)
@@ -487,7 +489,7 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
                  host_ids=ids, host_positions=positions)
 
 
-def _work_list(tables, heads, choose_rows=False, eight_bit=False):
+def _work_list(tables, heads, choose_rows=False):
     """(work pairs, count, query rows per item) of a paged call over `tables`
     (host arrays). choose_rows: the tile height qx_paged_attention_tile_rows
     picks for these sequences (the call must then pass it); otherwise the
@@ -500,18 +502,6 @@ def _work_list(tables, heads, choose_rows=False, eight_bit=False):
     seqs = len(used)
     causal = int(tables.get("causal", True))
     rows = 0
-    if eight_bit:
-        found = ctypes.c_int64()
-        _lib.call("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data, seqs, hq, hk,
-                  causal, ctypes.byref(found))
-        unit = found.value
-        tiles = 1 if unit > 0 else -(-np.diff(cu_q) // 32)
-        parts = 1 if not unit else np.maximum(-(-used // abs(unit)), 1)
-        cap = int((np.ones(seqs, dtype=np.int64) * tiles * parts).sum())
-        work = np.zeros(2 * max(cap, 1), dtype=np.int32)
-        n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
-                       hk, causal, unit, work.ctypes.data, cap)
-        return work[:2 * n], n, unit
     if choose_rows:
         rows = _lib.count("qx_paged_attention_tile_rows", cu_q.ctypes.data, used.ctypes.data,
                           seqs, hq, hk, d, causal)
@@ -520,6 +510,28 @@ def _work_list(tables, heads, choose_rows=False, eight_bit=False):
     n = _lib.count("qx_paged_attention_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq, hk,
                    d, causal, rows, work.ctypes.data, cap)
     return work[:2 * n], n, rows
+
+
+def _work_list8(tables, heads):
+    """The same of a call over an 8-bit arena's pages; the third value is
+    qx_paged_attention8_unit's."""
+    from quail_amd import _lib
+    hq, hk, _ = heads
+    cu_q = np.ascontiguousarray(tables["cu_q"], dtype=np.int32)
+    used = np.ascontiguousarray(tables["used"], dtype=np.int32)
+    seqs = len(used)
+    causal = int(tables.get("causal", True))
+    found = ctypes.c_int64()
+    _lib.call("qx_paged_attention8_unit", cu_q.ctypes.data, used.ctypes.data, seqs, hq, hk,
+              causal, ctypes.byref(found))
+    unit = found.value
+    tiles = 1 if unit > 0 else -(-np.diff(cu_q) // 32)
+    parts = 1 if not unit else np.maximum(-(-used // abs(unit)), 1)
+    cap = int((np.ones(seqs, dtype=np.int64) * tiles * parts).sum())
+    work = np.zeros(2 * max(cap, 1), dtype=np.int32)
+    n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq, hk,
+                   causal, unit, work.ctypes.data, cap)
+    return work[:2 * n], n, unit
 
 
 def _final_query(cu_q, used, table, final):
@@ -613,7 +625,8 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
     tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),
                   max_used=int(host["used"].max(initial=0)))
-    work, n_work, rows = _work_list(host, heads, choose_rows=True, eight_bit=eight_bit)
+    work, n_work, rows = (_work_list8(host, heads) if eight_bit else
+                          _work_list(host, heads, choose_rows=True))
     if n_work:
         import torch
         tables.update(work=torch.from_numpy(work).to(cu_q.device), n_work=n_work, work_rows=rows)
