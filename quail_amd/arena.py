@@ -87,6 +87,9 @@ class KVArena:
         if self.eight_bit:
             self.scales = torch.full((self.num_layers, num_pages, heads, 2), 127,
                                      dtype=torch.uint8, device=self.device)
+            self._layer_scales = list(self.scales.unbind(0))
+            self._pointers = [(k.data_ptr(), v.data_ptr(), s.data_ptr())
+                              for k, v, s in zip(self.k, self.v, self._layer_scales)]
         self._claims = {}
 
     @property
@@ -398,7 +401,11 @@ class KVArena:
     def layer_scales(self, layer: int):
         """The E8M0 bytes of one layer of an 8-bit arena: (num_pages,
         num_kv_heads, 2), K's and V's."""
-        return self.scales[layer]
+        return self._layer_scales[layer]
+
+    def layer_pointers(self, layer: int):
+        """The addresses of a layer's K codes, V codes and scales (8 bits)."""
+        return self._pointers[layer]
 
     def paged_kv(self, layer: int):
         heads, dim = self.kv_shape

@@ -24,6 +24,7 @@ import torch
 from quail_amd import _lib
 
 GROUP = 128
+PAGE_ROWS = 16   # tokens per page of an 8-bit arena
 
 # GEMM tile configurations (csrc/gemm_fp8.hip), in two arithmetic families.
 # Promotion family (30, 31): each 128-K block's products summed from zero by
@@ -613,11 +614,6 @@ class Engine:
     def _eight_bit(self):
         return getattr(self.arena, "eight_bit", False)
 
-    def _pools8(self, layer):
-        """The pointers of a layer's K codes, V codes and scales."""
-        k_pool, v_pool = self.arena.layer_kv(layer)
-        return _ptr(k_pool), _ptr(v_pool), _ptr(self.arena.layer_scales(layer))
-
     def _write_pages(self, qkv, positions, attn, phases, layer, q=None):
         """K (normed and rotated) and V of the page items' qkv rows into an
         8-bit arena's pages, phase by phase, and their rows of q into `q`."""
@@ -633,11 +629,12 @@ class Engine:
         cache = self._rope_cache()
         for items in phases:
             self._check_items(items)
-            _lib.call("qx_qk_norm_rope_kv8", _ptr(qkv), qkv.stride(0), _ptr(q),
-                      0 if q is None else q.stride(0), *self._pools8(layer), _ptr(items),
-                      items.shape[0], _ptr(cache), int(cache.dtype == torch.float32),
-                      _ptr(positions), _ptr(attn.q_norm.weight), _ptr(attn.k_norm.weight), hq, hk,
-                      d, float(attn.q_norm.variance_epsilon), _stream())
+            _lib.call("qx_qk_norm_rope_kv8", qkv.data_ptr(), qkv.stride(0), _ptr(q),
+                      0 if q is None else q.stride(0), *self.arena.layer_pointers(layer),
+                      items.data_ptr(), items.shape[0], cache.data_ptr(),
+                      int(cache.dtype == torch.float32), positions.data_ptr(),
+                      attn.q_norm.weight.data_ptr(), attn.k_norm.weight.data_ptr(), hq, hk, d,
+                      float(attn.q_norm.variance_epsilon), _stream())
 
     def _write_page_rows(self, k3, v3, phases, layer):
         """The same from K and V rows as they are (bf16)."""
@@ -647,7 +644,7 @@ class Engine:
         for items in phases:
             self._check_items(items)
             _lib.call("qx_kv8_write", _ptr(k3), k3.stride(0), _ptr(v3), v3.stride(0),
-                      *self._pools8(layer), _ptr(items), items.shape[0], self.num_kv_heads,
+                      *self.arena.layer_pointers(layer), _ptr(items), items.shape[0], self.num_kv_heads,
                       self.head_dim, _stream())
 
     @staticmethod
@@ -859,24 +856,26 @@ class Engine:
         log-sum-exp into `lse`."""
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         n = q3.shape[0] if q_index is None else q_index.shape[0]
-        table, seqs = tables["table"], tables["used"].shape[0]
-        max_q, max_used = int(tables["max_q"]), int(tables["max_used"])
+        table, used = tables["table"], tables["used"]
+        seqs, max_q, max_used = used.shape[0], int(tables["max_q"]), int(tables["max_used"])
         # the call's items and their keys, when the plan or pack carries them
-        work = tables.get("work")
-        if not torch.is_tensor(work):
+        work, n_work, unit = tables.get("work"), 0, 0
+        if torch.is_tensor(work):
+            n_work, unit = int(tables["n_work"]), int(tables["work_rows"])
+        else:
             work = None
-        n_work = int(tables.get("n_work", 0)) if work is not None else 0
-        unit = int(tables.get("work_rows", 0)) if work is not None else 0
         size = _attention8_workspace(seqs, n, max_q, max_used, hq, hk, d, int(work is not None),
                                      unit)
         space = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
-        o8, s8 = (None, None) if quant is None else quant
-        o = out if quant is None else o8
-        _lib.call("qx_paged_attention8", _ptr(q3), q3.stride(0), _ptr(q_index),
-                  *self._pools8(layer), _ptr(tables["cu_q"]), _ptr(tables["used"]), _ptr(table),
-                  table.stride(0), seqs, n, max_q, max_used, hq, hk, d, self.arena.page_tokens,
-                  float(scale), int(tables.get("causal", True)), _ptr(out), _ptr(o8), o.stride(0),
-                  _ptr(s8), 0 if s8 is None else self._scale_ld(s8), _ptr(lse),
+        if quant is None:
+            to = out.data_ptr(), None, out.stride(0), None, 0
+        else:
+            o8, s8 = quant
+            to = None, o8.data_ptr(), o8.stride(0), s8.data_ptr(), self._scale_ld(s8)
+        _lib.call("qx_paged_attention8", q3.data_ptr(), q3.stride(0), _ptr(q_index),
+                  *self.arena.layer_pointers(layer), tables["cu_q"].data_ptr(), used.data_ptr(),
+                  table.data_ptr(), table.stride(0), seqs, n, max_q, max_used, hq, hk, d,
+                  PAGE_ROWS, scale, int(tables.get("causal", True)), *to, _ptr(lse),
                   0 if lse is None else lse.stride(0), _ptr(work), n_work, unit, _ptr(space), size,
                   _stream())
 
@@ -895,7 +894,7 @@ class Engine:
         rows = int(tables["cu_q"].shape[0]) - 1
         if rows != tables["used"].shape[0]:
             raise ValueError(f"{rows} query ranges for {tables['used'].shape[0]} sequences")
-        scale = d ** -0.5 if softmax_scale is None else softmax_scale
+        scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
         out = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
         lse = torch.empty((hq, n), dtype=torch.float32, device=q3.device)
         if not n:
@@ -905,8 +904,7 @@ class Engine:
         else:
             k_pool, v_pool = self.arena.layer_kv(layer)
             self._check_pools(k_pool, v_pool)
-            self._lse_call(q3, None, k_pool, v_pool, tables, tables["table"], None, float(scale),
-                           out, lse)
+            self._lse_call(q3, None, k_pool, v_pool, tables, tables["table"], None, scale, out, lse)
         return out, lse
 
     def attention_unified(self, q3, k3, v3, meta, *, softmax_scale=None, output=None):
