@@ -68,6 +68,9 @@ def parse():
     p.add_argument("--v-dtype", choices=("fp16", "bf16"), default="fp16",
                    help="type of the arena's V pages: fp16 (this engine's arena) or bf16 "
                         "(the reference KVArena's layout)")
+    p.add_argument("--kv-bits", type=int, choices=(16, 8), default=16,
+                   help="bits of the arena's K and V: 16, or 8 (e4m3 codes with a scale per "
+                        "page and KV head)")
     p.add_argument("--cpu-seconds", type=float, default=15.0,
                    help="target wall time of the CPU baseline sample (0 skips it)")
     p.add_argument("--copy-mib", type=int, default=0,
@@ -467,8 +470,8 @@ def main():
         retain_answer_head(model, wl.label_ids[:2])
     num_pages = 3 * wl.chunk_budget // wl.page_tokens + 64
     v_dtype = torch.bfloat16 if args.v_dtype == "bf16" else torch.float16
-    arena = KVArena(cfg.layers, num_pages, wl.page_tokens, cfg.kv_heads, cfg.head_dim,
-                    v_dtype=v_dtype)
+    pages = dict(dtype=torch.float8_e4m3fn) if args.kv_bits == 8 else dict(v_dtype=v_dtype)
+    arena = KVArena(cfg.layers, num_pages, wl.page_tokens, cfg.kv_heads, cfg.head_dim, **pages)
     pipe = Qwen3Pipeline(model, arena)
     # the stage's AI function: AI.IF bits, AI.SCORE values, or the
     # AI.CLASSIFY label logits at each document's last row
@@ -607,7 +610,7 @@ def main():
             "workload": describe(wl, cfg, args.attention),
             "documents": docs, "fresh_tokens": fresh, "packs": stats[0]["chunks"],
             "borrowed_tokens": stats[0]["borrowed_tokens"], "attention_pairs": pairs,
-            "parallelism": "none (1 GPU)", "v_pages": args.v_dtype,
+            "parallelism": "none (1 GPU)", "v_pages": "e4m3" if args.kv_bits == 8 else args.v_dtype,
         },
         "prefill_tok_s": round(tok_s, 1),
         "e2e_roofline_frac": round(e2e_frac, 4),

@@ -442,6 +442,8 @@ max_used bound the sequences' rows and keys.
  * its keys [i * unit, (i + 1) * unit)), else items are (sequence, query tile |
  * i << 16), whole tiles (0) or their keys in splits of -unit; a second launch
  * joins the splits. _work returns the items' number (<= capacity) or -1.
+ * positions (may be NULL; D == 128, no q_index): q is the qkv projection's, and
+ * is normed and rotated as it is loaded, as in qx_paged_attention_qnorm.
  * workspace: qx_paged_attention8_workspace bytes of the caller's (has_work:
  * whether the call gets a list), 16-byte aligned (NULL where that is 0), used
  * by this call alone until the stream has passed it.
@@ -461,7 +463,8 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
                         int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
                         int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
                         const int* work, int64_t n_work, int64_t unit, void* workspace,
-                        int64_t workspace_bytes, hipStream_t stream);
+                        int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
+                        int cs_is_f32, const void* q_w, float eps, hipStream_t stream);
 
 /*
  * Replaces Engine.merge_attn_quant / the merge_attn_quant Triton kernel

@@ -55,7 +55,7 @@ SIGNATURES = {
     "qx_paged_attention8_unit": [_p, _p, _i64, _i64, _i64, _i32, _p],
     "qx_paged_attention8": [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                             _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _i64, _p, _i64, _p, _i64,
-                            _p, _i64, _i64, _p, _i64, _p],
+                            _p, _i64, _i64, _p, _i64, _p, _p, _i32, _p, _f32, _p],
     "qx_paged_attention8_work": [_p, _p, _i64, _i64, _i64, _i32, _i64, _p, _i64],
     "qx_copy_pages": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p],
     "qx_pages_compact": [_p, _p, _p, _i64, _p],

@@ -17,6 +17,7 @@
 #include <utility>
 #include <vector>
 
+#include "q_norm.h"
 #include "qx_common.h"
 #include "qx_status.h"
 
@@ -110,6 +111,58 @@ __device__ __forceinline__ void store_row(const Attn8Args& p, int64_t row, int h
                  pack2_bf16(y[6], y[7]));
 }
 
+// q-norm and RoPE of one column of the few-row kernel: the lanes of a group g4
+// hold the row's columns (k / 2) * 64 + g4 * 16 + (k & 1) * 8 .. + 8, so that
+// the rotation's pairs, 64 apart, are the lane's own chunks k and k + 2.
+template <int QN>
+__device__ __forceinline__ void q_norm_columns(v8bf (&qf)[4], const QNormArgs& qn, int64_t pos,
+                                               int g4) {
+  float x[4][8], ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[k][e] = (float)qf[k][e];
+      ss += x[k][e] * x[k][e];
+    }
+  ss += __shfl_xor(ss, 16, 64);
+  ss += __shfl_xor(ss, 32, 64);
+  const float rstd = norm_rstd<128>(ss, qn.eps);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = g4 * 16 + k * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float a[4], b[4], wa[4], wb[4], cosv[4], sinv[4], oa[4], ob[4];
+      bf16x4_to_f32(*reinterpret_cast<const uint2*>(qn.qw + c + 4 * h), wa);
+      bf16x4_to_f32(*reinterpret_cast<const uint2*>(qn.qw + 64 + c + 4 * h), wb);
+      if constexpr (QN == 2) {
+        const float* cs = reinterpret_cast<const float*>(qn.cs) + pos * 128 + c + 4 * h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          cosv[e] = cs[e];
+          sinv[e] = cs[64 + e];
+        }
+      } else {
+        const uint16_t* cs = reinterpret_cast<const uint16_t*>(qn.cs) + pos * 128 + c + 4 * h;
+        bf16x4_to_f32(*reinterpret_cast<const uint2*>(cs), cosv);
+        bf16x4_to_f32(*reinterpret_cast<const uint2*>(cs + 64), sinv);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = x[k][4 * h + e];
+        b[e] = x[k + 2][4 * h + e];
+      }
+      norm_rope4(a, b, wa, wb, cosv, sinv, rstd, oa, ob);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        qf[k][4 * h + e] = (__bf16)oa[e];
+        qf[k + 2][4 * h + e] = (__bf16)ob[e];
+      }
+    }
+  }
+}
+
 // Few query rows over long caches. The workgroup's 16 * NB columns are
 // (row, head of the KV head's group) pairs of one sequence; its 4 waves take
 // turns at steps of 32 keys (two pages) of the split [split * chunk, ...):
@@ -125,9 +178,9 @@ __device__ __forceinline__ void store_row(const Attn8Args& p, int64_t row, int h
 // touches land in different banks.
 constexpr int kRing = 2;
 
-template <int D, int NB>
+template <int D, int NB, int QN = 0>
 __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, const int* work,
-                                                                int seqs) {
+                                                                int seqs, QNormArgs qn) {
   static_assert(kMaxChunk / kPage <= 256, "a page id for each thread");
   constexpr int CH = D / 16;              // 16-byte chunks per code row
   constexpr int NC = D / 32;              // MFMA k-steps over the head dim
@@ -220,6 +273,7 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
     for (int k = 0; k < NC; ++k)
       qf[n][k] = *reinterpret_cast<const v8bf*>(q + (k >> 1) * (D == 128 ? 64 : 0) + g4 * 16 +
                                                 (k & 1) * 8);
+    if constexpr (QN != 0) q_norm_columns<QN>(qf[n], qn, qn.pos[row], g4);
 #pragma unroll
     for (int k = 0; k < NC; ++k) asm volatile("" ::"v"(qf[n][k]));
   }
@@ -426,10 +480,11 @@ constexpr float kLazyLog2 = 8.0f;
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-template <int D, int HPB, int QSUB>
+template <int D, int HPB, int QSUB, int QN = 0>
 __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, const int* work,
-                                                                 int zgroups, int seqs) {
-  static_assert(HPB * QSUB == 4, "four waves");
+                                                                 int zgroups, int seqs,
+                                                                 QNormArgs qn) {
+  static_assert(HPB * QSUB == 4 && (QN == 0 || D == 128), "four waves; q-norm at D = 128");
   constexpr int BQ = 32 * QSUB;
   constexpr int NC = D / 16;       // MFMA k-steps of S
   constexpr int NDS = D / 32;      // 32-row d tiles of O^T
@@ -491,10 +546,13 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   // another does not
   const int cut = p.causal ? max(0, min(used, off + qt * BQ + 1) - k0) / kBK : INT32_MAX;
 
+  int64_t q_pos = 0;  // of this lane's row, for its cos and sin
+  if constexpr (QN != 0) q_pos = qn.pos[q0 + (r_ok ? r : q_len - 1)];
   if (tid < npages) pages[tid] = page;
   for (int i = tid + 256; i < npages; i += 256) pages[i] = trow[k0 / kPage + i];
   if (tid == 0) nans = 0;
-  __syncthreads();
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): q_pos may be on its way still
+  lds_barrier();
 
   const int64_t kv_row = (int64_t)p.HK * D;
   const uint8_t* kbase = p.kp + kvh * D;
@@ -718,10 +776,12 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   int checked = cut;  // the first tile whose NaN codes were left out
   if (ntiles > 0) {
     uint4 k1[LOADS];
+    QNormIn<QN == 0 ? 1 : QN> qin;
     load(0, kbase, kreg);
     load(0, vbase, vreg);
     if (ntiles > 1) load(1, kbase, k1);
-    for (int i = tid; i < npages; i += 256) bytes[i] = p.scales[(int64_t)pages[i] * p.HK + kvh];
+    uint16_t pair = 0;
+    if (tid < npages) pair = p.scales[(int64_t)page * p.HK + kvh];
     {
       const int rr = r_ok ? r : q_len - 1;
       const int64_t row = p.q_index ? p.q_index[q0 + rr] : (int64_t)(q0 + rr);
@@ -729,13 +789,29 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 #pragma unroll
       for (int c = 0; c < NC; ++c) qf[c] = *reinterpret_cast<const v8bf*>(q + c * 16 + half * 8);
     }
-    __syncthreads();
+    if constexpr (QN != 0) {
+      q_norm_load_weights(qin, qn, half);
+      q_norm_load_row(qin, qn, q_pos, half);
+    }
+    if (tid < npages) bytes[tid] = pair;
+    for (int i = tid + 256; i < npages; i += 256)
+      bytes[i] = p.scales[(int64_t)pages[i] * p.HK + kvh];
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    lds_barrier();
     store_all(0, &k_lds[0][0], kreg, false);
     store_all(0, &v_lds[0][0], vreg, true);
     if (ntiles > 1) {
       store_all(1, &k_lds[1][0], k1, false);
       load(1, vbase, vreg);
       if (ntiles > 2) load(2, kbase, kreg);
+    }
+    if constexpr (QN != 0) {
+      v8s raw[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) raw[c] = __builtin_bit_cast(v8s, qf[c]);
+      q_norm_rope_apply(raw, qin, qn.eps);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) qf[c] = __builtin_bit_cast(v8bf, raw[c]);
     }
     step_end();
 #pragma unroll
@@ -980,17 +1056,19 @@ void merge_launch(const Attn8Args& a, int64_t seqs, int64_t max_q, hipStream_t s
                        stream, a);
 }
 
-template <int D>
-void tile_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t seqs, int64_t max_q,
-                 hipStream_t stream) {
+// q as the call has it: normed (QN 0), or the projection's with a bf16 (1) or
+// fp32 (2) cos/sin cache
+template <int D, int QN>
+void tile_launch(const Attn8Args& a, const QNormArgs& qn, const int* work, int64_t n_work,
+                 int64_t seqs, int64_t max_q, hipStream_t stream) {
   const int G = a.HQ / a.HK, hpb = tile_heads(G), rows = tile_height(G);
   const int zgroups = a.HQ / hpb;
   const dim3 grid = work ? dim3((unsigned)(n_work * zgroups))
                          : dim3((unsigned)((max_q + rows - 1) / rows), (unsigned)seqs,
                                 (unsigned)zgroups);
 #define QX_TILE(H, Q)                                                                          \
-  hipLaunchKernelGGL((attention8_tile_kernel<D, H, Q>), grid, dim3(256), 0, stream, a, work,   \
-                     zgroups, (int)seqs)
+  hipLaunchKernelGGL((attention8_tile_kernel<D, H, Q, QN>), grid, dim3(256), 0, stream, a,     \
+                     work, zgroups, (int)seqs, qn)
   if (hpb == 4) QX_TILE(4, 1);
   else if (hpb == 2) QX_TILE(2, 2);
   else QX_TILE(1, 4);
@@ -998,16 +1076,27 @@ void tile_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t se
   merge_launch<D>(a, seqs, max_q, stream);
 }
 
-template <int D, int NB>
-void few_launch(const Attn8Args& a, const int* work, int64_t n_work, int64_t seqs, int64_t max_q,
-                hipStream_t stream) {
-  const int G = a.HQ / a.HK;
-  const int64_t groups = (max_q * G + 16 * NB - 1) / (16 * NB);
+template <int D, int QN>
+void few_launch(const Attn8Args& a, const QNormArgs& qn, const int* work, int64_t n_work,
+                int64_t seqs, int64_t max_q, hipStream_t stream) {
+  const int G = a.HQ / a.HK, cols = 16 * few_blocks(max_q, G);
+  const int64_t groups = (max_q * G + cols - 1) / cols;
   const dim3 grid(work ? (unsigned)n_work : (unsigned)a.splits, (unsigned)(a.HK * groups),
                   work ? 1u : (unsigned)seqs);
-  hipLaunchKernelGGL((attention8_few_kernel<D, NB>), grid, dim3(256), 0, stream, a, work,
-                     (int)seqs);
+  if (cols == 16)
+    hipLaunchKernelGGL((attention8_few_kernel<D, 1, QN>), grid, dim3(256), 0, stream, a, work,
+                       (int)seqs, qn);
+  else
+    hipLaunchKernelGGL((attention8_few_kernel<D, 2, QN>), grid, dim3(256), 0, stream, a, work,
+                       (int)seqs, qn);
   merge_launch<D>(a, seqs, max_q, stream);
+}
+
+template <int D, int QN>
+void attention8_launch(const Attn8Args& a, const QNormArgs& qn, const int* work, int64_t n_work,
+                       int64_t seqs, int64_t max_q, hipStream_t stream) {
+  if (a.tile_rows) tile_launch<D, QN>(a, qn, work, n_work, seqs, max_q, stream);
+  else few_launch<D, QN>(a, qn, work, n_work, seqs, max_q, stream);
 }
 
 // What a call's work items are: keys per split of the few-row kernel (> 0),
@@ -1129,7 +1218,8 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
                         int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
                         int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
                         const int* work, int64_t n_work, int64_t unit, void* workspace,
-                        int64_t workspace_bytes, hipStream_t stream) {
+                        int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
+                        int cs_is_f32, const void* q_w, float eps, hipStream_t stream) {
   QX_CHECK(q && k_pool && v_pool && scales && cu_q && used && table, "attention8: null pointer");
   QX_CHECK((out_bf16 != nullptr) != (out_fp8 != nullptr), "attention8: one output, bf16 or e4m3");
   QX_CHECK(D == 64 || D == 128, "attention8: head_dim %lld", (long long)D);
@@ -1145,6 +1235,9 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   QX_CHECK((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out_bf16) & 15) == 0 &&
                ((uintptr_t)out_fp8 & 7) == 0 && ((uintptr_t)scales & 1) == 0,
            "attention8: alignment");
+  QX_CHECK(!positions || (D == 128 && cos_sin && q_w && !q_index &&
+                          (((uintptr_t)cos_sin | (uintptr_t)q_w) & 15) == 0),
+           "attention8: q-norm on load takes D = 128, cos_sin and q_w, and no q_index");
   QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
   QX_CHECK(!work || (n_work >= 0 && n_work * HQ < (1LL << 24)), "attention8: work items");
   QX_CHECK((work || !unit) && (unit <= 0 ? unit % kBK == 0 && unit >= -kMaxKeys
@@ -1171,16 +1264,11 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   a.rows = rows;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + (int64_t)a.splits * rows * HQ * D;
-  if (unit <= 0) {
-    if (D == 128) tile_launch<128>(a, work, n_work, seqs, max_q, stream);
-    else tile_launch<64>(a, work, n_work, seqs, max_q, stream);
-  } else if (D == 128) {
-    if (nb == 1) few_launch<128, 1>(a, work, n_work, seqs, max_q, stream);
-    else few_launch<128, 2>(a, work, n_work, seqs, max_q, stream);
-  } else {
-    if (nb == 1) few_launch<64, 1>(a, work, n_work, seqs, max_q, stream);
-    else few_launch<64, 2>(a, work, n_work, seqs, max_q, stream);
-  }
+  const QNormArgs qn{positions, cos_sin, (const uint16_t*)q_w, eps};
+  if (D == 64) attention8_launch<64, 0>(a, qn, work, n_work, seqs, max_q, stream);
+  else if (!positions) attention8_launch<128, 0>(a, qn, work, n_work, seqs, max_q, stream);
+  else if (!cs_is_f32) attention8_launch<128, 1>(a, qn, work, n_work, seqs, max_q, stream);
+  else attention8_launch<128, 2>(a, qn, work, n_work, seqs, max_q, stream);
   QX_LAUNCH_STATUS();
 }
 

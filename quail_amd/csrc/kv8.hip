@@ -24,9 +24,28 @@ __device__ __forceinline__ int scale_byte(float amax) {
   return max((int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8, 1);
 }
 
-// Infinities count as the largest finite value (e4m3 has none); NaN stays.
-__device__ __forceinline__ float finite(float x) {
-  return x != x ? x : fminf(fmaxf(x, -kF32Max), kF32Max);
+// v of lane ^ 4: within a row of 16 lanes, the banks of four 0 and 2 take the
+// next bank's, 1 and 3 the one's before
+__device__ __forceinline__ float xor4(float v) {
+  const int x = __float_as_int(v);
+  const int a = __builtin_amdgcn_update_dpp(x, x, 0x104, 0xf, 0x5, false);  // row_shl:4
+  return __int_as_float(__builtin_amdgcn_update_dpp(a, x, 0x114, 0xf, 0xa, false));  // row_shr:4
+}
+
+// group_sum<width>'s sums in its order (width 8 or 4), on vector operands
+// instead of LDS permutes
+template <int width>
+__device__ __forceinline__ float row_sum(float v) {
+  if (width == 8) v += xor4(v);
+  v += dpp_f32<0x4e>(v);  // lane ^ 2
+  return v + dpp_f32<0xb1>(v);  // lane ^ 1
+}
+
+// the maximum over the wave, likewise
+__device__ __forceinline__ float wave_max(float v) {
+  v = group_max<16>(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
 // e4m3 codes of 8 values times 2^shift
@@ -63,8 +82,10 @@ __device__ __forceinline__ uint4 load_once(const uint16_t* p) {
 // that every load is 16 bytes wide), D / 16 lanes a row, and the wave a
 // head's 16 rows in registers between their maximum and their codes; the
 // next head's rows load meanwhile, and a row's cos and sin serve every head.
-// A pack of 15,654 rows (32 + 8 + 8 heads of 128, 353 MB) 78 us, 4.55 TB/s
-// (a large copy on the same card: 4.8); one token each for 8 sequences 5 us.
+// Sums and maxima over lanes run on vector operands (through LDS permutes
+// they took 8% of a pack's write). A pack of 15,654 rows (32 + 8 + 8 heads of
+// 128, 353 MB) 71 us, 4.9 TB/s (a large copy on the same card: 4.8); one token
+// each for 8 sequences 4.6 us.
 struct WriteArgs {
   const uint16_t *x, *v;  // qkv rows, or K rows and V rows
   int64_t x_ld, v_ld;
@@ -172,7 +193,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs p) {
         // the qk-norm-rope pass's tree over 4-column groups: its last level
         // pairs the lane's own two
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s[e] = group_sum<LPR>(norm_part4(a[e], b[e]));
+        for (int e = 0; e < 2; ++e) s[e] = row_sum<LPR>(norm_part4(a[e], b[e]));
         const float rstd = norm_rstd<D>(s[0] + s[1], p.eps);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -211,14 +232,19 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs p) {
         }
       } else if (fresh[t]) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          y[t][k] = finite(y[t][k]);
-          amax = fmaxf(amax, fabsf(y[t][k]));
-        }
+        for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(y[t][k]));
       }
     }
     if (!q) {
-      amax = group_max<64>(amax);
+      amax = wave_max(amax);
+      if (amax > kF32Max) {  // an infinity counts as the largest float (e4m3 has none); NaN stays
+        amax = kF32Max;
+#pragma unroll
+        for (int t = 0; t < PASSES; ++t)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            y[t][k] = y[t][k] != y[t][k] ? y[t][k] : fminf(fmaxf(y[t][k], -kF32Max), kF32Max);
+      }
       const int need = scale_byte(amax);
       const int b = keep > 0 ? max(b_old, need) : need;
       const bool move = src != dst || b != b_old;  // the kept rows change
@@ -267,9 +293,10 @@ int kv8_write_launch(WriteArgs& a, bool qkv, int64_t n_items, int64_t HK, int64_
   QX_CHECK(HK > 0 && n_items >= 0, "kv8_write: heads %lld, items %lld", (long long)HK,
            (long long)n_items);
   if (n_items == 0) return QX_OK;
-  // a wave takes 4 heads of an item where the items are many (1: 86.0 us for
-  // the pack above, 2: 80.9, 4: 79.7, 8: 82.4), else one (a few tokens: latency)
-  a.heads = n_items * a.slots > 8192 ? 4 : 1;
+  // heads per wave: as many as leave 6144 waves (the card holds 3072 of these
+  // at once). The pack above, with q (48 slots) 1: 79.2 us, 2: 72.9, 4: 71.3;
+  // its K and V alone (16 slots) 31.1, 28.5, 30.8
+  for (a.heads = 4; a.heads > 1 && n_items * a.slots / a.heads < 6144;) a.heads /= 2;
   a.groups = (a.slots + a.heads - 1) / a.heads;
   a.waves = n_items * a.groups;
   QX_CHECK(a.waves <= (1LL << 26) - 4, "kv8_write: %lld items of %d heads exceed one launch",

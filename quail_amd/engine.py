@@ -573,18 +573,21 @@ class Engine:
         projection left it; this layer's paged attention then normalizes and
         rotates q as it loads it (qx_paged_attention_qnorm), with the same
         arithmetic (bit for bit). Returns the raw q columns of qkv (a view).
-        The attention of an 8-bit arena takes q normed and rotated: there
-        this is qk_norm_rope_kv."""
-        if self._eight_bit():
-            return self.qk_norm_rope_kv(qkv, positions, attn, meta)
+        An 8-bit arena's pages are written by their page items, as
+        qk_norm_rope_kv does."""
         n = qkv.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if d != GROUP or qkv.shape[1] < (hq + 2 * hk) * d:
             raise ValueError(f"kv_norm_rope: head_dim {d}, qkv width {qkv.shape[1]}")
+        layer = meta["layer"]
+        if self._eight_bit():
+            self._write_pages(qkv, positions, attn, meta["unified"]["page_writes"], layer)
+            meta["kv_fresh_layer"] = layer
+            meta["q_norm_on_load"] = (positions, attn)
+            return qkv[:, :hq * d]
         dst = meta["unified"]["row_dst"]
         if dst.shape[0] != n:
             raise ValueError(f"row_dst has {dst.shape[0]} rows, qkv {n}")
-        layer = meta["layer"]
         k_pool, v_pool = self.arena.layer_kv(layer)
         self._check_pools(k_pool, v_pool)
         cache = self._rope_cache()
@@ -850,10 +853,12 @@ class Engine:
                   lse.stride(0), _ptr(work), n_work, rows, int(v.dtype == torch.bfloat16),
                   _stream())
 
-    def _attend8(self, q3, tables, layer, scale, *, q_index=None, out=None, quant=None, lse=None):
+    def _attend8(self, q3, tables, layer, scale, *, q_index=None, out=None, quant=None, lse=None,
+                 qnorm=None):
         """One qx_paged_attention8 call over `tables`: bf16 rows into `out`, or
         the o_proj input into quant = (e4m3 rows, scales), and each row's
-        log-sum-exp into `lse`."""
+        log-sum-exp into `lse`. qnorm = (positions of q3's rows, attention
+        module): q3 is the projection's, normed and rotated as it is loaded."""
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         n = q3.shape[0] if q_index is None else q_index.shape[0]
         table, used = tables["table"], tables["used"]
@@ -872,12 +877,20 @@ class Engine:
         else:
             o8, s8 = quant
             to = None, o8.data_ptr(), o8.stride(0), s8.data_ptr(), self._scale_ld(s8)
+        norm = None, None, 0, None, 0.0
+        if qnorm is not None:
+            positions, attn = qnorm
+            if positions.shape != (n,) or positions.dtype != torch.int64:
+                raise ValueError(f"{n} rows need as many int64 positions")
+            cache = self._rope_cache()
+            norm = (positions.data_ptr(), cache.data_ptr(), int(cache.dtype == torch.float32),
+                    attn.q_norm.weight.data_ptr(), float(attn.q_norm.variance_epsilon))
         _lib.call("qx_paged_attention8", q3.data_ptr(), q3.stride(0), _ptr(q_index),
                   *self.arena.layer_pointers(layer), tables["cu_q"].data_ptr(), used.data_ptr(),
                   table.data_ptr(), table.stride(0), seqs, n, max_q, max_used, hq, hk, d,
                   PAGE_ROWS, scale, int(tables.get("causal", True)), *to, _ptr(lse),
                   0 if lse is None else lse.stride(0), _ptr(work), n_work, unit, _ptr(space), size,
-                  _stream())
+                  *norm, _stream())
 
     def read_pages(self, q3, tables, layer, *, softmax_scale=None):
         """Attention of q3's rows (n, HQ, D), normed and rotated, over pages
@@ -938,7 +951,8 @@ class Engine:
         packs may borrow it), then attend only for `rows` (the pass's final
         rows) through meta["final_query"], one query per row seeing exactly
         the keys it sees inside its own sequence. Returns the o_proj input of
-        those rows, bit-identical to theirs in the full call."""
+        those rows, bit-identical to theirs in the full call (over an 8-bit
+        arena's pages the few rows' keys are summed in another order)."""
         n = q.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         meta = chunk.meta
@@ -971,10 +985,10 @@ class Engine:
             o_s = self._col_major_scales(n, hq * d, q3.device)
         if self._eight_bit():
             if d == GROUP:
-                self._attend8(q3, tables, layer, scale, quant=(o_q, o_s))
+                self._attend8(q3, tables, layer, float(scale), quant=(o_q, o_s), qnorm=qnorm)
             else:
                 o = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
-                self._attend8(q3, tables, layer, scale, out=o)
+                self._attend8(q3, tables, layer, float(scale), out=o, qnorm=qnorm)
                 self.quant(o, output=(o_q, o_s))
             return o_q, o_s
         k_pool, v_pool = self.arena.layer_kv(layer)

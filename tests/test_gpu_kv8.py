@@ -398,6 +398,44 @@ def test_o_proj_input_is_the_quantized_rows(q_lens, used):
     assert torch.equal(got_s, want_s)
 
 
+@pytest.mark.parametrize("cache_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q_lens,used", [((1, 3, 1), (300, 1500, 7)), ((40, 70, 1), (40, 200, 90)),
+                                         ((12,), (9000,))])
+def test_q_norm_on_load_is_the_pass_then_the_attention(q_lens, used, cache_dtype):
+    """The projection's q, normed and rotated as the attention loads it, gives
+    what the pass's bf16 q gives: bit for bit over query tiles (one sum
+    tree); over few rows the sum of squares adds in another order, so a q may
+    be the next bf16: 2^-7 of a score's products, and of the weights."""
+    g = torch.Generator().manual_seed(21)
+    hq, hk, d = 32, 8, 128
+    arena = engine_arena(1000)
+    fill(arena, g)
+    attn, cache = _Attn(d, g), rope_cache(10000, d, cache_dtype)
+    eng = engine_of(arena, hq, cache)
+    plan, cu_q, u, table = plan_of(arena, hq, q_lens, used, g)
+    n = int(cu_q[-1])
+    qkv = torch.randn(n, 48 * d, generator=g).to(torch.bfloat16).to(DEV)
+    pos = torch.cat([torch.arange(b - a, b) for a, b in zip(q_lens, used)]).clamp(min=0).to(DEV)
+    normed, _ = eng.qk_norm_rope(qkv, pos, attn)
+    want, want_lse = eng.read_pages(normed.view(n, hq, d), plan, 0)
+    got, lse = torch.empty_like(want), torch.empty_like(want_lse)
+    eng._attend8(qkv[:, :hq * d].view(n, hq, d), plan, 0, d ** -0.5, out=got, lse=lse,
+                 qnorm=(pos, attn))
+    if plan["work_rows"] <= 0:
+        assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    else:
+        k, v = arena.layer_kv(0)
+        _, _, size, reach = ref.attend(normed.view(n, hq, d), k, v, arena.layer_scales(0),
+                                       cu_q.tolist(), u.tolist(), table, True)
+        off = 2.0 ** -7 * reach
+        assert bool(((lse - want_lse).abs().t() <= off + 1e-5).all())
+        bound = 2 * (2.0 ** -7 + torch.expm1(2 * off))[..., None] * size
+        assert bool(((got.float() - want.float()).abs().view(n, hq, d) <= bound).all())
+    with pytest.raises(ValueError, match="positions"):
+        eng._attend8(qkv[:, :hq * d].view(n, hq, d), plan, 0, d ** -0.5, out=got, lse=lse,
+                     qnorm=(pos[1:], attn))
+
+
 def test_rows_do_not_depend_on_the_list_or_on_padding_columns():
     """A plan without its list of items, a table of more columns than the
     sequences have pages, query rows that are columns of wider rows: the same

@@ -271,13 +271,13 @@ def test_entry_points_refuse_bad_arguments():
         a = dict(q=16, q_ld=4096, k=16, v=16, s=16, cu=16, used=16, table=16, tld=8, seqs=1, rows=1,
                  mq=1, mu=64, hq=32, hk=8, d=128, page=16, out=16, out8=None, o_ld=4096, os=None,
                  os_ld=0, lse=None, lse_ld=0, work=None, n_work=0, unit=0, ws=None,
-                 wsb=0)
+                 wsb=0, pos=None, cs=16, qw=16)
         a.update(kw)
         _lib.call("qx_paged_attention8", a["q"], a["q_ld"], None, a["k"], a["v"], a["s"], a["cu"],
                   a["used"], a["table"], a["tld"], a["seqs"], a["rows"], a["mq"], a["mu"], a["hq"],
                   a["hk"], a["d"], a["page"], 0.1, 1, a["out"], a["out8"], a["o_ld"], a["os"],
                   a["os_ld"], a["lse"], a["lse_ld"], a["work"], a["n_work"], a["unit"], a["ws"],
-                  a["wsb"], None)
+                  a["wsb"], a["pos"], a["cs"], 0, a["qw"], 1e-6, None)
 
     for kw, match in ((dict(q=None), "null"), (dict(table=None), "null"), (dict(out=None), "output"),
                       (dict(out8=16), "output"), (dict(d=96), "head_dim"), (dict(hk=5), "heads"),
@@ -289,6 +289,8 @@ def test_entry_points_refuse_bad_arguments():
                       (dict(seqs=65536), "grid"), (dict(mu=40000), "workspace"),
                       (dict(mu=40000, ws=16, wsb=100), "workspace"),
                       (dict(work=16, n_work=-1), "work"), (dict(work=16, n_work=1 << 24), "work"),
+                      (dict(pos=16, d=64), "q-norm"),
+                      (dict(pos=16, cs=None), "q-norm"), (dict(pos=16, qw=8), "q-norm"),
                       (dict(unit=128), "items"), (dict(work=16, n_work=1, unit=100), "items"),
                       (dict(work=16, n_work=1, unit=8192), "items"),
                       (dict(work=16, n_work=1, unit=-100), "items"),
