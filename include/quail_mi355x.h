@@ -434,7 +434,7 @@ int qx_attention_lse_tiled(const void* q, int64_t q_ld, const int64_t* q_index, 
  * qx_attention_lse. Exactly one of out_bf16 (rows of o_ld elements) and
  * out_fp8 (D == 128; out_scales[h*os_ld + row]); lse (may be NULL) as in
  * qx_attention_lse; a row that sees no key gets 0 and -inf. max_q and
-max_used bound the sequences' rows and keys.
+ * max_used bound the sequences' rows and keys; scale is positive.
  *
  * work, n_work, unit: the items of the call, or NULL, 0, 0. The host functions
  * qx_paged_attention8_unit and _work make them from host copies of cu_q and

@@ -249,6 +249,9 @@ class KVArena:
         if not self.storage.is_cuda:
             raise ValueError("page copies run on the GPU; this arena is on the CPU")
         from quail_amd.engine import _stream
+        for page in (*src, *dst):
+            if not 0 <= page < self.num_pages:   # also before it is cut to 32 bits
+                raise ValueError(f"page {page} of {self.num_pages}")
         ids = ctypes.c_int32 * max(1, len(src))
         heads, dim = self.kv_shape
         size = self.storage.element_size()
@@ -292,6 +295,8 @@ class KVArena:
         table = acct.table_pages(key)
         if len(shared) != full or len(table) < acct.pages_needed(tokens):
             raise ValueError("the key's leading pages were dropped")
+        if rest and children and not self.storage.is_cuda:
+            raise ValueError("page copies run on the GPU; this arena is on the CPU")
         need = acct.pages_needed(capacity) - full
         if need * len(children) > acct.free_pages:
             return None

@@ -493,8 +493,7 @@ def _work_list(tables, heads, choose_rows=False):
     """(work pairs, count, query rows per item) of a paged call over `tables`
     (host arrays). choose_rows: the tile height qx_paged_attention_tile_rows
     picks for these sequences (the call must then pass it); otherwise the
-    default (0). eight_bit: for a call over an 8-bit arena's pages (the third value
-    is then the keys per item, 0 for query tiles)."""
+    default (0)."""
     from quail_amd import _lib
     hq, hk, d = heads
     cu_q = np.ascontiguousarray(tables["cu_q"], dtype=np.int32)
@@ -623,6 +622,7 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
     if host["used"].max(initial=0) > table.shape[1] * PAGE_ROWS:
         raise ValueError(f"{host['used'].max()} keys in {table.shape[1]} pages")
     tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
+                  made_for=(int(host["cu_q"][-1]), *heads, bool(eight_bit)),
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),
                   max_used=int(host["used"].max(initial=0)))
     work, n_work, rows = (_work_list8(host, heads) if eight_bit else

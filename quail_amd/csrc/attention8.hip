@@ -504,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
     zg = blockIdx.x % zgroups;
     s = work[2 * item];
     qt = work[2 * item + 1] & 0xffff;
-    split = work[2 * item + 1] >> 16;
+    split = work[2 * item + 1] >> 16 & 0x7fff;
   } else {
     s = blockIdx.y;
     qt = gridDim.x - 1 - blockIdx.x;
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   const int page = trow[min(k0 / kPage + tid, last_entry)];
   const int q0 = p.cu_q[sc], q_len = p.cu_q[sc + 1] - q0;
   const int used = min(p.used[sc], p.max_used);
-  if (s < 0 || s >= seqs || split < 0 || (split && split >= p.splits) || qt * BQ >= q_len) return;
+  if (s < 0 || s >= seqs || (split && split >= p.splits) || qt * BQ >= q_len) return;
   const int G = p.HQ / p.HK;
   const int per_kv = G / HPB;
   const int kvh = zg / per_kv;
@@ -1238,6 +1238,7 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   QX_CHECK(!positions || (D == 128 && cos_sin && q_w && !q_index &&
                           (((uintptr_t)cos_sin | (uintptr_t)q_w) & 15) == 0),
            "attention8: q-norm on load takes D = 128, cos_sin and q_w, and no q_index");
+  QX_CHECK(scale > 0.f && scale <= 3.402823466e38f, "attention8: scale %g", (double)scale);
   QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
   QX_CHECK(!work || (n_work >= 0 && n_work * HQ < (1LL << 24)), "attention8: work items");
   QX_CHECK((work || !unit) && (unit <= 0 ? unit % kBK == 0 && unit >= -kMaxKeys
@@ -1245,9 +1246,10 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
            "attention8: work items of %lld keys", (long long)unit);
   if (seqs == 0 || max_q == 0 || rows == 0 || (work && n_work == 0)) return QX_OK;
   const int64_t G = HQ / HK;
-  const int nb = few_blocks(max_q, G);
-  QX_CHECK(HK * ((max_q * G + 16 * nb - 1) / (16 * nb)) < 65536, "attention8: %lld rows a sequence",
-           (long long)max_q);
+  if (!work) unit = call_unit(seqs * max_used, max_q, max_used, HK, G);
+  const int64_t cols = 16 * few_blocks(max_q, G);
+  QX_CHECK(max_q * HQ < (1LL << 31) && (unit <= 0 || HK * ((max_q * G + cols - 1) / cols) < 65536),
+           "attention8: %lld rows a sequence", (long long)max_q);
   const int64_t need =
       qx_paged_attention8_workspace(seqs, rows, max_q, max_used, HQ, HK, D, work != nullptr, unit);
   QX_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
@@ -1257,7 +1259,6 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
               (const uint16_t*)scales, cu_q, used, table, table_ld, (int)max_used, (int)HQ, (int)HK,
               causal, scale * 1.4426950408889634f, (uint16_t*)out_bf16, (uint8_t*)out_fp8, o_ld,
               out_scales, os_ld, lse, lse_ld};
-  if (!work) unit = call_unit(seqs * max_used, max_q, max_used, HK, G);
   a.chunk = (int)(unit < 0 ? -unit : unit);
   a.splits = unit ? (int)std::max<int64_t>(1, (max_used + a.chunk - 1) / a.chunk) : 1;
   a.tile_rows = unit > 0 ? 0 : tile_height(G);

@@ -644,6 +644,8 @@ class Engine:
         for t in (k3, v3):
             if t.dtype != torch.bfloat16:
                 raise ValueError(f"KV rows of {t.dtype}: 8-bit pages are written from bf16 rows")
+            if t.stride(-1) != 1 or (t.dim() == 3 and t.stride(1) != t.shape[2]):
+                raise ValueError("a KV row's heads are contiguous")
         for items in phases:
             self._check_items(items)
             _lib.call("qx_kv8_write", _ptr(k3), k3.stride(0), _ptr(v3), v3.stride(0),
@@ -907,6 +909,10 @@ class Engine:
         rows = int(tables["cu_q"].shape[0]) - 1
         if rows != tables["used"].shape[0]:
             raise ValueError(f"{rows} query ranges for {tables['used'].shape[0]} sequences")
+        made_for = tables.get("made_for")
+        if made_for not in (None, (n, hq, self.num_kv_heads, d, self._eight_bit())):
+            raise ValueError(f"a plan for {made_for} (rows, HQ, HK, D, 8 bits), not "
+                             f"{(n, hq, self.num_kv_heads, d, self._eight_bit())}")
         scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
         out = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
         lse = torch.empty((hq, n), dtype=torch.float32, device=q3.device)

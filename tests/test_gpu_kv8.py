@@ -723,3 +723,41 @@ def test_the_engine_refuses_what_8_bit_pages_do_not_take():
     out, lse = eng.read_pages(q[:0], attention_plan(ints(0), ints(), torch.zeros(
         0, 1, dtype=torch.int32, device=DEV), heads=(32, 8, 128)), 0)
     assert out.shape == (0, 4096) and lse.shape == (32, 0)
+
+
+def test_read_pages_refuses_a_plan_made_for_other_rows_heads_or_pages():
+    from quail_amd.chunk import attention_plan
+    arena = engine_arena(4)
+    eng = engine_of(arena, 32)
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    where = ints(0, 2), ints(20), ints(1, 2).view(1, 2)
+    q = torch.zeros(2, 32, 128, dtype=torch.bfloat16, device=DEV)
+    for rows, heads, eight_bit in ((1, (32, 8, 128), True), (2, (16, 8, 128), True),
+                                   (2, (32, 8, 128), False)):
+        plan = attention_plan(*where, heads=heads, eight_bit=eight_bit)
+        with pytest.raises(ValueError, match="a plan for"):
+            eng.read_pages(q[:rows], plan, 0)
+    with pytest.raises(ValueError, match="of 4"):
+        arena.copy_pages([0], [(1 << 32) + 1])
+    rows = torch.zeros(1, 8, 256, dtype=torch.bfloat16, device=DEV)[:, :, :128]
+    with pytest.raises(ValueError, match="contiguous"):
+        eng._write_page_rows(rows, rows, (torch.zeros(1, 5, dtype=torch.int32, device=DEV),), 0)
+
+
+def test_a_long_sequence_of_many_heads_per_kv_head():
+    """40,000 rows at 16 heads a KV head: more rows than few-row blocks fit
+    in a grid. The last rows against float64; the rest finite."""
+    from quail_amd.chunk import attention_plan
+    hq, hk, d, n = 128, 8, 64, 40000
+    pages = -(-n // PAGE)
+    arena = KVArena(1, pages, PAGE, hk, d, dtype=FP8)
+    g = torch.Generator().manual_seed(31)
+    fill(arena, g)
+    cu_q, used, table = sequences(g, [n], [n], pages)
+    q = torch.randn(n, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    plan = attention_plan(*(torch.from_numpy(a).to(DEV) for a in (cu_q, used, table)),
+                          heads=(hq, hk, d))
+    out, lse = engine_of(arena, hq).read_pages(q, plan, 0)
+    assert bool(torch.isfinite(out).all())
+    last = np.asarray([0, 3], dtype=np.int32)
+    check_rows(out[-3:], lse[:, -3:], q[-3:], arena, last, used, table, True)

@@ -8,7 +8,7 @@ import torch
 from oracle import kv8_ref as ref
 from quail_amd import _lib
 from quail_amd.arena import FP8, KVArena
-from quail_amd.chunk import pack_chunk, page_writes
+from quail_amd.chunk import attention_plan, pack_chunk, page_writes
 from quail_amd.pages import PageArena
 
 PAGE = 16
@@ -334,3 +334,28 @@ def test_entry_points_refuse_bad_arguments():
         with pytest.raises(_lib.QxError, match=match):
             copy(*args, **kw)
     copy([], [])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf")])
+def test_attention_refuses_scales_that_are_not_positive(scale):
+    with pytest.raises(_lib.QxError, match="scale"):
+        _lib.call("qx_paged_attention8", 16, 4096, None, 16, 16, 16, 16, 16, 16, 8, 1, 1, 1, 64, 32, 8,
+                  128, 16, scale, 1, 16, None, 4096, None, 0, None, 0, None, 0, 0, None, 0, None, None,
+                  0, None, 1e-6, None)
+
+
+def test_what_a_cpu_arena_cannot_copy_changes_nothing():
+    arena = KVArena(1, 8, PAGE, 2, 64, dtype=FP8, device="cpu")
+    arena.alloc("doc", 20)
+    with pytest.raises(ValueError, match="CPU"):
+        arena.fork("doc", ["a", "b"])                # the partial page needs a copy
+    assert not arena.is_resident("a") and not arena.is_resident("b") and arena.free_pages == 6
+    for src, dst in (([0], [1 << 32]), ([(1 << 32) + 1], [2]), ([-1], [2])):
+        with pytest.raises(ValueError, match="of 8|CPU"):
+            arena.copy_pages(src, dst)
+
+
+def test_an_attention_plan_names_what_it_was_made_for():
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32)  # noqa: E731
+    plan = attention_plan(ints(0, 1, 3), ints(20, 5), ints(1, 2, 3, 0).view(2, 2), heads=(4, 2, 64))
+    assert plan["made_for"] == (3, 4, 2, 64, True)
