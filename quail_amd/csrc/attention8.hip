@@ -557,9 +557,13 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   const int64_t kv_row = (int64_t)p.HK * D;
   const uint8_t* kbase = p.kp + kvh * D;
   const uint8_t* vbase = p.vp + kvh * D;
-  // 16-byte chunk swizzles of the bf16 rows, as the 16-bit kernel's
+  // A bf16 row in LDS: the first halves of its 16-column blocks, then their
+  // second halves, so that the lanes that store a row, a block each, write
+  // neighbouring 16-byte chunks (with the halves side by side they wrote every
+  // second chunk, and 11% of the kernel's time were bank conflicts); the
+  // chunks are swizzled by the key for the reads.
   auto kswz = [](int key) { return D == 128 ? key & 15 : (key >> 1) & 7; };
-  auto vswz = [](int key) { return D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; };
+  auto vswz = [](int key) { return D == 128 ? (key & 3) << 1 : ((key >> 1) & 1) << 1; };
   // Q^T fragments (B operand): lane holds row `col`, d = c * 16 + half * 8 .. + 8
   v8bf qf[NC];
   // this wave's page of a tile: lane's 16 codes of row j * KPL + lane / CH
@@ -579,16 +583,16 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
       reg[j] = *reinterpret_cast<const uint4*>(base + page * kPage * kv_row + place(t, j));
   };
   // the scale of this wave's page of a tile
-  auto scale_of = [&](int t, bool v) -> float {
-    const int slot = min(t * (kBK / kPage) + wave, npages - 1);
-    const int pair = __builtin_amdgcn_readfirstlane(bytes[slot]);
-    return e8m0(v ? pair >> 8 : pair & 255);
+  auto bytes_of = [&](int t) -> int { return bytes[min(t * (kBK / kPage) + wave, npages - 1)]; };
+  auto scale_of = [&](int pair, bool v) -> float {
+    const int b = __builtin_amdgcn_readfirstlane(pair);
+    return e8m0(v ? b >> 8 : b & 255);
   };
   // where this lane's 16 codes of row row0 + j KPL go, as bf16: st_k ^ 128 j
-  // (st_v) past j KPL rows, and their second half at that ^ 16
+  // (st_v) past j KPL rows, and their second half at that ^ 16 CH
   const int st_row = (wave * kPage + row0) * VROW;
-  const int st_k = st_row + (((2 * chunk) ^ kswz(row0)) * 16);
-  const int st_v = st_row + (((2 * chunk) ^ vswz(row0)) * 16);
+  const int st_k = st_row + ((chunk ^ kswz(row0)) * 16);
+  const int st_v = st_row + ((chunk ^ vswz(row0)) * 16);
   auto store = [&](uint8_t* tile, uint4 reg, int j, int at, float scale, bool v, bool check) {
     uint32_t w[4] = {reg.x, reg.y, reg.z, reg.w};
     if (check) {
@@ -607,10 +611,10 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
     }
     uint8_t* to = tile + j * KPL * VROW + (v ? at : at ^ (128 * j));
     *reinterpret_cast<uint4*>(to) = make_uint4(b[0], b[1], b[2], b[3]);
-    *reinterpret_cast<uint4*>(tile + j * KPL * VROW + ((v ? at : at ^ (128 * j)) ^ 16)) = make_uint4(b[4], b[5], b[6], b[7]);
+    *reinterpret_cast<uint4*>(tile + j * KPL * VROW + ((v ? at : at ^ (128 * j)) ^ (16 * CH))) = make_uint4(b[4], b[5], b[6], b[7]);
   };
   auto store_all = [&](int t, uint8_t* tile, const uint4 (&reg)[LOADS], bool v) {
-    const float scale = scale_of(t, v);
+    const float scale = scale_of(bytes_of(t), v);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) store(tile, reg[j], j, v ? st_v : st_k, scale, v, v && t >= cut);
   };
@@ -619,14 +623,14 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) in_page[j] = (uint32_t)((row0 + j * KPL) * (int)kv_row + chunk * 16);
   // K fragment (A operand of S^T): key `col` (+ 32), d chunk 2c + half, at
-  // k_base ^ 32 c (the swizzle moves chunks within the row)
-  const int k_base = col * VROW + ((half ^ kswz(col)) * 16);
+  // k_base ^ 16 c (the swizzle moves chunks within the row)
+  const int k_base = col * VROW + ((CH * half ^ kswz(col)) * 16);
   // V^T fragment by transposing reads: lane 16 g + x reads 4 halfwords of key
   // 4 * half + x / 4 (+ 8) at column 16 (g & 1) + 4 (x & 3) of a 32-d tile,
-  // d tile d at v_base ^ 64 d
+  // d tile d at v_base ^ 32 d
   const int v_key = 4 * half + ((lane & 15) >> 2);
   const int v_base = v_key * VROW +
-                     (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz(v_key)) * 16) + 8 * (lane & 1);
+                     (((((lane >> 4) & 1) + CH * ((lane & 3) >> 1)) ^ vswz(v_key)) * 16) + 8 * (lane & 1);
 
   v16f o[NDS];
 #pragma unroll
@@ -638,10 +642,10 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   auto read_k = [&](const uint8_t* kl, int kb, int c, v8bf (&f)[2]) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
-      f[ks] = *reinterpret_cast<const v8bf*>(kl + ks * 32 * VROW + (kb ^ (32 * c)));
+      f[ks] = *reinterpret_cast<const v8bf*>(kl + ks * 32 * VROW + (kb ^ (16 * c)));
   };
   auto read_v = [&](const uint8_t* vl, int vb, int kc, int d) -> v8bf {
-    const uint8_t* at = vl + ((kc >> 1) * 32 + (kc & 1) * 16) * VROW + (vb ^ (64 * d));
+    const uint8_t* at = vl + ((kc >> 1) * 32 + (kc & 1) * 16) * VROW + (vb ^ (32 * d));
     const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
     const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * VROW));
     const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -657,26 +661,12 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
       for (int i = 0; i < 16; ++i)
         sacc[ks][i] = ks * 32 + (i >> 2) * 8 + (i & 3) < room ? sacc[ks][i] : -INFINITY;
   };
-  auto rescale = [&](const v16f (&sacc)[2], float& alpha, float& m_use) {
-    float part[4];
+  // the largest of scores 8 g .. 8 g + 8 of a tile
+  auto part_max = [&](const v16f (&sacc)[2], int g) {
+    float m = sacc[g >> 1][(g & 1) * 8];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      part[g] = sacc[g >> 1][(g & 1) * 8];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) part[g] = fmaxf(part[g], sacc[g >> 1][(g & 1) * 8 + i]);
-    }
-    const float tmax = max_halves(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-    const float m_cand = fmaxf(m_run, tmax);
-    const bool move = (m_cand - m_run) * p.scale_log2 > kLazyLog2;
-    alpha = move ? __builtin_amdgcn_exp2f((m_run - m_cand) * p.scale_log2) : 1.0f;
-    m_run = move ? m_cand : m_run;
-    m_use = m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(move)) {
-#pragma unroll
-      for (int d = 0; d < NDS; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
-    }
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, sacc[g >> 1][(g & 1) * 8 + i]);
+    return m;
   };
   auto step_end = [&]() {
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
@@ -685,8 +675,9 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   // Step t: softmax and PV of tile t beside S of tile t + 1. Tiles reach LDS
   // a step before their use: K of tile t + 2 and V of tile t + 1 are stored
   // from the registers that step t - 1 loaded, and the next ones load. The
-  // exponentials run between the S MFMAs, two behind each, the conversions
-  // and stores between the PV MFMAs, in an order that sched_barrier keeps.
+  // new maximum and the exponentials run between the S MFMAs, the conversions
+  // and stores between the PV MFMAs, in an order that sched_barrier keeps (the
+  // maximum before the first MFMA: 1-2% slower).
   // FAST: no row's mask reaches tiles t and t + 1, and tiles up to t + 3 are
   // whole.
   enum { kFast, kNext, kLast };
@@ -701,17 +692,16 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
     constexpr int kAhead = 1;  // chunks of K read before their MFMAs: more were as fast, and took registers
     v8bf kf[NC][2];
     int page_v = 0, page_k = 0;
-    float scale_k = 1.f, scale_v = 1.f;
+    int pair_k = 0, pair_v = 0;
     if (!LAST) {
 #pragma unroll
       for (int c = 0; c < kAhead; ++c) read_k(kl, kb, c, kf[c]);
     }
     if (!FAST) mask_tile(t, s_cur);
-    float alpha, m_use;
-    rescale(s_cur, alpha, m_use);
-    float psum = 0.f;
+    float part[4], alpha = 1.f, m_use = 0.f, psum = 0.f;
+    bool move = false;
     v8bf pf[4], vf[4][NDS];
-    constexpr int PER = 16 / NC;  // scores behind each MFMA
+    constexpr int LEAD = NC / 2;  // MFMAs behind which the new maximum is found
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -724,8 +714,8 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
             page_k = pages[FAST ? (t + 3) * (kBK / kPage) + wave : slot_of(t + 3)];
           }
           if (c == 1 && ks == 1) {
-            scale_v = scale_of(t + 1, true);
-            scale_k = scale_of(t + 2, false);
+            pair_v = bytes_of(t + 1);
+            pair_k = bytes_of(t + 2);
           }
         }
         if (c == NC - 1) {  // V of the first 16 keys
@@ -734,9 +724,30 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
         }
         if (!LAST)
           s_next[ks] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[c][ks], qf[c], c == 0 ? v16f{} : s_next[ks], 0, 0, 0);
+        const int slot = 2 * c + ks;
+        if (slot < LEAD / 2) {
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          const int i = (c * 2 + ks) * PER + u;
+          for (int g = 0; g < 4; ++g)
+            if (g * LEAD / 8 == slot) part[g] = part_max(s_cur, g);
+        }
+        if (slot == LEAD / 2) {
+          const float tmax = max_halves(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+          const float m_cand = fmaxf(m_run, tmax);
+          move = (m_cand - m_run) * p.scale_log2 > kLazyLog2;
+          alpha = move ? __builtin_amdgcn_exp2f((m_run - m_cand) * p.scale_log2) : 1.0f;
+          m_run = move ? m_cand : m_run;
+          m_use = m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
+        }
+        if (slot == LEAD - 1 && __builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+          for (int d = 0; d < NDS; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        }
+        constexpr int REST = 2 * NC - LEAD;  // MFMAs behind which the 32 exponentials run
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (slot < LEAD || i < 32 * (slot - LEAD) / REST || i >= 32 * (slot - LEAD + 1) / REST) continue;
           const float pv = __builtin_amdgcn_exp2f(fmaf(s_cur[i >> 4][i & 15], p.scale_log2, -m_use));
           psum += pv;
           pf[i >> 3][i & 7] = (__bf16)pv;
@@ -744,6 +755,8 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
       }
     if (!LAST) __builtin_amdgcn_sched_barrier(0);
     l_run = l_run * alpha + sum_halves(psum);
+    const float scale_v = LAST ? 1.f : scale_of(pair_v, true);
+    const float scale_k = LAST ? 1.f : scale_of(pair_k, false);
     constexpr int SLOTS = 4 * NDS;  // MFMAs of PV; 2 LOADS stores go behind every few
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc)
