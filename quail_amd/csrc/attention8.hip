@@ -10,7 +10,9 @@
 // matrix cores over the codes themselves: K's scale multiplies a page's 16
 // scores and V's its 16 probabilities, both in fp32 (a power of two each).
 // P is rounded to bf16 (2^-9 of a weight, about what the bf16 output rounds
-// by); scores, maxima, sums and outputs stay in fp32.
+// by); scores, maxima, sums and outputs stay in fp32. (P in fp16 with V's
+// scales in the softmax's exponent keeps 11 bits, but loses the weights of
+// pages whose scale is far below another's; 3% slower on long documents.)
 #include <algorithm>
 #include <new>
 #include <type_traits>
@@ -175,7 +177,13 @@ __device__ __forceinline__ void q_norm_columns(v8bf (&qf)[4], const QNormArgs& q
 // stands when its 32 k slots are numbered (l / 16) * 8 + page * 4 + r, and
 // V^T in that order comes from the row-major codes by ds_read_b64_tr_b8.
 // Both tiles are XOR-swizzled by 16-byte chunks: the rows that one LDS read
-// touches land in different banks.
+// touches land in different banks (the conflict counter reads 0).
+//
+// Bound by reading the codes: 200 one-row sequences of ~2100 keys (32 + 8
+// heads of 128, 856 MB) 165 us, 5.2 TB/s, where a kernel that only loads in
+// this pattern reaches 5.5; 2 sequences of 40,000 keys with 3 rows of 64
+// heads (164 MB, 512 workgroups: one round, its start and end in the open)
+// 42 us. One row over 300 keys: 7.5 us, four memory round trips.
 constexpr int kRing = 2;
 
 template <int D, int NB, int QN = 0>
@@ -465,6 +473,14 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
 // cores. (Scores from the codes themselves on the FP8 cores, with q as the
 // sum of two e4m3 numbers, take the same matrix time and no conversion, but
 // those cores drop what lies 2^-12 below the largest product of a sum.)
+//
+// Bound by the issue of two waves a SIMD (256 registers each): two documents
+// of 8000 rows (32 + 8 heads of 128, 1.07 TFLOP) 1.03 ms, 1.04 PFLOP/s (a
+// large bf16 product on this card 1.21), matrix cores 48% busy and vector
+// units 56%, of which half is exponentials. Short documents add what an item
+// costs outside its steps: 46 of ~340 rows (107 GFLOP, 291 MB) 161 us. With
+// few rows the longest item's steps count, 1.3 us each alone on a CU: 21
+// rows on 60 of ~1000 keys (up to 2064) 54 us.
 constexpr int kBK = 64;
 
 // the keys that the last row of a query tile sees, which the tile visits
@@ -926,7 +942,9 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 // Join the splits of each (row, head), WAVES waves per pair: a lane weighs
 // one split (in every wave alike), and each group of 16 lanes adds up every
 // (4 WAVES)-th split's output. A split without a key has weight 0 and an
-// output that nobody wrote: it is read and not used.
+// output that nobody wrote: it is read and not used. A launch of 4 to 7 us
+// (latency: work, then (m, l), then outputs), beside 14 to 166 us of the
+// kernels that it joins.
 template <int D, int WAVES>
 __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
   constexpr int PER = D / 16;  // columns per lane
@@ -1131,7 +1149,7 @@ int64_t list_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ, in
   //     rows on one document of 8000 tokens: 156 us whole, 25; on 8 of ~900:
   //     34, 21; 100 on 8 of ~8000: 228, 142);
   //   - into 512 where it has 24 more and a quarter more (12 rows on 60
-  //     documents of ~4000: 203, 192); not for less (21 rows on 60 of ~900, 33
+  //     documents of ~4000: 203, 192); not for less (21 rows on 60 of ~1000, 33
   //     steps against 15: 56 us whole, 74; one document's 2000 rows: 60, 87).
   const int rows = tile_height(G);
   int64_t steps = 0, longest = 0;

@@ -328,7 +328,9 @@ struct CopyRegion {
 };
 
 // blockIdx.x: page of the list; blockIdx.y: pool (the codes' pools, then the
-// scales'); blockIdx.z: part of the page.
+// scales'); blockIdx.z: part of the page. Bound by HBM: 1000 pages of 36
+// layers (16 KiB of codes each for K and V, 2.36 GB read and written) 480 us,
+// 4.9 TB/s, a large copy's rate; 37 pages (87 MB) 18 us.
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyRegion big, CopyRegion small,
                                                          CopyIds ids) {
   const int pool = blockIdx.y;
