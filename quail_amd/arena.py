@@ -57,6 +57,8 @@ class KVArena:
             raise ValueError("K pages are bf16; V pages bf16 or fp16")
         self.torch = torch
         self.dtype = dtype
+        # whether K and V are e4m3 codes with a scale per (page, KV head)
+        self.eight_bit = dtype == FP8
         self.v_dtype = v_dtype
         self.device = device
         self.num_layers = num_layers
@@ -91,11 +93,6 @@ class KVArena:
             self._pointers = [(k.data_ptr(), v.data_ptr(), s.data_ptr())
                               for k, v, s in zip(self.k, self.v, self._layer_scales)]
         self._claims = {}
-
-    @property
-    def eight_bit(self) -> bool:
-        """Whether K and V are e4m3 codes with a scale per (page, KV head)."""
-        return self.dtype == FP8
 
     # ---- sizes -------------------------------------------------------------
 

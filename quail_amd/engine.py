@@ -548,7 +548,7 @@ class Engine:
             raise ValueError(f"qkv width {qkv.shape[1]} < {(hq + 2 * hk) * d}")
         layer = meta["layer"]
         if self._eight_bit():
-            q = torch.empty((n, hq * d), dtype=torch.bfloat16, device=qkv.device)
+            q = torch.empty(n, hq * d, dtype=torch.bfloat16, device=qkv.device)
             self._write_pages(qkv, positions, attn, meta["unified"]["page_writes"], layer, q)
             meta["kv_fresh_layer"] = layer
             return q
@@ -623,7 +623,7 @@ class Engine:
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if qkv.shape[1] < (hq + 2 * hk) * d:
             raise ValueError(f"qkv width {qkv.shape[1]} < {(hq + 2 * hk) * d}")
-        if positions.shape != (qkv.shape[0],) or positions.dtype != torch.int64 or \
+        if positions.shape != qkv.shape[:1] or positions.dtype != torch.int64 or \
                 not positions.is_contiguous():
             raise ValueError(f"positions: {qkv.shape[0]} contiguous int64, not "
                              f"{tuple(positions.shape)} {positions.dtype}")
@@ -904,21 +904,24 @@ class Engine:
         if (hq, d) != (self.num_q_heads, self.head_dim) or q3.dtype != torch.bfloat16:
             raise ValueError(f"query rows of {tuple(q3.shape)} {q3.dtype} for "
                              f"{self.num_q_heads} heads of {self.head_dim} in bf16")
-        if q3.stride(2) != 1 or (hq > 1 and q3.stride(1) != d):
+        _, by_head, by_column = q3.stride()
+        if by_column != 1 or (hq > 1 and by_head != d):
             raise ValueError("a query row's heads are contiguous")
-        rows = int(tables["cu_q"].shape[0]) - 1
-        if rows != tables["used"].shape[0]:
-            raise ValueError(f"{rows} query ranges for {tables['used'].shape[0]} sequences")
+        eight_bit = self._eight_bit()
         made_for = tables.get("made_for")
-        if made_for not in (None, (n, hq, self.num_kv_heads, d, self._eight_bit())):
+        if made_for is None:
+            if tables["cu_q"].shape[0] != tables["used"].shape[0] + 1:
+                raise ValueError(f"{tables['cu_q'].shape[0]} bounds of query ranges for "
+                                 f"{tables['used'].shape[0]} sequences")
+        elif made_for != (n, hq, self.num_kv_heads, d, eight_bit):
             raise ValueError(f"a plan for {made_for} (rows, HQ, HK, D, 8 bits), not "
-                             f"{(n, hq, self.num_kv_heads, d, self._eight_bit())}")
+                             f"{(n, hq, self.num_kv_heads, d, eight_bit)}")
         scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
-        out = torch.empty((n, hq * d), dtype=torch.bfloat16, device=q3.device)
-        lse = torch.empty((hq, n), dtype=torch.float32, device=q3.device)
+        out = torch.empty(n, hq * d, dtype=torch.bfloat16, device=q3.device)
+        lse = torch.empty(hq, n, dtype=torch.float32, device=q3.device)
         if not n:
             return out, lse
-        if self._eight_bit():
+        if eight_bit:
             self._attend8(q3, tables, layer, scale, out=out, lse=lse)
         else:
             k_pool, v_pool = self.arena.layer_kv(layer)
