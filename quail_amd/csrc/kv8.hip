@@ -293,8 +293,8 @@ int kv8_write_launch(WriteArgs& a, bool qkv, int64_t n_items, int64_t HK, int64_
   QX_CHECK(HK > 0 && n_items >= 0, "kv8_write: heads %lld, items %lld", (long long)HK,
            (long long)n_items);
   if (n_items == 0) return QX_OK;
-  // heads per wave: as many as leave 6144 waves (the card holds 3072 of these
-  // at once). The pack above, with q (48 slots) 1: 79.2 us, 2: 72.9, 4: 71.3;
+  // heads per wave: as many as leave 6144 waves (twice what the card holds of
+  // these at once). The pack above, with q (48 slots) 1: 79.2 us, 2: 72.9, 4: 71.3;
   // its K and V alone (16 slots) 31.1, 28.5, 30.8
   for (a.heads = 4; a.heads > 1 && n_items * a.slots / a.heads < 6144;) a.heads /= 2;
   a.groups = (a.slots + a.heads - 1) / a.heads;
