@@ -621,8 +621,14 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
         raise ValueError("cu_q rises from 0 and used is not negative")
     if host["used"].max(initial=0) > table.shape[1] * PAGE_ROWS:
         raise ValueError(f"{host['used'].max()} keys in {table.shape[1]} pages")
+    # the pages that are read (entries past a sequence's own may hold anything)
+    live = np.arange(table.shape[1]) < -(-host["used"][:, None] // PAGE_ROWS)
+    pages = table.cpu().numpy()[live]
+    if (pages < 0).any():
+        raise ValueError(f"page {pages.min()} in the table")
     tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
                   made_for=(int(host["cu_q"][-1]), *heads, bool(eight_bit)),
+                  pages=int(pages.max(initial=-1)) + 1,
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),
                   max_used=int(host["used"].max(initial=0)))
     work, n_work, rows = (_work_list8(host, heads) if eight_bit else

@@ -916,6 +916,9 @@ class Engine:
         elif made_for != (n, hq, self.num_kv_heads, d, eight_bit):
             raise ValueError(f"a plan for {made_for} (rows, HQ, HK, D, 8 bits), not "
                              f"{(n, hq, self.num_kv_heads, d, eight_bit)}")
+        elif tables["pages"] > self.arena.num_pages:
+            raise ValueError(f"page {tables['pages'] - 1} in the plan's table, "
+                             f"{self.arena.num_pages} in the arena")
         scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
         out = torch.empty(n, hq * d, dtype=torch.bfloat16, device=q3.device)
         lse = torch.empty(hq, n, dtype=torch.float32, device=q3.device)

@@ -761,3 +761,17 @@ def test_a_long_sequence_of_many_heads_per_kv_head():
     assert bool(torch.isfinite(out).all())
     last = np.asarray([0, 3], dtype=np.int32)
     check_rows(out[-3:], lse[:, -3:], q[-3:], arena, last, used, table, True)
+
+
+def test_read_pages_refuses_pages_that_the_arena_does_not_have():
+    from quail_amd.chunk import attention_plan
+    arena = engine_arena(4)
+    fill(arena, torch.Generator().manual_seed(5))    # a new arena holds any bytes, NaN codes too
+    eng = engine_of(arena, 32)
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    q = torch.zeros(1, 32, 128, dtype=torch.bfloat16, device=DEV)
+    plan = attention_plan(ints(0, 1), ints(20), ints(3, 4).view(1, 2), heads=(32, 8, 128))
+    with pytest.raises(ValueError, match="page 4"):
+        eng.read_pages(q, plan, 0)
+    plan = attention_plan(ints(0, 1), ints(16), ints(3, 4).view(1, 2), heads=(32, 8, 128))
+    assert bool(torch.isfinite(eng.read_pages(q, plan, 0)[0]).all())

@@ -359,3 +359,13 @@ def test_an_attention_plan_names_what_it_was_made_for():
     ints = lambda *a: torch.tensor(a, dtype=torch.int32)  # noqa: E731
     plan = attention_plan(ints(0, 1, 3), ints(20, 5), ints(1, 2, 3, 0).view(2, 2), heads=(4, 2, 64))
     assert plan["made_for"] == (3, 4, 2, 64, True)
+
+
+def test_an_attention_plan_checks_the_pages_that_are_read():
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32)  # noqa: E731
+    table = ints(1, 7, -1, 3, 99, -5).view(2, 3)
+    plan = attention_plan(ints(0, 1, 2), ints(32, 16), table, heads=(4, 2, 64))
+    assert plan["pages"] == 8                        # entries past a sequence's keys are not read
+    with pytest.raises(ValueError, match="page -1"):
+        attention_plan(ints(0, 1, 2), ints(33, 16), table, heads=(4, 2, 64))
+    assert attention_plan(ints(0, 1, 2), ints(0, 0), table, heads=(4, 2, 64))["pages"] == 0
