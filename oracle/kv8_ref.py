@@ -63,8 +63,15 @@ def values(codes, scales, side):
     return codes.double() * s.repeat_interleave(PAGE, 0)[..., None]
 
 
+def _rows(pool, rows):
+    if pool.dtype == FP8:       # indexed as bytes
+        return pool.view(torch.uint8)[rows].view(FP8).double()
+    return pool[rows].double()
+
+
 def attend(q, k_pool, v_pool, scales, cu_q, used, table, causal, scale=None):
-    """Attention rows (n, HQ, D), log-sum-exps (n, HQ), and for error bounds
+    """Over codes and their scales (or 16-bit rows and scales of 1):
+    attention rows (n, HQ, D), log-sum-exps (n, HQ), and for error bounds
     sum_j p_j |v_j| (n, HQ, D) and max_j scale * sum |q||k_j| (n, HQ)."""
     n, hq, d = q.shape
     hk = k_pool.shape[1]
@@ -80,8 +87,7 @@ def attend(q, k_pool, v_pool, scales, cu_q, used, table, causal, scale=None):
         pages = torch.as_tensor(table[s][:-(-keys // PAGE)], device=q.device).long()
         rows = (pages[:, None] * PAGE + torch.arange(PAGE, device=q.device)).view(-1)[:keys]
         sc = torch.exp2(scales[pages].double() - 127).repeat_interleave(PAGE, 0)[:keys]
-        k = k_pool.view(torch.uint8)[rows].view(FP8).double() * sc[..., :1]
-        v = v_pool.view(torch.uint8)[rows].view(FP8).double() * sc[..., 1:]
+        k, v = (_rows(pool, rows) * sc[..., i:i + 1] for i, pool in enumerate((k_pool, v_pool)))
         for i in range(r0, r1):
             seen = min(keys, keys - (r1 - r0) + (i - r0) + 1) if causal else keys
             if seen <= 0:

@@ -9,7 +9,7 @@
 // (attention.hip). Codes are exact in bf16, so both products run on the bf16
 // matrix cores over the codes themselves: K's scale multiplies a page's 16
 // scores and V's its 16 probabilities, both in fp32 (a power of two each).
-// P is rounded to bf16 (2^-9 of a weight, about what the bf16 output rounds
+// P is rounded to bf16 (at most 2^-8 of a weight, what the bf16 output rounds
 // by); scores, maxima, sums and outputs stay in fp32. (P in fp16 with V's
 // scales in the softmax's exponent keeps 11 bits, but loses the weights of
 // pages whose scale is far below another's; 3% slower on long documents.)

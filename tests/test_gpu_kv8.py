@@ -775,3 +775,29 @@ def test_read_pages_refuses_pages_that_the_arena_does_not_have():
         eng.read_pages(q, plan, 0)
     plan = attention_plan(ints(0, 1), ints(16), ints(3, 4).view(1, 2), heads=(32, 8, 128))
     assert bool(torch.isfinite(eng.read_pages(q, plan, 0)[0]).all())
+
+
+@pytest.mark.parametrize("v_dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (4, 2, 64)])
+@pytest.mark.parametrize("q_lens,used,causal", [((1, 1, 3), (300, 17, 64), True),
+                                                ((40, 21, 1), (90, 500, 33), True),
+                                                ((70, 2), (40, 1100), False)])
+def test_read_pages_of_a_16_bit_arena(v_dtype, hq, hk, d, q_lens, used, causal):
+    """The same call over bf16 K and 16-bit V: the oracle's codes are the
+    values, its scales 1; P is rounded to V's type (2^-8 at most)."""
+    from types import SimpleNamespace
+
+    from quail_amd.chunk import attention_plan
+    g = torch.Generator().manual_seed(41)
+    pages = sum(-(-u // PAGE) for u in used) + 3
+    arena = KVArena(1, pages, PAGE, hk, d, v_dtype=v_dtype)
+    for pool in arena.layer_kv(0):
+        pool.copy_(torch.randn(pool.shape, generator=g))
+    cu_q, used, table = sequences(g, q_lens, used, pages)
+    q = torch.randn(int(cu_q[-1]), hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    plan = attention_plan(*(torch.from_numpy(a).to(DEV) for a in (cu_q, used, table)),
+                          heads=(hq, hk, d), causal=causal, eight_bit=False)
+    out, lse = engine_of(arena, hq).read_pages(q, plan, 0)
+    ones = torch.full((pages, hk, 2), 127, dtype=torch.uint8, device=DEV)
+    same = SimpleNamespace(layer_kv=arena.layer_kv, layer_scales=lambda layer: ones)
+    check_rows(out, lse, q, same, cu_q, used, table, causal)
