@@ -18,7 +18,7 @@ bytes a token takes and a reader moves): each pool holds e4m3 codes, and
 KV head), (num_layers, num_pages, num_kv_heads, 2).
 """
 
-import ctypes
+from array import array
 
 import numpy as np
 import torch
@@ -245,22 +245,28 @@ class KVArena:
             raise ValueError(f"{len(src)} source pages for {len(dst)} destinations")
         if not self.storage.is_cuda:
             raise ValueError("page copies run on the GPU; this arena is on the CPU")
+        try:
+            src, dst = array("i", src), array("i", dst)
+        except OverflowError as err:
+            raise ValueError(f"page ids of {self.num_pages} pages: {err}") from err
+        device = self.storage.device.index
+        if device != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                self._copy_pages(src, dst)
+        else:
+            self._copy_pages(src, dst)
+
+    def _copy_pages(self, src, dst):
         from quail_amd.engine import _stream
-        for page in (*src, *dst):
-            if not 0 <= page < self.num_pages:   # also before it is cut to 32 bits
-                raise ValueError(f"page {page} of {self.num_pages}")
-        ids = ctypes.c_int32 * max(1, len(src))
         heads, dim = self.kv_shape
-        size = self.storage.element_size()
-        page = self.page_tokens * heads * dim * size
-        pool = self.num_pages * page
+        page = self.page_tokens * heads * dim * self.storage.element_size()
         scales = (None, 0, 0, 0)
         if self.eight_bit:
             scales = (self.scales.data_ptr(), self.num_layers, 2 * heads * self.num_pages, 2 * heads)
         try:
-            with torch.cuda.device(self.storage.device):
-                _lib.call("qx_copy_pages", self.storage.data_ptr(), 2 * self.num_layers, pool, page,
-                          *scales, ids(*src), ids(*dst), len(src), self.num_pages, _stream())
+            _lib.call("qx_copy_pages", self.storage.data_ptr(), 2 * self.num_layers,
+                      self.num_pages * page, page, *scales, src.buffer_info()[0],
+                      dst.buffer_info()[0], len(src), self.num_pages, _stream())
         except _lib.QxError as err:
             if "hipError" in str(err):
                 raise
