@@ -382,10 +382,11 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
         o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[n][d], 0, 0, 0);
     }
   }
-  if (__builtin_amdgcn_ballot_w64(nans != 0)) {  // rare: this wave's keys in the cut, again
+  if (__builtin_amdgcn_ballot_w64(nans != 0)) {  // rare: the keys of this wave's steps in the cut, again
     for (int t = 0; t < mine; ++t) {
       const int key0 = 32 * (4 * t + wave);
-      for (int key = max(key0, cut); key < min(key0 + 32, k1 - k0); ++key) {
+      if (key0 + 32 <= cut) continue;  // its NaN codes went into the products
+      for (int key = key0; key < min(key0 + 32, k1 - k0); ++key) {
         const uint8_t* v = vbase + ((int64_t)pages[key / kPage] * kPage + key % kPage) * kv_row;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
