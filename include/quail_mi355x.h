@@ -261,15 +261,16 @@ int qx_kv_scatter(const void* k, int64_t k_ld, const void* v, int64_t v_ld, void
  * whose pools are bf16): k_pool and v_pool hold e4m3 codes, rows of HK*D
  * bytes, and scales one byte for K and one for V per (page of 16 rows, KV
  * head), at scales[(page*HK + head)*2 + (0 for K, 1 for V)]: an E8M0 byte b
- * in [1, 247] that stands for 2^(b - 127). A row's value is code * 2^(b - 127).
+ * in [1, 247] that stands for 2^(b - 127). A row's value is code * 2^(b - 127);
+ * under 247 codes are at most 240, so that every value is a finite bf16.
  *
  * Both calls write whole page items. items (device): 5 int32 per item,
  * {destination page, source page, keep, row0, count}, keep + count <= 16: the
  * page's rows [0, keep) are the source page's (mostly the destination itself;
  * another for a copied partial page), the next `count` are the fresh rows
  * row0, row0 + 1, ...; rows past them stay as they are. The scale's byte is
- * the least b with max |fresh| <= 448 * 2^(b - 127) (infinities count as the
- * largest float, NaN not at all), or with keep > 0 the larger of that and
+ * the least b with max |fresh| <= 448 * 2^(b - 127) (values past 240 * 2^120,
+ * infinities among them, are written as that, NaN not counted), or with keep > 0 the larger of that and
  * the source page's; kept codes then move by that power of two, exactly
  * unless they become subnormal. A call writes each destination page once,
  * and no item's source is another item's destination.

@@ -11,6 +11,7 @@ from oracle.fp8 import FP8_MAX
 
 PAGE = 16
 FP8 = torch.float8_e4m3fn
+LAST_SCALE = 247    # of the largest float
 
 
 def scale_byte(amax: float) -> int:
@@ -26,6 +27,8 @@ def codes_of(x: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     scaled value is rounded once: float64 -> float32 would round first, so
     values are moved to the e4m3 grid in float64."""
     y = (x * torch.exp2(127.0 - b.double())).clamp(-FP8_MAX, FP8_MAX)
+    # under the last scale 256 would stand for 2^128: the codes end at 240
+    y = torch.where(b == LAST_SCALE, y.clamp(-240.0, 240.0), y)
     step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
     return (torch.round(y / step) * step).float().to(FP8)     # round half to even
 

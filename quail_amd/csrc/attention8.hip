@@ -469,7 +469,7 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
 // sequence x HPB heads that share a KV head, one wave per (tile, head); keys
 // come in 64-key tiles (four pages, one per wave to move), software
 // pipelined with one barrier a step. A page's codes travel HBM -> registers,
-// become bf16, scaled (exact), once per workgroup, and lie in LDS as the
+// become bf16, scaled (exact down to bf16's least number), once per workgroup, and lie in LDS as the
 // 16-bit kernel's tiles do, so that both products run on the bf16 matrix
 // cores. (Scores from the codes themselves on the FP8 cores, with q as the
 // sum of two e4m3 numbers, take the same matrix time and no conversion, but

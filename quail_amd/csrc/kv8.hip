@@ -14,12 +14,18 @@ namespace qx {
 namespace {
 
 constexpr int kPage = 16;  // tokens per arena page
-constexpr float kF32Max = 3.402823466e38f;
+// The last scale (2^120, for values past 448 * 2^119) holds codes up to 240
+// alone: 256 would stand for 2^128, which bf16 and fp32 do not have, and a
+// reader's weight of 0 times infinity is NaN. 240 for a value up to 256 is off
+// by at most 2^-4 of it, as a code's rounding is.
+constexpr int kLastScale = 247;
+constexpr float kLargest = 240.f * 0x1p120f;
 
 // The E8M0 byte of the least power of two s with amax <= 448 s, at least 1:
 // with amax = 1.m * 2^e that is 2^(e - 8), and twice that where 1.m > 1.75.
 // Adding the distance from the fraction of 1.75 to the next power of two
-// carries into the exponent exactly where the fraction is past it.
+// carries into the exponent exactly where the fraction is past it. (An infinity:
+// 247, as the largest float.)
 __device__ __forceinline__ int scale_byte(float amax) {
   return max((int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8, 1);
 }
@@ -237,15 +243,14 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs p) {
     }
     if (!q) {
       amax = wave_max(amax);
-      if (amax > kF32Max) {  // an infinity counts as the largest float (e4m3 has none); NaN stays
-        amax = kF32Max;
+      const int need = scale_byte(amax);
+      if (need == kLastScale) {  // infinities (e4m3 has none) and what they share a page with; NaN stays
 #pragma unroll
         for (int t = 0; t < PASSES; ++t)
 #pragma unroll
           for (int k = 0; k < 16; ++k)
-            y[t][k] = y[t][k] != y[t][k] ? y[t][k] : fminf(fmaxf(y[t][k], -kF32Max), kF32Max);
+            y[t][k] = y[t][k] != y[t][k] ? y[t][k] : fminf(fmaxf(y[t][k], -kLargest), kLargest);
       }
-      const int need = scale_byte(amax);
       const int b = keep > 0 ? max(b_old, need) : need;
       const bool move = src != dst || b != b_old;  // the kept rows change
       uint8_t* pool = v ? p.vp : p.kp;

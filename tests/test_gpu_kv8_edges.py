@@ -1,10 +1,13 @@
 """The 8-bit KV arena on the GPU where masks, infinities, NaN and long keys
 meet: what test_gpu_kv8.py's sizes leave out. Bounds as there."""
 
+import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_kv8 import DEV, PAGE, engine_arena, engine_of, fill, plan_of, same_codes
+from oracle import kv8_ref as ref
+from tests.test_gpu_kv8 import (DEV, PAGE, check_rows, engine_arena, engine_of, fill, plan_of,
+                                same_codes)
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +39,52 @@ def test_nan_values_below_the_cut_reach_every_row_that_sees_them(hq, hk, d, q_le
     want[seen, -(hq // hk):, d - 1] = float("nan")
     assert same_codes(out.view(q_len, hq, d), want)
     assert torch.equal(lse, clean_lse)
+
+
+def write_rows(arena, hq, k3, v3, table):
+    """Rows 0.. of one sequence into its pages, as they are."""
+    items = torch.tensor([(int(table[0, p]), int(table[0, p]), 0, PAGE * p,
+                           min(PAGE, len(k3) - PAGE * p)) for p in range(-(-len(k3) // PAGE))],
+                         dtype=torch.int32, device=DEV)
+    engine_of(arena, hq)._write_page_rows(k3, v3, (items,), 0)
+    return items.tolist()
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (24, 8, 64), (8, 8, 128), (4, 2, 64)])
+@pytest.mark.parametrize("value", [float("inf"), 3.3895313892515355e38])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_infinite_keys_and_values_stay_out_of_rows_that_do_not_see_them(hq, hk, d, value, side):
+    """An infinity, or bf16's largest number, is stored as a finite value (at
+    most 240 * 2^120), so that a weight of 0 times it is 0: rows that do not
+    see its page are as without it, bit for bit, and those that see a V one
+    match float64 over the stored codes."""
+    g = torch.Generator().manual_seed(52)
+    used, at = 48, 36
+    arena = engine_arena(4, hk, d)
+    fill(arena, g)
+    k3, v3 = (torch.randn(used, hk, d, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    bad = [k3.clone(), v3.clone()]
+    bad["kv".index(side)][at, 0, 5] = value
+    bad["kv".index(side)][at + 1, hk - 1, 3] = -value
+    for q_len in (40, 33, 8, 1):
+        plan, cu_q, u, table = plan_of(arena, hq, (q_len,), (used,), torch.Generator().manual_seed(1))
+        q = torch.randn(q_len, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+        eng = engine_of(arena, hq)
+        write_rows(arena, hq, k3, v3, table)
+        clean, clean_lse = eng.read_pages(q, plan, 0)
+        pools = [p.cpu() for p in arena.layer_kv(0)] + [arena.layer_scales(0).cpu()]
+        items = write_rows(arena, hq, *bad, table)
+        ref.write_items(*pools, *(t.double().cpu() for t in bad), items)
+        for got, want in zip(arena.layer_kv(0), pools):
+            assert same_codes(got, want)
+        assert torch.equal(arena.layer_scales(0).cpu(), pools[2])
+        for i in (0, 1):
+            size = ref.values(pools[i], pools[2], i)[np.r_[tuple(
+                slice(PAGE * p, PAGE * p + PAGE) for p in table[0, :3].tolist())]]
+            assert float(size.abs().max()) <= 240 * 2.0 ** 120
+        out, lse = eng.read_pages(q, plan, 0)
+        before = max(0, 2 * PAGE - (used - q_len))      # rows that see none of the last page
+        assert torch.equal(out[:before], clean[:before])
+        assert torch.equal(lse[:, :before], clean_lse[:, :before])
+        if side == "v":
+            check_rows(out, lse, q, arena, cu_q, u, table, True)
