@@ -942,8 +942,8 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 
 // Join the splits of each (row, head), WAVES waves per pair: a lane weighs
 // one split (in every wave alike), and each group of 16 lanes adds up every
-// (4 WAVES)-th split's output. A split without a key has weight 0 and an
-// output that nobody wrote: it is read and not used. A launch of 4 to 7 us
+// (4 WAVES)-th split's output. A split without a key has an output that
+// nobody wrote: it is read and not used. A launch of 4 to 7 us
 // (latency: work, then (m, l), then outputs), beside 14 to 166 us of the
 // kernels that it joins.
 template <int D, int WAVES>
@@ -977,6 +977,7 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
     const float top = fmaxf(mm, group_max<64>(mine.x));
     const float top_use = top == -INFINITY ? 0.f : top;
     const float w = __builtin_amdgcn_exp2f(mine.x - top_use);
+    const float out_w = mine.x == -INFINITY ? -1.f : w;  // no key, no output; 0 is a weight (of NaN, too)
     const float keep = __builtin_amdgcn_exp2f(mm - top_use);
     ll = ll * keep + group_sum<64>(mine.y * w);
     mm = top;
@@ -990,8 +991,8 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         const int at = i + u * GROUPS;
-        wi[u] = __shfl(w, min(at, 63), 64);
-        if (at >= n) wi[u] = 0.f;
+        wi[u] = __shfl(out_w, min(at, 63), 64);
+        if (at >= n) wi[u] = -1.f;
 #pragma unroll
         for (int k = 0; k < PER / 4; ++k)
           a[u][k] = *reinterpret_cast<const v4f*>(po + (first + min(at, n - 1)) * step * D + 4 * k);
@@ -1000,7 +1001,7 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
       for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
         for (int k = 0; k < PER; ++k)
-          y[k] = wi[u] != 0.f ? fmaf(a[u][k >> 2][k & 3], wi[u], y[k]) : y[k];
+          y[k] = wi[u] < 0.f ? y[k] : fmaf(a[u][k >> 2][k & 3], wi[u], y[k]);
     }
   }
   if constexpr (WAVES > 1) {

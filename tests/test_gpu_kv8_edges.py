@@ -88,3 +88,30 @@ def test_infinite_keys_and_values_stay_out_of_rows_that_do_not_see_them(hq, hk, 
         assert torch.equal(lse[:, :before], clean_lse[:, :before])
         if side == "v":
             check_rows(out, lse, q, arena, cu_q, u, table, True)
+
+
+@pytest.mark.parametrize("q_len", [1, 2, 40])
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (24, 8, 64)])
+def test_nan_values_of_a_split_without_weight_reach_the_rows(q_len, hq, hk, d):
+    """A NaN of V among keys that a row sees with a weight that underflows,
+    in a split of its own: the row is NaN there, as it is unsplit."""
+    from quail_amd.chunk import attention_plan
+    g = torch.Generator().manual_seed(53)
+    used = 9000
+    arena = engine_arena(-(-used // PAGE), hk, d)
+    fill(arena, g)
+    k, v = arena.layer_kv(0)
+    arena.layer_scales(0).fill_(127)
+    k.fill_(400.0)
+    k[:4096] = -400.0       # whole splits, of 2048 keys at most
+    v.view(torch.uint8)[5, 0, 7] = 0x7f
+    table = torch.arange(arena.num_pages, dtype=torch.int32, device=DEV).view(1, -1)
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    q = torch.full((q_len, hq, d), 8.0, dtype=torch.bfloat16, device=DEV)
+    plan = attention_plan(ints(0, q_len), ints(used), table, heads=(hq, hk, d))
+    assert 0 < abs(plan["work_rows"]) < used
+    out, lse = engine_of(arena, hq).read_pages(q, plan, 0)
+    nan = torch.zeros(hq, d, dtype=torch.bool, device=DEV)
+    nan[:hq // hk, 7] = True
+    assert torch.equal(torch.isnan(out.view(q_len, hq, d)), nan.expand(q_len, -1, -1))
+    assert bool(torch.isfinite(lse).all())
