@@ -448,6 +448,19 @@ int qx_attention_lse_tiled(const void* q, int64_t q_ld, const int64_t* q_index, 
  * workspace: qx_paged_attention8_workspace bytes of the caller's (has_work:
  * whether the call gets a list), 16-byte aligned (NULL where that is 0), used
  * by this call alone until the stream has passed it.
+ *
+ * That workspace has room for every row in as many splits as the longest
+ * sequence has, and the second launch looks at every sequence. With few rows
+ * over long keys beside many rows, qx_paged_attention8_joined pays for what
+ * is split alone: the host function qx_paged_attention8_joins takes the list
+ * and writes slots (n_work ints: the first row of an item's partial results,
+ * -1 for an item that is not split) and joins (4 ints for each split tile: its
+ * first query row, its rows, the first row of its partial results, its
+ * splits; `capacity` of them, n_work / 2 are always enough), both copied to
+ * the device for the call, and the number of partial rows; it returns the
+ * number of joins or -1. The call's workspace is
+ * part_rows * HQ * (D + 2) * 4 bytes. Rows are those of qx_paged_attention8,
+ * bit for bit.
  */
 int qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
                              int64_t HK, int causal, int64_t* unit);
@@ -466,6 +479,19 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
                         const int* work, int64_t n_work, int64_t unit, void* workspace,
                         int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
                         int cs_is_f32, const void* q_w, float eps, hipStream_t stream);
+int64_t qx_paged_attention8_joins(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                                  int64_t HK, int causal, int64_t unit, const int* work,
+                                  int64_t n_work, int* slots, int* joins, int64_t capacity,
+                                  int64_t* part_rows);
+int qx_paged_attention8_joined(
+    const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool, const void* v_pool,
+    const void* scales, const int* cu_q, const int* used, const int* table, int64_t table_ld,
+    int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
+    int64_t page, float scale, int causal, void* out_bf16, void* out_fp8, int64_t o_ld,
+    float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld, const int* work, int64_t n_work,
+    int64_t unit, const int* slots, const int* joins, int64_t n_joins, int64_t part_rows,
+    void* workspace, int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
+    int cs_is_f32, const void* q_w, float eps, hipStream_t stream);
 
 /*
  * Replaces Engine.merge_attn_quant / the merge_attn_quant Triton kernel

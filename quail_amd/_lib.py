@@ -57,6 +57,12 @@ SIGNATURES = {
                             _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _i64, _p, _i64, _p, _i64,
                             _p, _i64, _i64, _p, _i64, _p, _p, _i32, _p, _f32, _p],
     "qx_paged_attention8_work": [_p, _p, _i64, _i64, _i64, _i32, _i64, _p, _i64],
+    "qx_paged_attention8_joins": [_p, _p, _i64, _i64, _i64, _i32, _i64, _p, _i64, _p, _p, _i64,
+                                  _p],
+    "qx_paged_attention8_joined": [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                                   _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _i64, _p,
+                                   _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64,
+                                   _p, _p, _i32, _p, _f32, _p],
     "qx_copy_pages": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p],
     "qx_pages_compact": [_p, _p, _p, _i64, _p],
     "qx_embed": [_p, _i64, _p, _p, _i64, _i64, _i64, _p],
@@ -106,7 +112,7 @@ SIGNATURES = {
 RETURNS_COUNT = {"qx_paged_attention_work", "qx_paged_attention_tile_rows",
                  "qx_paged_attention_max_keys", "qx_vocab_logprobs_workspace",
                  "qx_vocab_logprobs_noalloc_max_bytes", "qx_paged_attention8_workspace",
-                 "qx_paged_attention8_work"}
+                 "qx_paged_attention8_work", "qx_paged_attention8_joins"}
 
 
 class QxUnavailable(RuntimeError):

@@ -242,9 +242,7 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
     if attention_heads is not None:
         for tables in (unified, meta["final_query"]):
             if tables is not None:
-                tables["work"], tables["n_work"], tables["work_rows"] = (
-                    _work_list8(tables, attention_heads) if eight_bit else
-                    _work_list(tables, attention_heads, choose_rows=True))
+                _add_work(tables, attention_heads, eight_bit)
     if timing is not None:
         timing["pack_py"] = timing.get("pack_py", 0.0) + (t1 - t0)
         timing["pack_unified"] = timing.get("pack_unified", 0.0) + (time.perf_counter() - t1)
@@ -468,9 +466,7 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
         for tables in (segments, reads, reads and reads.get("nodes")):
             if tables:
                 # call B alone reads the arena's pages
-                tables["work"], tables["n_work"], tables["work_rows"] = (
-                    _work_list8(tables, attention_heads) if eight_bit and tables is reads else
-                    _work_list(tables, attention_heads, choose_rows=True))
+                _add_work(tables, attention_heads, eight_bit and tables is reads)
     ids = _cat(id_parts)
     positions = _cat(pos_parts)
     final = _cat(finals)
@@ -511,9 +507,20 @@ def _work_list(tables, heads, choose_rows=False):
     return work[:2 * n], n, rows
 
 
+def _add_work(tables, heads, eight_bit):
+    """The list of a call's items into its tables."""
+    if eight_bit:
+        (tables["work"], tables["n_work"], tables["work_rows"],
+         tables["work_joins"]) = _work_list8(tables, heads)
+    else:
+        tables["work"], tables["n_work"], tables["work_rows"] = _work_list(
+            tables, heads, choose_rows=True)
+
+
 def _work_list8(tables, heads):
-    """The same of a call over an 8-bit arena's pages; the third value is
-    qx_paged_attention8_unit's."""
+    """The same of a call over an 8-bit arena's pages: (work pairs, then each
+    item's slot, then the joins of qx_paged_attention8_joins; count;
+    qx_paged_attention8_unit's value; (joins, partial rows))."""
     from quail_amd import _lib
     hq, hk, _ = heads
     cu_q = np.ascontiguousarray(tables["cu_q"], dtype=np.int32)
@@ -530,7 +537,12 @@ def _work_list8(tables, heads):
     work = np.zeros(2 * max(cap, 1), dtype=np.int32)
     n = _lib.count("qx_paged_attention8_work", cu_q.ctypes.data, used.ctypes.data, seqs, hq, hk,
                    causal, unit, work.ctypes.data, cap)
-    return work[:2 * n], n, unit
+    slots, joins = np.zeros(max(n, 1), dtype=np.int32), np.zeros((n // 2 + 1, 4), dtype=np.int32)
+    n_joins = _lib.count("qx_paged_attention8_joins", cu_q.ctypes.data, used.ctypes.data, seqs, hq,
+                         hk, causal, unit, work.ctypes.data, n, slots.ctypes.data,
+                         joins.ctypes.data, len(joins), ctypes.byref(found))
+    work = np.concatenate([work[:2 * n], slots[:n], joins[:n_joins].reshape(-1)])
+    return work, n, unit, (n_joins, found.value)
 
 
 def _final_query(cu_q, used, table, final):
@@ -631,11 +643,11 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
                   pages=int(pages.max(initial=-1)) + 1,
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),
                   max_used=int(host["used"].max(initial=0)))
-    work, n_work, rows = (_work_list8(host, heads) if eight_bit else
-                          _work_list(host, heads, choose_rows=True))
-    if n_work:
+    _add_work(host, heads, eight_bit)
+    if host["n_work"]:
         import torch
-        tables.update(work=torch.from_numpy(work).to(cu_q.device), n_work=n_work, work_rows=rows)
+        tables.update({k: v for k, v in host.items() if k.startswith(("work", "n_work"))},
+                      work=torch.from_numpy(host["work"]).to(cu_q.device))
     return tables
 
 

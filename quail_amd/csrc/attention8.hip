@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <new>
 #include <type_traits>
+#include <unordered_map>
 #include <utility>
 #include <vector>
 
@@ -49,11 +50,25 @@ struct Attn8Args {
   float* lse;
   int64_t lse_ld;
   // keys per split (0: whole sequences), the most splits of a sequence, the
-  // query rows of a tile (0: few rows), and the splits' partial results
+  // query rows of a tile (0: few rows), and the splits' partial results: rows
+  // of HQ heads. Without slots split i of query row r has row i * rows + r;
+  // with them a split item has its own rows from slots[item] on, one for each
+  // of its query rows, out of `rows` in all.
   int chunk, splits, tile_rows;
   int64_t rows;
   float *part_o, *part_ml;
+  const int *slots, *joins;
+  int n_joins;
 };
+
+// Where query row `row`, the in_item-th of an item of item_rows, keeps the
+// partial result of split `split`; -1: nowhere (a slot that is not the call's).
+__device__ __forceinline__ int64_t part_row(const Attn8Args& p, int64_t item, int split, int64_t row,
+                                            int in_item, int item_rows) {
+  if (!p.slots) return split * p.rows + row;
+  const int slot = p.slots[item];
+  return slot < 0 || slot + item_rows > p.rows ? -1 : slot + in_item;
+}
 
 // 2^(b - 127) of an E8M0 byte b >= 1
 __device__ __forceinline__ float e8m0(int b) { return __uint_as_float((uint32_t)b << 23); }
@@ -444,7 +459,9 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
     const int64_t row = q0 + c / G;
     const int head = kvh * G + c % G;
     if (used > p.chunk) {
-      const int64_t at = ((int64_t)split * p.rows + row) * p.HQ + head;
+      const int64_t part = part_row(p, blockIdx.x, split, row, c / G, q_len);
+      if (part < 0) continue;
+      const int64_t at = part * p.HQ + head;
       if (j == 0) {
         p.part_ml[2 * at] = mm;
         p.part_ml[2 * at + 1] = ll;
@@ -890,8 +907,10 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
   // the wave's rows go out through LDS so that a store writes whole rows,
   // 16-byte chunks XOR-swizzled by the row
   if (!whole) {  // a split: its state as it stands
-    const int64_t at = ((int64_t)split * p.rows + q0 + r) * p.HQ + head;
-    if (r_ok) {
+    const int64_t part = part_row(p, blockIdx.x / zgroups, split, q0 + r, r - qt * BQ,
+                                  min(BQ, q_len - qt * BQ));
+    const int64_t at = part * p.HQ + head;
+    if (r_ok && part >= 0) {
 #pragma unroll
       for (int d = 0; d < NDS; ++d)
 #pragma unroll
@@ -946,6 +965,11 @@ __global__ __launch_bounds__(256, 2) void attention8_tile_kernel(Attn8Args p, co
 // nobody wrote: it is read and not used. A launch of 4 to 7 us
 // (latency: work, then (m, l), then outputs), beside 14 to 166 us of the
 // kernels that it joins.
+// joins: 4 ints for each split tile (or sequence of few rows), {first query
+// row, rows, first row of partial results, splits}, blockIdx.y of them; the
+// grid and the partial results then cost what is split (over every sequence, a
+// pack of 46 documents beside 21 rows on 40,000 keys started 323,000
+// workgroups to join 21 rows). Without them: every sequence.
 template <int D, int WAVES>
 __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
   constexpr int PER = D / 16;  // columns per lane
@@ -953,21 +977,33 @@ __global__ __launch_bounds__(256) void split_merge_kernel(Attn8Args p) {
   __shared__ v4f part[WAVES > 1 ? GROUPS * D / 4 : 1];
   const int wave = threadIdx.x >> 6;
   const int in_seq = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
-  const int s = blockIdx.y;
-  const int q0 = p.cu_q[s], q_len = p.cu_q[s + 1] - q0;
-  const int used = min(p.used[s], p.max_used);
-  if (in_seq >= q_len * p.HQ) return;
-  const int keys = p.tile_rows
-                       ? tile_keys(used, q_len, in_seq / p.HQ / p.tile_rows, p.tile_rows, p.causal)
-                       : used;
-  if (keys <= p.chunk) return;  // not split: its rows went out whole
-  const int splits = (keys + p.chunk - 1) / p.chunk;
-  const int64_t row = q0 + in_seq / p.HQ;
   const int head = in_seq % p.HQ;
-  const int64_t pair = row * p.HQ + head;
+  int splits;
+  int64_t row, pair, step;
+  if (p.joins) {
+    const int* join = p.joins + 4 * blockIdx.y;
+    const int rows = join[1];
+    splits = join[3];
+    if (in_seq >= rows * p.HQ || join[2] < 0 || join[2] + (int64_t)rows * splits > p.rows) return;
+    row = join[0] + in_seq / p.HQ;
+    pair = (int64_t)(join[2] + in_seq / p.HQ) * p.HQ + head;
+    step = (int64_t)rows * p.HQ;
+  } else {
+    const int s = blockIdx.y;
+    const int q0 = p.cu_q[s], q_len = p.cu_q[s + 1] - q0;
+    const int used = min(p.used[s], p.max_used);
+    if (in_seq >= q_len * p.HQ) return;
+    const int keys = p.tile_rows
+                         ? tile_keys(used, q_len, in_seq / p.HQ / p.tile_rows, p.tile_rows, p.causal)
+                         : used;
+    if (keys <= p.chunk) return;  // not split: its rows went out whole
+    splits = (keys + p.chunk - 1) / p.chunk;
+    row = q0 + in_seq / p.HQ;
+    pair = row * p.HQ + head;
+    step = p.rows * p.HQ;
+  }
   const int lane = threadIdx.x & 63, j = lane & 15;
   const int g = (WAVES == 1 ? 0 : 4 * wave) + (lane >> 4);
-  const int64_t step = p.rows * p.HQ;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + pair;
   const float* po = p.part_o + pair * D + PER * j;
   float mm = -INFINITY, ll = 0.f, y[PER] = {};
@@ -1080,6 +1116,11 @@ inline bool few_rows(int64_t max_q, int64_t G) { return max_q * G <= 32; }
 
 template <int D>
 void merge_launch(const Attn8Args& a, int64_t seqs, int64_t max_q, hipStream_t stream) {
+  if (a.slots) {  // only what is split
+    seqs = a.n_joins;
+    if (a.tile_rows) max_q = std::min<int64_t>(max_q, a.tile_rows);
+    if (seqs == 0) return;
+  }
   if (a.splits > 16)
     hipLaunchKernelGGL((split_merge_kernel<D, 4>), dim3((unsigned)(max_q * a.HQ), (unsigned)seqs),
                        dim3(256), 0, stream, a);
@@ -1232,6 +1273,57 @@ int64_t qx_paged_attention8_work(const int* cu_q, const int* used, int64_t seqs,
   }
 }
 
+// The split tiles of a list, in the list's order of their first parts.
+static int64_t join_list(const int* cu_q, const int* used, int64_t seqs, int rows, int causal,
+                         int64_t unit, const int* work, int64_t n_work, int* slots, int* joins,
+                         int64_t capacity, int64_t* part_rows) {
+  std::unordered_map<int64_t, int64_t> first;  // (sequence, tile) -> first row of partial results
+  int64_t n = 0, total = 0;
+  for (int64_t i = 0; i < n_work; ++i) {
+    const int s = work[2 * i];
+    const int qt = rows ? work[2 * i + 1] & 0xffff : 0;
+    const int split = rows ? work[2 * i + 1] >> 16 : work[2 * i + 1];
+    QX_CHECK(s >= 0 && s < seqs && split >= 0, "attention8_joins: item %lld is none of this call's",
+             (long long)i);
+    const int q_len = cu_q[s + 1] - cu_q[s];
+    const int64_t keys = rows ? tile_keys(used[s], q_len, qt, rows, causal) : used[s];
+    slots[i] = -1;
+    if (!unit || keys <= unit) continue;
+    const int row0 = rows ? qt * rows : 0, here = rows ? std::min(rows, q_len - row0) : q_len;
+    const int64_t parts = (keys + unit - 1) / unit;
+    QX_CHECK(here > 0 && split < parts, "attention8_joins: item %lld is none of this call's",
+             (long long)i);
+    const auto at = first.emplace((int64_t)s << 32 | qt, total);
+    if (at.second) {
+      QX_CHECK(n < capacity, "attention8_joins: more split tiles than the %lld there is room for",
+               (long long)capacity);
+      QX_CHECK(total + here * parts <= INT32_MAX, "attention8_joins: too many partial rows");
+      const int join[4] = {cu_q[s] + row0, here, (int)total, (int)parts};
+      std::copy(join, join + 4, joins + 4 * n++);
+      total += here * parts;
+    }
+    slots[i] = (int)at.first->second + split * here;
+  }
+  *part_rows = total;
+  return n;
+}
+
+int64_t qx_paged_attention8_joins(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                                  int64_t HK, int causal, int64_t unit, const int* work,
+                                  int64_t n_work, int* slots, int* joins, int64_t capacity,
+                                  int64_t* part_rows) {
+  QX_CHECK(cu_q && used && part_rows && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0 &&
+               n_work >= 0 && (n_work == 0 || (work && slots)) && (capacity <= 0 || joins),
+           "attention8_joins: arguments");
+  try {
+    return join_list(cu_q, used, seqs, unit > 0 ? 0 : tile_height(HQ / HK), causal,
+                     unit < 0 ? -unit : unit, work, n_work, slots, joins, capacity, part_rows);
+  } catch (const std::bad_alloc&) {
+    set_error("attention8_joins: out of host memory");
+    return QX_EINVAL;
+  }
+}
+
 int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used,
                                       int64_t HQ, int64_t HK, int64_t D, int has_work,
                                       int64_t unit) {
@@ -1244,15 +1336,16 @@ int64_t qx_paged_attention8_workspace(int64_t seqs, int64_t rows, int64_t max_q,
   return splits > 1 ? splits * rows * HQ * (D + 2) * 4 : 0;
 }
 
-int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
-                        const void* v_pool, const void* scales, const int* cu_q, const int* used,
-                        const int* table, int64_t table_ld, int64_t seqs, int64_t rows,
-                        int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
-                        int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
-                        int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
-                        const int* work, int64_t n_work, int64_t unit, void* workspace,
-                        int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
-                        int cs_is_f32, const void* q_w, float eps, hipStream_t stream) {
+static int attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
+                      const void* v_pool, const void* scales, const int* cu_q, const int* used,
+                      const int* table, int64_t table_ld, int64_t seqs, int64_t rows,
+                      int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
+                      int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
+                      int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
+                      const int* work, int64_t n_work, int64_t unit, const int* slots,
+                      const int* joins, int64_t n_joins, int64_t part_rows, void* workspace,
+                      int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
+                      int cs_is_f32, const void* q_w, float eps, hipStream_t stream) {
   QX_CHECK(q && k_pool && v_pool && scales && cu_q && used && table, "attention8: null pointer");
   QX_CHECK((out_bf16 != nullptr) != (out_fp8 != nullptr), "attention8: one output, bf16 or e4m3");
   QX_CHECK(D == 64 || D == 128, "attention8: head_dim %lld", (long long)D);
@@ -1277,6 +1370,9 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   QX_CHECK((work || !unit) && (unit <= 0 ? unit % kBK == 0 && unit >= -kMaxKeys
                                          : unit % 128 == 0 && unit <= kMaxChunk),
            "attention8: work items of %lld keys", (long long)unit);
+  QX_CHECK(!slots || (work && n_joins >= 0 && n_joins < 65536 && (joins || n_joins == 0) &&
+                      part_rows >= 0 && part_rows <= INT32_MAX && (part_rows > 0) == (n_joins > 0)),
+           "attention8: %lld joins of %lld partial rows", (long long)n_joins, (long long)part_rows);
   if (seqs == 0 || max_q == 0 || rows == 0 || (work && n_work == 0)) return QX_OK;
   const int64_t G = HQ / HK;
   if (!work) unit = call_unit(seqs * max_used, max_q, max_used, HK, G);
@@ -1284,7 +1380,9 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   QX_CHECK(max_q * HQ < (1LL << 31) && (unit <= 0 || HK * ((max_q * G + cols - 1) / cols) < 65536),
            "attention8: %lld rows a sequence", (long long)max_q);
   const int64_t need =
-      qx_paged_attention8_workspace(seqs, rows, max_q, max_used, HQ, HK, D, work != nullptr, unit);
+      slots ? part_rows * HQ * (D + 2) * 4
+            : qx_paged_attention8_workspace(seqs, rows, max_q, max_used, HQ, HK, D,
+                                            work != nullptr, unit);
   QX_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
            "attention8: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
            (long long)need);
@@ -1295,9 +1393,12 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   a.chunk = (int)(unit < 0 ? -unit : unit);
   a.splits = unit ? (int)std::max<int64_t>(1, (max_used + a.chunk - 1) / a.chunk) : 1;
   a.tile_rows = unit > 0 ? 0 : tile_height(G);
-  a.rows = rows;
+  a.rows = slots ? part_rows : rows;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + (int64_t)a.splits * rows * HQ * D;
+  a.part_ml = a.part_o + (slots ? part_rows : a.splits * rows) * HQ * D;
+  a.slots = slots;
+  a.joins = joins;
+  a.n_joins = (int)n_joins;
   const QNormArgs qn{positions, cos_sin, (const uint16_t*)q_w, eps};
   if (D == 64) attention8_launch<64, 0>(a, qn, work, n_work, seqs, max_q, stream);
   else if (!positions) attention8_launch<128, 0>(a, qn, work, n_work, seqs, max_q, stream);
@@ -1305,5 +1406,39 @@ int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, con
   else attention8_launch<128, 2>(a, qn, work, n_work, seqs, max_q, stream);
   QX_LAUNCH_STATUS();
 }
+
+#define QX_ATTN8_FIRST                                                                            \
+  q, q_ld, q_index, k_pool, v_pool, scales, cu_q, used, table, table_ld, seqs, rows, max_q,       \
+      max_used, HQ, HK, D, page, scale, causal, out_bf16, out_fp8, o_ld, out_scales, os_ld, lse,  \
+      lse_ld, work, n_work, unit
+#define QX_ATTN8_LAST \
+  workspace, workspace_bytes, positions, cos_sin, cs_is_f32, q_w, eps, stream
+
+int qx_paged_attention8(const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool,
+                        const void* v_pool, const void* scales, const int* cu_q, const int* used,
+                        const int* table, int64_t table_ld, int64_t seqs, int64_t rows,
+                        int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
+                        int64_t page, float scale, int causal, void* out_bf16, void* out_fp8,
+                        int64_t o_ld, float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld,
+                        const int* work, int64_t n_work, int64_t unit, void* workspace,
+                        int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
+                        int cs_is_f32, const void* q_w, float eps, hipStream_t stream) {
+  return attention8(QX_ATTN8_FIRST, nullptr, nullptr, 0, 0, QX_ATTN8_LAST);
+}
+
+int qx_paged_attention8_joined(
+    const void* q, int64_t q_ld, const int64_t* q_index, const void* k_pool, const void* v_pool,
+    const void* scales, const int* cu_q, const int* used, const int* table, int64_t table_ld,
+    int64_t seqs, int64_t rows, int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK, int64_t D,
+    int64_t page, float scale, int causal, void* out_bf16, void* out_fp8, int64_t o_ld,
+    float* out_scales, int64_t os_ld, float* lse, int64_t lse_ld, const int* work, int64_t n_work,
+    int64_t unit, const int* slots, const int* joins, int64_t n_joins, int64_t part_rows,
+    void* workspace, int64_t workspace_bytes, const int64_t* positions, const void* cos_sin,
+    int cs_is_f32, const void* q_w, float eps, hipStream_t stream) {
+  QX_CHECK(work && slots, "attention8_joined: null pointer");
+  return attention8(QX_ATTN8_FIRST, slots, joins, n_joins, part_rows, QX_ATTN8_LAST);
+}
+#undef QX_ATTN8_FIRST
+#undef QX_ATTN8_LAST
 
 }  // extern "C"

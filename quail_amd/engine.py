@@ -865,14 +865,18 @@ class Engine:
         n = q3.shape[0] if q_index is None else q_index.shape[0]
         table, used = tables["table"], tables["used"]
         seqs, max_q, max_used = used.shape[0], int(tables["max_q"]), int(tables["max_used"])
-        # the call's items and their keys, when the plan or pack carries them
-        work, n_work, unit = tables.get("work"), 0, 0
+        # the call's items, their keys and the joins of split ones, when the
+        # plan or pack carries them
+        work, name = tables.get("work"), "qx_paged_attention8"
         if torch.is_tensor(work):
-            n_work, unit = int(tables["n_work"]), int(tables["work_rows"])
+            n_work, (n_joins, part_rows) = tables["n_work"], tables["work_joins"]
+            at, name = work.data_ptr(), "qx_paged_attention8_joined"
+            work = (at, n_work, tables["work_rows"], at + 8 * n_work, at + 12 * n_work, n_joins,
+                    part_rows)
+            size = part_rows * hq * (d + 2) * 4
         else:
-            work = None
-        size = _attention8_workspace(seqs, n, max_q, max_used, hq, hk, d, int(work is not None),
-                                     unit)
+            work = None, 0, 0
+            size = _attention8_workspace(seqs, n, max_q, max_used, hq, hk, d, 0, 0)
         space = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
         if quant is None:
             to = out.data_ptr(), None, out.stride(0), None, 0
@@ -887,11 +891,11 @@ class Engine:
             cache = self._rope_cache()
             norm = (positions.data_ptr(), cache.data_ptr(), int(cache.dtype == torch.float32),
                     attn.q_norm.weight.data_ptr(), float(attn.q_norm.variance_epsilon))
-        _lib.call("qx_paged_attention8", q3.data_ptr(), q3.stride(0), _ptr(q_index),
+        _lib.call(name, q3.data_ptr(), q3.stride(0), _ptr(q_index),
                   *self.arena.layer_pointers(layer), tables["cu_q"].data_ptr(), used.data_ptr(),
                   table.data_ptr(), table.stride(0), seqs, n, max_q, max_used, hq, hk, d,
                   PAGE_ROWS, scale, int(tables.get("causal", True)), *to, _ptr(lse),
-                  0 if lse is None else lse.stride(0), _ptr(work), n_work, unit, _ptr(space), size,
+                  0 if lse is None else lse.stride(0), *work, _ptr(space), size,
                   *norm, _stream())
 
     def read_pages(self, q3, tables, layer, *, softmax_scale=None):

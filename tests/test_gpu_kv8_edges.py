@@ -115,3 +115,51 @@ def test_nan_values_of_a_split_without_weight_reach_the_rows(q_len, hq, hk, d):
     nan[:hq // hk, 7] = True
     assert torch.equal(torch.isnan(out.view(q_len, hq, d)), nan.expand(q_len, -1, -1))
     assert bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (24, 8, 64), (8, 8, 128), (64, 8, 128)])
+@pytest.mark.parametrize("q_lens,used", [([100] * 12 + [21, 3], [100] * 12 + [20000, 9000]),
+                                         ([1, 2, 1, 2, 0], [30, 9000, 64, 2100, 5]),
+                                         ([40, 150], [9000, 150])])
+def test_joins_give_the_rows_of_the_call_that_looks_at_every_sequence(hq, hk, d, q_lens, used):
+    """A few rows over long keys among many rows: bit for bit the rows that
+    the list without joins gives, in scratch memory of the split rows alone."""
+    from quail_amd import _lib
+    g = torch.Generator().manual_seed(54)
+    arena = engine_arena(sum(-(-u // PAGE) for u in used) + 3, hk, d)
+    fill(arena, g)
+    plan, cu_q, u, table = plan_of(arena, hq, q_lens, used, g)
+    n_joins, part_rows = plan["work_joins"]
+    assert 0 < n_joins and part_rows < 4096
+    n = int(cu_q[-1])
+    q = torch.randn(n, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    eng = engine_of(arena, hq)
+    out, lse = eng.read_pages(q, plan, 0)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out, lse = eng.read_pages(q, plan, 0)
+    torch.cuda.synchronize()
+    scratch = part_rows * hq * (d + 2) * 4
+    rows = out.numel() * 2 + lse.numel() * 4
+    assert torch.cuda.max_memory_allocated() - before <= 2 * rows + scratch + (1 << 16)
+    # the same list, every row in as many splits as the longest sequence has
+    sizes = len(q_lens), n, plan["max_q"], plan["max_used"], hq, hk, d
+    size = _lib.count("qx_paged_attention8_workspace", *sizes, 1, plan["work_rows"])
+    space = torch.empty(size, dtype=torch.uint8, device=DEV)
+    out2, lse2 = torch.empty_like(out), torch.empty_like(lse)
+    _lib.call("qx_paged_attention8", q.data_ptr(), q.stride(0), None, *arena.layer_pointers(0),
+              plan["cu_q"].data_ptr(), plan["used"].data_ptr(), plan["table"].data_ptr(),
+              plan["table"].stride(0), *sizes, PAGE, d ** -0.5, 1, out2.data_ptr(), None,
+              out2.stride(0), None, 0, lse2.data_ptr(), lse2.stride(0), plan["work"].data_ptr(),
+              plan["n_work"], plan["work_rows"], space.data_ptr(), size, None, None, 0, None, 0.0,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    for s in (i for i, m in enumerate(q_lens) if m and used[i] != 100):
+        at = slice(int(cu_q[s]), int(cu_q[s + 1]))
+        if q_lens[s] > 100:
+            at = slice(at.start, at.start + 2)          # its first rows: the fewest keys
+            part = np.asarray([0, 2], dtype=np.int32), u[s:s + 1] - q_lens[s] + 2
+        else:
+            part = np.asarray([0, q_lens[s]], dtype=np.int32), u[s:s + 1]
+        check_rows(out[at], lse[:, at], q[at], arena, *part, table[s:s + 1], True)
