@@ -621,7 +621,11 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
     itself (Engine.read_pages): sequence s has query rows cu_q[s] .. cu_q[s+1]
     and keys [0, used[s]) through table[s]. cu_q, used and table are int32
     tensors on the device; heads = (HQ, HK, D); eight_bit: whether the arena
-    that is read keeps 8-bit pages."""
+    that is read keeps 8-bit pages.
+
+    The plan is of the tables as they are now, and holds copies: what the
+    caller changes in its own afterwards is not read. Sequences that grow
+    between calls need a plan each time, or tables without one (read_pages)."""
     for name, t, dims in (("cu_q", cu_q, 1), ("used", used, 1), ("table", table, 2)):
         if str(t.dtype) != "torch.int32" or t.dim() != dims or t.stride(dims - 1) != 1:
             raise ValueError(f"{name}: int32 of {dims} dimension(s), rows contiguous")
@@ -638,7 +642,7 @@ def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):
     pages = table.cpu().numpy()[live]
     if (pages < 0).any():
         raise ValueError(f"page {pages.min()} in the table")
-    tables = dict(cu_q=cu_q, used=used, table=table, causal=causal,
+    tables = dict(cu_q=cu_q.clone(), used=used.clone(), table=table.clone(), causal=causal,
                   made_for=(int(host["cu_q"][-1]), *heads, bool(eight_bit)),
                   pages=int(pages.max(initial=-1)) + 1,
                   max_q=int(np.diff(host["cu_q"]).max(initial=0)),

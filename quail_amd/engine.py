@@ -903,7 +903,12 @@ class Engine:
         the arena holds: `tables` as quail_amd.chunk.attention_plan or a
         pack's reads give them (cu_q, used, table, max_q, max_used, causal).
         Returns (bf16 rows (n, HQ*D), log-sum-exps (HQ, n) fp32); a row that
-        sees no key gets 0 and -inf."""
+        sees no key gets 0 and -inf.
+
+        Sequences that grow between calls, or between a captured call's
+        replays, take tables without a plan: a dict of cu_q, used and table
+        (int32, read by each call as they then are), causal, max_q and max_used,
+        bounds of the rows and keys that a sequence may come to have."""
         n, hq, d = q3.shape
         if (hq, d) != (self.num_q_heads, self.head_dim) or q3.dtype != torch.bfloat16:
             raise ValueError(f"query rows of {tuple(q3.shape)} {q3.dtype} for "
