@@ -922,6 +922,11 @@ class Engine:
             if tables["cu_q"].shape[0] != tables["used"].shape[0] + 1:
                 raise ValueError(f"{tables['cu_q'].shape[0]} bounds of query ranges for "
                                  f"{tables['used'].shape[0]} sequences")
+            seqs, pages = tables["table"].shape
+            if seqs < tables["used"].shape[0] or tables["max_used"] > pages * PAGE_ROWS:
+                raise ValueError(f"{tables['used'].shape[0]} sequences of up to "
+                                 f"{tables['max_used']} keys in a table of {seqs} times {pages} "
+                                 "pages")
         elif made_for != (n, hq, self.num_kv_heads, d, eight_bit):
             raise ValueError(f"a plan for {made_for} (rows, HQ, HK, D, 8 bits), not "
                              f"{(n, hq, self.num_kv_heads, d, eight_bit)}")

@@ -64,3 +64,17 @@ def test_captured_reads_of_growing_sequences_take_tables_without_a_plan(hq, hk, 
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, eager))
         check_rows(*held, q, arena, cu_q, used, table, True)
+
+
+def test_tables_without_a_plan_that_do_not_hold_their_bound_are_refused():
+    arena = engine_arena(8)
+    fill(arena, torch.Generator().manual_seed(73))
+    eng = engine_of(arena, 32)
+    ints = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    q = torch.zeros(1, 32, 128, dtype=torch.bfloat16, device=DEV)
+    tables = dict(cu_q=ints(0, 1), used=ints(5), table=ints(1, 2).view(1, 2), causal=True, max_q=1,
+                  max_used=32)
+    assert bool(torch.isfinite(eng.read_pages(q, tables, 0)[0]).all())
+    for bad in (dict(max_used=33), dict(table=ints(1, 2).view(1, 2)[:0])):
+        with pytest.raises(ValueError, match="in a table of"):
+            eng.read_pages(q, dict(tables, **bad), 0)
