@@ -273,7 +273,8 @@ int qx_kv_scatter(const void* k, int64_t k_ld, const void* v, int64_t v_ld, void
  * infinities among them, are written as that, NaN not counted), or with keep > 0 the larger of that and
  * the source page's; kept codes then move by that power of two, exactly
  * unless they become subnormal. A call writes each destination page once,
- * and no item's source is another item's destination.
+ * and no item's source is another item's destination. An item of destination
+ * -1 (keep 0) writes no page; with q_out its rows' q.
  *
  * qx_qk_norm_rope_kv8: rows of the qkv projection, as in
  * qx_qk_norm_rope_kv: K through its norm and RoPE in fp32 and from there to

@@ -235,7 +235,8 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
         rows_in_order=bool(src.size == n_tok and np.array_equal(src, np.arange(n_tok))))
     eight_bit = getattr(arena, "eight_bit", False)
     if eight_bit:
-        unified["page_writes"] = page_writes(src, dst, unified["tail_src"], unified["tail_dst"])
+        unified["page_writes"] = page_writes(src, dst, unified["tail_src"], unified["tail_dst"],
+                                             rows=n_tok)
     meta = dict(layer=0, unified=unified, cu_a=cu_a,
                 max_a=int(np.diff(cu_a).max()) if len(cu_a) > 1 else 0,
                 final_query=_final_query(cu_q, used, table, final))
@@ -565,13 +566,16 @@ def _final_query(cu_q, used, table, final):
 PAGE_ROWS = 16
 
 
-def page_writes(src, dst, tail_src=None, tail_dst=None):
+def page_writes(src, dst, tail_src=None, tail_dst=None, rows=None):
     """The page items of a pack's KV writes to an 8-bit arena, whose scale
     covers a page: pack row src[i] goes to pool row dst[i], after pool rows
     tail_src were copied to tail_dst (a partial page's rows into another's
     same slots). Returns a tuple of (n, 5) int32 arrays, (destination page,
     source page, kept rows, first pack row, rows), to be written one after
-    the other: the writes of each page in order, copied pages last.
+    the other: the writes of each page in order, copied pages last. With
+    `rows`, of the pack in all, rows that go to no page (dst < 0, or not in
+    src) come as items of page -1: the pass that writes the pages writes
+    their q (Engine.qk_norm_rope_kv), as it does every other row's.
 
     Rows of one page form runs of consecutive pack rows in consecutive slots;
     a run keeps the slots before it. A run that starts at or before the slot
@@ -579,8 +583,9 @@ def page_writes(src, dst, tail_src=None, tail_dst=None):
     src, dst = np.asarray(src, dtype=np.int64), np.asarray(dst, dtype=np.int64)
     live = dst >= 0
     src, dst = src[live], dst[live]
+    loose = _loose_items(src, rows)
     if not len(dst):
-        return ()
+        return (loose,) if len(loose) else ()
     page = dst // PAGE_ROWS
     first = np.ones(len(dst), dtype=bool)
     first[1:] = (np.diff(dst) != 1) | (np.diff(src) != 1) | (np.diff(page) != 0)
@@ -613,7 +618,27 @@ def page_writes(src, dst, tail_src=None, tail_dst=None):
         source[hit] = tail_src[where[pos[hit]]] // PAGE_ROWS
         phase[hit] = phase.max() + 1    # once every source page is whole
     items = np.stack([page, source, keep, row0, count], 1).astype(np.int32)
-    return tuple(np.ascontiguousarray(items[phase == p]) for p in np.unique(phase))
+    phases = [np.ascontiguousarray(items[phase == p]) for p in np.unique(phase)]
+    if len(loose):
+        phases[0] = np.concatenate([phases[0], loose])
+    return tuple(phases)
+
+
+def _loose_items(src, rows):
+    """Items of page -1 for the rows [0, rows) that are not in src."""
+    seen = np.zeros(rows or 0, dtype=bool)
+    if len(seen):
+        seen[src] = True
+    left = np.flatnonzero(~seen)
+    if not len(left):
+        return np.empty((0, 5), dtype=np.int32)
+    first = np.ones(len(left), dtype=bool)
+    first[1:] = (np.diff(left) != 1) | (left[1:] % PAGE_ROWS == 0)
+    at = np.flatnonzero(first)
+    items = np.zeros((len(at), 5), dtype=np.int32)
+    items[:, :2], items[:, 3] = -1, left[at]
+    items[:, 4] = np.diff(np.append(at, len(left)))
+    return items
 
 
 def attention_plan(cu_q, used, table, *, heads, causal=True, eight_bit=True):

@@ -78,7 +78,8 @@ __device__ __forceinline__ uint4 load_once(const uint16_t* p) {
 // rest of the page stays as it is. The scale is the fresh rows' own, or the
 // larger of that and the source page's where rows are kept: the kept codes
 // then move by a power of two, exactly unless they become subnormal.
-// Slots of an item: HK of K, HK of V, then (QKV, with a q output) HQ of q.
+// Slots of an item: HK of K, HK of V, then (QKV, with a q output) HQ of q;
+// an item of page -1 has the last ones alone.
 // QKV: rows are the qkv projection's; q and K go through their norm and RoPE
 // (the sums and products of norm_part4 and norm_rope4, in their order) and K
 // from fp32 to its code in one rounding. Otherwise k and v are rows as the
@@ -117,9 +118,11 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs p) {
   const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (wid >= p.waves) return;
   const int* item = p.items + wid / p.groups * 5;
-  const int first = (int)(wid % p.groups) * p.heads;
-  const int last = min(first + p.heads, p.slots);
   const int dst = item[0], src = item[1], keep = item[2], row0 = item[3], count = item[4];
+  const int head0 = (int)(wid % p.groups) * p.heads;
+  const int first = max(head0, dst < 0 ? 2 * p.HK : 0);  // rows of no page: their q alone
+  const int last = min(head0 + p.heads, p.slots);
+  if (first >= last) return;
   const int j = lane % LPR;
   const int64_t kv_row = (int64_t)p.HK * D;
   // this lane's rows of the page, clamped to fresh ones for the loads

@@ -541,7 +541,8 @@ class Engine:
         over qkv). Returns q; this layer's write_kv then copies only the
         retained tails. An 8-bit arena's pages are written by the page items
         meta["unified"]["page_writes"], which hold every row once and the
-        retained tails too."""
+        retained tails too; q's rows are written by these items (page_writes'
+        `rows` adds those that go to no page)."""
         n = qkv.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if qkv.shape[1] < (hq + 2 * hk) * d:
