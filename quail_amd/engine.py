@@ -887,8 +887,9 @@ class Engine:
         norm = None, None, 0, None, 0.0
         if qnorm is not None:
             positions, attn = qnorm
-            if positions.shape != (n,) or positions.dtype != torch.int64:
-                raise ValueError(f"{n} rows need as many int64 positions")
+            if positions.shape != (n,) or positions.dtype != torch.int64 or \
+                    not positions.is_contiguous():
+                raise ValueError(f"{n} rows need as many contiguous int64 positions")
             cache = self._rope_cache()
             norm = (positions.data_ptr(), cache.data_ptr(), int(cache.dtype == torch.float32),
                     attn.q_norm.weight.data_ptr(), float(attn.q_norm.variance_epsilon))
