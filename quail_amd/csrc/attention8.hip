@@ -1222,8 +1222,8 @@ using namespace qx;
 
 extern "C" {
 
-int64_t qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
-                                 int64_t HK, int causal, int64_t* unit) {
+int qx_paged_attention8_unit(const int* cu_q, const int* used, int64_t seqs, int64_t HQ,
+                             int64_t HK, int causal, int64_t* unit) {
   QX_CHECK(cu_q && used && unit && seqs >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
            "attention8_unit: arguments");
   *unit = list_unit(cu_q, used, seqs, HQ, HK, causal);
