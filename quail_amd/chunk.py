@@ -234,16 +234,21 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
         # dst[i], which lets qk_norm_rope write it in place
         rows_in_order=bool(src.size == n_tok and np.array_equal(src, np.arange(n_tok))))
     eight_bit = getattr(arena, "eight_bit", False)
-    if eight_bit:
-        unified["page_writes"] = page_writes(src, dst, unified["tail_src"], unified["tail_dst"],
-                                             rows=n_tok)
-    meta = dict(layer=0, unified=unified, cu_a=cu_a,
-                max_a=int(np.diff(cu_a).max()) if len(cu_a) > 1 else 0,
-                final_query=_final_query(cu_q, used, table, final))
-    if attention_heads is not None:
-        for tables in (unified, meta["final_query"]):
-            if tables is not None:
-                _add_work(tables, attention_heads, eight_bit)
+    try:
+        if eight_bit:
+            unified["page_writes"] = page_writes(src, dst, unified["tail_src"],
+                                                 unified["tail_dst"], rows=n_tok)
+        meta = dict(layer=0, unified=unified, cu_a=cu_a,
+                    max_a=int(np.diff(cu_a).max()) if len(cu_a) > 1 else 0,
+                    final_query=_final_query(cu_q, used, table, final))
+        if attention_heads is not None:
+            for tables in (unified, meta["final_query"]):
+                if tables is not None:
+                    _add_work(tables, attention_heads, eight_bit)
+    except Exception:
+        for key in temporary_keys:      # nothing stays allocated
+            acct.free_key(key)
+        raise
     if timing is not None:
         timing["pack_py"] = timing.get("pack_py", 0.0) + (t1 - t0)
         timing["pack_unified"] = timing.get("pack_unified", 0.0) + (time.perf_counter() - t1)
