@@ -236,8 +236,7 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
     eight_bit = getattr(arena, "eight_bit", False)
     try:
         if eight_bit:
-            unified["page_writes"] = page_writes(src, dst, unified["tail_src"],
-                                                 unified["tail_dst"], rows=n_tok)
+            unified["page_writes"] = page_writes(src, dst, *_read_tails(unified), rows=n_tok)
         meta = dict(layer=0, unified=unified, cu_a=cu_a,
                     max_a=int(np.diff(cu_a).max()) if len(cu_a) > 1 else 0,
                     final_query=_final_query(cu_q, used, table, final))
@@ -627,6 +626,16 @@ def page_writes(src, dst, tail_src=None, tail_dst=None, rows=None):
     if len(loose):
         phases[0] = np.concatenate([phases[0], loose])
     return tuple(phases)
+
+
+def _read_tails(unified):
+    """(tail_src, tail_dst) of a pack without the copies for suffixes of no
+    row, whose sequences nothing reads."""
+    tail_src, tail_dst = unified["tail_src"], unified["tail_dst"]
+    if tail_src is None:
+        return None, None
+    read = np.isin(tail_dst // PAGE_ROWS, unified["dst"] // PAGE_ROWS)
+    return tail_src[read], tail_dst[read]
 
 
 def _loose_items(src, rows):
