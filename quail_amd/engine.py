@@ -17,6 +17,7 @@ Layouts are the reference's: FP8 activations are e4m3fn (n, K) with
 """
 
 import functools
+import math
 import os
 
 import torch
@@ -940,6 +941,8 @@ class Engine:
         lse = torch.empty(hq, n, dtype=torch.float32, device=q3.device)
         if not n:
             return out, lse
+        if not tables["max_used"]:      # no sequence has a key: the table may have no column
+            return out.zero_(), lse.fill_(-math.inf)
         if eight_bit:
             self._attend8(q3, tables, layer, scale, out=out, lse=lse)
         else:

@@ -40,3 +40,14 @@ def test_q_norm_on_load_takes_contiguous_int64_positions(engine, positions):
     norm = SimpleNamespace(weight=torch.ones(128, dtype=torch.bfloat16), variance_epsilon=1e-6)
     with pytest.raises(ValueError, match="positions"):
         eng._attend8(q, plan, 0, 0.1, out=out, qnorm=(positions, SimpleNamespace(q_norm=norm)))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_sequences_without_a_key_need_no_page(engine, causal):
+    """A table of no columns: rows of 0, log-sum-exps of -inf."""
+    eng = engine()
+    plan = attention_plan(ints(0, 1, 3), ints(0, 0), torch.zeros(2, 0, dtype=torch.int32),
+                          heads=(4, 2, 128), causal=causal)
+    out, lse = eng.read_pages(torch.ones(3, 4, 128, dtype=torch.bfloat16), plan, 0)
+    assert out.shape == (3, 512) and not out.any() and lse.shape == (4, 3)
+    assert bool((lse == -float("inf")).all())
