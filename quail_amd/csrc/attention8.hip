@@ -1366,7 +1366,11 @@ static int attention8(const void* q, int64_t q_ld, const int64_t* q_index, const
            "attention8: q-norm on load takes D = 128, cos_sin and q_w, and no q_index");
   QX_CHECK(scale > 0.f && scale <= 3.402823466e38f, "attention8: scale %g", (double)scale);
   QX_CHECK(seqs < 65536, "attention8: %lld sequences exceed the grid", (long long)seqs);
-  QX_CHECK(!work || (n_work >= 0 && n_work * HQ < (1LL << 24)), "attention8: work items");
+  const int64_t G = HQ / HK, cols = 16 * few_blocks(max_q, G);
+  const int64_t col_groups = (max_q * G + cols - 1) / cols;
+  const int64_t per_item = unit > 0 ? HK * col_groups : HQ / tile_heads(G);  // 2^32 threads a launch
+  QX_CHECK(!work || (n_work >= 0 && n_work < (1LL << 24) && n_work * per_item < (1LL << 24)),
+           "attention8: %lld work items", (long long)n_work);
   QX_CHECK((work || !unit) && (unit <= 0 ? unit % kBK == 0 && unit >= -kMaxKeys
                                          : unit % 128 == 0 && unit <= kMaxChunk),
            "attention8: work items of %lld keys", (long long)unit);
@@ -1374,10 +1378,8 @@ static int attention8(const void* q, int64_t q_ld, const int64_t* q_index, const
                       part_rows >= 0 && part_rows <= INT32_MAX && (part_rows > 0) == (n_joins > 0)),
            "attention8: %lld joins of %lld partial rows", (long long)n_joins, (long long)part_rows);
   if (seqs == 0 || max_q == 0 || rows == 0 || (work && n_work == 0)) return QX_OK;
-  const int64_t G = HQ / HK;
   if (!work) unit = call_unit(seqs * max_used, max_q, max_used, HK, G);
-  const int64_t cols = 16 * few_blocks(max_q, G);
-  QX_CHECK(max_q * HQ < (1LL << 31) && (unit <= 0 || HK * ((max_q * G + cols - 1) / cols) < 65536),
+  QX_CHECK(max_q * HQ < (1LL << 31) && (unit <= 0 || HK * col_groups < 65536),
            "attention8: %lld rows a sequence", (long long)max_q);
   const int64_t need =
       slots ? part_rows * HQ * (D + 2) * 4

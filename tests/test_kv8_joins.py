@@ -114,3 +114,20 @@ def test_joins_refuse_lists_of_another_call_and_too_little_room():
                       (dict(size=2 * 32 * 130 * 4 - 1), "workspace"), (dict(unit=-100), "items")):
         with pytest.raises(_lib.QxError, match=match):
             attend(**kw)
+
+
+@pytest.mark.parametrize("hq,hk,unit,most", [(64, 8, 128, 1 << 21), (32, 8, 0, 1 << 21), (8, 8, 0, 1 << 21),
+                                             (128, 8, -64, 1 << 19)])
+def test_items_are_refused_where_a_launch_ends_and_not_before(hq, hk, unit, most):
+    """2^24 workgroups of 256 threads; what comes next in the checks, the
+    missing scratch memory or joins, says that the items were taken."""
+    def attend(n_work):
+        _lib.call("qx_paged_attention8_joined", 16, 16384, None, 16, 16, 16, 16, 16, 16, 8, 1, 1, 1,
+                  256, hq, hk, 128, 16, 0.1, 1, 16, None, 16384, None, 0, None, 0, 16, n_work, unit,
+                  16, None, 1, 1, None, 0, None, None, 0, None, 1e-6, None)
+
+    with pytest.raises(_lib.QxError, match="joins"):
+        attend(most - 1)
+    for n in (most, 1 << 60, -1):
+        with pytest.raises(_lib.QxError, match="work items"):
+            attend(n)
