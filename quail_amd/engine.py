@@ -576,7 +576,8 @@ class Engine:
         rotates q as it loads it (qx_paged_attention_qnorm), with the same
         arithmetic (bit for bit). Returns the raw q columns of qkv (a view).
         An 8-bit arena's pages are written by their page items, as
-        qk_norm_rope_kv does."""
+        qk_norm_rope_kv does; over few rows its attention adds a row's squares
+        in another order, so that a q may come out as the next bf16."""
         n = qkv.shape[0]
         hq, hk, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         if d != GROUP or qkv.shape[1] < (hq + 2 * hk) * d:
