@@ -163,3 +163,31 @@ def test_joins_give_the_rows_of_the_call_that_looks_at_every_sequence(hq, hk, d,
         else:
             part = np.asarray([0, q_lens[s]], dtype=np.int32), u[s:s + 1]
         check_rows(out[at], lse[:, at], q[at], arena, *part, table[s:s + 1], True)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (24, 8, 64), (16, 8, 128)])
+@pytest.mark.parametrize("q_len,used", [(40, 9000), (70, 700), (130, 130), (200, 20000)])
+@pytest.mark.parametrize("back", [-30, 0, 1, 40, 64, 65, 129])
+def test_nan_values_near_the_cut_of_query_tiles(hq, hk, d, q_len, used, back):
+    """The same over query tiles, whole and split over their keys: the NaN
+    `back` keys before the first that the first row does not see."""
+    g = torch.Generator().manual_seed(55)
+    arena = engine_arena(-(-used // PAGE) + 1, hk, d)
+    fill(arena, g)
+    plan, cu_q, u, table = plan_of(arena, hq, (q_len,), (used,), g)
+    assert plan["work_rows"] <= 0
+    q = torch.randn(q_len, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    eng = engine_of(arena, hq)
+    clean, clean_lse = eng.read_pages(q, plan, 0)
+    at = max(0, used - q_len + 1 - back)
+    row = int(table[0, at // PAGE]) * PAGE + at % PAGE
+    v = arena.layer_kv(0)[1]
+    v.view(torch.uint8)[row, 0, 5] = 0x7f
+    v.view(torch.uint8)[row, hk - 1, d - 1] = 0xff
+    out, lse = eng.read_pages(q, plan, 0)
+    first = max(0, at - (used - q_len))
+    want = clean.view(q_len, hq, d).clone()
+    want[first:, :hq // hk, 5] = float("nan")
+    want[first:, -(hq // hk):, d - 1] = float("nan")
+    assert same_codes(out.view(q_len, hq, d), want)
+    assert torch.equal(lse, clean_lse)
