@@ -136,13 +136,15 @@ def test_joins_give_the_rows_of_the_call_that_looks_at_every_sequence(hq, hk, d,
     eng = engine_of(arena, hq)
     out, lse = eng.read_pages(q, plan, 0)
     torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
     torch.cuda.reset_peak_memory_stats()
     out, lse = eng.read_pages(q, plan, 0)
     torch.cuda.synchronize()
     scratch = part_rows * hq * (d + 2) * 4
     rows = out.numel() * 2 + lse.numel() * 4
-    assert torch.cuda.max_memory_allocated() - before <= 2 * rows + scratch + (1 << 16)
+    # as asked for (a cached block may be up to 1 MiB larger)
+    peak = torch.cuda.memory_stats()["requested_bytes.all.peak"] - before
+    assert peak <= 2 * rows + scratch + (1 << 16)
     # the same list, every row in as many splits as the longest sequence has
     sizes = len(q_lens), n, plan["max_q"], plan["max_used"], hq, hk, d
     size = _lib.count("qx_paged_attention8_workspace", *sizes, 1, plan["work_rows"])
