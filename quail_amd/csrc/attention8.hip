@@ -9,10 +9,14 @@
 // (attention.hip). Codes are exact in bf16, so both products run on the bf16
 // matrix cores over the codes themselves: K's scale multiplies a page's 16
 // scores and V's its 16 probabilities, both in fp32 (a power of two each).
-// P is rounded to bf16 (at most 2^-8 of a weight, what the bf16 output rounds
-// by); scores, maxima, sums and outputs stay in fp32. (P in fp16 with V's
-// scales in the softmax's exponent keeps 11 bits, but loses the weights of
-// pages whose scale is far below another's; 3% slower on long documents.)
+// P is rounded to bf16 in query tiles (at most 2^-8 of a weight, what the
+// bf16 output rounds by); few rows, whose matrix cores wait for memory, take
+// what that rounding left as a second product (2^-16; rows then are off by
+// 0.0015 to 0.0017 of their size where one product gave 0.0019 to 0.0024;
+// 0.5 to 3% of a call's time). Scores, maxima, sums and outputs stay in fp32.
+// (P in fp16 with V's scales in the softmax's exponent keeps 11 bits, but
+// loses the weights of pages whose scale is far below another's; 3% slower on
+// long documents.)
 #include <algorithm>
 #include <new>
 #include <type_traits>
@@ -195,10 +199,10 @@ __device__ __forceinline__ void q_norm_columns(v8bf (&qf)[4], const QNormArgs& q
 // touches land in different banks (the conflict counter reads 0).
 //
 // Bound by reading the codes: 200 one-row sequences of ~2100 keys (32 + 8
-// heads of 128, 856 MB) 165 us, 5.2 TB/s, where a kernel that only loads in
+// heads of 128, 856 MB) 166 us, 5.2 TB/s, where a kernel that only loads in
 // this pattern reaches 5.5; 2 sequences of 40,000 keys with 3 rows of 64
 // heads (164 MB, 512 workgroups: one round, its start and end in the open)
-// 42 us. One row over 300 keys: 7.5 us, four memory round trips.
+// 43 us. One row over 300 keys: 7.5 us, four memory round trips.
 constexpr int kRing = 2;
 
 template <int D, int NB, int QN = 0>
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
         }
       }
     }
-    v8bf pf[NB];
+    v8bf pf[NB], pr[NB];  // P and what its rounding to bf16 left
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       const int room = lim[n] - k0 - key0 - g4 * 4;  // key pgi * 16 + r of this lane is below it
@@ -372,7 +376,9 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
       for (int e = 0; e < 8; ++e) {
         const float pe = __builtin_amdgcn_exp2f(z[e] - m_use);
         sum += pe;
-        pf[n][e] = (__bf16)(pe * vs[e >> 2]);
+        const float pv = pe * vs[e >> 2];
+        pf[n][e] = (__bf16)pv;
+        pr[n][e] = (__bf16)(pv - (float)pf[n][e]);
       }
       l[n] = l[n] * alpha + sum;
 #pragma unroll
@@ -393,8 +399,10 @@ __global__ __launch_bounds__(256, 2) void attention8_few_kernel(Attn8Args p, con
       }
       const v8bf vf = codes_bf16(w[0], w[1]);
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int n = 0; n < NB; ++n) {
         o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[n][d], 0, 0, 0);
+        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pr[n], o[n][d], 0, 0, 0);
+      }
     }
   }
   if (__builtin_amdgcn_ballot_w64(nans != 0)) {  // rare: the keys of this wave's steps in the cut, again

@@ -193,3 +193,28 @@ def test_nan_values_near_the_cut_of_query_tiles(hq, hk, d, q_len, used, back):
     want[first:, -(hq // hk):, d - 1] = float("nan")
     assert same_codes(out.view(q_len, hq, d), want)
     assert torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(32, 8, 128), (24, 8, 64), (16, 8, 128), (64, 8, 128)])
+@pytest.mark.parametrize("q_lens,used", [((1,), (300,)), ((2, 1), (40, 3000)), ((3, 1, 1), (9000, 17, 200)),
+                                         ((1,) * 20, tuple(range(5, 105, 5)))])
+def test_few_rows_are_off_by_the_rounding_of_the_output(hq, hk, d, q_lens, used):
+    """P goes into the products to 2^-16 of a weight (its rounding to bf16 and
+    what that left, rounded again): beside the output's own rounding there are
+    only that, the exponent's 2^-20, the scores' and fp32 sums' errors."""
+    g = torch.Generator().manual_seed(56)
+    arena = engine_arena(sum(-(-u // PAGE) for u in used) + 3, hk, d)
+    fill(arena, g)
+    plan, cu_q, u, table = plan_of(arena, hq, q_lens, used, g)
+    assert plan["work_rows"] > 0
+    n = int(cu_q[-1])
+    q = torch.randn(n, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    out, _ = engine_of(arena, hq).read_pages(q, plan, 0)
+    k, v = arena.layer_kv(0)
+    want, _, size, reach = ref.attend(q, k, v, arena.layer_scales(0), cu_q.tolist(), u.tolist(),
+                                      table, True)
+    score = (d + 8) * 2.0 ** -24 * reach[..., None]
+    weight = 2.0 ** -16 + 2 * score + 2.0 ** -20 + max(used) * 2.0 ** -24
+    bound = 2.0 ** -8 * want.abs() + 1.01 * weight * size
+    over = (out.view(n, hq, d).double() - want).abs() - bound
+    assert float(over.max()) <= 1e-30
