@@ -262,19 +262,20 @@ int qx_kv_scatter(const void* k, int64_t k_ld, const void* v, int64_t v_ld, void
  * bytes, and scales one byte for K and one for V per (page of 16 rows, KV
  * head), at scales[(page*HK + head)*2 + (0 for K, 1 for V)]: an E8M0 byte b
  * in [1, 247] that stands for 2^(b - 127). A row's value is code * 2^(b - 127);
- * under 247 codes are at most 240, so that every value is a finite bf16.
+ * where b = 247 codes are at most 240, so that every value is a finite bf16.
  *
  * Both calls write whole page items. items (device): 5 int32 per item,
  * {destination page, source page, keep, row0, count}, keep + count <= 16: the
  * page's rows [0, keep) are the source page's (mostly the destination itself;
  * another for a copied partial page), the next `count` are the fresh rows
  * row0, row0 + 1, ...; rows past them stay as they are. The scale's byte is
- * the least b with max |fresh| <= 448 * 2^(b - 127) (values past 240 * 2^120,
- * infinities among them, are written as that, NaN not counted), or with keep > 0 the larger of that and
- * the source page's; kept codes then move by that power of two, exactly
- * unless they become subnormal. A call writes each destination page once,
- * and no item's source is another item's destination. An item of destination
- * -1 (keep 0) writes no page; with q_out its rows' q.
+ * the least b <= 247 with max |fresh| <= 448 * 2^(b - 127) (values past 240 *
+ * 2^120, infinities among them, are written as that; NaN does not count), or
+ * with keep > 0 the larger of that and the source page's; kept codes then
+ * move by that power of two, exactly unless they become subnormal. A call
+ * writes each destination page once, and no item's source is another item's
+ * destination. An item of destination -1 (keep 0) writes no page; with q_out
+ * its rows' q.
  *
  * qx_qk_norm_rope_kv8: rows of the qkv projection, as in
  * qx_qk_norm_rope_kv: K through its norm and RoPE in fp32 and from there to

@@ -632,17 +632,20 @@ def _read_tails(unified):
     """(tail_src, tail_dst) of a pack without the copies for suffixes of no
     row, whose sequences nothing reads."""
     tail_src, tail_dst = unified["tail_src"], unified["tail_dst"]
-    if tail_src is None:
-        return None, None
+    if tail_src is None or (np.diff(unified["cu_q"]) > 0).all():
+        return tail_src, tail_dst
     read = np.isin(tail_dst // PAGE_ROWS, unified["dst"] // PAGE_ROWS)
     return tail_src[read], tail_dst[read]
 
 
 def _loose_items(src, rows):
     """Items of page -1 for the rows [0, rows) that are not in src."""
-    seen = np.zeros(rows or 0, dtype=bool)
-    if len(seen):
-        seen[src] = True
+    if rows is None:
+        return np.empty((0, 5), dtype=np.int32)
+    if len(src) and not 0 <= src.min() <= src.max() < rows:
+        raise ValueError(f"rows {src.min()} to {src.max()} of {rows}")
+    seen = np.zeros(rows, dtype=bool)
+    seen[src] = True
     left = np.flatnonzero(~seen)
     if not len(left):
         return np.empty((0, 5), dtype=np.int32)

@@ -29,3 +29,9 @@ def test_every_row_is_in_one_item(seed):
     rows = [r for p in phases for _, _, _, r0, c in p.tolist() for r in range(r0, r0 + c)]
     assert sorted(rows) == list(range(n + 5))
     assert all(0 < c and k + c <= 16 for p in phases for _, _, k, _, c in p.tolist())
+
+
+def test_rows_past_the_batch_are_refused():
+    for src in ([3], [-1]):
+        with pytest.raises(ValueError, match="of 3"):
+            page_writes(src, [16], rows=3)
