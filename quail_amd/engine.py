@@ -923,6 +923,10 @@ class Engine:
         eight_bit = self._eight_bit()
         made_for = tables.get("made_for")
         if made_for is None:
+            for name, dims in (("cu_q", 1), ("used", 1), ("table", 2)):
+                t = tables[name]
+                if t.dtype != torch.int32 or t.dim() != dims or t.stride(-1) != 1:
+                    raise ValueError(f"{name}: int32 of {dims} dimension(s), rows contiguous")
             if tables["cu_q"].shape[0] != tables["used"].shape[0] + 1:
                 raise ValueError(f"{tables['cu_q'].shape[0]} bounds of query ranges for "
                                  f"{tables['used'].shape[0]} sequences")

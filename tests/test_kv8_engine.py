@@ -51,3 +51,16 @@ def test_sequences_without_a_key_need_no_page(engine, causal):
     out, lse = eng.read_pages(torch.ones(3, 4, 128, dtype=torch.bfloat16), plan, 0)
     assert out.shape == (3, 512) and not out.any() and lse.shape == (4, 3)
     assert bool((lse == -float("inf")).all())
+
+
+@pytest.mark.parametrize("name,bad", [("used", torch.tensor([20, 5])), ("cu_q", torch.tensor([0, 1, 3])),
+                                      ("table", torch.zeros(2, 2, dtype=torch.int64)),
+                                      ("table", torch.zeros(2, 2, dtype=torch.int32).t()),
+                                      ("table", torch.zeros(4, dtype=torch.int32)),
+                                      ("used", torch.zeros(4, dtype=torch.int32)[::2]),
+                                      ("used", ints(20, 5, 3)), ("max_used", 33)])
+def test_tables_without_a_plan_are_checked(engine, name, bad):
+    tables = dict(cu_q=ints(0, 1, 3), used=ints(20, 5), table=ints(1, 2, 3, 0).view(2, 2), causal=True,
+                  max_q=2, max_used=32)
+    with pytest.raises(ValueError, match=f"^{name}: int32|bounds of query|in a table of"):
+        engine().read_pages(torch.zeros(3, 4, 128, dtype=torch.bfloat16), {**tables, name: bad}, 0)
