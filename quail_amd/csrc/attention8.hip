@@ -202,7 +202,7 @@ __device__ __forceinline__ void q_norm_columns(v8bf (&qf)[4], const QNormArgs& q
 // heads of 128, 856 MB) 166 us, 5.2 TB/s, where a kernel that only loads in
 // this pattern reaches 5.5; 2 sequences of 40,000 keys with 3 rows of 64
 // heads (164 MB, 512 workgroups: one round, its start and end in the open)
-// 43 us. One row over 300 keys: 7.5 us, four memory round trips.
+// 43 us. One row over 300 keys: 7.8 us, four memory round trips.
 constexpr int kRing = 2;
 
 template <int D, int NB, int QN = 0>
