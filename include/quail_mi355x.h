@@ -305,6 +305,23 @@ int qx_copy_pages(void* pools, int64_t n_pools, int64_t pool_stride, int64_t pag
                   const int* src, const int* dst, int64_t count, int64_t num_pages,
                   hipStream_t stream);
 
+/*
+ * Rotary positions of n rows of q (HQ heads) and k (HK heads; either may be
+ * 0): for each pair (a, b) of the first rotary_dim columns of a head,
+ * (i, i + rotary_dim/2) or with interleaved (2i, 2i + 1),
+ *   (a cos t - b sin t, b cos t + a sin t),  t = 2 pi positions[row] turns[i],
+ * cos and sin times `factor`, t's whole turns dropped in 64 bits (any
+ * position), products and sums in fp32, one rounding to the rows' type (type
+ * 0: bf16, 1: fp16, 2: fp32). The other columns are copied. turns: rotary_dim/2
+ * doubles on the device. A row's heads lie D elements apart; the outputs are
+ * the rows themselves or overlap none of them. No counterpart in the
+ * reference, whose rotary module is vLLM's with its table of cos and sin.
+ */
+int qx_rotary(const void* q, int64_t q_ld, const void* k, int64_t k_ld, void* q_out,
+              int64_t qo_ld, void* k_out, int64_t ko_ld, const int64_t* positions,
+              const double* turns, float factor, int64_t n, int64_t HQ, int64_t HK, int64_t D,
+              int64_t rotary_dim, int interleaved, int type, hipStream_t stream);
+
 /* out[i] = table[ids[i]] (bf16 rows). Replaces vLLM embed_tokens (qwen3.py:123). */
 int qx_embed(const void* table, int64_t t_ld, const int64_t* ids, void* out, int64_t o_ld,
              int64_t n, int64_t H, hipStream_t stream);

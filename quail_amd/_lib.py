@@ -65,6 +65,8 @@ SIGNATURES = {
                                    _p, _p, _i32, _p, _f32, _p],
     "qx_copy_pages": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p],
     "qx_pages_compact": [_p, _p, _p, _i64, _p],
+    "qx_rotary": [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _f32, _i64, _i64, _i64, _i64, _i64,
+                  _i32, _i32, _p],
     "qx_embed": [_p, _i64, _p, _p, _i64, _i64, _i64, _p],
     "qx_paged_attention": [_p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
                            _i64, _i64, _f32, _i32, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _i32,

@@ -11,8 +11,9 @@ download, no vLLM) and returns the object `quail_amd.model.build_synthetic`
 returns, so `Qwen3Pipeline` runs it unchanged.
 
 Only what the Qwen3 FP8 path needs is accepted: `Qwen3ForCausalLM`, FP8
-e4m3 weights with 128x128 blocks and dynamic activation scales, no rope
-scaling, no sliding window. Anything else raises.
+e4m3 weights with 128x128 blocks and dynamic activation scales, no sliding
+window, and rope scaling (linear, YaRN: quail_amd.rotary) only where the caller
+asks for it with scaled_rope. Anything else raises.
 """
 
 import json
@@ -22,12 +23,24 @@ from types import SimpleNamespace
 import torch
 
 from quail_amd.model import (BLOCK, Embedding, Qwen3Config, _linear, _norm, rope_cache)
+from quail_amd.rotary import RotaryEmbedding
 
 INDEX = "model.safetensors.index.json"
 
 
-def config_from_json(config: dict, name: str = "checkpoint") -> Qwen3Config:
-    """Qwen3Config from a Hugging Face config.json dictionary.
+def _scaled_rope(config: dict) -> dict | None:
+    """The rope scaling a config.json asks for, or None."""
+    for name in ("rope_scaling", "rope_parameters"):
+        rope = config.get(name) or {}
+        if rope.get("rope_type", rope.get("type", "default")) != "default":
+            return dict(rope)
+    return None
+
+
+def config_from_json(config: dict, name: str = "checkpoint", scaled_rope: bool = False) -> Qwen3Config:
+    """Qwen3Config from a Hugging Face config.json dictionary. With
+    scaled_rope, one whose rope is scaled is taken too; its max_positions are
+    the scaled context where that is longer.
 
     Raises:
         ValueError: not a Qwen3 FP8 block-quantized checkpoint this engine runs.
@@ -42,12 +55,12 @@ def config_from_json(config: dict, name: str = "checkpoint") -> Qwen3Config:
             or quant.get("activation_scheme", "dynamic") != "dynamic"):
         raise ValueError(f"{name}: needs FP8 e4m3 weights in {BLOCK}x{BLOCK} blocks with "
                          f"dynamic activation scales, got quantization_config={quant}")
-    if config.get("rope_scaling"):
+    if config.get("rope_scaling") and not scaled_rope:
         raise ValueError(f"{name}: rope_scaling {config['rope_scaling']} is not supported")
     # transformers 5 writes the rotary settings as rope_parameters
     # {"rope_type", "rope_theta", ...} instead of a top-level rope_theta
     rope = config.get("rope_parameters") or {}
-    if rope.get("rope_type", "default") != "default":
+    if rope.get("rope_type", "default") != "default" and not scaled_rope:
         raise ValueError(f"{name}: rope_parameters {rope} is not supported (only default rope)")
     theta = config.get("rope_theta", rope.get("rope_theta"))
     if config.get("use_sliding_window"):
@@ -56,6 +69,11 @@ def config_from_json(config: dict, name: str = "checkpoint") -> Qwen3Config:
         raise ValueError(f"{name}: attention bias is not supported")
     if config.get("hidden_act", "silu") != "silu":
         raise ValueError(f"{name}: hidden_act {config.get('hidden_act')!r} is not silu")
+    positions = int(config.get("max_position_embeddings", 40960))
+    scaling = _scaled_rope(config) if scaled_rope else None
+    if scaling:
+        trained = int(scaling.get("original_max_position_embeddings") or positions)
+        positions = max(positions, int(trained * float(scaling.get("factor") or 1)))
     heads = int(config["num_attention_heads"])
     hidden = int(config["hidden_size"])
     return Qwen3Config(
@@ -69,16 +87,16 @@ def config_from_json(config: dict, name: str = "checkpoint") -> Qwen3Config:
         vocab=int(config["vocab_size"]),
         eps=float(config.get("rms_norm_eps", 1e-6)),
         theta=float(10000.0 if theta is None else theta),
-        max_positions=int(config.get("max_position_embeddings", 40960)),
+        max_positions=positions,
         tied_head=bool(config.get("tie_word_embeddings", False)),
     )
 
 
-def read_config(path) -> Qwen3Config:
+def read_config(path, scaled_rope: bool = False) -> Qwen3Config:
     """The Qwen3Config of a checkpoint directory (its config.json)."""
     path = Path(path)
     with open(path / "config.json") as f:
-        return config_from_json(json.load(f), name=path.name)
+        return config_from_json(json.load(f), name=path.name, scaled_rope=scaled_rope)
 
 
 class _Tensors:
@@ -125,7 +143,7 @@ def _expect(t: torch.Tensor, name: str, dtype, shape):
     return t
 
 
-def load_qwen3_fp8(path, device="cuda", num_layers: int | None = None):
+def load_qwen3_fp8(path, device="cuda", num_layers: int | None = None, scaled_rope: bool = False):
     """Load a local Qwen3 FP8 checkpoint into the pipeline's module surface.
 
     Args:
@@ -134,6 +152,8 @@ def load_qwen3_fp8(path, device="cuda", num_layers: int | None = None):
         device: where the weights go.
         num_layers: keep only the first layers (model_loading.keep_layers,
             model_loading.py:263-285); every layer's tensors must exist.
+        scaled_rope: take the rope scaling that the config asks for, linear or
+            YaRN (refused otherwise); `rotary_emb` is then a RotaryEmbedding.
 
     Returns:
         An object with `model.layers[i].self_attn.{qkv_proj, o_proj, q_norm,
@@ -143,7 +163,7 @@ def load_qwen3_fp8(path, device="cuda", num_layers: int | None = None):
         when the head is tied) and `config` (a Qwen3Config).
     """
     path = Path(path)
-    cfg = read_config(path)
+    cfg = read_config(path, scaled_rope)
     if num_layers is not None and not 0 < num_layers <= cfg.layers:
         raise ValueError(f"the checkpoint has {cfg.layers} layers; cannot keep {num_layers}")
     tensors = _Tensors(path)
@@ -167,9 +187,16 @@ def load_qwen3_fp8(path, device="cuda", num_layers: int | None = None):
         w = _expect(tensors.get(f"{name}.weight"), f"{name}.weight", bf16, (n,))
         return _norm(w.to(device), cfg.eps)
 
-    cos_sin = rope_cache(d, cfg.max_positions, cfg.theta, device=device)
-    rotary = SimpleNamespace(cos_sin_cache=cos_sin, head_size=d, base=cfg.theta,
-                             is_neox_style=True)
+    config = json.loads((path / "config.json").read_text())
+    scaling = _scaled_rope(config) if scaled_rope else None
+    if scaling:
+        scaling.setdefault("original_max_position_embeddings", config.get("max_position_embeddings"))
+        rotary = RotaryEmbedding(d, base=cfg.theta, max_positions=cfg.max_positions,
+                                 scaling=scaling, device=device)
+    else:
+        cos_sin = rope_cache(d, cfg.max_positions, cfg.theta, device=device)
+        rotary = SimpleNamespace(cos_sin_cache=cos_sin, head_size=d, base=cfg.theta,
+                                 is_neox_style=True)
     layers = []
     for i in range(cfg.layers if num_layers is None else num_layers):
         p = f"model.layers.{i}"
