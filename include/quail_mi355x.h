@@ -322,6 +322,33 @@ int qx_rotary(const void* q, int64_t q_ld, const void* k, int64_t k_ld, void* q_
               const double* turns, float factor, int64_t n, int64_t HQ, int64_t HK, int64_t D,
               int64_t rotary_dim, int interleaved, int type, hipStream_t stream);
 
+/*
+ * Thinning (no counterpart in the reference): for each layer, sequence s and
+ * KV head the rows [0, k), k = min(used[s], keep), of its pages come to hold
+ * the first `sinks` rows, the last `recent` and the heaviest of the others by
+ * `weights` (the first of equal ones; a NaN is heavier than every number; layers,
+ * sequences and heads w_layer, w_seq and w_head floats apart). Kept rows below
+ * k stay; the j-th dropped slot below k takes the j-th kept row at or past k.
+ * kept, (layers, seqs, HK, min(keep, cols)): the row each slot holds, as it was
+ * numbered before, -1 past k; out, (layers, seqs, HK, cols): the slots'
+ * weights, 0 past k. Rows at or past k stay as they were; a call repeated on
+ * the same weights changes nothing.
+ * pools: K and V of each layer in turn, pool_stride bytes apart, rows of HK * D
+ * values of element_bytes 2, or e4m3 codes (1) with scales as qx_kv8_write lays
+ * them out, layers scale_stride bytes apart: a page that a row moves into then
+ * takes the largest scale its rows come with, codes of others move by the power
+ * of two between (exactly unless they become subnormal), and keep is whole
+ * pages. No page may be in two of the call's tables. max_used bounds `used`
+ * (larger entries count as max_used), at most qx_paged_attention_max_keys and
+ * cols. sinks + recent <= keep. weights, kept and out overlap nowhere.
+ */
+int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* scales,
+                 int64_t scale_stride, const float* weights, int64_t w_layer, int64_t w_seq,
+                 int64_t w_head, const int* used, const int* table, int64_t table_ld,
+                 int64_t layers, int64_t seqs, int64_t HK, int64_t D, int64_t page,
+                 int64_t max_used, int64_t cols, int64_t keep, int64_t sinks, int64_t recent,
+                 int* kept, float* out, hipStream_t stream);
+
 /* out[i] = table[ids[i]] (bf16 rows). Replaces vLLM embed_tokens (qwen3.py:123). */
 int qx_embed(const void* table, int64_t t_ld, const int64_t* ids, void* out, int64_t o_ld,
              int64_t n, int64_t H, hipStream_t stream);

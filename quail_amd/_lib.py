@@ -65,6 +65,7 @@ SIGNATURES = {
                                    _p, _p, _i32, _p, _f32, _p],
     "qx_copy_pages": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p],
     "qx_pages_compact": [_p, _p, _p, _i64, _p],
+    "qx_thin_rows": [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p] + 11 * [_i64] + [_p, _p, _p],
     "qx_rotary": [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _f32, _i64, _i64, _i64, _i64, _i64,
                   _i32, _i32, _p],
     "qx_embed": [_p, _i64, _p, _p, _i64, _i64, _i64, _p],

@@ -93,6 +93,9 @@ class KVArena:
             self._pointers = [(k.data_ptr(), v.data_ptr(), s.data_ptr())
                               for k, v, s in zip(self.k, self.v, self._layer_scales)]
         self._claims = {}
+        # keys whose rows are no longer their first tokens, and their ids in the
+        # accounting (a key of the same name that comes later has another)
+        self._thinned = {}
 
     # ---- sizes -------------------------------------------------------------
 
@@ -145,11 +148,13 @@ class KVArena:
         if borrow is None:
             return []
         parent, shared = borrow
+        self.check_whole(parent)
         return self.accounting.shared_pages(parent, shared)
 
     def can_borrow(self, parent, shared: int) -> bool:
         acct = self.accounting
-        return acct.is_resident(parent) and shared <= acct.key_tokens(parent)
+        return (acct.is_resident(parent) and not self.is_thinned(parent)
+                and shared <= acct.key_tokens(parent))
 
     def alloc(self, key, tokens: int, capacity_tokens=None, base_tokens=None, borrow=None):
         """Pages for a fresh key, or None when the free list is short.
@@ -193,6 +198,7 @@ class KVArena:
         the parent it borrows from; then it is activated (pinned). False
         leaves it as it was (evictions may have happened)."""
         acct = self.accounting
+        self.check_whole(key)
         if acct.is_resident(key):
             held = len(acct.table_pages(key))
         else:
@@ -212,6 +218,7 @@ class KVArena:
     def activate(self, key, tokens: int, capacity_tokens=None, base_tokens=None, borrow=None):
         """Make a prefix active (pinned), evicting retained KV when needed."""
         acct = self.accounting
+        self.check_whole(key)
         capacity = tokens if capacity_tokens is None else capacity_tokens
         if acct.is_resident(key):
             acct.pin(key)
@@ -288,6 +295,8 @@ class KVArena:
         capacity = tokens if capacity_tokens is None else capacity_tokens
         if not 0 <= tokens <= held:
             raise ValueError(f"fork of {tokens} tokens from a key that holds {held}")
+        if tokens != held:
+            self.check_whole(key)
         if capacity < tokens:
             raise ValueError(f"capacity of {capacity} tokens for a fork of {tokens}")
         for child in children:
@@ -306,6 +315,8 @@ class KVArena:
         pages = [acct.alloc(child, tokens, capacity, borrowed=shared) for child in children]
         if rest and children:
             self.copy_pages([table[full]] * len(children), [own[0] for own in pages])
+        if self.is_thinned(key):
+            self._thinned.update((child, acct.key_id(child)) for child in children)
         return pages
 
     def compact(self) -> int:
@@ -330,7 +341,12 @@ class KVArena:
         if claim is not None:
             claim.free_asked = True
             return 0
-        return self.accounting.free_key(key)
+        return self._free(key)
+
+    def _free(self, key) -> int:
+        freed = self.accounting.free_key(key)
+        self._thinned.pop(key, None)
+        return freed
 
     def pin(self, key) -> None:
         self.accounting.pin(key)
@@ -339,8 +355,145 @@ class KVArena:
         """Keep a key's first `tokens` (all of them by default) for a later
         operator; it becomes evictable."""
         if tokens is not None:
+            if tokens != self.accounting.key_tokens(key):
+                self.check_whole(key)
             self.accounting.rewind(key, tokens)
         self.accounting.retain(key, priority)
+
+    # ---- thinning ------------------------------------------------------------------
+
+    def thin_rows(self, tables, weights, keep, *, sinks=0, recent=0):
+        """Keep the heaviest rows of sequences that a caller lays out: of every
+        (layer, sequence, KV head) the first `sinks` rows, the last `recent`
+        and the heaviest of the others by `weights`, min(used, keep) in all
+        (ties: the first; a NaN is heavier than every number). Kept rows below
+        `keep` stay where they are, the j-th dropped place takes the j-th kept
+        row past them (current stream), and rows from `keep` on stay as they
+        were: the caller reads min(used, keep) rows afterwards. Keys keep the
+        rotation they were written with.
+
+        tables: used (int32, one per sequence), table (int32 rows of pages) and
+        max_used, a bound of used, as a plan or read_pages' tables have them;
+        no page is in two sequences. weights: fp32 (layers, sequences, KV heads,
+        columns), as Engine.key_weights gathers them. 8-bit pages are kept whole:
+        `keep` is then a multiple of their 16 rows.
+
+        Returns (kept, weights): int32 (layers, sequences, KV heads, min(keep,
+        columns)), the row that each slot holds as it was numbered before, -1
+        past min(used, keep); and the slots' weights in the shape of `weights`,
+        0 past them."""
+        from quail_amd.engine import _stream
+        used, table = tables["used"], tables["table"]
+        heads, dim = self.kv_shape
+        for name, t, dims in (("used", used, 1), ("table", table, 2)):
+            if t.dtype != torch.int32 or t.dim() != dims or t.stride(-1) != 1:
+                raise ValueError(f"{name}: int32 of {dims} dimension(s), rows contiguous")
+        seqs, max_used = used.shape[0], int(tables["max_used"])
+        if weights.dtype != torch.float32 or weights.dim() != 4 or \
+                weights.shape[:3] != (self.num_layers, seqs, heads) or \
+                (weights.shape[3] > 1 and weights.stride(3) != 1):
+            raise ValueError(f"weights: fp32 ({self.num_layers} layers, {seqs} sequences, {heads} heads, "
+                             f"columns), columns contiguous, not {tuple(weights.shape)} "
+                             f"{weights.dtype}")
+        cols = weights.shape[3]
+        if table.shape[0] < seqs or max_used > table.shape[1] * self.page_tokens:
+            raise ValueError(f"{seqs} sequences of up to {max_used} rows in a table of "
+                             f"{table.shape[0]} times {table.shape[1]} pages")
+        if max_used > cols:
+            raise ValueError(f"{cols} columns of weights for up to {max_used} rows")
+        if tables.get("pages", 0) > self.num_pages:
+            raise ValueError(f"page {tables['pages'] - 1} in the plan's table, {self.num_pages} in the "
+                             "arena")
+        if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"{sinks} first and {recent} last rows of {keep} that stay")
+        if self.eight_bit and keep % self.page_tokens:
+            raise ValueError(f"8-bit pages are kept whole: {keep} rows are not a multiple of "
+                             f"{self.page_tokens}")
+        device = self.storage.get_device()
+        if device < 0:
+            raise ValueError("rows are thinned on the GPU; this arena is on the CPU")
+        if not used.get_device() == table.get_device() == weights.get_device() == device:
+            raise ValueError(f"tables and weights on the arena's GPU {device}")
+        shape = (self.num_layers, seqs, heads)
+        kept = torch.empty(*shape, min(keep, cols), dtype=torch.int32, device=weights.device)
+        out = torch.empty(*shape, cols, dtype=torch.float32, device=weights.device)
+        scales = (None, 0) if self.scales is None else (self.scales.data_ptr(), self.scales.stride(0))
+        pool = self.num_pages * self.page_tokens * heads * dim * self.storage.element_size()
+        args = (self.storage.data_ptr(), pool, self.storage.element_size(), *scales,
+                weights.data_ptr(), *weights.stride()[:3], used.data_ptr(), table.data_ptr(),
+                table.stride(0), *shape, dim, self.page_tokens, max_used, cols, keep, sinks, recent,
+                kept.data_ptr(), out.data_ptr())
+        try:
+            if device == torch.cuda.current_device():
+                _lib.call("qx_thin_rows", *args, _stream())
+            else:
+                with torch.cuda.device(device):
+                    _lib.call("qx_thin_rows", *args, _stream())
+        except _lib.QxError as err:
+            if "hipError" in str(err):
+                raise
+            raise ValueError(str(err)) from err
+        return kept, out
+
+    def thin(self, keys, weights, keep, *, sinks=0, recent=0):
+        """thin_rows of resident keys, whose pages past `keep` rows go free.
+        `weights` has a row per key, in the keys' order. A thinned key's rows
+        are no longer its first tokens: it is read and continued by a caller
+        (read_pages, append_rows, fork of all it holds), not lent, packed or
+        activated again. ValueError where a key lends or borrows pages, is held
+        or is being read, or is named twice."""
+        acct = self.accounting
+        keys = list(keys)
+        if len(set(keys)) != len(keys):
+            raise ValueError("a key is thinned once")
+        pages = set()
+        for key in keys:
+            if key in self._claims:
+                raise ValueError(f"{key!r} is held for borrowers or being read")
+            if acct.borrowed_pages(key):
+                raise ValueError(f"{key!r} borrows pages")
+            pages.update(acct.owned_pages(key))
+        for other in acct.resident_keys():
+            if not pages.isdisjoint(acct.borrowed_pages(other)):
+                raise ValueError(f"{other!r} borrows pages of the keys")
+        if not keys:
+            return self.thin_rows(dict(used=torch.zeros(0, dtype=torch.int32, device=weights.device),
+                                       table=torch.zeros(0, 0, dtype=torch.int32,
+                                                         device=weights.device), max_used=0),
+                                  weights, keep, sinks=sinks, recent=recent)
+        table, used = self.block_table(keys)
+        if any(len(acct.table_pages(key)) < acct.pages_needed(n) for key, n in zip(keys, used.tolist())):
+            raise ValueError("a key's leading pages were dropped")
+        tables = dict(used=torch.from_numpy(used).to(self.storage.device),
+                      table=torch.from_numpy(table).to(self.storage.device), max_used=int(used.max()))
+        found = self.thin_rows(tables, weights, keep, sinks=sinks, recent=recent)
+        for key, n in zip(keys, used.tolist()):
+            if n > keep:
+                acct.rewind(key, keep)
+                self._thinned[key] = acct.key_id(key)
+        return found
+
+    def append_rows(self, key, count: int):
+        """Room for `count` more rows of a resident key: their pool rows (host
+        int64), or None with nothing changed when the free list is short."""
+        acct = self.accounting
+        tokens = acct.key_tokens(key)
+        if count < 0:
+            raise ValueError(f"{count} more rows")
+        if acct.grow(key, tokens + count) is None:
+            return None
+        acct.set_tokens(key, tokens + count)
+        return self.capacity_rows(key)[tokens:tokens + count]
+
+    def is_thinned(self, key) -> bool:
+        """Whether a resident key's rows are no longer its first tokens."""
+        ident = self._thinned.get(key)
+        return ident is not None and self.is_resident(key) and self.accounting.key_id(key) == ident
+
+    def check_whole(self, key) -> None:
+        """ValueError for a thinned key."""
+        if self._thinned and self.is_thinned(key):
+            raise ValueError(f"{key!r} was thinned: its rows are not its first tokens")
 
     # ---- holds and reads: keys that admitted or queued readers need -------------
 
@@ -358,7 +511,7 @@ class KVArena:
             return
         del self._claims[key]
         if claim.free_asked:
-            self.accounting.free_key(key)
+            self._free(key)
 
     def hold(self, key, borrowers: int) -> None:
         """Keep a key for `borrowers` documents that will read its pages."""

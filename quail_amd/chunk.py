@@ -109,6 +109,12 @@ def _pack_arrays(handle):
     return out
 
 
+def _check_whole(arena, key):
+    check = getattr(arena, "check_whole", None)
+    if check is not None:
+        check(key)
+
+
 def _suffix_reads(g, s_row0, slen):
     """The answer rows of a group's suffixes (chunk.py:726-764): the marked
     rows of its one suffix (`read_mask`), the last `read_rows[j]` rows of
@@ -168,6 +174,7 @@ def pack_chunk(arena, groups, *, attention_mode="unified", mask="causal", timing
         key = g["key"]
         if not acct.is_resident(key):
             raise ValueError(f"group {key!r}: the paged unified path needs arena pages")
+        _check_whole(arena, key)
         if g.get("paths") is not None:
             raise ValueError(f"group {key!r}: paths pack one suffix, every row read, under "
                              f"tree attention")
@@ -311,6 +318,9 @@ def _pack_tree(arena, groups, *, timing=None, attention_heads=None):
         f = int(g["f"])
         start = int(g.get("start", 0))
         paged = arena.is_resident(key)
+        _check_whole(arena, key)
+        if g.get("read_key") is not None:
+            _check_whole(arena, g["read_key"])
         row0 = n_tok
         sids, slen = _as_suffixes(g["suffixes"])
         n = len(slen)
