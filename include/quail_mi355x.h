@@ -323,6 +323,32 @@ int qx_rotary(const void* q, int64_t q_ld, const void* k, int64_t k_ld, void* q_
               int64_t rotary_dim, int interleaved, int type, hipStream_t stream);
 
 /*
+ * The attention weight that keys have gathered (no counterpart in the
+ * reference): for sequence s, KV head h and key j < cols
+ *   out[s, h, j] = base[s, h, j] + sum over the sequence's query rows i that see j and the
+ *       heads g of h's group of exp(scale q[i, g] . k[j, h] - lse[g, i])
+ * with base 0 where it is NULL (or `out` itself). q rows, cu_q, used, table and
+ * causal as in qx_paged_attention8; lse[g * lse_ld + i] as that call or
+ * qx_attention_lse wrote it; k_pool holds bf16 rows, or with scales the codes of
+ * an 8-bit arena's pages. max_q and max_used bound the sequences' rows and keys
+ * (max_used at most qx_paged_attention_max_keys and cols); `rows` is that of q
+ * and lse. Sequences and heads of base and out lie base_seq, base_head, out_seq
+ * and out_head floats apart. Sums are fp32, in an order that max_q, HQ / HK and
+ * the sequence's own sizes fix. workspace: qx_key_weights_workspace bytes of the
+ * caller's, 16-byte aligned (NULL where that is 0; at most 128 MiB, or one
+ * sequence's), used by this call alone until the stream has passed it.
+ */
+int64_t qx_key_weights_workspace(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ,
+                                 int64_t HK);
+int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld,
+                   const void* k_pool, const void* scales, const int* cu_q, const int* used,
+                   const int* table, int64_t table_ld, int64_t seqs, int64_t rows, int64_t max_q,
+                   int64_t max_used, int64_t HQ, int64_t HK, int64_t D, int64_t page, float scale,
+                   int causal, const float* base, int64_t base_seq, int64_t base_head, float* out,
+                   int64_t out_seq, int64_t out_head, int64_t cols, void* workspace,
+                   int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * Thinning (no counterpart in the reference): for each layer, sequence s and
  * KV head the rows [0, k), k = min(used[s], keep), of its pages come to hold
  * the first `sinks` rows, the last `recent` and the heaviest of the others by

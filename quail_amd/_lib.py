@@ -65,6 +65,9 @@ SIGNATURES = {
                                    _p, _p, _i32, _p, _f32, _p],
     "qx_copy_pages": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p],
     "qx_pages_compact": [_p, _p, _p, _i64, _p],
+    "qx_key_weights_workspace": 5 * [_i64],
+    "qx_key_weights": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p] + 9 * [_i64] + [
+        _f32, _i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],
     "qx_thin_rows": [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p] + 11 * [_i64] + [_p, _p, _p],
     "qx_rotary": [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _f32, _i64, _i64, _i64, _i64, _i64,
                   _i32, _i32, _p],
@@ -115,7 +118,8 @@ SIGNATURES = {
 RETURNS_COUNT = {"qx_paged_attention_work", "qx_paged_attention_tile_rows",
                  "qx_paged_attention_max_keys", "qx_vocab_logprobs_workspace",
                  "qx_vocab_logprobs_noalloc_max_bytes", "qx_paged_attention8_workspace",
-                 "qx_paged_attention8_work", "qx_paged_attention8_joins"}
+                 "qx_paged_attention8_work", "qx_paged_attention8_joins",
+                 "qx_key_weights_workspace"}
 
 
 class QxUnavailable(RuntimeError):

@@ -1,0 +1,403 @@
+// The attention weight that each key has gathered: for sequence s, KV head h
+// and key j
+//   out[s, h, j] = base[s, h, j] + sum over rows i that see j and heads g of h's group of
+//                  exp(scale q[i, g] . k[j, h] - lse[g, i])
+// over pages of 16 rows, bf16 or e4m3 codes with a scale per (page, head).
+//
+// A wave holds kKW keys of one KV head in registers, as the A operand of
+// v_mfma_f32_32x32x16_bf16, and the (row, head of the group) pairs of the
+// sequence stream past it as its columns, kCols of them a step, through LDS
+// (four waves share them). Rows are keys, so a column's log-sum-exp is one value
+// a lane and a key's sum stays in one register across the steps: a score costs
+// one multiply-add, one exponential and one addition, and lanes are added up
+// once, at the end. Sums are fp32, in an order that the call's sizes fix.
+//
+// Where there are few rows a launch of one workgroup per (sequence, head, key
+// tile) writes the result itself (whole sequences' rows in one workgroup).
+// Many rows are cut into chunks, an item per (sequence, head, key tile, chunk)
+// that sees anything, taken in turn by workgroups that find their items from the
+// sequences' lengths; their sums go to scratch memory and a second launch adds
+// them up, chunk by chunk.
+#include "qx_common.h"
+#include "qx_status.h"
+
+#include <algorithm>
+
+namespace qx {
+namespace {
+
+constexpr int kPage = 16;
+constexpr int kMaxKeys = 2560 * kPage;
+constexpr int kKW = 64;              // keys of a wave
+constexpr int kTile = 4 * kKW;       // keys of a workgroup
+constexpr int kCols = 64;            // (row, head) columns of a step
+constexpr int kSeqs = 2048;          // sequences of one launch (their items' bounds in LDS)
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WeightsArgs {
+  const uint16_t* q;
+  int64_t q_ld;
+  const float* lse;
+  int64_t lse_ld;
+  const uint8_t *k, *scales;
+  const int *cu_q, *used, *table;
+  int64_t table_ld;
+  const float* base;
+  int64_t base_s, base_h;
+  float* out;
+  int64_t out_s, out_h;
+  float* part;
+  int seqs, HK, G, rows, max_q, max_used, cols, tiles, chunk;  // chunk: rows of an item
+  uint32_t magic;  // ceil(2^32 / G), G > 1
+  float scale_log2;
+  int causal;
+};
+
+// A sequence: its first row, rows, keys
+struct Seq {
+  int q0, n, used;
+};
+
+__device__ __forceinline__ Seq seq_of(const WeightsArgs& p, int s) {
+  Seq x;
+  x.q0 = min(max(p.cu_q[s], 0), p.rows);
+  x.n = min(min(max(p.cu_q[s + 1] - x.q0, 0), p.rows - x.q0), p.max_q);
+  x.used = min(max(p.used[s], 0), p.max_used);
+  return x;
+}
+
+// keys that row i of the sequence sees: [0, seen)
+__device__ __forceinline__ int seen_by(const WeightsArgs& p, const Seq& x, int i) {
+  return p.causal ? x.used - x.n + i + 1 : x.used;
+}
+
+// the first row that sees key k0 (k0 < used)
+__device__ __forceinline__ int first_row(const WeightsArgs& p, const Seq& x, int k0) {
+  return p.causal ? max(0, k0 - (x.used - x.n)) : 0;
+}
+
+// key tiles that rows [.., hi) of the sequence see anything of
+__device__ __forceinline__ int tiles_seen(const WeightsArgs& p, const Seq& x, int hi) {
+  return (max(min(seen_by(p, x, hi - 1), x.used), 0) + kTile - 1) / kTile;
+}
+
+// acc[i], i < 32, summed over the 32 lanes of a half wave: lane l's is i = l & 31
+__device__ __forceinline__ float sum_lanes(float (&acc)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float send = up ? acc[i] : acc[i + o];
+      acc[i] = (up ? acc[i + o] : acc[i]) + __shfl_xor(send, o, 64);
+    }
+  }
+  return acc[0];
+}
+
+// The sums of one item: keys [k0, k0 + kTile) of head h over rows [lo, hi) of
+// the sequence. Lane l of wave w returns that of key
+// k0 + w * kKW + 32 ((l & 31) >> 4) + 8 ((l & 15) >> 2) + 4 (l >> 5) + (l & 3).
+template <int D, bool F8>
+__device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, int s, int h, int k0,
+                                           int lo, int hi, uint8_t (&stage)[2][kCols * D * 2]) {
+  constexpr int CH = D / 8;        // 16-byte chunks of a row
+  constexpr int C = D / 16;        // MFMAs of a dot product
+  constexpr int LOADS = kCols * CH / 256;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int half = lane >> 5, col = lane & 31;
+  const int kw = k0 + wave * kKW;
+  // the wave's keys; past the last one, the last again (their sums are dropped)
+  v8bf kf[2][C];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int key = min(kw + t * 32 + col, x.used - 1);
+    const int64_t page = p.table[s * p.table_ld + key / kPage];
+    const int64_t at = ((page * kPage + key % kPage) * p.HK + h) * D + half * 8;
+    if constexpr (F8) {
+      const float scale = __uint_as_float(max((uint32_t)p.scales[(page * p.HK + h) * 2], 1u) << 23);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p.k + at + c * 16);
+        const uint4 b = make_uint4(
+            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.x, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w.x, 1) * scale),
+            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.x, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w.x, 3) * scale),
+            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.y, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w.y, 1) * scale),
+            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.y, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w.y, 3) * scale));
+        kf[t][c] = __builtin_bit_cast(v8bf, b);
+      }
+    } else {
+      const uint16_t* k = reinterpret_cast<const uint16_t*>(p.k) + at;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        kf[t][c] = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(k + c * 16));
+    }
+  }
+  const int nf = (hi - lo) * p.G;  // columns of the item
+  const int steps = (nf + kCols - 1) / kCols;
+  const uint16_t* q = p.q + (int64_t)(x.q0 + lo) * p.q_ld + (int64_t)h * p.G * D;
+  const float* lse = p.lse + (int64_t)h * p.G * p.lse_ld + x.q0 + lo;
+  // column f: row f / G, head f % G
+  auto row_of = [&](int f) { return p.G == 1 ? f : (int)__umulhi((uint32_t)f, p.magic); };
+  // a row's chunks lie in LDS at c ^ swizzle, so that the 16 rows that a
+  // quarter wave reads together lie in different banks
+  auto swizzle = [&](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  auto load = [&](int step, int buffer) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int r = j * (256 / CH) + tid / CH;
+      const int f = min(step * kCols + r, nf - 1);
+      const int row = row_of(f), g = f - row * p.G;
+      const int c = tid % CH ^ swizzle(r);
+      lds_dma16(q + row * p.q_ld + g * D + c * 8,
+                &stage[buffer][(j * 256 + wave * 64) * 16]);
+    }
+  };
+  float acc[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+  const int end = min(kw + kKW, x.used);  // past the wave's last key
+  __syncthreads();                        // an earlier item's reads of the stages
+  load(0, 0);
+  for (int step = 0; step < steps; ++step) {
+    float bias[2];
+    int lim[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int f = step * kCols + t * 32 + col, fc = min(f, nf - 1);
+      const int row = row_of(fc), g = fc - row * p.G;
+      bias[t] = lse[g * p.lse_ld + row] * -kLog2e;
+      lim[t] = f < nf ? seen_by(p, x, lo + row) : 0;
+    }
+    // this step's rows have landed, and the last step's are read
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (step + 1 < steps) load(step + 1, (step + 1) & 1);
+    const uint8_t* st = stage[step & 1];
+    const bool whole = (step + 1) * kCols <= nf &&
+                       seen_by(p, x, lo + row_of(step * kCols)) >= end;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (step * kCols + t * 32 >= nf) break;
+      v16f sc[2] = {};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int r = t * 32 + col;
+        const v8bf qf = *reinterpret_cast<const v8bf*>(st + r * D * 2 + ((2 * c + half) ^ swizzle(r)) * 16);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u][c], qf, sc[u], 0, 0, 0);
+      }
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          acc[i] += __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias[t]));
+      } else {
+        const int last = lim[t] - kw - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int key = (i >> 4) * 32 + ((i & 15) >> 2) * 8 + (i & 3);
+          const float w = __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias[t]));
+          acc[i] += key < last ? w : 0.f;
+        }
+      }
+    }
+  }
+  return sum_lanes(acc, lane);
+}
+
+__device__ __forceinline__ int lane_key(int lane) {
+  return ((lane & 31) >> 4) * 32 + ((lane & 15) >> 2) * 8 + (lane >> 5) * 4 + (lane & 3);
+}
+
+// One workgroup per (key tile, sequence, head), heads fastest.
+template <int D, bool F8>
+__global__ __launch_bounds__(256, 2) void key_weights_direct_kernel(WeightsArgs p) {
+  __shared__ __align__(16) uint8_t stage[2][kCols * D * 2];
+  const int id = blockIdx.x;
+  const int h = id % p.HK, s = id / p.HK % p.seqs, k0 = id / p.HK / p.seqs * kTile;
+  const Seq x = seq_of(p, s);
+  const int lane = threadIdx.x & 63;
+  const int j = k0 + (threadIdx.x >> 6) * kKW + lane_key(lane);
+  float sum = 0.f;
+  const int lo = first_row(p, x, k0);
+  if (k0 < x.used && lo < x.n) {
+    const float v = item_sums<D, F8>(p, x, s, h, k0, lo, x.n, stage);
+    sum = j < x.used ? v : 0.f;
+  }
+  if (j >= p.cols) return;
+  if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
+  p.out[s * p.out_s + h * p.out_h + j] = sum;
+}
+
+// Items of a sequence: (chunk, key tile it sees, head), heads fastest
+__device__ __forceinline__ int items_of(const WeightsArgs& p, const Seq& x) {
+  int n = 0;
+  for (int lo = 0; lo < x.n; lo += p.chunk) n += tiles_seen(p, x, min(lo + p.chunk, x.n));
+  return n * p.HK;
+}
+
+template <int D, bool F8>
+__global__ __launch_bounds__(256, 2) void key_weights_chunk_kernel(WeightsArgs p) {
+  __shared__ __align__(16) uint8_t stage[2][kCols * D * 2];
+  __shared__ int bound[kSeqs + 1];  // items of the sequences before
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (tid < 64) {
+    int carry = 0;
+    for (int s0 = 0; s0 < p.seqs; s0 += 64) {
+      const int s = s0 + lane;
+      const int mine = s < p.seqs ? items_of(p, seq_of(p, s)) : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += y;
+      }
+      if (s < p.seqs) bound[s + 1] = carry + sum;
+      carry += __shfl(sum, 63, 64);
+    }
+    if (lane == 0) bound[0] = 0;
+  }
+  __syncthreads();
+  const int total = bound[p.seqs];
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    int a = 0, b = p.seqs;  // bound[a] <= item < bound[b]
+    while (b - a > 1) {
+      const int m = (a + b) / 2;
+      if (bound[m] <= item) a = m; else b = m;
+    }
+    const int s = a;
+    const Seq x = seq_of(p, s);
+    const int h = (item - bound[s]) % p.HK;
+    int i = (item - bound[s]) / p.HK, lo = 0;
+    for (;; lo += p.chunk) {
+      const int n = tiles_seen(p, x, min(lo + p.chunk, x.n));
+      if (i < n) break;
+      i -= n;
+    }
+    const int k0 = i * kTile, hi = min(lo + p.chunk, x.n);
+    const float v = item_sums<D, F8>(p, x, s, h, k0, max(lo, first_row(p, x, k0)), hi, stage);
+    const int64_t at = ((int64_t)(lo / p.chunk * p.seqs + s) * p.HK + h) * p.tiles * kTile;
+    p.part[at + k0 + (tid >> 6) * kKW + lane_key(lane)] = v;
+  }
+}
+
+__global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
+  const int h = blockIdx.y % p.HK, s = blockIdx.y / p.HK;
+  const int j = blockIdx.x * kTile + threadIdx.x;
+  if (j >= p.cols) return;
+  const Seq x = seq_of(p, s);
+  float sum = 0.f;
+  if (j < x.used) {
+    const int first = first_row(p, x, j / kTile * kTile);
+    for (int c = first / p.chunk; c * p.chunk < x.n; ++c)
+      sum += p.part[((int64_t)(c * p.seqs + s) * p.HK + h) * p.tiles * kTile + j];
+  }
+  if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
+  p.out[s * p.out_s + h * p.out_h + j] = sum;
+}
+
+// Rows of an item: whole sequences (0 returned) where they are few
+int64_t chunk_rows(int64_t max_q, int64_t G) {
+  const int64_t rows = (512 * 4 + G - 1) / G;  // 32 steps
+  return max_q <= rows ? 0 : rows;
+}
+
+int64_t tiles_of(int64_t max_used) { return (max_used + kTile - 1) / kTile; }
+
+// Sequences of one pair of launches over chunks, whose sums take
+// `per_sequence` bytes each: within kScratch of scratch memory
+constexpr int64_t kScratch = 128 << 20;
+int64_t batch_of(int64_t seqs, int64_t per_sequence) {
+  const int64_t fit = std::max<int64_t>(1, kScratch / std::max<int64_t>(per_sequence, 1));
+  return std::min<int64_t>({seqs, fit, kSeqs});
+}
+int64_t part_bytes(int64_t max_q, int64_t max_used, int64_t HK, int64_t chunk) {
+  return (max_q + chunk - 1) / chunk * HK * tiles_of(max_used) * kTile * (int64_t)sizeof(float);
+}
+
+}  // namespace
+}  // namespace qx
+
+using namespace qx;
+
+extern "C" {
+
+int64_t qx_key_weights_workspace(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ,
+                                 int64_t HK) {
+  QX_CHECK(seqs >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
+           "key_weights_workspace: sizes");
+  const int64_t rows = chunk_rows(max_q, HQ / HK);
+  if (rows == 0) return 0;
+  const int64_t bytes = part_bytes(max_q, max_used, HK, rows);
+  return batch_of(seqs, bytes) * bytes;
+}
+
+int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld,
+                   const void* k_pool, const void* scales, const int* cu_q, const int* used,
+                   const int* table, int64_t table_ld, int64_t seqs, int64_t rows, int64_t max_q,
+                   int64_t max_used, int64_t HQ, int64_t HK, int64_t D, int64_t page, float scale,
+                   int causal, const float* base, int64_t base_seq, int64_t base_head, float* out,
+                   int64_t out_seq, int64_t out_head, int64_t cols, void* workspace,
+                   int64_t workspace_bytes, hipStream_t stream) {
+  QX_CHECK(D == 64 || D == 128, "key_weights: head_dim %lld (64 or 128)", (long long)D);
+  QX_CHECK(HQ > 0 && HK > 0 && HQ % HK == 0 && HQ <= 4096, "key_weights: heads %lld/%lld",
+           (long long)HQ, (long long)HK);
+  QX_CHECK(page == kPage, "key_weights: page of %lld tokens (16)", (long long)page);
+  QX_CHECK(seqs >= 0 && rows >= 0 && rows < (1LL << 31) && max_q >= 0 && max_used >= 0 &&
+               max_used <= kMaxKeys && max_used <= cols && cols < (1LL << 30),
+           "key_weights: %lld rows, up to %lld keys of %lld columns (at most %d)", (long long)rows,
+           (long long)max_used, (long long)cols, kMaxKeys);
+  QX_CHECK(max_q * (HQ / HK) * (HQ / HK) < (1LL << 31), "key_weights: a sequence of %lld rows",
+           (long long)max_q);
+  QX_CHECK(q_ld % 8 == 0 && (((uintptr_t)q | (uintptr_t)k_pool) & 15) == 0 && lse_ld >= rows,
+           "key_weights: strides or alignment");
+  QX_CHECK(scale == scale && scale - scale == 0.f, "key_weights: scale %g", (double)scale);
+  if (seqs == 0 || cols == 0) return QX_OK;
+  QX_CHECK(cu_q && used && out && (rows == 0 || max_used == 0 || (q && lse && k_pool && table)),
+           "key_weights: null pointer");
+  const int64_t need = qx_key_weights_workspace(seqs, max_q, max_used, HQ, HK);
+  QX_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+           "key_weights: a workspace of %lld bytes, %lld given", (long long)need,
+           (long long)workspace_bytes);
+  const int64_t G = HQ / HK, chunk = chunk_rows(max_q, G);
+  const int64_t tiles = chunk ? tiles_of(max_used) : tiles_of(cols);
+  const int64_t batch = chunk ? batch_of(seqs, part_bytes(max_q, max_used, HK, chunk))
+                              : std::min<int64_t>(seqs, kSeqs);
+  for (int64_t s0 = 0; s0 < seqs; s0 += batch) {
+    const int64_t n = std::min(seqs - s0, batch);
+    WeightsArgs a{(const uint16_t*)q, q_ld, lse, lse_ld, (const uint8_t*)k_pool,
+                  (const uint8_t*)scales, cu_q + s0, used + s0, table + s0 * table_ld, table_ld,
+                  base ? base + s0 * base_seq : nullptr, base_seq, base_head, out + s0 * out_seq,
+                  out_seq, out_head, (float*)workspace, (int)n, (int)HK, (int)G, (int)rows, (int)max_q,
+                  rows ? (int)max_used : 0, (int)cols, (int)tiles, (int)chunk,
+                  (uint32_t)(((1LL << 32) + G - 1) / G), scale * kLog2e, causal};
+#define QX_KEYS(K, grid)                                                                       \
+  if (scales) {                                                                                \
+    if (D == 128) hipLaunchKernelGGL((K<128, true>), grid, dim3(256), 0, stream, a);           \
+    else hipLaunchKernelGGL((K<64, true>), grid, dim3(256), 0, stream, a);                     \
+  } else {                                                                                     \
+    if (D == 128) hipLaunchKernelGGL((K<128, false>), grid, dim3(256), 0, stream, a);          \
+    else hipLaunchKernelGGL((K<64, false>), grid, dim3(256), 0, stream, a);                    \
+  }
+    if (!chunk) {
+      QX_CHECK(tiles * n * HK < (1LL << 24), "key_weights: %lld key tiles exceed one launch",
+               (long long)(tiles * n * HK));
+      QX_KEYS(key_weights_direct_kernel, dim3((unsigned)(tiles * n * HK)));
+    } else {
+      QX_CHECK(n * HK < 65536 && (max_q + chunk - 1) / chunk * tiles * n * HK < (1LL << 31),
+               "key_weights: %lld sequences of %lld heads exceed one launch", (long long)n,
+               (long long)HK);
+      QX_KEYS(key_weights_chunk_kernel, dim3(1024));
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return (int)e;
+      hipLaunchKernelGGL(key_weights_join_kernel, dim3((unsigned)tiles_of(cols), (unsigned)(n * HK)),
+                         dim3(256), 0, stream, a);
+    }
+#undef QX_KEYS
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return QX_OK;
+}
+
+}  // extern "C"

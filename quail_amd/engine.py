@@ -16,6 +16,7 @@ Layouts are the reference's: FP8 activations are e4m3fn (n, K) with
 (N/128, K/128).
 """
 
+import contextlib
 import functools
 import math
 import os
@@ -243,6 +244,11 @@ def _swiglu_launches(n: int, k: int, m: int) -> tuple:
 @functools.lru_cache(maxsize=4096)
 def _attention8_workspace(*sizes):
     return _lib.count("qx_paged_attention8_workspace", *sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _key_weights_workspace(*sizes):
+    return _lib.count("qx_key_weights_workspace", *sizes)
 
 
 class Engine:
@@ -902,17 +908,9 @@ class Engine:
                   0 if lse is None else lse.stride(0), *work, _ptr(space), size,
                   *norm, _stream())
 
-    def read_pages(self, q3, tables, layer, *, softmax_scale=None):
-        """Attention of q3's rows (n, HQ, D), normed and rotated, over pages
-        the arena holds: `tables` as quail_amd.chunk.attention_plan or a
-        pack's reads give them (cu_q, used, table, max_q, max_used, causal).
-        Returns (bf16 rows (n, HQ*D), log-sum-exps (HQ, n) fp32); a row that
-        sees no key gets 0 and -inf.
-
-        Sequences that grow between calls, or between a captured call's
-        replays, take tables without a plan: a dict of cu_q, used and table
-        (int32, read by each call as they then are), causal, max_q and max_used,
-        bounds of the rows and keys that a sequence may come to have."""
+    def _check_reads(self, q3, tables):
+        """Refuses query rows and tables (a plan, or tables without one) that
+        calls over the arena's pages do not take; returns q3's (n, HQ, D)."""
         n, hq, d = q3.shape
         if (hq, d) != (self.num_q_heads, self.head_dim) or q3.dtype != torch.bfloat16:
             raise ValueError(f"query rows of {tuple(q3.shape)} {q3.dtype} for "
@@ -941,6 +939,21 @@ class Engine:
         elif tables["pages"] > self.arena.num_pages:
             raise ValueError(f"page {tables['pages'] - 1} in the plan's table, "
                              f"{self.arena.num_pages} in the arena")
+        return n, hq, d
+
+    def read_pages(self, q3, tables, layer, *, softmax_scale=None):
+        """Attention of q3's rows (n, HQ, D), normed and rotated, over pages
+        the arena holds: `tables` as quail_amd.chunk.attention_plan or a
+        pack's reads give them (cu_q, used, table, max_q, max_used, causal).
+        Returns (bf16 rows (n, HQ*D), log-sum-exps (HQ, n) fp32); a row that
+        sees no key gets 0 and -inf.
+
+        Sequences that grow between calls, or between a captured call's
+        replays, take tables without a plan: a dict of cu_q, used and table
+        (int32, read by each call as they then are), causal, max_q and max_used,
+        bounds of the rows and keys that a sequence may come to have."""
+        n, hq, d = self._check_reads(q3, tables)
+        eight_bit = self._eight_bit()
         scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
         out = torch.empty(n, hq * d, dtype=torch.bfloat16, device=q3.device)
         lse = torch.empty(hq, n, dtype=torch.float32, device=q3.device)
@@ -955,6 +968,64 @@ class Engine:
             self._check_pools(k_pool, v_pool)
             self._lse_call(q3, None, k_pool, v_pool, tables, tables["table"], None, scale, out, lse)
         return out, lse
+
+    def key_weights(self, q3, lse, tables, layer, *, weights=None, out=None, softmax_scale=None):
+        """The attention weight that each key has gathered over q3's rows:
+        for every sequence, KV head and key the sum of the softmax
+        probabilities, exp(scale q . k - lse), over the rows that see the key
+        and the query heads of the group, on top of `weights` where they are
+        given. q3, `tables` (a plan made for this arena, or tables without
+        one) and softmax_scale as read_pages took them, and lse (HQ, n) as it
+        gave them; rows that see no key add nothing.
+
+        weights: fp32 (sequences, KV heads, columns), at least max_used columns.
+        Returns them, as a new tensor or in `out` of the same shape (which may
+        be `weights`): without either, of the tables' width in rows. Columns
+        past a sequence's keys stay as they were (0 without `weights`). The
+        sums are fp32, in the same order at each call of the same sizes."""
+        n, hq, d = self._check_reads(q3, tables)
+        hk = self.num_kv_heads
+        if lse.shape != (hq, n) or lse.dtype != torch.float32 or (n > 1 and lse.stride(1) != 1):
+            raise ValueError(f"log-sum-exps: fp32 ({hq}, {n}), rows contiguous, not "
+                             f"{tuple(lse.shape)} {lse.dtype}")
+        table, used = tables["table"], tables["used"]
+        seqs, max_q, max_used = used.shape[0], int(tables["max_q"]), int(tables["max_used"])
+        device = q3.get_device()
+        if out is None:
+            like = weights
+            cols = table.shape[1] * PAGE_ROWS if like is None else like.shape[-1]
+            out = torch.empty(seqs, hk, cols, dtype=torch.float32, device=q3.device)
+        for name, t in (("weights", weights), ("out", out)):
+            if t is not None and (t.dtype != torch.float32 or t.shape != (seqs, hk, out.shape[-1])
+                                  or (t.shape[2] > 1 and t.stride(2) != 1)):
+                raise ValueError(f"{name}: fp32 ({seqs} sequences, {hk} heads, columns), columns "
+                                 f"contiguous, not {tuple(t.shape)} {t.dtype}")
+        cols = out.shape[2]
+        if cols < max_used:
+            raise ValueError(f"{cols} columns of weights for up to {max_used} keys")
+        if out.stride(0) == 0 and seqs > 1 or out.stride(1) == 0 and hk > 1:
+            raise ValueError("out: sequences and heads overlap")
+        eight_bit = self._eight_bit()
+        k_pool = self.arena.layer_kv(layer)[0]
+        if not eight_bit:
+            self._check_pools(*self.arena.layer_kv(layer))
+        for t in (lse, used, table, k_pool, out, weights):
+            if t is not None and (device < 0 or t.get_device() != device):
+                raise ValueError(f"query rows on {q3.device}, {tuple(t.shape)} on {t.device}")
+        scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
+        size = _key_weights_workspace(seqs, max_q, max_used, hq, hk)
+        args = (q3.data_ptr(), q3.stride(0), lse.data_ptr(), lse.stride(0) if hq > 1 else n,
+                k_pool.data_ptr(), _ptr(self.arena.layer_scales(layer)) if eight_bit else None,
+                tables["cu_q"].data_ptr(), used.data_ptr(), table.data_ptr(), table.stride(0), seqs,
+                n, max_q, max_used, hq, hk, d, self.arena.page_tokens, scale,
+                int(tables.get("causal", True)), _ptr(weights),
+                *((0, 0) if weights is None else weights.stride()[:2]), out.data_ptr(),
+                *out.stride()[:2], cols)
+        with contextlib.nullcontext() if device == torch.cuda.current_device() else \
+                torch.cuda.device(device):
+            space = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
+            _lib.call("qx_key_weights", *args, _ptr(space), size, _stream())
+        return out
 
     def attention_unified(self, q3, k3, v3, meta, *, softmax_scale=None, output=None):
         """Write the chunk's KV to its pages, then one paged causal call with
