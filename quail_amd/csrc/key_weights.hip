@@ -28,8 +28,6 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kMaxKeys = 2560 * kPage;
-constexpr int kKW = 64;              // keys of a wave
-constexpr int kTile = 4 * kKW;       // keys of a workgroup
 constexpr int kCols = 64;            // (row, head) columns of a step
 constexpr int kSeqs = 2048;          // sequences of one launch (their items' bounds in LDS)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -48,10 +46,13 @@ struct WeightsArgs {
   int64_t out_s, out_h;
   float* part;
   int seqs, HK, G, rows, max_q, max_used, cols, tiles, chunk;  // chunk: rows of an item
-  uint32_t magic;  // ceil(2^32 / G), G > 1
+  int step_rows, blocks;  // rows of a step; steps that a row's heads take (G > kCols)
   float scale_log2;
   int causal;
 };
+
+// Keys of a workgroup whose waves hold KT tiles of 32
+constexpr int tile_keys(int KT) { return 4 * 32 * KT; }
 
 // A sequence: its first row, rows, keys
 struct Seq {
@@ -77,14 +78,21 @@ __device__ __forceinline__ int first_row(const WeightsArgs& p, const Seq& x, int
 }
 
 // key tiles that rows [.., hi) of the sequence see anything of
-__device__ __forceinline__ int tiles_seen(const WeightsArgs& p, const Seq& x, int hi) {
-  return (max(min(seen_by(p, x, hi - 1), x.used), 0) + kTile - 1) / kTile;
+__device__ __forceinline__ int tiles_seen(const WeightsArgs& p, const Seq& x, int hi, int tile) {
+  return (max(min(seen_by(p, x, hi - 1), x.used), 0) + tile - 1) / tile;
 }
 
-// acc[i], i < 32, summed over the 32 lanes of a half wave: lane l's is i = l & 31
-__device__ __forceinline__ float sum_lanes(float (&acc)[32], int lane) {
+// acc[i], i < 16 KT, summed over the 32 lanes of a half wave: lane l's is
+// i = l & (16 KT - 1)
+template <int N>
+__device__ __forceinline__ float sum_lanes(float (&acc)[N], int lane) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
+    if (o >= N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+      continue;
+    }
     const bool up = lane & o;
 #pragma unroll
     for (int i = 0; i < o; ++i) {
@@ -95,108 +103,169 @@ __device__ __forceinline__ float sum_lanes(float (&acc)[32], int lane) {
   return acc[0];
 }
 
-// The sums of one item: keys [k0, k0 + kTile) of head h over rows [lo, hi) of
-// the sequence. Lane l of wave w returns that of key
-// k0 + w * kKW + 32 ((l & 31) >> 4) + 8 ((l & 15) >> 2) + 4 (l >> 5) + (l & 3).
-template <int D, bool F8>
+// the key, within its wave's, whose sum a lane gets
+__device__ __forceinline__ int lane_key(int lane) {
+  return ((lane & 31) >> 4) * 32 + ((lane & 15) >> 2) * 8 + (lane >> 5) * 4 + (lane & 3);
+}
+
+// LDS of a workgroup: three stages of a step's rows, and their log-sum-exps.
+// The waves' keys come in through the last two stages.
+constexpr int kStage = kCols * 256;
+constexpr int kLds = 3 * kStage + 3 * kCols * 4;
+
+// The sums of one item: keys [k0, k0 + tile_keys(KT)) of head h over rows
+// [lo, hi) of the sequence. Lane l of wave w returns that of key k0 +
+// w * 32 KT + lane_key(l) (KT 1: of lanes with l & 16 nothing new).
+template <int D, bool F8, int KT>
 __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, int s, int h, int k0,
-                                           int lo, int hi, uint8_t (&stage)[2][kCols * D * 2]) {
-  constexpr int CH = D / 8;        // 16-byte chunks of a row
-  constexpr int C = D / 16;        // MFMAs of a dot product
+                                           int lo, int hi, uint8_t* lds) {
+  constexpr int CH = D / 8;  // 16-byte chunks of a query row
+  constexpr int C = D / 16;  // MFMAs of a dot product
   constexpr int LOADS = kCols * CH / 256;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = opaque(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const int half = lane >> 5, col = lane & 31;
-  const int kw = k0 + wave * kKW;
-  // the wave's keys; past the last one, the last again (their sums are dropped)
-  v8bf kf[2][C];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int key = min(kw + t * 32 + col, x.used - 1);
-    const int64_t page = p.table[s * p.table_ld + key / kPage];
-    const int64_t at = ((page * kPage + key % kPage) * p.HK + h) * D + half * 8;
-    if constexpr (F8) {
-      const float scale = __uint_as_float(max((uint32_t)p.scales[(page * p.HK + h) * 2], 1u) << 23);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p.k + at + c * 16);
-        const uint4 b = make_uint4(
-            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.x, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w.x, 1) * scale),
-            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.x, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w.x, 3) * scale),
-            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.y, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w.y, 1) * scale),
-            pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.y, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w.y, 3) * scale));
-        kf[t][c] = __builtin_bit_cast(v8bf, b);
-      }
-    } else {
-      const uint16_t* k = reinterpret_cast<const uint16_t*>(p.k) + at;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        kf[t][c] = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(k + c * 16));
-    }
-  }
-  const int nf = (hi - lo) * p.G;  // columns of the item
-  const int steps = (nf + kCols - 1) / kCols;
+  const int kw = k0 + wave * 32 * KT;
+  const int steps = (hi - lo + p.step_rows - 1) / p.step_rows * p.blocks;
   const uint16_t* q = p.q + (int64_t)(x.q0 + lo) * p.q_ld + (int64_t)h * p.G * D;
   const float* lse = p.lse + (int64_t)h * p.G * p.lse_ld + x.q0 + lo;
-  // column f: row f / G, head f % G
-  auto row_of = [&](int f) { return p.G == 1 ? f : (int)__umulhi((uint32_t)f, p.magic); };
+  // Column c of a step: row c / heads of it, head c % heads of the block; past
+  // the rows or heads there are, the last ones again, with weight 0.
+  const int heads = min(p.G, kCols);
   // a row's chunks lie in LDS at c ^ swizzle, so that the 16 rows that a
   // quarter wave reads together lie in different banks
-  auto swizzle = [&](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
-  auto load = [&](int step, int buffer) {
+  auto swizzle = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  int slot_row[LOADS], slot_at[LOADS];  // of the rows this lane loads: row of the step, elements
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int c = j * (256 / CH) + tid / CH;
+    slot_row[j] = min(c / heads, p.step_rows - 1);
+    slot_at[j] = c % heads * D + (tid % CH ^ swizzle(c)) * 8;
+  }
+  const int lse_c = wave * 16 + (lane & 15);
+  const int lse_row = min(lse_c / heads, p.step_rows - 1), lse_g = lse_c % heads;
+  auto load = [&](int step) {
+    const int r0 = p.blocks == 1 ? step * p.step_rows : step / p.blocks;  // blocks > 1: a row a step
+    const int g0 = p.blocks == 1 ? 0 : step % p.blocks * kCols;
+    const int buffer = step % 3, last = hi - lo - 1;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int r = j * (256 / CH) + tid / CH;
-      const int f = min(step * kCols + r, nf - 1);
-      const int row = row_of(f), g = f - row * p.G;
-      const int c = tid % CH ^ swizzle(r);
-      lds_dma16(q + row * p.q_ld + g * D + c * 8,
-                &stage[buffer][(j * 256 + wave * 64) * 16]);
+      int at = slot_at[j];
+      if (p.blocks > 1) at += min(g0, p.G - 1 - at / D) * D;
+      lds_dma16(q + min(r0 + slot_row[j], last) * p.q_ld + at,
+                lds + buffer * kStage + (j * 256 + wave * 64) * 16);
     }
+    if (lane < 16)
+      lds_dma4(lse + min(lse_g + g0, p.G - 1) * p.lse_ld + min(r0 + lse_row, last),
+               lds + 3 * kStage + buffer * kCols * 4 + wave * 64);
   };
-  float acc[32];
+  __syncthreads();  // an earlier item's reads of the stages
+  load(0);
+  // The wave's keys; past the last one, the last again (their sums are
+  // dropped). They come through LDS, whole rows a request: read from memory as
+  // the fragments lie, 32 bytes of each of 32 rows, a row's lines came several
+  // times (two contexts of 40,000 keys 97 us)
+  v8bf kf[KT][C];
+  {
+    constexpr int RB = F8 ? D : 2 * D, RCH = RB / 16;  // bytes and chunks of a key's row
+    constexpr int RPL = 64 / RCH;                      // rows of one request
+    constexpr int ROUND = RB == 256 ? 32 : 32 * KT;    // keys at a time, in 8 KiB
+    auto key_swizzle = [](int r) { return RB == 256 ? r & 15 : RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
+    uint8_t* mine = lds + kStage + wave * 8192;
+    const int* table = p.table + s * p.table_ld;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-  const int end = min(kw + kKW, x.used);  // past the wave's last key
-  __syncthreads();                        // an earlier item's reads of the stages
-  load(0, 0);
-  for (int step = 0; step < steps; ++step) {
-    float bias[2];
-    int lim[2];
+    for (int t0 = 0; t0 < KT; t0 += ROUND / 32) {
+      int64_t row[ROUND / RPL];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int f = step * kCols + t * 32 + col, fc = min(f, nf - 1);
-      const int row = row_of(fc), g = fc - row * p.G;
-      bias[t] = lse[g * p.lse_ld + row] * -kLog2e;
-      lim[t] = f < nf ? seen_by(p, x, lo + row) : 0;
+      for (int j = 0; j < ROUND / RPL; ++j) {
+        const int key = min(kw + t0 * 32 + j * RPL + lane / RCH, x.used - 1);
+        row[j] = (int64_t)table[key / kPage] * kPage + key % kPage;
+      }
+#pragma unroll
+      for (int j = 0; j < ROUND / RPL; ++j) {
+        const int c = lane % RCH ^ key_swizzle(j * RPL + lane / RCH);
+        lds_dma16(p.k + (row[j] * p.HK + h) * RB + c * 16, mine + j * 1024);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int t = 0; t < ROUND / 32; ++t) {
+        const int r = t * 32 + col;
+        if constexpr (F8) {
+          const int key = min(kw + (t0 + t) * 32 + col, x.used - 1);
+          const uint32_t b = p.scales[((int64_t)table[key / kPage] * p.HK + h) * 2];
+          const float scale = __uint_as_float(max(b, 1u) << 23);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const uint2 w = *reinterpret_cast<const uint2*>(mine + r * RB + (c ^ key_swizzle(r)) * 16 + half * 8);
+            const uint4 f = make_uint4(
+                pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.x, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w.x, 1) * scale),
+                pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.x, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w.x, 3) * scale),
+                pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.y, 0) * scale, __builtin_amdgcn_cvt_f32_fp8(w.y, 1) * scale),
+                pack2_bf16(__builtin_amdgcn_cvt_f32_fp8(w.y, 2) * scale, __builtin_amdgcn_cvt_f32_fp8(w.y, 3) * scale));
+            kf[t0 + t][c] = __builtin_bit_cast(v8bf, f);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            kf[t0 + t][c] = *reinterpret_cast<const v8bf*>(mine + r * RB + ((2 * c + half) ^ key_swizzle(r)) * 16);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    // this step's rows have landed, and the last step's are read
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (step + 1 < steps) load(step + 1, (step + 1) & 1);
-    const uint8_t* st = stage[step & 1];
-    const bool whole = (step + 1) * kCols <= nf &&
-                       seen_by(p, x, lo + row_of(step * kCols)) >= end;
+  }
+  lds_barrier();  // every wave has its keys
+  if (steps > 1) load(1);
+  float acc[16 * KT];
+#pragma unroll
+  for (int i = 0; i < 16 * KT; ++i) acc[i] = 0.f;
+  const int end = min(kw + 32 * KT, x.used);  // past the wave's last key
+  int col_row[2], col_g[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int c = t * 32 + col;
+    col_row[t] = c / heads < p.step_rows ? c / heads : 1 << 30;
+    col_g[t] = c % heads;
+  }
+  for (int step = 0; step < steps; ++step) {
+    // this step's rows have landed (the next one's may be on their way), and
+    // the last step's are read
+    if (step + 1 < steps) {
+      wait_vmcnt<LOADS + 1>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (step + 2 < steps) load(step + 2);
+    const int r0 = p.blocks == 1 ? step * p.step_rows : step / p.blocks;
+    const int g0 = p.blocks == 1 ? 0 : step % p.blocks * kCols;
+    const int left = hi - lo - r0;  // rows from the step's first on
+    if (kw >= min(seen_by(p, x, lo + r0 + min(left, p.step_rows) - 1), end)) continue;
+    const uint8_t* st = lds + step % 3 * kStage;
+    const float* sl = reinterpret_cast<const float*>(lds + 3 * kStage) + step % 3 * kCols;
+    const bool whole = seen_by(p, x, lo + r0) >= end;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (step * kCols + t * 32 >= nf) break;
-      v16f sc[2] = {};
+      if (t * 32 >= left * heads) break;
+      const bool live = col_row[t] < left && col_g[t] + g0 < p.G;
+      const float bias = live ? sl[t * 32 + col] * -kLog2e : -__builtin_inff();
+      v16f sc[KT] = {};
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int r = t * 32 + col;
         const v8bf qf = *reinterpret_cast<const v8bf*>(st + r * D * 2 + ((2 * c + half) ^ swizzle(r)) * 16);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < KT; ++u)
           sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u][c], qf, sc[u], 0, 0, 0);
       }
       if (whole) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          acc[i] += __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias[t]));
+        for (int i = 0; i < 16 * KT; ++i)
+          acc[i] += __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias));
       } else {
-        const int last = lim[t] - kw - 4 * half;
+        const int last = (live ? seen_by(p, x, lo + r0 + col_row[t]) : 0) - kw - 4 * half;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < 16 * KT; ++i) {
           const int key = (i >> 4) * 32 + ((i & 15) >> 2) * 8 + (i & 3);
-          const float w = __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias[t]));
+          const float w = __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias));
           acc[i] += key < last ? w : 0.f;
         }
       }
@@ -205,47 +274,44 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
   return sum_lanes(acc, lane);
 }
 
-__device__ __forceinline__ int lane_key(int lane) {
-  return ((lane & 31) >> 4) * 32 + ((lane & 15) >> 2) * 8 + (lane >> 5) * 4 + (lane & 3);
-}
-
 // One workgroup per (key tile, sequence, head), heads fastest.
-template <int D, bool F8>
+template <int D, bool F8, int KT>
 __global__ __launch_bounds__(256, 2) void key_weights_direct_kernel(WeightsArgs p) {
-  __shared__ __align__(16) uint8_t stage[2][kCols * D * 2];
+  __shared__ __align__(16) uint8_t lds[kLds];
   const int id = blockIdx.x;
-  const int h = id % p.HK, s = id / p.HK % p.seqs, k0 = id / p.HK / p.seqs * kTile;
+  const int h = id % p.HK, s = id / p.HK % p.seqs, k0 = id / p.HK / p.seqs * tile_keys(KT);
   const Seq x = seq_of(p, s);
   const int lane = threadIdx.x & 63;
-  const int j = k0 + (threadIdx.x >> 6) * kKW + lane_key(lane);
+  const int j = k0 + (threadIdx.x >> 6) * 32 * KT + lane_key(lane & (KT == 1 ? 47 : 63));
   float sum = 0.f;
   const int lo = first_row(p, x, k0);
   if (k0 < x.used && lo < x.n) {
-    const float v = item_sums<D, F8>(p, x, s, h, k0, lo, x.n, stage);
+    const float v = item_sums<D, F8, KT>(p, x, s, h, k0, lo, x.n, lds);
     sum = j < x.used ? v : 0.f;
   }
-  if (j >= p.cols) return;
+  if (j >= p.cols || (KT == 1 && (lane & 16))) return;
   if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
   p.out[s * p.out_s + h * p.out_h + j] = sum;
 }
 
 // Items of a sequence: (chunk, key tile it sees, head), heads fastest
-__device__ __forceinline__ int items_of(const WeightsArgs& p, const Seq& x) {
+__device__ __forceinline__ int items_of(const WeightsArgs& p, const Seq& x, int tile) {
   int n = 0;
-  for (int lo = 0; lo < x.n; lo += p.chunk) n += tiles_seen(p, x, min(lo + p.chunk, x.n));
+  for (int lo = 0; lo < x.n; lo += p.chunk) n += tiles_seen(p, x, min(lo + p.chunk, x.n), tile);
   return n * p.HK;
 }
 
 template <int D, bool F8>
 __global__ __launch_bounds__(256, 2) void key_weights_chunk_kernel(WeightsArgs p) {
-  __shared__ __align__(16) uint8_t stage[2][kCols * D * 2];
+  constexpr int KT = 2, TILE = tile_keys(KT);
+  __shared__ __align__(16) uint8_t lds[kLds];
   __shared__ int bound[kSeqs + 1];  // items of the sequences before
   const int tid = threadIdx.x, lane = tid & 63;
   if (tid < 64) {
     int carry = 0;
     for (int s0 = 0; s0 < p.seqs; s0 += 64) {
       const int s = s0 + lane;
-      const int mine = s < p.seqs ? items_of(p, seq_of(p, s)) : 0;
+      const int mine = s < p.seqs ? items_of(p, seq_of(p, s), TILE) : 0;
       int sum = mine;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -270,27 +336,28 @@ __global__ __launch_bounds__(256, 2) void key_weights_chunk_kernel(WeightsArgs p
     const int h = (item - bound[s]) % p.HK;
     int i = (item - bound[s]) / p.HK, lo = 0;
     for (;; lo += p.chunk) {
-      const int n = tiles_seen(p, x, min(lo + p.chunk, x.n));
+      const int n = tiles_seen(p, x, min(lo + p.chunk, x.n), TILE);
       if (i < n) break;
       i -= n;
     }
-    const int k0 = i * kTile, hi = min(lo + p.chunk, x.n);
-    const float v = item_sums<D, F8>(p, x, s, h, k0, max(lo, first_row(p, x, k0)), hi, stage);
-    const int64_t at = ((int64_t)(lo / p.chunk * p.seqs + s) * p.HK + h) * p.tiles * kTile;
-    p.part[at + k0 + (tid >> 6) * kKW + lane_key(lane)] = v;
+    const int k0 = i * TILE, hi = min(lo + p.chunk, x.n);
+    const float v = item_sums<D, F8, KT>(p, x, s, h, k0, max(lo, first_row(p, x, k0)), hi, lds);
+    const int64_t at = ((int64_t)(lo / p.chunk * p.seqs + s) * p.HK + h) * p.tiles * TILE;
+    p.part[at + k0 + (tid >> 6) * 32 * KT + lane_key(lane)] = v;
   }
 }
 
 __global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
+  constexpr int TILE = tile_keys(2);
   const int h = blockIdx.y % p.HK, s = blockIdx.y / p.HK;
-  const int j = blockIdx.x * kTile + threadIdx.x;
+  const int j = blockIdx.x * 256 + threadIdx.x;
   if (j >= p.cols) return;
   const Seq x = seq_of(p, s);
   float sum = 0.f;
   if (j < x.used) {
-    const int first = first_row(p, x, j / kTile * kTile);
+    const int first = first_row(p, x, j / TILE * TILE);
     for (int c = first / p.chunk; c * p.chunk < x.n; ++c)
-      sum += p.part[((int64_t)(c * p.seqs + s) * p.HK + h) * p.tiles * kTile + j];
+      sum += p.part[((int64_t)(c * p.seqs + s) * p.HK + h) * p.tiles * TILE + j];
   }
   if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
   p.out[s * p.out_s + h * p.out_h + j] = sum;
@@ -302,7 +369,7 @@ int64_t chunk_rows(int64_t max_q, int64_t G) {
   return max_q <= rows ? 0 : rows;
 }
 
-int64_t tiles_of(int64_t max_used) { return (max_used + kTile - 1) / kTile; }
+int64_t tiles_of(int64_t keys, int KT) { return (keys + tile_keys(KT) - 1) / tile_keys(KT); }
 
 // Sequences of one pair of launches over chunks, whose sums take
 // `per_sequence` bytes each: within kScratch of scratch memory
@@ -312,7 +379,8 @@ int64_t batch_of(int64_t seqs, int64_t per_sequence) {
   return std::min<int64_t>({seqs, fit, kSeqs});
 }
 int64_t part_bytes(int64_t max_q, int64_t max_used, int64_t HK, int64_t chunk) {
-  return (max_q + chunk - 1) / chunk * HK * tiles_of(max_used) * kTile * (int64_t)sizeof(float);
+  return (max_q + chunk - 1) / chunk * HK * tiles_of(max_used, 2) * tile_keys(2) *
+         (int64_t)sizeof(float);
 }
 
 }  // namespace
@@ -347,7 +415,7 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
                max_used <= kMaxKeys && max_used <= cols && cols < (1LL << 30),
            "key_weights: %lld rows, up to %lld keys of %lld columns (at most %d)", (long long)rows,
            (long long)max_used, (long long)cols, kMaxKeys);
-  QX_CHECK(max_q * (HQ / HK) * (HQ / HK) < (1LL << 31), "key_weights: a sequence of %lld rows",
+  QX_CHECK(max_q < (1LL << 28) && max_q * (HQ / HK) < (1LL << 31), "key_weights: a sequence of %lld rows",
            (long long)max_q);
   QX_CHECK(q_ld % 8 == 0 && (((uintptr_t)q | (uintptr_t)k_pool) & 15) == 0 && lse_ld >= rows,
            "key_weights: strides or alignment");
@@ -360,7 +428,10 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
            "key_weights: a workspace of %lld bytes, %lld given", (long long)need,
            (long long)workspace_bytes);
   const int64_t G = HQ / HK, chunk = chunk_rows(max_q, G);
-  const int64_t tiles = chunk ? tiles_of(max_used) : tiles_of(cols);
+  // few columns: keys are read once and hardly computed with, so that more and
+  // smaller workgroups read them sooner
+  const int KT = chunk || max_q * G > 4 * kCols ? 2 : 1;
+  const int64_t tiles = chunk ? tiles_of(max_used, KT) : tiles_of(cols, KT);
   const int64_t batch = chunk ? batch_of(seqs, part_bytes(max_q, max_used, HK, chunk))
                               : std::min<int64_t>(seqs, kSeqs);
   for (int64_t s0 = 0; s0 < seqs; s0 += batch) {
@@ -370,27 +441,33 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
                   base ? base + s0 * base_seq : nullptr, base_seq, base_head, out + s0 * out_seq,
                   out_seq, out_head, (float*)workspace, (int)n, (int)HK, (int)G, (int)rows, (int)max_q,
                   rows ? (int)max_used : 0, (int)cols, (int)tiles, (int)chunk,
-                  (uint32_t)(((1LL << 32) + G - 1) / G), scale * kLog2e, causal};
-#define QX_KEYS(K, grid)                                                                       \
-  if (scales) {                                                                                \
-    if (D == 128) hipLaunchKernelGGL((K<128, true>), grid, dim3(256), 0, stream, a);           \
-    else hipLaunchKernelGGL((K<64, true>), grid, dim3(256), 0, stream, a);                     \
-  } else {                                                                                     \
-    if (D == 128) hipLaunchKernelGGL((K<128, false>), grid, dim3(256), 0, stream, a);          \
-    else hipLaunchKernelGGL((K<64, false>), grid, dim3(256), 0, stream, a);                    \
+                  G > kCols ? 1 : (int)(kCols / G), (int)((G + kCols - 1) / kCols), scale * kLog2e,
+                  causal};
+#define QX_KEYS(K, grid, ...)                                                                    \
+  if (scales) {                                                                                  \
+    if (D == 128) hipLaunchKernelGGL((K<128, true __VA_ARGS__>), grid, dim3(256), 0, stream, a); \
+    else hipLaunchKernelGGL((K<64, true __VA_ARGS__>), grid, dim3(256), 0, stream, a);           \
+  } else {                                                                                       \
+    if (D == 128) hipLaunchKernelGGL((K<128, false __VA_ARGS__>), grid, dim3(256), 0, stream, a); \
+    else hipLaunchKernelGGL((K<64, false __VA_ARGS__>), grid, dim3(256), 0, stream, a);          \
   }
     if (!chunk) {
       QX_CHECK(tiles * n * HK < (1LL << 24), "key_weights: %lld key tiles exceed one launch",
                (long long)(tiles * n * HK));
-      QX_KEYS(key_weights_direct_kernel, dim3((unsigned)(tiles * n * HK)));
+      const dim3 grid((unsigned)(tiles * n * HK));
+      if (KT == 1) {
+        QX_KEYS(key_weights_direct_kernel, grid, , 1)
+      } else {
+        QX_KEYS(key_weights_direct_kernel, grid, , 2)
+      }
     } else {
       QX_CHECK(n * HK < 65536 && (max_q + chunk - 1) / chunk * tiles * n * HK < (1LL << 31),
                "key_weights: %lld sequences of %lld heads exceed one launch", (long long)n,
                (long long)HK);
-      QX_KEYS(key_weights_chunk_kernel, dim3(1024));
+      QX_KEYS(key_weights_chunk_kernel, dim3(512))
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
-      hipLaunchKernelGGL(key_weights_join_kernel, dim3((unsigned)tiles_of(cols), (unsigned)(n * HK)),
+      hipLaunchKernelGGL(key_weights_join_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)(n * HK)),
                          dim3(256), 0, stream, a);
     }
 #undef QX_KEYS
