@@ -22,6 +22,7 @@
 #include "qx_status.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace qx {
 namespace {
@@ -82,25 +83,35 @@ __device__ __forceinline__ int tiles_seen(const WeightsArgs& p, const Seq& x, in
   return (max(min(seen_by(p, x, hi - 1), x.used), 0) + tile - 1) / tile;
 }
 
-// acc[i], i < 16 KT, summed over the 32 lanes of a half wave: lane l's is
-// i = l & (16 KT - 1)
-template <int N>
-__device__ __forceinline__ float sum_lanes(float (&acc)[N], int lane) {
+// acc[i], i < N, summed over the 32 lanes of a half wave: lane l's is
+// i = l & (N - 1). Lanes O apart exchange halves of what is left (each O its own
+// function: as one loop, the registers' numbers became selects)
+template <int O, int N>
+__device__ __forceinline__ void sum_lanes(float (&acc)[N], int lane) {
+  if constexpr (O >= N) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (o >= N) {
+    for (int i = 0; i < N; ++i) acc[i] += __shfl_xor(acc[i], O, 64);
+  } else {
+    const bool up = lane & O;
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
-      continue;
-    }
-    const bool up = lane & o;
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float send = up ? acc[i] : acc[i + o];
-      acc[i] = (up ? acc[i + o] : acc[i]) + __shfl_xor(send, o, 64);
+    for (int i = 0; i < O; ++i) {
+      const float send = up ? acc[i] : acc[i + O], own = up ? acc[i + O] : acc[i];
+      acc[i] = own + __shfl_xor(send, O, 64);
     }
   }
-  return acc[0];
+  if constexpr (O > 1) sum_lanes<O / 2>(acc, lane);
+}
+
+// 16 bytes per lane (4 for dma4) to LDS from a uniform base and a lane's own
+// offset in bytes, as lds_dma16
+__device__ __forceinline__ void dma16(const void* base, uint32_t offset, const uint8_t* lds) {
+  const uint32_t addr = (uint32_t)(uintptr_t)(lds_u8*)lds;
+  asm volatile(
+      "s_nop 1\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "{m0}"(addr), "v"(offset), "s"(base)
+      : "memory");
 }
 
 // the key, within its wave's, whose sum a lane gets
@@ -122,7 +133,8 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
   constexpr int CH = D / 8;  // 16-byte chunks of a query row
   constexpr int C = D / 16;  // MFMAs of a dot product
   constexpr int LOADS = kCols * CH / 256;
-  const int tid = opaque(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  const int tid = opaque(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int kw = k0 + wave * 32 * KT;
   const int steps = (hi - lo + p.step_rows - 1) / p.step_rows * p.blocks;
@@ -134,28 +146,27 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
   // a row's chunks lie in LDS at c ^ swizzle, so that the 16 rows that a
   // quarter wave reads together lie in different banks
   auto swizzle = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
-  int slot_row[LOADS], slot_at[LOADS];  // of the rows this lane loads: row of the step, elements
+  const int q_bytes = (int)p.q_ld * 2;
+  auto place = [&](int c) { return min(c / heads, p.step_rows - 1) << 16 | c % heads; };
+  int slot[LOADS];  // rows and heads of the columns this lane loads
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) {
-    const int c = j * (256 / CH) + tid / CH;
-    slot_row[j] = min(c / heads, p.step_rows - 1);
-    slot_at[j] = c % heads * D + (tid % CH ^ swizzle(c)) * 8;
-  }
-  const int lse_c = wave * 16 + (lane & 15);
-  const int lse_row = min(lse_c / heads, p.step_rows - 1), lse_g = lse_c % heads;
+  for (int j = 0; j < LOADS; ++j) slot[j] = place(j * (256 / CH) + tid / CH);
+  const int chunk = (tid % CH ^ swizzle(tid / CH)) * 16;  // the same for all (their distance is whole 16s)
+  const int lse_slot = place(wave * 16 + (lane & 15));
   auto load = [&](int step) {
     const int r0 = p.blocks == 1 ? step * p.step_rows : step / p.blocks;  // blocks > 1: a row a step
     const int g0 = p.blocks == 1 ? 0 : step % p.blocks * kCols;
     const int buffer = step % 3, last = hi - lo - 1;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      int at = slot_at[j];
-      if (p.blocks > 1) at += min(g0, p.G - 1 - at / D) * D;
-      lds_dma16(q + min(r0 + slot_row[j], last) * p.q_ld + at,
-                lds + buffer * kStage + (j * 256 + wave * 64) * 16);
+      int at = (slot[j] & 0xffff) * (2 * D) + chunk;
+      if (p.blocks > 1) at = min((slot[j] & 0xffff) + g0, p.G - 1) * (2 * D) + chunk;
+      // rows of an item and their length are below 2^12 and 2^20
+      dma16(q, __umul24(min(r0 + (slot[j] >> 16), last), q_bytes) + at,
+            lds + buffer * kStage + (j * 256 + wave * 64) * 16);
     }
     if (lane < 16)
-      lds_dma4(lse + min(lse_g + g0, p.G - 1) * p.lse_ld + min(r0 + lse_row, last),
+      lds_dma4(lse + min((lse_slot & 0xffff) + g0, p.G - 1) * p.lse_ld + min(r0 + (lse_slot >> 16), last),
                lds + 3 * kStage + buffer * kCols * 4 + wave * 64);
   };
   __syncthreads();  // an earlier item's reads of the stages
@@ -218,16 +229,17 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
 #pragma unroll
   for (int i = 0; i < 16 * KT; ++i) acc[i] = 0.f;
   const int end = min(kw + 32 * KT, x.used);  // past the wave's last key
-  int col_row[2], col_g[2];
+  // rows and heads of the lane's columns; a step's last columns may be none
+  int at_col[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int c = t * 32 + col;
-    col_row[t] = c / heads < p.step_rows ? c / heads : 1 << 30;
-    col_g[t] = c % heads;
+    at_col[t] = c / heads < p.step_rows ? place(c) : -1;
   }
-  for (int step = 0; step < steps; ++step) {
-    // this step's rows have landed (the next one's may be on their way), and
-    // the last step's are read
+  const int frag = col * D * 2 + (half ^ swizzle(col)) * 16;  // of chunk `half`; 2 c + half is at ^ 32 c
+  // this step's rows have landed (the next one's may be on their way), and the
+  // last step's are read
+  auto arrive = [&](int step) {
     if (step + 1 < steps) {
       wait_vmcnt<LOADS + 1>();
     } else {
@@ -235,43 +247,98 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (step + 2 < steps) load(step + 2);
-    const int r0 = p.blocks == 1 ? step * p.step_rows : step / p.blocks;
+  };
+  auto first_of = [&](int step) { return p.blocks == 1 ? step * p.step_rows : step / p.blocks; };
+  auto is_live = [&](int t, int step, int left) {
     const int g0 = p.blocks == 1 ? 0 : step % p.blocks * kCols;
-    const int left = hi - lo - r0;  // rows from the step's first on
-    if (kw >= min(seen_by(p, x, lo + r0 + min(left, p.step_rows) - 1), end)) continue;
-    const uint8_t* st = lds + step % 3 * kStage;
-    const float* sl = reinterpret_cast<const float*>(lds + 3 * kStage) + step % 3 * kCols;
-    const bool whole = seen_by(p, x, lo + r0) >= end;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t * 32 >= left * heads) break;
-      const bool live = col_row[t] < left && col_g[t] + g0 < p.G;
-      const float bias = live ? sl[t * 32 + col] * -kLog2e : -__builtin_inff();
+    return (uint32_t)(at_col[t] >> 16) < (uint32_t)left && (at_col[t] & 0xffff) + g0 < p.G;
+  };
+  const float* all_lse = reinterpret_cast<const float*>(lds + 3 * kStage);
+  auto bias_of = [&](int t, int step, bool live) {
+    const float v = all_lse[step % 3 * kCols + t * 32 + col] * -kLog2e;
+    return live ? v : -__builtin_inff();
+  };
+  constexpr int AHEAD = 3;
+  auto fragment = [&](int step, int t, int c) {
+    return *reinterpret_cast<const v8bf*>(lds + step % 3 * kStage + t * 64 * D + (opaque(frag) ^ c * 32));
+  };
+  // steps whose first row does not see all of the wave's keys: each score
+  // against the keys that its column sees
+  int step = 0;
+  for (; step < steps; ++step) {
+    const int r0 = first_of(step), left = hi - lo - r0;  // rows from the step's first on
+    if (seen_by(p, x, lo + r0) >= end) break;
+    arrive(step);
+    if (kw >= seen_by(p, x, lo + r0 + min(left, p.step_rows) - 1)) continue;
+#pragma unroll 1
+    for (int t = 0; t < 2 && t * 32 < left * heads; ++t) {
+      const bool live = is_live(t, step, left);
+      const float bias = bias_of(t, step, live);
+      const int last = (live ? seen_by(p, x, lo + r0 + (at_col[t] >> 16)) : 0) - kw - 4 * half;
       v16f sc[KT] = {};
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int r = t * 32 + col;
-        const v8bf qf = *reinterpret_cast<const v8bf*>(st + r * D * 2 + ((2 * c + half) ^ swizzle(r)) * 16);
+        const v8bf qf = fragment(step, t, c);
 #pragma unroll
         for (int u = 0; u < KT; ++u)
           sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u][c], qf, sc[u], 0, 0, 0);
       }
-      if (whole) {
 #pragma unroll
-        for (int i = 0; i < 16 * KT; ++i)
-          acc[i] += __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias));
-      } else {
-        const int last = (live ? seen_by(p, x, lo + r0 + col_row[t]) : 0) - kw - 4 * half;
-#pragma unroll
-        for (int i = 0; i < 16 * KT; ++i) {
-          const int key = (i >> 4) * 32 + ((i & 15) >> 2) * 8 + (i & 3);
-          const float w = __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias));
-          acc[i] += key < last ? w : 0.f;
-        }
+      for (int i = 0; i < 16 * KT; ++i) {
+        const int key = (i >> 4) * 32 + ((i & 15) >> 2) * 8 + (i & 3);
+        const float w = __builtin_amdgcn_exp2f(fmaf(sc[i >> 4][i & 15], p.scale_log2, bias));
+        acc[i] += key < last ? w : 0.f;
       }
     }
   }
-  return sum_lanes(acc, lane);
+  if (step < steps && kw < x.used) {
+    // The rest: the products of 32 columns with the wave's keys, and behind each
+    // of them a share of the exponentials of the 32 columns before. (The waves of
+    // a SIMD run the same steps at about the same time, so the matrix core and
+    // the vector unit overlap only within a wave.)
+    struct Scores {
+      v16f sc[KT];
+      float bias;
+    } s0, s1;
+    auto add = [&](const Scores& y, int i0, int i1) {
+#pragma unroll
+      for (int i = i0; i < i1; ++i)
+        acc[i] += __builtin_amdgcn_exp2f(fmaf(y.sc[i >> 4][i & 15], p.scale_log2, y.bias));
+    };
+    auto products = [&](int t, Scores& y, const Scores& old) {
+      v8bf qf[AHEAD];
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c) qf[c] = fragment(step, t, c);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+          y.sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u][c], qf[c % AHEAD],
+                                                             c == 0 ? v16f{} : y.sc[u], 0, 0, 0);
+        if (c + AHEAD < C) qf[c % AHEAD] = fragment(step, t, c + AHEAD);
+        add(old, c * 16 * KT / C, (c + 1) * 16 * KT / C);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    s1.bias = -__builtin_inff();  // nothing is left of the steps before
+#pragma unroll
+    for (int u = 0; u < KT; ++u) s1.sc[u] = v16f{};
+    for (; step < steps; ++step) {
+      const int left = hi - lo - first_of(step);
+      arrive(step);
+      // (no branch between the two: the exponentials would move behind it)
+      const float bias = bias_of(1, step, is_live(1, step, left));
+      s0.bias = bias_of(0, step, is_live(0, step, left));
+      products(0, s0, s1);
+      s1.bias = bias;
+      products(1, s1, s0);
+    }
+    add(s1, 0, 16 * KT);
+  } else {
+    for (; step < steps; ++step) arrive(step);
+  }
+  sum_lanes<16>(acc, lane);
+  return acc[0];
 }
 
 // One workgroup per (key tile, sequence, head), heads fastest.
@@ -331,10 +398,12 @@ __global__ __launch_bounds__(256, 2) void key_weights_chunk_kernel(WeightsArgs p
       const int m = (a + b) / 2;
       if (bound[m] <= item) a = m; else b = m;
     }
-    const int s = a;
+    // (found by way of LDS; every lane has the same)
+    const int s = __builtin_amdgcn_readfirstlane(a);
     const Seq x = seq_of(p, s);
-    const int h = (item - bound[s]) % p.HK;
-    int i = (item - bound[s]) / p.HK, lo = 0;
+    const int of = item - __builtin_amdgcn_readfirstlane(bound[s]);
+    const int h = of % p.HK;
+    int i = of / p.HK, lo = 0;
     for (;; lo += p.chunk) {
       const int n = tiles_seen(p, x, min(lo + p.chunk, x.n), TILE);
       if (i < n) break;
@@ -417,6 +486,8 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
            (long long)max_used, (long long)cols, kMaxKeys);
   QX_CHECK(max_q < (1LL << 28) && max_q * (HQ / HK) < (1LL << 31), "key_weights: a sequence of %lld rows",
            (long long)max_q);
+  QX_CHECK(q_ld >= 0 && q_ld < (1LL << 19), "key_weights: rows %lld elements apart (below 2^19)",
+           (long long)q_ld);
   QX_CHECK(q_ld % 8 == 0 && (((uintptr_t)q | (uintptr_t)k_pool) & 15) == 0 && lse_ld >= rows,
            "key_weights: strides or alignment");
   QX_CHECK(scale == scale && scale - scale == 0.f, "key_weights: scale %g", (double)scale);
