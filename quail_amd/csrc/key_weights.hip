@@ -30,7 +30,9 @@ namespace {
 constexpr int kPage = 16;
 constexpr int kMaxKeys = 2560 * kPage;
 constexpr int kCols = 64;            // (row, head) columns of a step
-constexpr int kSeqs = 2048;          // sequences of one launch (their items' bounds in LDS)
+constexpr int kSeqs = 2048;          // sequences of one launch (their bounds in LDS)
+constexpr int kShares = 512;         // workgroups that the work is shared by: two a CU
+constexpr int kMinShare = 2;         // groups of a share, at least
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct WeightsArgs {
@@ -46,8 +48,11 @@ struct WeightsArgs {
   float* out;
   int64_t out_s, out_h;
   float* part;
-  int seqs, HK, G, rows, max_q, max_used, cols, tiles, chunk;  // chunk: rows of an item
+  int* bound;
+  int seqs, HK, G, rows, max_q, max_used, cols, tiles;
   int step_rows, blocks;  // rows of a step; steps that a row's heads take (G > kCols)
+  int drop;               // groups that a tile has fewer than the one before
+  int row_limit;          // rows whose elements 32 bits of bytes reach
   float scale_log2;
   int causal;
 };
@@ -78,9 +83,32 @@ __device__ __forceinline__ int first_row(const WeightsArgs& p, const Seq& x, int
   return p.causal ? max(0, k0 - (x.used - x.n)) : 0;
 }
 
-// key tiles that rows [.., hi) of the sequence see anything of
-__device__ __forceinline__ int tiles_seen(const WeightsArgs& p, const Seq& x, int hi, int tile) {
-  return (max(min(seen_by(p, x, hi - 1), x.used), 0) + tile - 1) / tile;
+// The work of a sequence, in groups of step_rows rows: its key tiles, those that
+// every row sees (`full` groups each), and of the others the first one's groups;
+// each next one has p.drop fewer (or up to one less than that where step_rows does
+// not divide a tile: the last groups then hold no row).
+struct Work {
+  int tiles, seen, full, rest;
+};
+
+__device__ __forceinline__ Work work_of(const WeightsArgs& p, const Seq& x, int tile) {
+  Work w{0, 0, 0, 0};
+  if (x.n == 0 || x.used == 0) return w;
+  w.tiles = (x.used + tile - 1) / tile;
+  w.full = (x.n + p.step_rows - 1) / p.step_rows;
+  const int older = x.used - x.n;  // keys that every row sees, and one more
+  w.seen = !p.causal ? w.tiles : older < 0 ? 0 : min(older / tile + 1, w.tiles);
+  if (w.seen < w.tiles) w.rest = (x.used - w.seen * tile + p.step_rows - 1) / p.step_rows;
+  return w;
+}
+
+// groups of tile t, and of the tiles before it
+__device__ __forceinline__ int groups_of(const Work& w, int drop, int t) {
+  return t < w.seen ? w.full : w.rest - (t - w.seen) * drop;
+}
+__device__ __forceinline__ int groups_before(const Work& w, int drop, int t) {
+  const int m = max(t - w.seen, 0);
+  return min(t, w.seen) * w.full + m * w.rest - drop * (m * (m - 1) / 2);
 }
 
 // acc[i], i < N, summed over the 32 lanes of a half wave: lane l's is
@@ -161,7 +189,7 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
     for (int j = 0; j < LOADS; ++j) {
       int at = (slot[j] & 0xffff) * (2 * D) + chunk;
       if (p.blocks > 1) at = min((slot[j] & 0xffff) + g0, p.G - 1) * (2 * D) + chunk;
-      // rows of an item and their length are below 2^12 and 2^20
+      // (an item's rows and their bytes are below 2^24, and together below 2^31)
       dma16(q, __umul24(min(r0 + (slot[j] >> 16), last), q_bytes) + at,
             lds + buffer * kStage + (j * 256 + wave * 64) * 16);
     }
@@ -361,95 +389,138 @@ __global__ __launch_bounds__(256, 2) void key_weights_direct_kernel(WeightsArgs 
   p.out[s * p.out_s + h * p.out_h + j] = sum;
 }
 
-// Items of a sequence: (chunk, key tile it sees, head), heads fastest
-__device__ __forceinline__ int items_of(const WeightsArgs& p, const Seq& x, int tile) {
-  int n = 0;
-  for (int lo = 0; lo < x.n; lo += p.chunk) n += tiles_seen(p, x, min(lo + p.chunk, x.n), tile);
-  return n * p.HK;
+// Groups of a head from each sequence on (bound[s], s <= seqs), by one wave
+__device__ __forceinline__ void bounds(const WeightsArgs& p, int lane, int tile, int* bound) {
+  int carry = 0;
+  for (int s0 = 0; s0 < p.seqs; s0 += 64) {
+    const int s = s0 + lane;
+    int sum = 0;
+    if (s < p.seqs) {
+      const Work w = work_of(p, seq_of(p, s), tile);
+      sum = groups_before(w, p.drop, w.tiles);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += y;
+    }
+    if (s < p.seqs) bound[s + 1] = carry + sum;
+    carry += __shfl(sum, 63, 64);
+  }
+  if (lane == 0) bound[0] = 0;
 }
 
+// groups of a workgroup
+__device__ __forceinline__ int share_of(int total, int workgroups) {
+  return max(kMinShare, (total + workgroups - 1) / workgroups);
+}
+
+// Many rows: the groups of all heads' sequences' key tiles, in that order, in
+// equal shares, one a workgroup. A share begins and ends anywhere; each tile's
+// part of it goes to scratch memory, at the tile's number plus the workgroup's
+// (both only rise along the order).
 template <int D, bool F8>
-__global__ __launch_bounds__(256, 2) void key_weights_chunk_kernel(WeightsArgs p) {
+__global__ __launch_bounds__(256, 2) void key_weights_share_kernel(WeightsArgs p) {
   constexpr int KT = 2, TILE = tile_keys(KT);
   __shared__ __align__(16) uint8_t lds[kLds];
-  __shared__ int bound[kSeqs + 1];  // items of the sequences before
+  __shared__ int bound[kSeqs + 1];
   const int tid = threadIdx.x, lane = tid & 63;
-  if (tid < 64) {
-    int carry = 0;
-    for (int s0 = 0; s0 < p.seqs; s0 += 64) {
-      const int s = s0 + lane;
-      const int mine = s < p.seqs ? items_of(p, seq_of(p, s), TILE) : 0;
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += y;
-      }
-      if (s < p.seqs) bound[s + 1] = carry + sum;
-      carry += __shfl(sum, 63, 64);
-    }
-    if (lane == 0) bound[0] = 0;
-  }
+  if (tid < 64) bounds(p, lane, TILE, bound);
   __syncthreads();
-  const int total = bound[p.seqs];
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    int a = 0, b = p.seqs;  // bound[a] <= item < bound[b]
+  if (blockIdx.x == 0)
+    for (int s = tid; s <= p.seqs; s += 256) p.bound[s] = bound[s];
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int of_head = uniform(bound[p.seqs]);
+  const int total = of_head * p.HK, share = share_of(total, gridDim.x);
+  // workgroups i, i + 8, ... run on one XCD: it takes neighbouring shares, whose
+  // query rows are the same
+  const int w = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  int at = min(w * share, total);
+  const int end = uniform(min(at + share, total));
+  if (at == end) return;
+  int h = at / of_head, in = at % of_head, s;
+  {
+    int a = 0, b = p.seqs;  // bound[a] <= in < bound[b]
     while (b - a > 1) {
       const int m = (a + b) / 2;
-      if (bound[m] <= item) a = m; else b = m;
+      if (bound[m] <= in) a = m; else b = m;
     }
-    // (found by way of LDS; every lane has the same)
-    const int s = __builtin_amdgcn_readfirstlane(a);
-    const Seq x = seq_of(p, s);
-    const int of = item - __builtin_amdgcn_readfirstlane(bound[s]);
-    const int h = of % p.HK;
-    int i = of / p.HK, lo = 0;
-    for (;; lo += p.chunk) {
-      const int n = tiles_seen(p, x, min(lo + p.chunk, x.n), TILE);
-      if (i < n) break;
-      i -= n;
-    }
-    const int k0 = i * TILE, hi = min(lo + p.chunk, x.n);
-    const float v = item_sums<D, F8, KT>(p, x, s, h, k0, max(lo, first_row(p, x, k0)), hi, lds);
-    const int64_t at = ((int64_t)(lo / p.chunk * p.seqs + s) * p.HK + h) * p.tiles * TILE;
-    p.part[at + k0 + (tid >> 6) * 32 * KT + lane_key(lane)] = v;
+    s = uniform(a);
+  }
+  in -= uniform(bound[s]);
+  Seq x = seq_of(p, s);
+  Work work = work_of(p, x, TILE);
+  int t = min(in / work.full, work.seen);
+  while (in >= groups_before(work, p.drop, t + 1)) ++t;
+  in -= groups_before(work, p.drop, t);
+  for (;;) {
+    // (the same in every lane, found by way of LDS)
+    h = uniform(h), s = uniform(s), t = uniform(t), in = uniform(in), at = uniform(at);
+    x = seq_of(p, s);
+    work = work_of(p, x, TILE);
+    const int groups = groups_of(work, p.drop, t);
+    const int here = min(groups - in, end - at);
+    const int k0 = t * TILE, first = first_row(p, x, k0);
+    const int lo = first + in * p.step_rows, hi = min(lo + here * p.step_rows, x.n);
+    float v = 0.f;
+    for (int l = lo; l < hi; l += p.row_limit)
+      v += item_sums<D, F8, KT>(p, x, s, h, k0, l, min(l + p.row_limit, hi), lds);
+    const int64_t part = ((int64_t)h * p.seqs + s) * p.tiles + t + w;
+    p.part[part * TILE + (tid >> 6) * 32 * KT + lane_key(lane)] = v;
+    at += here;
+    if (at == end) return;
+    in = 0;
+    if (++t < work.tiles) continue;
+    t = 0;
+    do {
+      if (++s == p.seqs) s = 0, ++h;
+      x = seq_of(p, s);
+      work = work_of(p, x, TILE);
+    } while (work.tiles == 0);
   }
 }
 
-__global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
+__global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p, int workgroups) {
   constexpr int TILE = tile_keys(2);
   const int h = blockIdx.y % p.HK, s = blockIdx.y / p.HK;
   const int j = blockIdx.x * 256 + threadIdx.x;
   if (j >= p.cols) return;
   const Seq x = seq_of(p, s);
+  const Work work = work_of(p, x, TILE);
+  const int t = j / TILE;
   float sum = 0.f;
-  if (j < x.used) {
-    const int first = first_row(p, x, j / TILE * TILE);
-    for (int c = first / p.chunk; c * p.chunk < x.n; ++c)
-      sum += p.part[((int64_t)(c * p.seqs + s) * p.HK + h) * p.tiles * TILE + j];
+  if (j < x.used && t < work.tiles) {
+    const int of_head = p.bound[p.seqs], share = share_of(of_head * p.HK, workgroups);
+    const int at = of_head * h + p.bound[s] + groups_before(work, p.drop, t);
+    const int last = (at + groups_of(work, p.drop, t) - 1) / share;
+    const float* part = p.part + (((int64_t)h * p.seqs + s) * p.tiles + t) * TILE + j % TILE;
+    for (int w = at / share; w <= last; ++w) sum += part[(int64_t)w * TILE];
   }
   if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
   p.out[s * p.out_s + h * p.out_h + j] = sum;
 }
 
-// Rows of an item: whole sequences (0 returned) where they are few
-int64_t chunk_rows(int64_t max_q, int64_t G) {
-  const int64_t rows = (512 * 4 + G - 1) / G;  // 32 steps
-  return max_q <= rows ? 0 : rows;
-}
+// Whether the rows go in shares: a key tile is worth several steps
+bool shared_rows(int64_t max_q, int64_t G) { return max_q * G > 2 * kCols; }
 
 int64_t tiles_of(int64_t keys, int KT) { return (keys + tile_keys(KT) - 1) / tile_keys(KT); }
 
-// Sequences of one pair of launches over chunks, whose sums take
-// `per_sequence` bytes each: within kScratch of scratch memory
-constexpr int64_t kScratch = 128 << 20;
-int64_t batch_of(int64_t seqs, int64_t per_sequence) {
-  const int64_t fit = std::max<int64_t>(1, kScratch / std::max<int64_t>(per_sequence, 1));
-  return std::min<int64_t>({seqs, fit, kSeqs});
+// Scratch memory of a pair of launches over shares: the sequences' bounds, then
+// the parts of (tile, workgroup)
+constexpr int kBoundBytes = (kSeqs + 64) * 4;
+int64_t part_bytes(int64_t seqs, int64_t max_used, int64_t HK) {
+  return kBoundBytes + (seqs * HK * tiles_of(max_used, 2) + kShares) * tile_keys(2) * 4;
 }
-int64_t part_bytes(int64_t max_q, int64_t max_used, int64_t HK, int64_t chunk) {
-  return (max_q + chunk - 1) / chunk * HK * tiles_of(max_used, 2) * tile_keys(2) *
-         (int64_t)sizeof(float);
+
+// Sequences of one pair of launches: within kScratch of scratch memory, and
+// groups that are counted in 31 bits
+constexpr int64_t kScratch = 128 << 20;
+int64_t batch_of(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK) {
+  const int64_t G = HQ / HK, rows = std::max<int64_t>(1, kCols / G);
+  const int64_t groups = std::max<int64_t>(1, (max_q + rows - 1) / rows * tiles_of(max_used, 2) * HK);
+  int64_t n = std::min<int64_t>({seqs, kSeqs, (1LL << 30) / groups});
+  n = std::min(n, kScratch / std::max<int64_t>(1, part_bytes(1, max_used, HK) - part_bytes(0, max_used, HK)));
+  return std::max<int64_t>(n, 1);
 }
 
 }  // namespace
@@ -463,10 +534,8 @@ int64_t qx_key_weights_workspace(int64_t seqs, int64_t max_q, int64_t max_used, 
                                  int64_t HK) {
   QX_CHECK(seqs >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
            "key_weights_workspace: sizes");
-  const int64_t rows = chunk_rows(max_q, HQ / HK);
-  if (rows == 0) return 0;
-  const int64_t bytes = part_bytes(max_q, max_used, HK, rows);
-  return batch_of(seqs, bytes) * bytes;
+  if (!shared_rows(max_q, HQ / HK) || seqs == 0) return 0;
+  return part_bytes(batch_of(seqs, max_q, max_used, HQ, HK), max_used, HK);
 }
 
 int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld,
@@ -498,22 +567,28 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
   QX_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
            "key_weights: a workspace of %lld bytes, %lld given", (long long)need,
            (long long)workspace_bytes);
-  const int64_t G = HQ / HK, chunk = chunk_rows(max_q, G);
-  // few columns: keys are read once and hardly computed with, so that more and
-  // smaller workgroups read them sooner
-  const int KT = chunk || max_q * G > 4 * kCols ? 2 : 1;
-  const int64_t tiles = chunk ? tiles_of(max_used, KT) : tiles_of(cols, KT);
-  const int64_t batch = chunk ? batch_of(seqs, part_bytes(max_q, max_used, HK, chunk))
-                              : std::min<int64_t>(seqs, kSeqs);
+  const int64_t G = HQ / HK;
+  const bool shares = shared_rows(max_q, G);
+  // one step a tile: keys are read once and hardly computed with, so that more
+  // and smaller workgroups read them sooner
+  const int KT = shares ? 2 : 1;
+  const int64_t tiles = tiles_of(shares ? max_used : cols, KT);
+  const int64_t step_rows = G > kCols ? 1 : kCols / G;
+  const int64_t batch = shares ? batch_of(seqs, max_q, max_used, HQ, HK) : std::min<int64_t>(seqs, kSeqs);
+  QX_CHECK(!shares || (max_q + step_rows - 1) / step_rows * tiles * HK < (1LL << 30),
+           "key_weights: %lld rows of %lld heads over %lld keys exceed one launch", (long long)max_q,
+           (long long)HQ, (long long)max_used);
   for (int64_t s0 = 0; s0 < seqs; s0 += batch) {
     const int64_t n = std::min(seqs - s0, batch);
     WeightsArgs a{(const uint16_t*)q, q_ld, lse, lse_ld, (const uint8_t*)k_pool,
                   (const uint8_t*)scales, cu_q + s0, used + s0, table + s0 * table_ld, table_ld,
                   base ? base + s0 * base_seq : nullptr, base_seq, base_head, out + s0 * out_seq,
-                  out_seq, out_head, (float*)workspace, (int)n, (int)HK, (int)G, (int)rows, (int)max_q,
-                  rows ? (int)max_used : 0, (int)cols, (int)tiles, (int)chunk,
-                  G > kCols ? 1 : (int)(kCols / G), (int)((G + kCols - 1) / kCols), scale * kLog2e,
-                  causal};
+                  out_seq, out_head, (float*)((char*)workspace + kBoundBytes), (int*)workspace, (int)n,
+                  (int)HK, (int)G, (int)rows, (int)max_q, rows ? (int)max_used : 0, (int)cols,
+                  (int)tiles, (int)step_rows, (int)((G + kCols - 1) / kCols),
+                  (int)(tile_keys(KT) / step_rows),
+                  (int)((1LL << 31) / std::max<int64_t>(2 * q_ld, 1 << 16) / step_rows * step_rows),
+                  scale * kLog2e, causal};
 #define QX_KEYS(K, grid, ...)                                                                    \
   if (scales) {                                                                                  \
     if (D == 128) hipLaunchKernelGGL((K<128, true __VA_ARGS__>), grid, dim3(256), 0, stream, a); \
@@ -522,24 +597,19 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
     if (D == 128) hipLaunchKernelGGL((K<128, false __VA_ARGS__>), grid, dim3(256), 0, stream, a); \
     else hipLaunchKernelGGL((K<64, false __VA_ARGS__>), grid, dim3(256), 0, stream, a);          \
   }
-    if (!chunk) {
+    if (!shares) {
       QX_CHECK(tiles * n * HK < (1LL << 24), "key_weights: %lld key tiles exceed one launch",
                (long long)(tiles * n * HK));
       const dim3 grid((unsigned)(tiles * n * HK));
-      if (KT == 1) {
-        QX_KEYS(key_weights_direct_kernel, grid, , 1)
-      } else {
-        QX_KEYS(key_weights_direct_kernel, grid, , 2)
-      }
+      QX_KEYS(key_weights_direct_kernel, grid, , 1)
     } else {
-      QX_CHECK(n * HK < 65536 && (max_q + chunk - 1) / chunk * tiles * n * HK < (1LL << 31),
-               "key_weights: %lld sequences of %lld heads exceed one launch", (long long)n,
-               (long long)HK);
-      QX_KEYS(key_weights_chunk_kernel, dim3(512))
+      QX_CHECK(n * HK < 65536, "key_weights: %lld sequences of %lld heads exceed one launch",
+               (long long)n, (long long)HK);
+      QX_KEYS(key_weights_share_kernel, dim3(kShares))
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
       hipLaunchKernelGGL(key_weights_join_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)(n * HK)),
-                         dim3(256), 0, stream, a);
+                         dim3(256), 0, stream, a, kShares);
     }
 #undef QX_KEYS
     const hipError_t e = hipGetLastError();
