@@ -32,6 +32,7 @@ constexpr int kMaxKeys = 2560 * kPage;
 constexpr int kCols = 64;            // (row, head) columns of a step
 constexpr int kSeqs = 2048;          // sequences of one launch (their bounds in LDS)
 constexpr int kShares = 512;         // workgroups that the work is shared by: two a CU
+constexpr int kStart = 8;            // groups that the start of a key tile takes as long as
 constexpr int kMinShare = 2;         // groups of a share, at least
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -51,6 +52,7 @@ struct WeightsArgs {
   int* bound;
   int seqs, HK, G, rows, max_q, max_used, cols, tiles;
   int step_rows, blocks;  // rows of a step; steps that a row's heads take (G > kCols)
+  int start;              // groups that a tile's start is counted as
   int drop;               // groups that a tile has fewer than the one before
   int row_limit;          // rows whose elements 32 bits of bytes reach
   float scale_log2;
@@ -95,10 +97,10 @@ __device__ __forceinline__ Work work_of(const WeightsArgs& p, const Seq& x, int 
   Work w{0, 0, 0, 0};
   if (x.n == 0 || x.used == 0) return w;
   w.tiles = (x.used + tile - 1) / tile;
-  w.full = (x.n + p.step_rows - 1) / p.step_rows;
+  w.full = p.start + (x.n + p.step_rows - 1) / p.step_rows;
   const int older = x.used - x.n;  // keys that every row sees, and one more
   w.seen = !p.causal ? w.tiles : older < 0 ? 0 : min(older / tile + 1, w.tiles);
-  if (w.seen < w.tiles) w.rest = (x.used - w.seen * tile + p.step_rows - 1) / p.step_rows;
+  if (w.seen < w.tiles) w.rest = p.start + (x.used - w.seen * tile + p.step_rows - 1) / p.step_rows;
   return w;
 }
 
@@ -288,7 +290,7 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
   };
   constexpr int AHEAD = 3;
   auto fragment = [&](int step, int t, int c) {
-    return *reinterpret_cast<const v8bf*>(lds + step % 3 * kStage + t * 64 * D + (opaque(frag) ^ c * 32));
+    return *reinterpret_cast<const v8bf*>(lds + step % 3 * kStage + t * 64 * D + (frag ^ c * 32));
   };
   // steps whose first row does not see all of the wave's keys: each score
   // against the keys that its column sees
@@ -461,7 +463,8 @@ __global__ __launch_bounds__(256, 2) void key_weights_share_kernel(WeightsArgs p
     const int groups = groups_of(work, p.drop, t);
     const int here = min(groups - in, end - at);
     const int k0 = t * TILE, first = first_row(p, x, k0);
-    const int lo = first + in * p.step_rows, hi = min(lo + here * p.step_rows, x.n);
+    const int lo = first + max(in - p.start, 0) * p.step_rows;
+    const int hi = min(first + max(in + here - p.start, 0) * p.step_rows, x.n);
     float v = 0.f;
     for (int l = lo; l < hi; l += p.row_limit)
       v += item_sums<D, F8, KT>(p, x, s, h, k0, l, min(l + p.row_limit, hi), lds);
@@ -517,7 +520,7 @@ int64_t part_bytes(int64_t seqs, int64_t max_used, int64_t HK) {
 constexpr int64_t kScratch = 128 << 20;
 int64_t batch_of(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ, int64_t HK) {
   const int64_t G = HQ / HK, rows = std::max<int64_t>(1, kCols / G);
-  const int64_t groups = std::max<int64_t>(1, (max_q + rows - 1) / rows * tiles_of(max_used, 2) * HK);
+  const int64_t groups = std::max<int64_t>(1, ((max_q + rows - 1) / rows + kStart) * tiles_of(max_used, 2) * HK);
   int64_t n = std::min<int64_t>({seqs, kSeqs, (1LL << 30) / groups});
   n = std::min(n, kScratch / std::max<int64_t>(1, part_bytes(1, max_used, HK) - part_bytes(0, max_used, HK)));
   return std::max<int64_t>(n, 1);
@@ -575,7 +578,7 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
   const int64_t tiles = tiles_of(shares ? max_used : cols, KT);
   const int64_t step_rows = G > kCols ? 1 : kCols / G;
   const int64_t batch = shares ? batch_of(seqs, max_q, max_used, HQ, HK) : std::min<int64_t>(seqs, kSeqs);
-  QX_CHECK(!shares || (max_q + step_rows - 1) / step_rows * tiles * HK < (1LL << 30),
+  QX_CHECK(!shares || ((max_q + step_rows - 1) / step_rows + kStart) * tiles * HK < (1LL << 30),
            "key_weights: %lld rows of %lld heads over %lld keys exceed one launch", (long long)max_q,
            (long long)HQ, (long long)max_used);
   for (int64_t s0 = 0; s0 < seqs; s0 += batch) {
@@ -586,7 +589,7 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
                   out_seq, out_head, (float*)((char*)workspace + kBoundBytes), (int*)workspace, (int)n,
                   (int)HK, (int)G, (int)rows, (int)max_q, rows ? (int)max_used : 0, (int)cols,
                   (int)tiles, (int)step_rows, (int)((G + kCols - 1) / kCols),
-                  (int)(tile_keys(KT) / step_rows),
+                  kStart, (int)(tile_keys(KT) / step_rows),
                   (int)((1LL << 31) / std::max<int64_t>(2 * q_ld, 1 << 16) / step_rows * step_rows),
                   scale * kLog2e, causal};
 #define QX_KEYS(K, grid, ...)                                                                    \
