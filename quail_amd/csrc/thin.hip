@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kMaxKeys = 2560 * kPage;  // as the paged attention's
+constexpr int64_t kFullWaves = 2048;     // waves that keep the card's memory busy
 
 struct ThinArgs {
   uint8_t* pools;  // K and V of layer 0, K of layer 1, ...
@@ -39,6 +40,7 @@ __device__ __forceinline__ uint32_t rank_of(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// the sum of v over the lanes before, and over all
 __device__ __forceinline__ int wave_sum_before(int v, int lane, int* total) {
   int x = v;
 #pragma unroll
@@ -55,21 +57,32 @@ __device__ __forceinline__ int lanes_before(uint64_t mask) {
                                    __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+// bits [lo, hi) of a word whose first bit is number `base`
+__device__ __forceinline__ uint64_t bits(int lo, int hi, int base) {
+  const int a = min(max(lo - base, 0), 64), b = min(max(hi - base, 0), 64);
+  const uint64_t below_b = b == 64 ? ~0ull : (1ull << b) - 1;
+  return a >= b ? 0 : below_b & ~((1ull << a) - 1);
+}
+
 // One (layer, sequence, head) per workgroup, its weights' ranks in registers,
-// E a thread (row e * NT + thread). The border, the rank of the last row kept, is
-// found 11, 11 and 10 bits at a time from histograms in LDS; rows are then
-// numbered by counting ballots, equal ranks, dropped slots and movers alike.
-// Bound by latency: a few passes over registers with barriers between, 4 bytes
-// a row from memory.
+// E a thread (row e * NT + thread); 0 stands for a row that is protected or not
+// there (no weight ranks so low). The border, the rank of the last row kept, is
+// found 11, 11 and 10 bits at a time from histograms in LDS, of which the second
+// and third count few rows. What stays is then a bit a row, in words of 64 rows
+// (the wave cells' ballots), and dropped slots and movers are numbered by words.
+// Bound by instructions, about 50 a row, and barriers; 8 bytes a row from and
+// to memory.
 template <int NT, int E>
 __global__ __launch_bounds__(NT) void thin_select_kernel(ThinArgs p) {
   constexpr int W = NT / 64, CELLS = E * W, BINS = 2048, PER = BINS / NT;
   __shared__ int hist[BINS];
-  __shared__ int cell[CELLS + 1];
+  __shared__ uint64_t stays[CELLS];
+  __shared__ int before[CELLS];  // flagged rows before a word's
   __shared__ int sums[W];
   __shared__ int found[3];  // bin, rows above it, rows in it
   __shared__ uint16_t movers[NT * E / 2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x;
   const int h = (int)(row % p.HK);
   const int64_t ls = row / p.HK;
@@ -88,28 +101,31 @@ __global__ __launch_bounds__(NT) void thin_select_kernel(ThinArgs p) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int i = e * NT + tid;
-    rank[e] = i >= p.sinks && i < late ? rank_of(w[i]) : 0;
+    rank[e] = i >= p.sinks && i < late ? __float_as_uint(w[i]) : 0;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = e * NT + tid;
+    if (i >= p.sinks && i < late) rank[e] = rank_of(__uint_as_float(rank[e]));
   }
   int want = k - p.sinks - p.recent;  // of the rows [sinks, late), which are more
+  const bool none = want == 0;
   uint32_t border = 0;
   int equal = 0;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
     for (int i = tid; i < BINS; i += NT) hist[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int i = e * NT + tid;
-      const bool in = i >= p.sinks && i < late &&
-                      (pass == 0 || (rank[e] >> (shift + bits)) == (border >> (shift + bits)));
-      if (!in) continue;
-      const int bin = (rank[e] >> shift) & ((1 << bits) - 1);
+      if (pass == 0 ? rank[e] == 0 : rank[e] >> (shift + width) != border >> (shift + width)) continue;
+      const int bin = (rank[e] >> shift) & ((1 << width) - 1);
       // a wave whose rows are all of one bin counts them at once (weights of
       // keys that never had any are all 0)
       const int first = __builtin_amdgcn_readfirstlane(bin);
-      const uint64_t active = __ballot(1);
-      if (__ballot(bin == first) == active) {
+      if (__ballot(bin != first) == 0) {
+        const uint64_t active = __ballot(1);
         if (lanes_before(active) == 0) atomicAdd(&hist[bin], (int)__popcll(active));
       } else {
         atomicAdd(&hist[bin], 1);
@@ -121,157 +137,175 @@ __global__ __launch_bounds__(NT) void thin_select_kernel(ThinArgs p) {
 #pragma unroll
     for (int b = 0; b < PER; ++b) mine += hist[BINS - 1 - (tid * PER + b)];
     int total;
-    int before = wave_sum_before(mine, lane, &total);
+    int above = wave_sum_before(mine, lane, &total);
     if (lane == 0) sums[wave] = total;
     __syncthreads();
-    for (int v = 0; v < wave; ++v) before += sums[v];
-    if (before < want && want <= before + mine) {
+    for (int v = 0; v < wave; ++v) above += sums[v];
+    if (above < want && want <= above + mine) {
 #pragma unroll
       for (int b = 0; b < PER; ++b) {
         const int bin = BINS - 1 - (tid * PER + b), n = hist[bin];
-        if (before < want && want <= before + n) {
+        if (above < want && want <= above + n) {
           found[0] = bin;
-          found[1] = before;
+          found[1] = above;
           found[2] = n;
         }
-        before += n;
+        above += n;
       }
     }
     __syncthreads();
-    if (want > 0) {
+    if (!none) {
       border |= (uint32_t)found[0] << shift;
       want -= found[1];
       equal = found[2];
     }
   }
-  const bool none = k == p.sinks + p.recent;  // no other row stays
-  // numbers a flag's rows: cell[c] = rows before wave cell c
-  auto number = [&](auto flag) {
+  // numbers the bits of flags(cell), W E words: before[cell], and all of them
+  auto number = [&](auto flags) {
+    int carry = 0;
+    for (int c0 = 0; c0 < CELLS; c0 += NT) {
+      const int c = c0 + tid;
+      const int mine = c < CELLS ? (int)__popcll(flags(c)) : 0;
+      int total;
+      int n = wave_sum_before(mine, lane, &total);
+      if (lane == 0) sums[wave] = total;
+      __syncthreads();
+      for (int v = 0; v < W; ++v) {
+        if (v == wave) n += carry;
+        if (v < wave) n += sums[v];
+      }
+      if (c < CELLS) before[c] = n;
+      for (int v = 0; v < W; ++v) carry += sums[v];
+      __syncthreads();
+    }
+    return carry;
+  };
+  // Word c = e * W + wave holds rows [64 c, 64 c + 64)
+  if (none) border = 0xffffffffu;  // and no tie stays
+  const bool ties = none || want != equal;  // not all of the border's rank
+  if (ties) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const uint64_t m = __ballot(flag(e));
-      if (lane == 0) cell[e * W + wave] = __popcll(m);
+      const uint64_t m = __ballot(rank[e] == border);
+      if (lane == 0) stays[e * W + wave] = m;
     }
     __syncthreads();
-    if (wave == 0) {
-      int carry = 0;
-      for (int c = 0; c < CELLS; c += 64) {
-        const int v = c + lane < CELLS ? cell[c + lane] : 0;
-        int total;
-        const int before = wave_sum_before(v, lane, &total);
-        if (c + lane < CELLS) cell[c + lane] = carry + before;
-        carry += total;
-      }
-      if (lane == 0) cell[CELLS] = carry;
-    }
-    __syncthreads();
-  };
-  // bit e: row e * NT + tid stays
-  uint64_t stays = 0;
-  const bool all_equal = want == equal;
-  if (!none && !all_equal)
-    number([&](int e) {
-      const int i = e * NT + tid;
-      return i >= p.sinks && i < late && rank[e] == border;
-    });
+    number([&](int c) { return stays[c]; });
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int i = e * NT + tid;
-    const bool middle = i >= p.sinks && i < late;
-    bool stay = i < used && !middle;
-    if (!none) {
-      bool tie = middle && rank[e] == border;
-      if (!all_equal) {
-        const uint64_t m = __ballot(tie);
-        tie = tie && cell[e * W + wave] + lanes_before(m) < want;
-      }
-      stay = stay || tie || (middle && rank[e] > border);
+    const int c = e * W + wave;
+    uint64_t m;
+    if (ties) {
+      const uint64_t same = stays[c];
+      const bool tie = (same >> lane & 1) && before[c] + lanes_before(same) < want;
+      m = __ballot(rank[e] > border || tie);
+    } else {
+      m = __ballot(rank[e] >= border);
     }
-    stays |= (uint64_t)stay << e;
+    m |= bits(0, p.sinks, 64 * c) | bits(late, used, 64 * c);
+    if (lane == 0) stays[c] = m;
   }
   __syncthreads();
-  // dropped slots come before all movers
-  auto flag = [&](int e) {
-    const int i = e * NT + tid;
-    const bool stay = stays >> e & 1;
-    return i < k ? !stay : stay;
+  // dropped slots below k, then (numbered behind them) movers from k on
+  auto flagged = [&](int c) {
+    const uint64_t m = stays[c], low = bits(0, k, 64 * c);
+    return (~m & low) | (m & ~low);
   };
-  number(flag);
-  const int holes = cell[CELLS] / 2;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = e * NT + tid;
-    const bool f = flag(e);
-    const uint64_t m = __ballot(f);
-    if (f && i >= k) movers[cell[e * W + wave] + lanes_before(m) - holes] = (uint16_t)i;
+  const int holes = number(flagged) / 2;
+  for (int i0 = k / 64 * 64; i0 < used; i0 += NT) {
+    const int i = i0 + tid, c = i >> 6;
+    if (c >= CELLS || i < k) continue;
+    const uint64_t m = flagged(c);
+    if (m >> (i & 63) & 1)
+      movers[before[c] + (int)__popcll(m & ((1ull << (i & 63)) - 1)) - holes] = (uint16_t)i;
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = e * NT + tid;
-    const bool f = flag(e);
-    const uint64_t m = __ballot(f);
-    if (i < k) {
-      const int src = f ? movers[cell[e * W + wave] + lanes_before(m)] : i;
-      kept[i] = src;
-      out[i] = w[src];
-    }
+  for (int i = tid; i < k; i += NT) {
+    const int c = i >> 6;
+    const uint64_t m = flagged(c);
+    const int src = m >> (i & 63) & 1 ? movers[before[c] + (int)__popcll(m & ((1ull << (i & 63)) - 1))] : i;
+    kept[i] = src;
+    out[i] = w[src];
   }
   for (int i = k + tid; i < p.cols; i += NT) out[i] = 0.f;
 }
 
-// 64 slots of a (layer, sequence, head) per wave: those whose row moves are
-// listed in LDS, then a row of D values goes by D * 2 / 16 lanes, 16 bytes each,
-// K and V of kBatch rows a lane in flight. Bound by HBM, in pieces of a head's
-// row.
-template <int D>
+// The moves of a wave: 64 * PL slots of a (layer, sequence, head), PL a lane.
+// Those whose row moves are listed in LDS, so that few moves among many slots
+// fill a wave too.
+struct Place {
+  int h;
+  int64_t layer, head;  // head: of kept
+  const int* table;
+  int slot;
+};
+
+template <int PL>
+__device__ __forceinline__ Place place_of(const ThinArgs& p, int64_t wid, int parts, int lane) {
+  Place x;
+  x.h = (int)(wid % p.HK);
+  const int64_t ls = wid / p.HK / parts;
+  x.layer = ls / p.seqs;
+  x.head = ls * p.HK + x.h;
+  x.table = p.table + ls % p.seqs * p.table_ld;
+  x.slot = ((int)(wid / p.HK % parts) * 64 + lane) * PL;
+  return x;
+}
+
+template <int PL>
+__device__ __forceinline__ void sources(const ThinArgs& p, const Place& x, int (&src)[PL]) {
+  const int* kept = p.kept + x.head * p.slots + x.slot;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) src[i] = x.slot + i < p.slots ? kept[i] : -1;
+}
+
+// A row of D values goes by D * 2 / 16 lanes, 16 bytes each, K and V of kBatch
+// rows a lane in flight. Bound by HBM, in pieces of a head's row.
+template <int D, int PL>
 __global__ __launch_bounds__(256) void thin_move_kernel(ThinArgs p, int64_t waves, int parts) {
   constexpr int LPR = D / 8, RPP = 64 / LPR, kBatch = 4;
-  __shared__ int64_t list[4][64][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ int64_t list[4][64 * PL][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wid = (int64_t)blockIdx.x * 4 + wave;
-  int n = 0;
-  int h = 0;
-  int64_t layer = 0;
-  if (wid < waves) {
-    h = (int)(wid % p.HK);
-    const int part = (int)(wid / p.HK % parts);
-    const int64_t ls = wid / p.HK / parts;
-    layer = ls / p.seqs;
-    const int* table = p.table + ls % p.seqs * p.table_ld;
-    const int slot = part * 64 + lane;
-    const int src = slot < p.slots ? p.kept[(ls * p.HK + h) * p.slots + slot] : -1;
-    const bool moves = src >= 0 && src != slot;
+  if (wid >= waves) return;
+  const Place x = place_of<PL>(p, wid, parts, lane);
+  int src[PL], n = 0;
+  sources<PL>(p, x, src);
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    const int slot = x.slot + i;
+    const bool moves = src[i] >= 0 && src[i] != slot;
     const uint64_t mask = __ballot(moves);
-    n = __popcll(mask);
     if (moves) {
-      int64_t* to = list[wave][lanes_before(mask)];
-      to[0] = (int64_t)table[slot / kPage] * kPage + slot % kPage;
-      to[1] = (int64_t)table[src / kPage] * kPage + src % kPage;
+      int64_t* to = list[wave][n + lanes_before(mask)];
+      to[0] = (int64_t)x.table[slot / kPage] * kPage + slot % kPage;
+      to[1] = (int64_t)x.table[src[i] / kPage] * kPage + src[i] % kPage;
     }
+    n += __popcll(mask);
   }
-  __syncthreads();
   if (n == 0) return;
-  uint8_t* k_pool = p.pools + 2 * layer * p.pool_stride + (int64_t)h * D * 2;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list
+  uint8_t* k_pool = p.pools + 2 * x.layer * p.pool_stride + (int64_t)x.h * D * 2;
   uint8_t* v_pool = k_pool + p.pool_stride;
   const int64_t row_bytes = (int64_t)p.HK * D * 2;
   const int at = lane % LPR * 16;
   for (int m0 = lane / LPR; m0 < n; m0 += RPP * kBatch) {
-    uint4 kv[kBatch][2];
+    v4i kv[kBatch][2];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int m = min(m0 + b * RPP, n - 1);  // a row again: no branch between the loads
       const int64_t from = list[wave][m][1] * row_bytes + at;
-      kv[b][0] = *reinterpret_cast<const uint4*>(k_pool + from);
-      kv[b][1] = *reinterpret_cast<const uint4*>(v_pool + from);
+      kv[b][0] = *reinterpret_cast<const v4i*>(k_pool + from);
+      kv[b][1] = *reinterpret_cast<const v4i*>(v_pool + from);
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int m = m0 + b * RPP;
       if (m >= n) continue;
       const int64_t to = list[wave][m][0] * row_bytes + at;
-      *reinterpret_cast<uint4*>(k_pool + to) = kv[b][0];
-      *reinterpret_cast<uint4*>(v_pool + to) = kv[b][1];
+      *reinterpret_cast<v4i*>(k_pool + to) = kv[b][0];
+      *reinterpret_cast<v4i*>(v_pool + to) = kv[b][1];
     }
   }
 }
@@ -287,93 +321,94 @@ __device__ __forceinline__ uint2 shifted8(uint2 c, int shift) {
   for (int i = 0; i < 8; ++i) y[i] = __builtin_ldexpf(y[i], shift);
   return make_uint2(pack4_fp8(y[0], y[1], y[2], y[3]), pack4_fp8(y[4], y[5], y[6], y[7]));
 }
-__device__ __forceinline__ uint4 shifted16(uint4 c, int shift) {
+__device__ __forceinline__ v4i shifted16(v4i c, int shift) {
   if (shift == 0) return c;
-  const uint2 a = shifted8(make_uint2(c.x, c.y), shift), b = shifted8(make_uint2(c.z, c.w), shift);
-  return make_uint4(a.x, a.y, b.x, b.y);
+  const uint2 a = shifted8(make_uint2(c[0], c[1]), shift), b = shifted8(make_uint2(c[2], c[3]), shift);
+  return v4i{(int)a.x, (int)a.y, (int)b.x, (int)b.y};
 }
 
 // The same over 8-bit pages. A page that a row moves into gets the largest
 // scale of those its rows come with (its own among them, where a row stays);
 // the codes of the others are shifted down to it, those of rows that stay too.
 // `keep` is whole pages, so no page is both read for a move and written.
-template <int D>
+template <int D, int PL>
 __global__ __launch_bounds__(256) void thin_move8_kernel(ThinArgs p, int64_t waves, int parts) {
   constexpr int LPR = D / 16, RPP = 64 / LPR, kBatch = 4;
-  __shared__ int64_t list[4][64][2];
-  __shared__ int shifts[4][64];  // K's and V's, 16 bits each
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int LPP = kPage / PL;  // lanes of a page
+  __shared__ int64_t list[4][64 * PL][2];
+  __shared__ int shifts[4][64 * PL];  // K's and V's, 16 bits each
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wid = (int64_t)blockIdx.x * 4 + wave;
-  int n = 0;
-  int h = 0;
-  int64_t layer = 0;
-  if (wid < waves) {
-    h = (int)(wid % p.HK);
-    const int part = (int)(wid / p.HK % parts);
-    const int64_t ls = wid / p.HK / parts;
-    layer = ls / p.seqs;
-    const int* table = p.table + ls % p.seqs * p.table_ld;
-    const int slot = part * 64 + lane;
-    const int src = slot < p.slots ? p.kept[(ls * p.HK + h) * p.slots + slot] : -1;
-    const bool moves = src >= 0 && src != slot;
-    const uint64_t moving = __ballot(moves);
-    if (moving) {
-      uint8_t* scales = p.scales + layer * p.scale_stride;
-      const bool page_moves = (moving >> (lane & 48) & 0xffff) != 0;
-      int64_t to = 0, from = 0;
-      int bk = 0, bv = 0;
-      if (page_moves) {  // then all 16 of its slots hold rows
-        to = table[slot / kPage];
-        from = table[src / kPage];
-        const uint8_t* b = scales + (from * p.HK + h) * 2;
-        bk = b[0];
-        bv = b[1];
-      }
-      int top_k = bk, top_v = bv;
+  if (wid >= waves) return;
+  const Place x = place_of<PL>(p, wid, parts, lane);
+  int src[PL], n = 0;
+  sources<PL>(p, x, src);
+  bool any = false;
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) {
-        top_k = max(top_k, __shfl_xor(top_k, o, 64));
-        top_v = max(top_v, __shfl_xor(top_v, o, 64));
-      }
-      const bool write = page_moves && (moves || bk != top_k || bv != top_v);
-      const uint64_t mask = __ballot(write);
-      n = __popcll(mask);
-      if (write) {
-        const int m = lanes_before(mask);
-        list[wave][m][0] = to * kPage + slot % kPage;
-        list[wave][m][1] = from * kPage + src % kPage;
-        shifts[wave][m] = ((top_k - bk) & 0xffff) | (top_v - bv) << 16;
-      }
-      if (page_moves && lane % kPage == 0) {
-        uint8_t* b = scales + (to * p.HK + h) * 2;
-        b[0] = (uint8_t)top_k;
-        b[1] = (uint8_t)top_v;
-      }
+  for (int i = 0; i < PL; ++i) any |= src[i] >= 0 && src[i] != x.slot + i;
+  const uint64_t moving = __ballot(any);
+  if (moving == 0) return;
+  uint8_t* scales = p.scales + x.layer * p.scale_stride;
+  // whether a row moves into the lane's page; then all 16 of its slots hold rows
+  const bool page_moves = (moving >> (lane / LPP * LPP) & ((1u << LPP) - 1)) != 0;
+  int64_t to = 0, from[PL];
+  int bk[PL], bv[PL], top_k = 0, top_v = 0;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    from[i] = 0;
+    bk[i] = bv[i] = 0;
+    if (page_moves) {
+      from[i] = x.table[src[i] / kPage];
+      const uint16_t b = *reinterpret_cast<const uint16_t*>(scales + (from[i] * p.HK + x.h) * 2);
+      bk[i] = b & 0xff;
+      bv[i] = b >> 8;
     }
+    top_k = max(top_k, bk[i]);
+    top_v = max(top_v, bv[i]);
   }
-  __syncthreads();
-  if (n == 0) return;
-  uint8_t* k_pool = p.pools + 2 * layer * p.pool_stride + (int64_t)h * D;
+  if (page_moves) to = x.table[x.slot / kPage];
+#pragma unroll
+  for (int o = LPP / 2; o > 0; o >>= 1) {
+    top_k = max(top_k, __shfl_xor(top_k, o, 64));
+    top_v = max(top_v, __shfl_xor(top_v, o, 64));
+  }
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    const int slot = x.slot + i;
+    const bool write = page_moves && (src[i] != slot || bk[i] != top_k || bv[i] != top_v);
+    const uint64_t mask = __ballot(write);
+    if (write) {
+      const int m = n + lanes_before(mask);
+      list[wave][m][0] = to * kPage + slot % kPage;
+      list[wave][m][1] = from[i] * kPage + src[i] % kPage;
+      shifts[wave][m] = (top_k - bk[i]) | (top_v - bv[i]) << 16;
+    }
+    n += __popcll(mask);
+  }
+  if (page_moves && lane % LPP == 0)
+    *reinterpret_cast<uint16_t*>(scales + (to * p.HK + x.h) * 2) = (uint16_t)(top_k | top_v << 8);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list
+  uint8_t* k_pool = p.pools + 2 * x.layer * p.pool_stride + (int64_t)x.h * D;
   uint8_t* v_pool = k_pool + p.pool_stride;
   const int64_t row_bytes = (int64_t)p.HK * D;
   const int at = lane % LPR * 16;
   for (int m0 = lane / LPR; m0 < n; m0 += RPP * kBatch) {
-    uint4 kv[kBatch][2];
+    v4i kv[kBatch][2];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int m = min(m0 + b * RPP, n - 1);  // a row again: no branch between the loads
-      const int64_t from = list[wave][m][1] * row_bytes + at;
-      kv[b][0] = *reinterpret_cast<const uint4*>(k_pool + from);
-      kv[b][1] = *reinterpret_cast<const uint4*>(v_pool + from);
+      const int m = min(m0 + b * RPP, n - 1);
+      const int64_t row = list[wave][m][1] * row_bytes + at;
+      kv[b][0] = *reinterpret_cast<const v4i*>(k_pool + row);
+      kv[b][1] = *reinterpret_cast<const v4i*>(v_pool + row);
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int m = m0 + b * RPP;
       if (m >= n) continue;
-      const int64_t to = list[wave][m][0] * row_bytes + at;
+      const int64_t row = list[wave][m][0] * row_bytes + at;
       const int shift = shifts[wave][m];
-      *reinterpret_cast<uint4*>(k_pool + to) = shifted16(kv[b][0], -(shift & 0xffff));
-      *reinterpret_cast<uint4*>(v_pool + to) = shifted16(kv[b][1], -(shift >> 16));
+      *reinterpret_cast<v4i*>(k_pool + row) = shifted16(kv[b][0], -(shift & 0xffff));
+      *reinterpret_cast<v4i*>(v_pool + row) = shifted16(kv[b][1], -(shift >> 16));
     }
   }
 }
@@ -429,17 +464,29 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (max_used <= keep) return QX_OK;  // no row moves
-  const int parts = (int)((slots + 63) / 64);
+  // slots a lane: 4 where that leaves waves enough (each then has more moves)
+  const int PL = rows * ((slots + 255) / 256) >= kFullWaves ? 4 : 1;
+  const int parts = (int)((slots + 64 * PL - 1) / (64 * PL));
   const int64_t waves = rows * parts;
   QX_CHECK(waves <= (1LL << 26) - 4, "thin_rows: %lld rows of %lld heads exceed one launch",
            (long long)slots, (long long)rows);
   const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
-#define QX_MOVE(K, DD) hipLaunchKernelGGL((K<DD>), grid, block, 0, stream, a, waves, parts)
+#define QX_MOVE(K, DD)                                                                     \
+  if (PL == 4) hipLaunchKernelGGL((K<DD, 4>), grid, block, 0, stream, a, waves, parts);    \
+  else hipLaunchKernelGGL((K<DD, 1>), grid, block, 0, stream, a, waves, parts)
   if (waves) {
     if (element_bytes == 2) {
-      if (D == 128) QX_MOVE(thin_move_kernel, 128); else QX_MOVE(thin_move_kernel, 64);
+      if (D == 128) {
+        QX_MOVE(thin_move_kernel, 128);
+      } else {
+        QX_MOVE(thin_move_kernel, 64);
+      }
     } else {
-      if (D == 128) QX_MOVE(thin_move8_kernel, 128); else QX_MOVE(thin_move8_kernel, 64);
+      if (D == 128) {
+        QX_MOVE(thin_move8_kernel, 128);
+      } else {
+        QX_MOVE(thin_move8_kernel, 64);
+      }
     }
   }
 #undef QX_MOVE
