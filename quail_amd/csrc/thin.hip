@@ -40,16 +40,29 @@ __device__ __forceinline__ uint32_t rank_of(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// the sum of v over the lanes before, and over all
-__device__ __forceinline__ int wave_sum_before(int v, int lane, int* total) {
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  *total = __shfl(x, 63, 64);
-  return x - v;
+// the sum of v over the lanes up to this one, on vector operands (through LDS
+// permutes the three scans took a third of a short call's time)
+__device__ __forceinline__ int wave_sum_to(int v) {
+#define QX_STEP(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false)
+  QX_STEP(0x111, 0xf);  // from 1, 2, 4 and 8 lanes below in the row of 16
+  QX_STEP(0x112, 0xf);
+  QX_STEP(0x114, 0xf);
+  QX_STEP(0x118, 0xf);
+  QX_STEP(0x142, 0xa);  // the row's last lane into the next row, of rows 1 and 3
+  QX_STEP(0x143, 0xc);  // lane 31 into the upper rows
+#undef QX_STEP
+  return v;
+}
+
+// the sum of v over the threads before, and over all of W waves; sums: W in LDS
+template <int W>
+__device__ __forceinline__ int block_sum_before(int v, int lane, int wave, int* sums, int* total) {
+  const int to = wave_sum_to(v);
+  if (lane == 63) sums[wave] = to;
+  __syncthreads();
+  const int waves = wave_sum_to(lane < W ? sums[lane] : 0);
+  *total = __builtin_amdgcn_readlane(waves, W - 1);
+  return to - v + (wave ? __builtin_amdgcn_readlane(waves, wave - 1) : 0);
 }
 
 __device__ __forceinline__ int lanes_before(uint64_t mask) {
@@ -69,15 +82,15 @@ __device__ __forceinline__ uint64_t bits(int lo, int hi, int base) {
 // there (no weight ranks so low). The border, the rank of the last row kept, is
 // found 11, 11 and 10 bits at a time from histograms in LDS, of which the second
 // and third count few rows. What stays is then a bit a row, in words of 64 rows
-// (the wave cells' ballots), and dropped slots and movers are numbered by words.
-// Bound by instructions, about 50 a row, and barriers; 8 bytes a row from and
-// to memory.
+// (a wave's ballots), and dropped slots and movers are numbered by words. Bound
+// by instructions (some 60 a row) and, where rows are few, by the barriers
+// between these steps; 8 bytes a row from and to memory.
 template <int NT, int E>
-__global__ __launch_bounds__(NT) void thin_select_kernel(ThinArgs p) {
-  constexpr int W = NT / 64, CELLS = E * W, BINS = 2048, PER = BINS / NT;
+__global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(ThinArgs p) {
+  constexpr int W = NT / 64, WORDS = E * W, BINS = 2048, PER = BINS / NT;
   __shared__ int hist[BINS];
-  __shared__ uint64_t stays[CELLS];
-  __shared__ int before[CELLS];  // flagged rows before a word's
+  __shared__ uint64_t stays[WORDS];
+  __shared__ int before[WORDS];  // flagged rows before a word's
   __shared__ int sums[W];
   __shared__ int found[3];  // bin, rows above it, rows in it
   __shared__ uint16_t movers[NT * E / 2];
@@ -97,92 +110,89 @@ __global__ __launch_bounds__(NT) void thin_select_kernel(ThinArgs p) {
     return;
   }
   const int k = p.keep, late = used - p.recent;
-  uint32_t rank[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = e * NT + tid;
-    rank[e] = i >= p.sinks && i < late ? __float_as_uint(w[i]) : 0;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = e * NT + tid;
-    if (i >= p.sinks && i < late) rank[e] = rank_of(__uint_as_float(rank[e]));
-  }
   int want = k - p.sinks - p.recent;  // of the rows [sinks, late), which are more
   const bool none = want == 0;
+  uint32_t rank[E];
   uint32_t border = 0;
   int equal = 0;
+  auto count = [&](int bin) {
+    // a wave whose rows are all of one bin counts them at once (weights of
+    // keys that never had any are all 0)
+    const int first = __builtin_amdgcn_readfirstlane(bin);
+    if (__ballot(bin != first) == 0) {
+      const uint64_t active = __ballot(1);
+      if (lanes_before(active) == 0) atomicAdd(&hist[bin], (int)__popcll(active));
+    } else {
+      atomicAdd(&hist[bin], 1);
+    }
+  };
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
     for (int i = tid; i < BINS; i += NT) hist[i] = 0;
     __syncthreads();
+    if (pass == 0) {
+      constexpr int AT_ONCE = E < 8 ? E : 8;  // loads in flight
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (pass == 0 ? rank[e] == 0 : rank[e] >> (shift + width) != border >> (shift + width)) continue;
-      const int bin = (rank[e] >> shift) & ((1 << width) - 1);
-      // a wave whose rows are all of one bin counts them at once (weights of
-      // keys that never had any are all 0)
-      const int first = __builtin_amdgcn_readfirstlane(bin);
-      if (__ballot(bin != first) == 0) {
-        const uint64_t active = __ballot(1);
-        if (lanes_before(active) == 0) atomicAdd(&hist[bin], (int)__popcll(active));
-      } else {
-        atomicAdd(&hist[bin], 1);
+      for (int e0 = 0; e0 < E; e0 += AT_ONCE) {
+        const int t = opaque(tid);
+#pragma unroll
+        for (int e = e0; e < e0 + AT_ONCE; ++e) rank[e] = __float_as_uint(w[min(e * NT + t, used - 1)]);
+#pragma unroll
+        for (int e = e0; e < e0 + AT_ONCE; ++e) {
+          const int first = e * NT + wave * 64;
+          rank[e] = rank_of(__uint_as_float(rank[e]));
+          if (first >= p.sinks && first + 64 <= late) {
+            count(rank[e] >> 21);
+          } else {
+            const int i = e * NT + t;
+            if (i >= p.sinks && i < late) count(rank[e] >> 21); else rank[e] = 0;
+          }
+        }
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (rank[e] >> (shift + width) == border >> (shift + width))
+          count((rank[e] >> shift) & ((1 << width) - 1));
     }
     __syncthreads();
     // bins from the top, PER a thread
-    int mine = 0;
+    int bins[PER], mine = 0;
 #pragma unroll
-    for (int b = 0; b < PER; ++b) mine += hist[BINS - 1 - (tid * PER + b)];
+    for (int b = 0; b < PER; ++b) mine += bins[b] = hist[BINS - 1 - (tid * PER + b)];
     int total;
-    int above = wave_sum_before(mine, lane, &total);
-    if (lane == 0) sums[wave] = total;
-    __syncthreads();
-    for (int v = 0; v < wave; ++v) above += sums[v];
+    int above = block_sum_before<W>(mine, lane, wave, sums, &total);
     if (above < want && want <= above + mine) {
 #pragma unroll
       for (int b = 0; b < PER; ++b) {
-        const int bin = BINS - 1 - (tid * PER + b), n = hist[bin];
-        if (above < want && want <= above + n) {
-          found[0] = bin;
+        if (above < want && want <= above + bins[b]) {
+          found[0] = BINS - 1 - (tid * PER + b);
           found[1] = above;
-          found[2] = n;
+          found[2] = bins[b];
         }
-        above += n;
+        above += bins[b];
       }
     }
     __syncthreads();
     if (!none) {
-      border |= (uint32_t)found[0] << shift;
-      want -= found[1];
-      equal = found[2];
+      border |= (uint32_t)__builtin_amdgcn_readfirstlane(found[0]) << shift;
+      want -= __builtin_amdgcn_readfirstlane(found[1]);
+      equal = __builtin_amdgcn_readfirstlane(found[2]);
     }
   }
-  // numbers the bits of flags(cell), W E words: before[cell], and all of them
+  // Word c holds rows [64 c, 64 c + 64); wave v has the words v, v + W, ...
+  // number(flags): the set bits of the words before each word, and of all
+  const int words = (used + NT - 1) / NT * W;
   auto number = [&](auto flags) {
-    int carry = 0;
-    for (int c0 = 0; c0 < CELLS; c0 += NT) {
-      const int c = c0 + tid;
-      const int mine = c < CELLS ? (int)__popcll(flags(c)) : 0;
-      int total;
-      int n = wave_sum_before(mine, lane, &total);
-      if (lane == 0) sums[wave] = total;
-      __syncthreads();
-      for (int v = 0; v < W; ++v) {
-        if (v == wave) n += carry;
-        if (v < wave) n += sums[v];
-      }
-      if (c < CELLS) before[c] = n;
-      for (int v = 0; v < W; ++v) carry += sums[v];
-      __syncthreads();
-    }
-    return carry;
+    int total;
+    static_assert(WORDS <= NT, "a word a thread");
+    const int n = block_sum_before<W>(tid < words ? (int)__popcll(flags(tid)) : 0, lane, wave, sums, &total);
+    if (tid < words) before[tid] = n;
+    __syncthreads();
+    return total;
   };
-  // Word c = e * W + wave holds rows [64 c, 64 c + 64)
-  if (none) border = 0xffffffffu;  // and no tie stays
-  const bool ties = none || want != equal;  // not all of the border's rank
+  const bool ties = want != equal;  // not all of the border's rank stay
   if (ties) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -195,38 +205,60 @@ __global__ __launch_bounds__(NT) void thin_select_kernel(ThinArgs p) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = e * W + wave;
-    uint64_t m;
+    uint64_t m = __ballot(ties ? rank[e] > border : rank[e] >= border);
     if (ties) {
       const uint64_t same = stays[c];
-      const bool tie = (same >> lane & 1) && before[c] + lanes_before(same) < want;
-      m = __ballot(rank[e] > border || tie);
-    } else {
-      m = __ballot(rank[e] >= border);
+      m |= __ballot((same >> lane & 1) && before[c] + lanes_before(same) < want);
     }
-    m |= bits(0, p.sinks, 64 * c) | bits(late, used, 64 * c);
+    if (none) m = 0;
+    if (64 * c < p.sinks || 64 * c + 64 > late) m |= bits(0, p.sinks, 64 * c) | bits(late, used, 64 * c);
     if (lane == 0) stays[c] = m;
   }
   __syncthreads();
   // dropped slots below k, then (numbered behind them) movers from k on
   auto flagged = [&](int c) {
-    const uint64_t m = stays[c], low = bits(0, k, 64 * c);
-    return (~m & low) | (m & ~low);
+    const uint64_t m = stays[c];
+    if (64 * c + 64 <= k) return ~m;
+    return 64 * c >= k ? m : m ^ bits(0, k, 64 * c);
   };
   const int holes = number(flagged) / 2;
-  for (int i0 = k / 64 * 64; i0 < used; i0 += NT) {
-    const int i = i0 + tid, c = i >> 6;
-    if (c >= CELLS || i < k) continue;
+  // row 64 c + lane's number among the flagged ones, or -1
+  auto number_of = [&](int c) {
     const uint64_t m = flagged(c);
-    if (m >> (i & 63) & 1)
-      movers[before[c] + (int)__popcll(m & ((1ull << (i & 63)) - 1)) - holes] = (uint16_t)i;
+    const int n = before[c] + lanes_before(m);
+    return m >> lane & 1 ? n : -1;
+  };
+  constexpr int AT_ONCE = 4;  // words of a wave in flight
+  for (int c0 = k / 64; c0 < words; c0 += AT_ONCE * W) {
+    int n[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int c = c0 + j * W + wave;
+      n[j] = c < words ? number_of(c) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      if (n[j] >= holes) movers[n[j] - holes] = (uint16_t)((c0 + j * W + wave) * 64 + lane);
   }
   __syncthreads();
-  for (int i = tid; i < k; i += NT) {
-    const int c = i >> 6;
-    const uint64_t m = flagged(c);
-    const int src = m >> (i & 63) & 1 ? movers[before[c] + (int)__popcll(m & ((1ull << (i & 63)) - 1))] : i;
-    kept[i] = src;
-    out[i] = w[src];
+  for (int c0 = 0; c0 * 64 < k; c0 += AT_ONCE * W) {
+    int src[AT_ONCE];
+    float f[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int c = min(c0 + j * W + wave, (k - 1) / 64), n = number_of(c);
+      src[j] = n < 0 ? c * 64 + lane : n < holes ? movers[n] : 0;  // (0: past k)
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) f[j] = w[min(src[j], used - 1)];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int i = (c0 + j * W + wave) * 64 + lane;
+      if (i < k) {
+        kept[i] = src[j];
+        out[i] = f[j];
+      }
+    }
   }
   for (int i = k + tid; i < p.cols; i += NT) out[i] = 0.f;
 }
