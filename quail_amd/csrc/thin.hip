@@ -17,7 +17,6 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kMaxKeys = 2560 * kPage;  // as the paged attention's
-constexpr int64_t kFullWaves = 2048;     // waves that keep the card's memory busy
 
 struct ThinArgs {
   uint8_t* pools;  // K and V of layer 0, K of layer 1, ...
@@ -263,9 +262,9 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
   for (int i = k + tid; i < p.cols; i += NT) out[i] = 0.f;
 }
 
-// The moves of a wave: 64 * PL slots of a (layer, sequence, head), PL a lane.
-// Those whose row moves are listed in LDS, so that few moves among many slots
-// fill a wave too.
+// The moves of a wave: 64 slots of a (layer, sequence, head), one a lane. Those
+// whose row moves are listed in LDS. (256 slots a wave, for more moves in each:
+// 8 to 10% slower, with few moves among the slots or many.)
 struct Place {
   int h;
   int64_t layer, head;  // head: of kept
@@ -273,7 +272,6 @@ struct Place {
   int slot;
 };
 
-template <int PL>
 __device__ __forceinline__ Place place_of(const ThinArgs& p, int64_t wid, int parts, int lane) {
   Place x;
   x.h = (int)(wid % p.HK);
@@ -281,40 +279,32 @@ __device__ __forceinline__ Place place_of(const ThinArgs& p, int64_t wid, int pa
   x.layer = ls / p.seqs;
   x.head = ls * p.HK + x.h;
   x.table = p.table + ls % p.seqs * p.table_ld;
-  x.slot = ((int)(wid / p.HK % parts) * 64 + lane) * PL;
+  x.slot = (int)(wid / p.HK % parts) * 64 + lane;
   return x;
 }
 
-template <int PL>
-__device__ __forceinline__ void sources(const ThinArgs& p, const Place& x, int (&src)[PL]) {
-  const int* kept = p.kept + x.head * p.slots + x.slot;
-#pragma unroll
-  for (int i = 0; i < PL; ++i) src[i] = x.slot + i < p.slots ? kept[i] : -1;
+__device__ __forceinline__ int source(const ThinArgs& p, const Place& x) {
+  return x.slot < p.slots ? p.kept[x.head * p.slots + x.slot] : -1;
 }
 
 // A row of D values goes by D * 2 / 16 lanes, 16 bytes each, K and V of kBatch
 // rows a lane in flight. Bound by HBM, in pieces of a head's row.
-template <int D, int PL>
+template <int D>
 __global__ __launch_bounds__(256) void thin_move_kernel(ThinArgs p, int64_t waves, int parts) {
   constexpr int LPR = D / 8, RPP = 64 / LPR, kBatch = 4;
-  __shared__ int64_t list[4][64 * PL][2];
+  __shared__ int64_t list[4][64][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wid = (int64_t)blockIdx.x * 4 + wave;
   if (wid >= waves) return;
-  const Place x = place_of<PL>(p, wid, parts, lane);
-  int src[PL], n = 0;
-  sources<PL>(p, x, src);
-#pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    const int slot = x.slot + i;
-    const bool moves = src[i] >= 0 && src[i] != slot;
-    const uint64_t mask = __ballot(moves);
-    if (moves) {
-      int64_t* to = list[wave][n + lanes_before(mask)];
-      to[0] = (int64_t)x.table[slot / kPage] * kPage + slot % kPage;
-      to[1] = (int64_t)x.table[src[i] / kPage] * kPage + src[i] % kPage;
-    }
-    n += __popcll(mask);
+  const Place x = place_of(p, wid, parts, lane);
+  const int src = source(p, x);
+  const bool moves = src >= 0 && src != x.slot;
+  const uint64_t mask = __ballot(moves);
+  const int n = __popcll(mask);
+  if (moves) {
+    int64_t* to = list[wave][lanes_before(mask)];
+    to[0] = (int64_t)x.table[x.slot / kPage] * kPage + x.slot % kPage;
+    to[1] = (int64_t)x.table[src / kPage] * kPage + src % kPage;
   }
   if (n == 0) return;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list
@@ -363,61 +353,47 @@ __device__ __forceinline__ v4i shifted16(v4i c, int shift) {
 // scale of those its rows come with (its own among them, where a row stays);
 // the codes of the others are shifted down to it, those of rows that stay too.
 // `keep` is whole pages, so no page is both read for a move and written.
-template <int D, int PL>
+template <int D>
 __global__ __launch_bounds__(256) void thin_move8_kernel(ThinArgs p, int64_t waves, int parts) {
   constexpr int LPR = D / 16, RPP = 64 / LPR, kBatch = 4;
-  constexpr int LPP = kPage / PL;  // lanes of a page
-  __shared__ int64_t list[4][64 * PL][2];
-  __shared__ int shifts[4][64 * PL];  // K's and V's, 16 bits each
+  __shared__ int64_t list[4][64][2];
+  __shared__ int shifts[4][64];  // K's and V's, 16 bits each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wid = (int64_t)blockIdx.x * 4 + wave;
   if (wid >= waves) return;
-  const Place x = place_of<PL>(p, wid, parts, lane);
-  int src[PL], n = 0;
-  sources<PL>(p, x, src);
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < PL; ++i) any |= src[i] >= 0 && src[i] != x.slot + i;
-  const uint64_t moving = __ballot(any);
+  const Place x = place_of(p, wid, parts, lane);
+  const int src = source(p, x);
+  const bool moves = src >= 0 && src != x.slot;
+  const uint64_t moving = __ballot(moves);
   if (moving == 0) return;
   uint8_t* scales = p.scales + x.layer * p.scale_stride;
   // whether a row moves into the lane's page; then all 16 of its slots hold rows
-  const bool page_moves = (moving >> (lane / LPP * LPP) & ((1u << LPP) - 1)) != 0;
-  int64_t to = 0, from[PL];
-  int bk[PL], bv[PL], top_k = 0, top_v = 0;
-#pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    from[i] = 0;
-    bk[i] = bv[i] = 0;
-    if (page_moves) {
-      from[i] = x.table[src[i] / kPage];
-      const uint16_t b = *reinterpret_cast<const uint16_t*>(scales + (from[i] * p.HK + x.h) * 2);
-      bk[i] = b & 0xff;
-      bv[i] = b >> 8;
-    }
-    top_k = max(top_k, bk[i]);
-    top_v = max(top_v, bv[i]);
+  const bool page_moves = (moving >> (lane & 48) & 0xffff) != 0;
+  int64_t to = 0, from = 0;
+  int bk = 0, bv = 0;
+  if (page_moves) {
+    to = x.table[x.slot / kPage];
+    from = x.table[src / kPage];
+    const uint16_t b = *reinterpret_cast<const uint16_t*>(scales + (from * p.HK + x.h) * 2);
+    bk = b & 0xff;
+    bv = b >> 8;
   }
-  if (page_moves) to = x.table[x.slot / kPage];
+  int top_k = bk, top_v = bv;
 #pragma unroll
-  for (int o = LPP / 2; o > 0; o >>= 1) {
+  for (int o = kPage / 2; o > 0; o >>= 1) {
     top_k = max(top_k, __shfl_xor(top_k, o, 64));
     top_v = max(top_v, __shfl_xor(top_v, o, 64));
   }
-#pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    const int slot = x.slot + i;
-    const bool write = page_moves && (src[i] != slot || bk[i] != top_k || bv[i] != top_v);
-    const uint64_t mask = __ballot(write);
-    if (write) {
-      const int m = n + lanes_before(mask);
-      list[wave][m][0] = to * kPage + slot % kPage;
-      list[wave][m][1] = from[i] * kPage + src[i] % kPage;
-      shifts[wave][m] = (top_k - bk[i]) | (top_v - bv[i]) << 16;
-    }
-    n += __popcll(mask);
+  const bool write = page_moves && (moves || bk != top_k || bv != top_v);
+  const uint64_t mask = __ballot(write);
+  const int n = __popcll(mask);
+  if (write) {
+    const int m = lanes_before(mask);
+    list[wave][m][0] = to * kPage + x.slot % kPage;
+    list[wave][m][1] = from * kPage + src % kPage;
+    shifts[wave][m] = (top_k - bk) | (top_v - bv) << 16;
   }
-  if (page_moves && lane % LPP == 0)
+  if (page_moves && lane % kPage == 0)
     *reinterpret_cast<uint16_t*>(scales + (to * p.HK + x.h) * 2) = (uint16_t)(top_k | top_v << 8);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own list
   uint8_t* k_pool = p.pools + 2 * x.layer * p.pool_stride + (int64_t)x.h * D;
@@ -496,29 +472,17 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (max_used <= keep) return QX_OK;  // no row moves
-  // slots a lane: 4 where that leaves waves enough (each then has more moves)
-  const int PL = rows * ((slots + 255) / 256) >= kFullWaves ? 4 : 1;
-  const int parts = (int)((slots + 64 * PL - 1) / (64 * PL));
+  const int parts = (int)((slots + 63) / 64);
   const int64_t waves = rows * parts;
   QX_CHECK(waves <= (1LL << 26) - 4, "thin_rows: %lld rows of %lld heads exceed one launch",
            (long long)slots, (long long)rows);
   const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
-#define QX_MOVE(K, DD)                                                                     \
-  if (PL == 4) hipLaunchKernelGGL((K<DD, 4>), grid, block, 0, stream, a, waves, parts);    \
-  else hipLaunchKernelGGL((K<DD, 1>), grid, block, 0, stream, a, waves, parts)
+#define QX_MOVE(K, DD) hipLaunchKernelGGL((K<DD>), grid, block, 0, stream, a, waves, parts)
   if (waves) {
     if (element_bytes == 2) {
-      if (D == 128) {
-        QX_MOVE(thin_move_kernel, 128);
-      } else {
-        QX_MOVE(thin_move_kernel, 64);
-      }
+      if (D == 128) QX_MOVE(thin_move_kernel, 128); else QX_MOVE(thin_move_kernel, 64);
     } else {
-      if (D == 128) {
-        QX_MOVE(thin_move8_kernel, 128);
-      } else {
-        QX_MOVE(thin_move8_kernel, 64);
-      }
+      if (D == 128) QX_MOVE(thin_move8_kernel, 128); else QX_MOVE(thin_move8_kernel, 64);
     }
   }
 #undef QX_MOVE
