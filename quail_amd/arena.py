@@ -382,7 +382,7 @@ class KVArena:
         columns)), the row that each slot holds as it was numbered before, -1
         past min(used, keep); and the slots' weights in the shape of `weights`,
         0 past them."""
-        from quail_amd.engine import _stream
+        from quail_amd.engine import _launch
         used, table = tables["used"], tables["table"]
         heads, dim = self.kv_shape
         for name, t, dims in (("used", used, 1), ("table", table, 2)):
@@ -416,7 +416,7 @@ class KVArena:
             raise ValueError(f"tables and weights on the arena's GPU {device}")
         shape = (self.num_layers, seqs, heads)
         kept = torch.empty(*shape, min(keep, cols), dtype=torch.int32, device=weights.device)
-        out = torch.empty(*shape, cols, dtype=torch.float32, device=weights.device)
+        out = torch.empty_like(weights, memory_format=torch.contiguous_format)
         scales = (None, 0) if self.scales is None else (self.scales.data_ptr(), self.scales.stride(0))
         pool = self.num_pages * self.page_tokens * heads * dim * self.storage.element_size()
         args = (self.storage.data_ptr(), pool, self.storage.element_size(), *scales,
@@ -424,11 +424,7 @@ class KVArena:
                 table.stride(0), *shape, dim, self.page_tokens, max_used, cols, keep, sinks, recent,
                 kept.data_ptr(), out.data_ptr())
         try:
-            if device == torch.cuda.current_device():
-                _lib.call("qx_thin_rows", *args, _stream())
-            else:
-                with torch.cuda.device(device):
-                    _lib.call("qx_thin_rows", *args, _stream())
+            _launch(device, "qx_thin_rows", *args)
         except _lib.QxError as err:
             if "hipError" in str(err):
                 raise

@@ -522,7 +522,8 @@ int64_t batch_of(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ, int6
   const int64_t G = HQ / HK, rows = std::max<int64_t>(1, kCols / G);
   const int64_t groups = std::max<int64_t>(1, ((max_q + rows - 1) / rows + kStart) * tiles_of(max_used, 2) * HK);
   int64_t n = std::min<int64_t>({seqs, kSeqs, (1LL << 30) / groups});
-  n = std::min(n, kScratch / std::max<int64_t>(1, part_bytes(1, max_used, HK) - part_bytes(0, max_used, HK)));
+  const int64_t fixed = part_bytes(0, max_used, HK), each = part_bytes(1, max_used, HK) - fixed;
+  n = std::min(n, (kScratch - fixed) / std::max<int64_t>(each, 1));
   return std::max<int64_t>(n, 1);
 }
 

@@ -16,7 +16,6 @@ Layouts are the reference's: FP8 activations are e4m3fn (n, K) with
 (N/128, K/128).
 """
 
-import contextlib
 import functools
 import math
 import os
@@ -87,6 +86,15 @@ def _stream():
     if _raw_stream is None or _current_device is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(_current_device())
+
+
+def _launch(device, name, *args):
+    """_lib.call(name, *args, stream) on the current stream of GPU `device`,
+    which is made the current one for the call where it is not."""
+    if device == (torch.cuda.current_device() if _current_device is None else _current_device()):
+        return _lib.call(name, *args, _stream())
+    with torch.cuda.device(device):
+        _lib.call(name, *args, _stream())
 
 
 def gemm_config(n: int, k: int, m: int) -> int:
@@ -992,9 +1000,8 @@ class Engine:
         seqs, max_q, max_used = used.shape[0], int(tables["max_q"]), int(tables["max_used"])
         device = q3.get_device()
         if out is None:
-            like = weights
-            cols = table.shape[1] * PAGE_ROWS if like is None else like.shape[-1]
-            out = torch.empty(seqs, hk, cols, dtype=torch.float32, device=q3.device)
+            out = torch.empty(seqs, hk, table.shape[1] * PAGE_ROWS, dtype=torch.float32, device=q3.device) \
+                if weights is None else torch.empty_like(weights, memory_format=torch.contiguous_format)
         for name, t in (("weights", weights), ("out", out)):
             if t is not None and (t.dtype != torch.float32 or t.shape != (seqs, hk, out.shape[-1])
                                   or (t.shape[2] > 1 and t.stride(2) != 1)):
@@ -1021,10 +1028,8 @@ class Engine:
                 int(tables.get("causal", True)), _ptr(weights),
                 *((0, 0) if weights is None else weights.stride()[:2]), out.data_ptr(),
                 *out.stride()[:2], cols)
-        with contextlib.nullcontext() if device == torch.cuda.current_device() else \
-                torch.cuda.device(device):
-            space = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
-            _lib.call("qx_key_weights", *args, _ptr(space), size, _stream())
+        space = torch.empty(size, dtype=torch.uint8, device=q3.device) if size else None
+        _launch(device, "qx_key_weights", *args, _ptr(space), size)
         return out
 
     def attention_unified(self, q3, k3, v3, meta, *, softmax_scale=None, output=None):

@@ -21,7 +21,7 @@ import math
 
 import torch
 
-from quail_amd import _lib
+from quail_amd.engine import _launch
 
 _KNOWN = {"default": set(), "linear": {"factor"},
           "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
@@ -133,24 +133,37 @@ class RotaryEmbedding:
     def _rows(self, name, x, n):
         """(heads, row stride) of rows (n, heads * head_dim) or (n, heads, head_dim)."""
         d = self.head_size
-        if x.dim() == 3:
-            ok = x.shape[2] == d and x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == d)
-            heads = x.shape[1]
+        shape, stride = x.shape, x.stride()
+        if len(shape) == 2:
+            heads, rest = divmod(shape[1], d)
+            ok = not rest and stride[1] == 1
         else:
-            ok = x.dim() == 2 and x.shape[1] % d == 0 and x.stride(1) == 1
-            heads = x.shape[-1] // d
-        if not ok or x.shape[0] != n or heads == 0:
-            raise ValueError(f"{name}: {n} rows of contiguous heads of {d}, not {tuple(x.shape)} "
-                             f"with strides {x.stride()}")
-        if n > 1 and x.stride(0) < heads * d:
-            raise ValueError(f"{name}: rows overlap (strides {x.stride()})")
-        return heads, x.stride(0) if n > 1 else heads * d
+            ok = len(shape) == 3 and shape[2] == d and stride[2] == 1
+            heads = shape[1] if ok else 0
+            ok = ok and (heads == 1 or stride[1] == d)
+        if not ok or shape[0] != n or heads == 0:
+            raise ValueError(f"{name}: {n} rows of contiguous heads of {d}, not {tuple(shape)} "
+                             f"with strides {stride}")
+        if n <= 1:
+            return heads, heads * d
+        if stride[0] < heads * d:
+            raise ValueError(f"{name}: rows overlap (strides {stride})")
+        return heads, stride[0]
+
+    def _result(self, x, heads, ld, y, n):
+        """(result, its row stride) for rows x: a new tensor, or y."""
+        if y is None:
+            return torch.empty_like(x, memory_format=torch.contiguous_format), heads * self.head_size
+        if y is x:
+            return x, ld
+        if y.dtype != x.dtype or y.shape != x.shape:
+            raise ValueError(f"out of {tuple(y.shape)} {y.dtype} for {tuple(x.shape)} {x.dtype}")
+        return y, self._rows("out", y, n)[1]
 
     def __call__(self, positions, q, k=None, *, out=None):
         """q and k (n rows, bf16, fp16 or fp32) rotated by `positions` (n,
         int64, any value), as new tensors or into out = (q's, k's), which may
         be the rows themselves. With q alone, `out` and the result are q's."""
-        from quail_amd.engine import _stream
         n = q.shape[0]
         if positions.shape != (n,) or positions.dtype != torch.int64 or \
                 not (n == 1 or positions.is_contiguous()):
@@ -159,34 +172,24 @@ class RotaryEmbedding:
         if kind is None or (k is not None and k.dtype != q.dtype):
             raise ValueError(f"rows of {q.dtype}{'' if k is None else f' and {k.dtype}'}: one of "
                              "bf16, fp16 and fp32")
+        q_to, k_to = (None, None) if out is None else (out, None) if k is None else out
+        hq, q_ld = self._rows("q", q, n)
+        qo, qo_ld = self._result(q, hq, q_ld, q_to, n)
+        tensors = (positions, self._turns, qo)
+        hk = k_ld = ko_ld = 0
+        kp = kop = None
+        if k is not None:
+            hk, k_ld = self._rows("k", k, n)
+            ko, ko_ld = self._result(k, hk, k_ld, k_to, n)
+            tensors += (k, ko)
+            kp, kop = k.data_ptr(), ko.data_ptr()
         device = q.get_device()
-        outs = (None, None) if out is None else (out, None) if k is None else out
-        rows, results, elsewhere = [], [], False
-        for name, x, y in (("q", q, outs[0]), ("k", k, outs[1])):
-            if x is None:
-                rows.append((None, 0, 0, None, 0))
-                continue
-            heads, ld = self._rows(name, x, n)
-            if y is None:
-                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            elif y.dtype != x.dtype or y.shape != x.shape:
-                raise ValueError(f"out of {tuple(y.shape)} {y.dtype} for {tuple(x.shape)} {x.dtype}")
-            elsewhere |= device < 0 or x.get_device() != device or y.get_device() != device
-            rows.append((x.data_ptr(), heads, ld, y.data_ptr(), self._rows("out", y, n)[1]))
-            results.append(y)
-        if elsewhere:
-            raise ValueError("rows and results are on one GPU")
-        if positions.get_device() != device or self._turns.get_device() != device:
-            raise ValueError(f"rows on GPU {device}, positions on {positions.device}, module on "
-                             f"{self._turns.device}")
-        (qp, hq, q_ld, qo, qo_ld), (kp, hk, k_ld, ko, ko_ld) = rows
+        if device < 0 or any(t.get_device() != device for t in tensors):
+            raise ValueError("rows, results, positions and the module are on one GPU, not "
+                             f"{q.device}, {', '.join(str(t.device) for t in tensors)}")
         if n:
-            args = (qp, q_ld, kp, k_ld, qo, qo_ld, ko, ko_ld, positions.data_ptr(),
-                    self._turns.data_ptr(), self.factor, n, hq, hk, self.head_size,
-                    self.rotary_dim, int(not self.is_neox_style), kind)
-            if device == torch.cuda.current_device():
-                _lib.call("qx_rotary", *args, _stream())
-            else:
-                with torch.cuda.device(device):
-                    _lib.call("qx_rotary", *args, _stream())
-        return results[0] if k is None else tuple(results)
+            args = (q.data_ptr(), q_ld, kp, k_ld, qo.data_ptr(), qo_ld, kop, ko_ld,
+                    positions.data_ptr(), self._turns.data_ptr(), self.factor, n, hq, hk,
+                    self.head_size, self.rotary_dim, int(not self.is_neox_style), kind)
+            _launch(device, "qx_rotary", *args)
+        return qo if k is None else (qo, ko)
