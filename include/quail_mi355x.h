@@ -333,10 +333,12 @@ int qx_rotary(const void* q, int64_t q_ld, const void* k, int64_t k_ld, void* q_
  * an 8-bit arena's pages. max_q and max_used bound the sequences' rows and keys
  * (max_used at most qx_paged_attention_max_keys and cols); `rows` is that of q
  * and lse. Sequences and heads of base and out lie base_seq, base_head, out_seq
- * and out_head floats apart. Sums are fp32, in an order that max_q, HQ / HK and
- * the sequence's own sizes fix. workspace: qx_key_weights_workspace bytes of the
- * caller's, 16-byte aligned (NULL where that is 0; at most 128 MiB, or one
- * sequence's), used by this call alone until the stream has passed it.
+ * and out_head floats apart, out overlaps nothing else. Sums are fp32, in an order
+ * that the bounds, the heads and the lengths of the call's sequences fix (the same
+ * call gives the same bits). q_ld is below 2^19. workspace:
+ * qx_key_weights_workspace bytes of the caller's, 16-byte aligned (NULL where that
+ * is 0; at most 128 MiB, or one sequence's), used by this call alone until the
+ * stream has passed it.
  */
 int64_t qx_key_weights_workspace(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ,
                                  int64_t HK);

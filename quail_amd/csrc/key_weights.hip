@@ -4,20 +4,25 @@
 //                  exp(scale q[i, g] . k[j, h] - lse[g, i])
 // over pages of 16 rows, bf16 or e4m3 codes with a scale per (page, head).
 //
-// A wave holds kKW keys of one KV head in registers, as the A operand of
+// A wave holds 32 KT keys of one KV head in registers, as the A operand of
 // v_mfma_f32_32x32x16_bf16, and the (row, head of the group) pairs of the
 // sequence stream past it as its columns, kCols of them a step, through LDS
 // (four waves share them). Rows are keys, so a column's log-sum-exp is one value
 // a lane and a key's sum stays in one register across the steps: a score costs
 // one multiply-add, one exponential and one addition, and lanes are added up
-// once, at the end. Sums are fp32, in an order that the call's sizes fix.
+// once, at the end. Sums are fp32, in an order that the call's lengths fix: no
+// atomics.
 //
-// Where there are few rows a launch of one workgroup per (sequence, head, key
-// tile) writes the result itself (whole sequences' rows in one workgroup).
-// Many rows are cut into chunks, an item per (sequence, head, key tile, chunk)
-// that sees anything, taken in turn by workgroups that find their items from the
-// sequences' lengths; their sums go to scratch memory and a second launch adds
-// them up, chunk by chunk.
+// Few rows (one token a sequence): a workgroup for each (sequence, head, key
+// tile) reads its keys once and writes the result itself; the keys' bytes bound
+// it. Many rows: 512 workgroups, two a CU, share the groups of rows of all tiles
+// evenly, whatever the sequences' lengths; a tile's parts go to scratch memory
+// and a second launch adds them up in the order of the rows. There a step of 64
+// columns with a wave's 64 keys is 32 MFMAs of 32 cycles (8003 rows of 32 heads,
+// causal, 218 us at the rate of a large product), and the 64 exponentials a lane
+// cost the vector unit as long, so that the two have to run side by side
+// (item_sums). 8003 rows of 32/8 heads of 128 take 261-278 us on several cards, an AI.IF pack of
+// 3900 rows over a kept prefix 71-74.
 #include "qx_common.h"
 #include "qx_status.h"
 
@@ -32,7 +37,8 @@ constexpr int kMaxKeys = 2560 * kPage;
 constexpr int kCols = 64;            // (row, head) columns of a step
 constexpr int kSeqs = 2048;          // sequences of one launch (their bounds in LDS)
 constexpr int kShares = 512;         // workgroups that the work is shared by: two a CU
-constexpr int kStart = 8;            // groups that the start of a key tile takes as long as
+constexpr int kStart = 8;            // groups that a key tile's start takes as long as (0: 8003 rows 332 us, 8: 288)
+constexpr int kFirst = 40;           // of 64: the part of a pair's groups that its first workgroup has
 constexpr int kMinShare = 2;         // groups of a share, at least
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -371,7 +377,10 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
   return acc[0];
 }
 
-// One workgroup per (key tile, sequence, head), heads fastest.
+// One workgroup per (key tile, sequence, head), heads fastest (a page's heads lie
+// side by side, and neighbouring workgroups read them at about the same time).
+// Two contexts of 40,000 keys, 8 heads of 128: 42-50 us, 328 MB with the weights
+// there before and after, 33 at the rate of a copy.
 template <int D, bool F8, int KT>
 __global__ __launch_bounds__(256, 2) void key_weights_direct_kernel(WeightsArgs p) {
   __shared__ __align__(16) uint8_t lds[kLds];
@@ -412,15 +421,24 @@ __device__ __forceinline__ void bounds(const WeightsArgs& p, int lane, int tile,
   if (lane == 0) bound[0] = 0;
 }
 
-// groups of a workgroup
-__device__ __forceinline__ int share_of(int total, int workgroups) {
-  return max(kMinShare, (total + workgroups - 1) / workgroups);
+// Shares go in pairs, one for each of the two workgroups that run on a CU: of
+// their waves the older issue first, so that the one which started first took
+// 203 us for half of 8003 rows and the other 275. It gets the larger share (of
+// 64ths 32: 286 us, an AI.IF pack 85; 36: 275 and 76; 40: 267 and 71; 44 on another
+// card 4% more than 40).
+struct Shares {
+  int first, both;  // groups of the first of a pair, and of the two
+};
+__device__ __forceinline__ Shares shares_of(int total) {
+  const int both = max(2 * kMinShare, (total + kShares / 2 - 1) / (kShares / 2));
+  return {(int)((int64_t)both * kFirst / 64), both};
 }
 
 // Many rows: the groups of all heads' sequences' key tiles, in that order, in
-// equal shares, one a workgroup. A share begins and ends anywhere; each tile's
-// part of it goes to scratch memory, at the tile's number plus the workgroup's
-// (both only rise along the order).
+// equal shares, one a workgroup (items of a tile and some of its rows, taken in
+// turn: an AI.IF pack 110 us where the shares took 88). A share begins and ends
+// anywhere; each tile's part of it goes to scratch memory, at the tile's number
+// plus the workgroup's (both only rise along the order).
 template <int D, bool F8>
 __global__ __launch_bounds__(256, 2) void key_weights_share_kernel(WeightsArgs p) {
   constexpr int KT = 2, TILE = tile_keys(KT);
@@ -433,12 +451,14 @@ __global__ __launch_bounds__(256, 2) void key_weights_share_kernel(WeightsArgs p
     for (int s = tid; s <= p.seqs; s += 256) p.bound[s] = bound[s];
   auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   const int of_head = uniform(bound[p.seqs]);
-  const int total = of_head * p.HK, share = share_of(total, gridDim.x);
-  // workgroups i, i + 8, ... run on one XCD: it takes neighbouring shares, whose
-  // query rows are the same
-  const int w = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
-  int at = min(w * share, total);
-  const int end = uniform(min(at + share, total));
+  const int total = of_head * p.HK;
+  const Shares share = shares_of(total);
+  // workgroups i, i + 8, ... run on one XCD, half of them first on their CUs: it
+  // takes neighbouring pairs, whose query rows are the same
+  const int nth = blockIdx.x / 8, half = kShares / 16;
+  const int pair = blockIdx.x % 8 * half + nth % half, w = 2 * pair + nth / half;
+  int at = min(pair * share.both + nth / half * share.first, total);
+  const int end = uniform(min(at + (nth / half ? share.both - share.first : share.first), total));
   if (at == end) return;
   int h = at / of_head, in = at % of_head, s;
   {
@@ -483,7 +503,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_share_kernel(WeightsArgs p
   }
 }
 
-__global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p, int workgroups) {
+__global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
   constexpr int TILE = tile_keys(2);
   const int h = blockIdx.y % p.HK, s = blockIdx.y / p.HK;
   const int j = blockIdx.x * 256 + threadIdx.x;
@@ -493,17 +513,23 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p, in
   const int t = j / TILE;
   float sum = 0.f;
   if (j < x.used && t < work.tiles) {
-    const int of_head = p.bound[p.seqs], share = share_of(of_head * p.HK, workgroups);
+    const int of_head = p.bound[p.seqs];
+    const Shares share = shares_of(of_head * p.HK);
+    auto share_at = [&](int group) {
+      const int pair = group / share.both;
+      return 2 * pair + (group - pair * share.both >= share.first);
+    };
     const int at = of_head * h + p.bound[s] + groups_before(work, p.drop, t);
-    const int last = (at + groups_of(work, p.drop, t) - 1) / share;
+    const int last = share_at(at + groups_of(work, p.drop, t) - 1);
     const float* part = p.part + (((int64_t)h * p.seqs + s) * p.tiles + t) * TILE + j % TILE;
-    for (int w = at / share; w <= last; ++w) sum += part[(int64_t)w * TILE];
+    for (int w = share_at(at); w <= last; ++w) sum += part[(int64_t)w * TILE];
   }
   if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
   p.out[s * p.out_s + h * p.out_h + j] = sum;
 }
 
-// Whether the rows go in shares: a key tile is worth several steps
+// Whether the rows go in shares: more than the two steps that a tile's workgroup
+// has no better to do in than read its keys
 bool shared_rows(int64_t max_q, int64_t G) { return max_q * G > 2 * kCols; }
 
 int64_t tiles_of(int64_t keys, int KT) { return (keys + tile_keys(KT) - 1) / tile_keys(KT); }
@@ -523,7 +549,7 @@ int64_t batch_of(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HQ, int6
   const int64_t groups = std::max<int64_t>(1, ((max_q + rows - 1) / rows + kStart) * tiles_of(max_used, 2) * HK);
   int64_t n = std::min<int64_t>({seqs, kSeqs, (1LL << 30) / groups});
   const int64_t fixed = part_bytes(0, max_used, HK), each = part_bytes(1, max_used, HK) - fixed;
-  n = std::min(n, (kScratch - fixed) / std::max<int64_t>(each, 1));
+  n = std::min({n, (kScratch - fixed) / std::max<int64_t>(each, 1), 65535 / HK});
   return std::max<int64_t>(n, 1);
 }
 
@@ -573,12 +599,16 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
            (long long)workspace_bytes);
   const int64_t G = HQ / HK;
   const bool shares = shared_rows(max_q, G);
-  // one step a tile: keys are read once and hardly computed with, so that more
-  // and smaller workgroups read them sooner
+  // few rows: smaller tiles, so that more workgroups read the keys (8 sequences
+  // of 700 keys 13.3 us, with the larger ones 22; two contexts of 40,000 41.8 and
+  // 41.2)
   const int KT = shares ? 2 : 1;
   const int64_t tiles = tiles_of(shares ? max_used : cols, KT);
   const int64_t step_rows = G > kCols ? 1 : kCols / G;
-  const int64_t batch = shares ? batch_of(seqs, max_q, max_used, HQ, HK) : std::min<int64_t>(seqs, kSeqs);
+  const int64_t batch = shares ? batch_of(seqs, max_q, max_used, HQ, HK)
+                               : std::min<int64_t>({seqs, kSeqs, ((1LL << 24) - 1) / (tiles * HK)});
+  QX_CHECK(batch > 0, "key_weights: %lld columns of %lld heads exceed one launch", (long long)cols,
+           (long long)HK);
   QX_CHECK(!shares || ((max_q + step_rows - 1) / step_rows + kStart) * tiles * HK < (1LL << 30),
            "key_weights: %lld rows of %lld heads over %lld keys exceed one launch", (long long)max_q,
            (long long)HQ, (long long)max_used);
@@ -602,18 +632,14 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
     else hipLaunchKernelGGL((K<64, false __VA_ARGS__>), grid, dim3(256), 0, stream, a);          \
   }
     if (!shares) {
-      QX_CHECK(tiles * n * HK < (1LL << 24), "key_weights: %lld key tiles exceed one launch",
-               (long long)(tiles * n * HK));
       const dim3 grid((unsigned)(tiles * n * HK));
       QX_KEYS(key_weights_direct_kernel, grid, , 1)
     } else {
-      QX_CHECK(n * HK < 65536, "key_weights: %lld sequences of %lld heads exceed one launch",
-               (long long)n, (long long)HK);
       QX_KEYS(key_weights_share_kernel, dim3(kShares))
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
       hipLaunchKernelGGL(key_weights_join_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)(n * HK)),
-                         dim3(256), 0, stream, a, kShares);
+                         dim3(256), 0, stream, a);
     }
 #undef QX_KEYS
     const hipError_t e = hipGetLastError();

@@ -990,7 +990,9 @@ class Engine:
         Returns them, as a new tensor or in `out` of the same shape (which may
         be `weights`): without either, of the tables' width in rows. Columns
         past a sequence's keys stay as they were (0 without `weights`). The
-        sums are fp32, in the same order at each call of the same sizes."""
+        sums are fp32, in an order that the lengths of the call's sequences fix:
+        equal calls give equal bits, and a sequence's last bits may depend on
+        what it is called with. `out` overlaps nothing but `weights`."""
         n, hq, d = self._check_reads(q3, tables)
         hk = self.num_kv_heads
         if lse.shape != (hq, n) or lse.dtype != torch.float32 or (n > 1 and lse.stride(1) != 1):

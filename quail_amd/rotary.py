@@ -163,7 +163,7 @@ class RotaryEmbedding:
     def __call__(self, positions, q, k=None, *, out=None):
         """q and k (n rows, bf16, fp16 or fp32) rotated by `positions` (n,
         int64, any value), as new tensors or into out = (q's, k's), which may
-        be the rows themselves. With q alone, `out` and the result are q's."""
+        be the rows themselves and overlap them in no other way. With q alone, `out` and the result are q's."""
         n = q.shape[0]
         if positions.shape != (n,) or positions.dtype != torch.int64 or \
                 not (n == 1 or positions.is_contiguous()):
