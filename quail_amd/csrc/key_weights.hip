@@ -21,8 +21,8 @@
 // columns with a wave's 64 keys is 32 MFMAs of 32 cycles (8003 rows of 32 heads,
 // causal, 218 us at the rate of a large product), and the 64 exponentials a lane
 // cost the vector unit as long, so that the two have to run side by side
-// (item_sums). 8003 rows of 32/8 heads of 128 take 261-278 us on several cards, an AI.IF pack of
-// 3900 rows over a kept prefix 71-74.
+// (item_sums). 8003 rows of 32/8 heads of 128 take 261-278 us on several cards, an
+// AI.IF pack of 46 sequences over a kept prefix 71-74.
 #include "qx_common.h"
 #include "qx_status.h"
 

@@ -29,31 +29,34 @@ __device__ __forceinline__ float to_f32(uint16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float to_f32(float v) { return v; }
 
-// N results to T, each rounded once (to nearest even)
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> load(const T* x) {
+  return *reinterpret_cast<const Pack<T, N>*>(x);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store(T* y, const Pack<T, N>& v) {
+  *reinterpret_cast<Pack<T, N>*>(y) = v;
+}
+
+// N results in T, each rounded once (to nearest even)
 template <int N>
-__device__ __forceinline__ void store(const float (&v)[N], Pack<uint16_t, N>* out) {
+__device__ __forceinline__ Pack<uint16_t, N> rounded(const float (&v)[N], const uint16_t*) {
   if constexpr (N == 1) {
-    out->x[0] = f32_to_bf16(v[0]);
+    return {{f32_to_bf16(v[0])}};
   } else {
     Pack<uint32_t, N / 2> w;
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) w.x[i] = pack2_bf16(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<Pack<uint32_t, N / 2>*>(out) = w;
+    return __builtin_bit_cast(Pack<uint16_t, N>, w);
   }
 }
-template <int N>
-__device__ __forceinline__ void store(const float (&v)[N], Pack<_Float16, N>* out) {
-  Pack<_Float16, N> w;
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> rounded(const float (&v)[N], const T*) {
+  Pack<T, N> w;
 #pragma unroll
-  for (int i = 0; i < N; ++i) w.x[i] = (_Float16)v[i];
-  *out = w;
-}
-template <int N>
-__device__ __forceinline__ void store(const float (&v)[N], Pack<float, N>* out) {
-  Pack<float, N> w;
-#pragma unroll
-  for (int i = 0; i < N; ++i) w.x[i] = v[i];
-  *out = w;
+  for (int i = 0; i < N; ++i) w.x[i] = (T)v[i];
+  return w;
 }
 
 // y_a = a cos t - b sin t, y_b = b cos t + a sin t for each pair (a, b) of a
@@ -63,11 +66,14 @@ __device__ __forceinline__ void store(const float (&v)[N], Pack<float, N>* out) 
 // a row of them serves every head of q and k.
 // A wave per row: its lanes compute the row's cos and sin into LDS, then take
 // units of N pairs' elements (16 bytes; N = 1: rows whose strides, alignment or
-// pairs do not allow that), `kBatch` of them in flight. Reads and writes each
-// row once: bound by HBM.
+// pairs do not allow that). Reads and writes each row once and is bound by HBM:
+// 32 query and 8 key heads of 128 in 2 bytes, 15,654 rows 64 us from memory (321 MB
+// at 5.0 TB/s; a copy reaches 5.1), 56 over and over. Waves enough hide the loads:
+// with two units of a lane in flight 57, three 60, five 62-67. Stores past the
+// caches 50, but what reads the rows next lost more (4000 rows and a copy of q 28.0
+// us, 24.8 so).
 template <typename T, int N, bool INTERLEAVED>
 __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs p) {
-  constexpr int kBatch = 5;
   __shared__ float cs[kWaves][2][kMaxPairs];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = (int64_t)blockIdx.x * kWaves + wave;
@@ -90,59 +96,42 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs p) {
   T* ko = static_cast<T*>(p.ko) + row * p.ko_ld;
   auto in = [&](int head) { return head < p.HQ ? q + head * p.D : k + (head - p.HQ) * p.D; };
   auto out = [&](int head) { return head < p.HQ ? qo + head * p.D : ko + (head - p.HQ) * p.D; };
-  typedef Pack<T, N> V;
   // a unit: N pairs of half layout (two packs), or the 2 N elements of N
   // interleaved ones
   const int units = pairs / N;
   const int step_h = 64 / units, step_u = 64 % units;
   int head = lane / units, u = lane % units;
-  for (; head < p.heads;) {
-    V a[kBatch], b[kBatch];
-    int hs[kBatch], us[kBatch];
+  while (head < p.heads) {
+    const int at_a = INTERLEAVED ? 2 * u * N : u * N, at_b = INTERLEAVED ? at_a + N : at_a + pairs;
+    const Pack<T, N> a = load<N>(in(head) + at_a), b = load<N>(in(head) + at_b);
+    const float *c = &cs[wave][0][u * N], *s = &cs[wave][1][u * N];
+    float xa[N], xb[N];
+    if constexpr (!INTERLEAVED || N == 1) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      hs[i] = head;
-      us[i] = u;
-      if (head < p.heads) {
-        const T* x = in(head);
-        a[i] = *reinterpret_cast<const V*>(x + (INTERLEAVED ? 2 * u * N : u * N));
-        b[i] = *reinterpret_cast<const V*>(x + (INTERLEAVED ? 2 * u * N + N : pairs + u * N));
+      for (int e = 0; e < N; ++e) {
+        const float va = to_f32(a.x[e]), vb = to_f32(b.x[e]);
+        xa[e] = va * c[e] - vb * s[e];
+        xb[e] = vb * c[e] + va * s[e];
       }
-      head += step_h;
-      u += step_u;
-      if (u >= units) {
-        u -= units;
-        ++head;
-      }
-    }
+    } else {  // each pack holds N / 2 pairs
+      auto turn = [&](const Pack<T, N>& v, float (&y)[N], int first) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (hs[i] >= p.heads) continue;
-      const float* c = &cs[wave][0][us[i] * N];
-      const float* s = &cs[wave][1][us[i] * N];
-      float xa[N], xb[N];
-      if constexpr (!INTERLEAVED || N == 1) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float va = to_f32(a[i].x[e]), vb = to_f32(b[i].x[e]);
-          xa[e] = va * c[e] - vb * s[e];
-          xb[e] = vb * c[e] + va * s[e];
+        for (int e = 0; e < N / 2; ++e) {
+          const float va = to_f32(v.x[2 * e]), vb = to_f32(v.x[2 * e + 1]);
+          y[2 * e] = va * c[first + e] - vb * s[first + e];
+          y[2 * e + 1] = vb * c[first + e] + va * s[first + e];
         }
-      } else {  // each pack holds N / 2 pairs
-        auto turn = [&](const V& v, float (&y)[N], int first) {
-#pragma unroll
-          for (int e = 0; e < N / 2; ++e) {
-            const float va = to_f32(v.x[2 * e]), vb = to_f32(v.x[2 * e + 1]);
-            y[2 * e] = va * c[first + e] - vb * s[first + e];
-            y[2 * e + 1] = vb * c[first + e] + va * s[first + e];
-          }
-        };
-        turn(a[i], xa, 0);
-        turn(b[i], xb, N / 2);
-      }
-      T* y = out(hs[i]);
-      store(xa, reinterpret_cast<V*>(y + (INTERLEAVED ? 2 * us[i] * N : us[i] * N)));
-      store(xb, reinterpret_cast<V*>(y + (INTERLEAVED ? 2 * us[i] * N + N : pairs + us[i] * N)));
+      };
+      turn(a, xa, 0);
+      turn(b, xb, N / 2);
+    }
+    store(out(head) + at_a, rounded(xa, (T*)nullptr));
+    store(out(head) + at_b, rounded(xb, (T*)nullptr));
+    head += step_h;
+    u += step_u;
+    if (u >= units) {
+      u -= units;
+      ++head;
     }
   }
   // the rest of each head as it is
@@ -152,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(RotaryArgs p) {
     const int h = i / rest, e = p.R + i % rest * N;
     const T *x = in(h) + e;
     T* y = out(h) + e;
-    if (x != y) *reinterpret_cast<V*>(y) = *reinterpret_cast<const V*>(x);
+    if (x != y) store(y, load<N>(x));
   }
 }
 
