@@ -476,6 +476,8 @@ class KVArena:
         tokens = acct.key_tokens(key)
         if count < 0:
             raise ValueError(f"{count} more rows")
+        if len(acct.table_pages(key)) < acct.pages_needed(tokens):
+            raise ValueError(f"{key!r}: leading pages were dropped")
         if acct.grow(key, tokens + count) is None:
             return None
         acct.set_tokens(key, tokens + count)

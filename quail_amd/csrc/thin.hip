@@ -457,6 +457,10 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   QX_CHECK(pools && weights && used && out && (kept || slots == 0) && (table || max_used == 0),
            "thin_rows: null pointer");
   QX_CHECK(rows < (1LL << 21), "thin_rows: %lld heads exceed one launch", (long long)rows);
+  const int parts = (int)((slots + 63) / 64);
+  const int64_t waves = rows * parts;
+  QX_CHECK(waves <= (1LL << 26) - 4, "thin_rows: %lld rows of %lld heads exceed one launch",
+           (long long)slots, (long long)rows);
   ThinArgs a{(uint8_t*)pools, pool_stride, (uint8_t*)scales, scale_stride, weights, w_layer, w_seq,
              w_head, used, table, table_ld, (int)seqs, (int)HK, (int)max_used, (int)cols,
              (int)(keep < kMaxKeys ? keep : kMaxKeys), (int)slots, (int)sinks, (int)recent, kept, out};
@@ -473,10 +477,6 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (max_used <= keep) return QX_OK;  // no row moves
-  const int parts = (int)((slots + 63) / 64);
-  const int64_t waves = rows * parts;
-  QX_CHECK(waves <= (1LL << 26) - 4, "thin_rows: %lld rows of %lld heads exceed one launch",
-           (long long)slots, (long long)rows);
   const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
 #define QX_MOVE(K, DD) hipLaunchKernelGGL((K<DD>), grid, block, 0, stream, a, waves, parts)
   if (waves) {

@@ -1018,12 +1018,13 @@ class Engine:
         k_pool = self.arena.layer_kv(layer)[0]
         if not eight_bit:
             self._check_pools(*self.arena.layer_kv(layer))
-        for t in (lse, used, table, k_pool, out, weights):
+        for t in (lse, tables["cu_q"], used, table, k_pool, out, weights):
             if t is not None and (device < 0 or t.get_device() != device):
                 raise ValueError(f"query rows on {q3.device}, {tuple(t.shape)} on {t.device}")
         scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
         size = _key_weights_workspace(seqs, max_q, max_used, hq, hk)
-        args = (q3.data_ptr(), q3.stride(0), lse.data_ptr(), lse.stride(0) if hq > 1 else n,
+        args = (q3.data_ptr(), q3.stride(0) if n > 1 else hq * d, lse.data_ptr(),
+                lse.stride(0) if hq > 1 else n,
                 k_pool.data_ptr(), _ptr(self.arena.layer_scales(layer)) if eight_bit else None,
                 tables["cu_q"].data_ptr(), used.data_ptr(), table.data_ptr(), table.stride(0), seqs,
                 n, max_q, max_used, hq, hk, d, self.arena.page_tokens, scale,

@@ -190,7 +190,8 @@ def load_qwen3_fp8(path, device="cuda", num_layers: int | None = None, scaled_ro
     config = json.loads((path / "config.json").read_text())
     scaling = _scaled_rope(config) if scaled_rope else None
     if scaling:
-        scaling.setdefault("original_max_position_embeddings", config.get("max_position_embeddings"))
+        if not scaling.get("original_max_position_embeddings"):
+            scaling["original_max_position_embeddings"] = config.get("max_position_embeddings", 40960)
         rotary = RotaryEmbedding(d, base=cfg.theta, max_positions=cfg.max_positions,
                                  scaling=scaling, device=device)
     else:

@@ -124,10 +124,17 @@ class RotaryEmbedding:
             if self.rotary_dim != self.head_size or not self.is_neox_style:
                 raise ValueError("the engine's passes rotate whole heads in half pairs; rows of "
                                  "other layouts are rotated by calling the module")
+            on_gpu = self.device.type == "cuda"
+            if on_gpu and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("cos_sin_cache is made at its first use, which a graph cannot "
+                                   "capture; read it once before")
             turns = torch.arange(self.max_positions, dtype=torch.float64,
                                  device=self.device)[:, None] * self._turns
             angle = (turns - turns.round()) * (2 * math.pi)
-            self._cache = (torch.cat([angle.cos(), angle.sin()], 1) * self.factor).to(self.dtype)
+            cache = (torch.cat([angle.cos(), angle.sin()], 1) * self.factor).to(self.dtype)
+            if on_gpu:   # other streams read it too
+                torch.cuda.current_stream(cache.device).synchronize()
+            self._cache = cache
         return self._cache
 
     def _rows(self, name, x, n):

@@ -164,6 +164,19 @@ def test_query_rows_apart_and_a_softmax_scale():
     assert torch.equal(eng.key_weights(q, wide[1:5, 8:33], plan, 0, softmax_scale=0.2), got)
 
 
+def test_one_row_of_a_wide_tensor():
+    g = torch.Generator().manual_seed(31)
+    arena = make(8, 2, 64, 16, g)
+    eng = engine_of(arena, 4)
+    cu_q, used, table = sequences(g, (1,), (90,), 8, 1)
+    tables = attention_plan(*(torch.from_numpy(a).to(DEV) for a in (cu_q, used, table)), heads=(4, 2, 64),
+                            causal=True, eight_bit=False)
+    wide = torch.randn(2, 2 ** 19 + 3, generator=g).to(torch.bfloat16).to(DEV)
+    q = wide[:1, 8:8 + 256].view(1, 4, 64)
+    _, lse = eng.read_pages(q.contiguous(), tables, 0)
+    check(eng.key_weights(q, lse, tables, 0), q, lse, arena, cu_q, used.tolist(), table, True)
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_what_lies_past_the_keys_and_in_masked_ones_stays_out(bits):
     """NaN rows past each sequence's keys, and NaN in a key that only the last

@@ -156,6 +156,17 @@ def test_replays_of_a_captured_call_read_positions_as_they_are():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_the_engines_table_is_not_made_inside_a_graph():
+    rot = RotaryEmbedding(64, max_positions=100)
+    x = torch.zeros(1, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="first use"):
+            rot.cos_sin_cache
+    assert rot.cos_sin_cache.shape == (100, 64)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_the_engines_pass_with_a_scaled_table_rotates_as_the_module(dtype):
     """Norm weights 1: the qk-norm-rope pass is the norm, then the rotation

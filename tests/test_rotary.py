@@ -142,6 +142,14 @@ def test_checkpoints_of_no_scaling_load_the_same_with_scaled_rope(tmp_path):
     assert torch.equal(*(m.model.layers[0].self_attn.rotary_emb.cos_sin_cache for m in (a, b)))
 
 
+def test_positions_not_named_are_the_checkpoints_own(tmp_path):
+    path = _checkpoint(tmp_path, max_position_embeddings=4096, rope_scaling={
+        "type": "yarn", "factor": 4.0, "original_max_position_embeddings": None})
+    rotary = load_qwen3_fp8(path, device="cpu", scaled_rope=True).model.layers[0].self_attn.rotary_emb
+    want, _ = frequencies(64, CONFIGS["tiny"].theta, YARN | {"original_max_position_embeddings": 4096})
+    assert torch.equal(rotary.inv_freq, want) and rotary.max_positions == 16384
+
+
 def test_unknown_scalings_are_refused(tmp_path):
     path = _checkpoint(tmp_path, rope_scaling={"rope_type": "dynamic", "factor": 4.0})
     with pytest.raises(ValueError, match="rope_type"):

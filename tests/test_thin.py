@@ -176,6 +176,16 @@ def test_keys_in_use_are_not_thinned(thinned):
     assert arena.thin([], torch.zeros(2, 0, 2, 96), 16)["used"].numel() == 0
 
 
+def test_rows_are_not_appended_behind_dropped_pages():
+    arena = cpu_arena()
+    arena.activate("a", 64)
+    arena.accounting.drop_leading("a", 1)
+    with pytest.raises(ValueError, match="dropped"):
+        arena.append_rows("a", 1)
+    with pytest.raises(ValueError, match="dropped"):
+        arena.thin(["a"], torch.zeros(2, 1, 2, 64), 16)
+
+
 def test_refused_thinning_changes_no_key():
     arena = cpu_arena()
     arena.activate("a", 64)
