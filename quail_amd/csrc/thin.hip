@@ -289,7 +289,8 @@ __device__ __forceinline__ int source(const ThinArgs& p, const Place& x) {
 
 // A row of D values goes by D * 2 / 16 lanes, 16 bytes each, K and V of kBatch
 // rows a lane in flight, past the caches (each is read and written once; 4%).
-// Bound by HBM, in pieces of a head's row.
+// Bound by HBM, in pieces of a head's row: 8003 rows to 2000 in 36 layers of 8 heads
+// of 128, both launches 110 us, 91 at a copy's rate.
 template <int D>
 __global__ __launch_bounds__(256) void thin_move_kernel(ThinArgs p, int64_t waves, int parts) {
   constexpr int LPR = D / 8, RPP = 64 / LPR, kBatch = 4;
@@ -464,12 +465,18 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   ThinArgs a{(uint8_t*)pools, pool_stride, (uint8_t*)scales, scale_stride, weights, w_layer, w_seq,
              w_head, used, table, table_ld, (int)seqs, (int)HK, (int)max_used, (int)cols,
              (int)(keep < kMaxKeys ? keep : kMaxKeys), (int)slots, (int)sinks, (int)recent, kept, out};
+  // A thread's rows as few as the bound allows (each step is done for all E), in
+  // as few waves as hold them in registers, since barriers among many cost more:
+  // of 2304 heads 1088 rows 26.5 us, by 16 waves 51; 4000 rows 49.5 and 65, 8000
+  // rows 80 and 93 (by 4 waves 49.5 and 82.5). 288 heads leave CUs to spare: 4000
+  // rows 16.8 and 17.1, 8000 rows 24.0 and 23.7 (by 4 waves 18.5 and 29). Of 20,000
+  // rows 24 a thread 46, 40 56.
 #define QX_THIN(NT, E) \
   hipLaunchKernelGGL((thin_select_kernel<NT, E>), dim3((unsigned)rows), dim3(NT), 0, stream, a)
   if (max_used <= 1024) QX_THIN(256, 4);
   else if (max_used <= 2048) QX_THIN(256, 8);
-  else if (max_used <= 4096) QX_THIN(1024, 4);
-  else if (max_used <= 8192) QX_THIN(1024, 8);
+  else if (max_used <= 4096) QX_THIN(512, 8);
+  else if (max_used <= 8192) QX_THIN(512, 16);
   else if (max_used <= 16384) QX_THIN(1024, 16);
   else if (max_used <= 24576) QX_THIN(1024, 24);
   else QX_THIN(1024, 40);
