@@ -13,9 +13,9 @@
 // once, at the end. Sums are fp32, in an order that the call's lengths fix: no
 // atomics.
 //
-// Few rows (one token a sequence): a workgroup for each (sequence, head, key
-// tile) reads its keys once and writes the result itself; the keys' bytes bound
-// it. Many rows: 512 workgroups, two a CU, share the groups of rows of all tiles
+// Few rows (a token or a question a sequence): a workgroup for each (sequence,
+// head, key tile) reads its keys once and writes the result itself; the keys' bytes
+// bound it. Many rows: 512 workgroups, two a CU, share the groups of rows of all tiles
 // evenly, whatever the sequences' lengths; a tile's parts go to scratch memory
 // and a second launch adds them up in the order of the rows. There a step of 64
 // columns with a wave's 64 keys is 32 MFMAs of 32 cycles (8003 rows of 32 heads,
@@ -528,11 +528,18 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
   p.out[s * p.out_s + h * p.out_h + j] = sum;
 }
 
-// Whether the rows go in shares: more than the two steps that a tile's workgroup
-// has no better to do in than read its keys
-bool shared_rows(int64_t max_q, int64_t G) { return max_q * G > 2 * kCols; }
-
 int64_t tiles_of(int64_t keys, int KT) { return (keys + tile_keys(KT) - 1) / tile_keys(KT); }
+
+// Whether the rows go in shares. Up to two steps a tile's workgroup has no more
+// to do than read its keys. Up to 12 and where its tiles are few, the shares' start
+// (bounds, a search, the second launch) costs more than they even out, in us by
+// tiles and shares: 8 contexts of up to 1600 keys (832 tiles), 64 rows of 4 heads a
+// group 14.8 and 22.2, 128 rows 23.6 and 29.8, 200 rows 31.6 and 38.5 (500: 61 and
+// 56); 60 of up to 900 (3840), 64 rows 47.6 and 51.2. Many tiles: 24 contexts of
+// up to 8000 (12096), 64 rows 147 and 132, 128 rows 236 and 201.
+bool shared_rows(int64_t seqs, int64_t max_q, int64_t max_used, int64_t HK, int64_t G) {
+  return max_q * G > 2 * kCols && (max_q * G > 12 * kCols || tiles_of(max_used, 1) * seqs * HK > 4000);
+}
 
 // Scratch memory of a pair of launches over shares: the sequences' bounds, then
 // the parts of (tile, workgroup)
@@ -564,7 +571,7 @@ int64_t qx_key_weights_workspace(int64_t seqs, int64_t max_q, int64_t max_used, 
                                  int64_t HK) {
   QX_CHECK(seqs >= 0 && max_q >= 0 && max_used >= 0 && HQ > 0 && HK > 0 && HQ % HK == 0,
            "key_weights_workspace: sizes");
-  if (!shared_rows(max_q, HQ / HK) || seqs == 0) return 0;
+  if (!shared_rows(seqs, max_q, max_used, HK, HQ / HK)) return 0;
   return part_bytes(batch_of(seqs, max_q, max_used, HQ, HK), max_used, HK);
 }
 
@@ -598,7 +605,7 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
            "key_weights: a workspace of %lld bytes, %lld given", (long long)need,
            (long long)workspace_bytes);
   const int64_t G = HQ / HK;
-  const bool shares = shared_rows(max_q, G);
+  const bool shares = shared_rows(seqs, max_q, max_used, HK, G);
   // few rows: smaller tiles, so that more workgroups read the keys (8 sequences
   // of 700 keys 13.3 us, with the larger ones 22; two contexts of 40,000 41.8 and
   // 41.2)
