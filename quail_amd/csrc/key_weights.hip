@@ -389,6 +389,8 @@ __global__ __launch_bounds__(256, 2) void key_weights_direct_kernel(WeightsArgs 
   const Seq x = seq_of(p, s);
   const int lane = threadIdx.x & 63;
   const int j = k0 + (threadIdx.x >> 6) * 32 * KT + lane_key(lane & (KT == 1 ? 47 : 63));
+  // (read ahead: behind the sums it would be one more way to memory)
+  const float prior = p.base && j < p.cols ? p.base[s * p.base_s + h * p.base_h + j] : 0.f;
   float sum = 0.f;
   const int lo = first_row(p, x, k0);
   if (k0 < x.used && lo < x.n) {
@@ -396,8 +398,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_direct_kernel(WeightsArgs 
     sum = j < x.used ? v : 0.f;
   }
   if (j >= p.cols || (KT == 1 && (lane & 16))) return;
-  if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
-  p.out[s * p.out_s + h * p.out_h + j] = sum;
+  p.out[s * p.out_s + h * p.out_h + j] = p.base ? sum + prior : sum;
 }
 
 // Groups of a head from each sequence on (bound[s], s <= seqs), by one wave
@@ -511,6 +512,7 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
   const Seq x = seq_of(p, s);
   const Work work = work_of(p, x, TILE);
   const int t = j / TILE;
+  const float prior = p.base ? p.base[s * p.base_s + h * p.base_h + j] : 0.f;
   float sum = 0.f;
   if (j < x.used && t < work.tiles) {
     const int of_head = p.bound[p.seqs];
@@ -524,8 +526,7 @@ __global__ __launch_bounds__(256) void key_weights_join_kernel(WeightsArgs p) {
     const float* part = p.part + (((int64_t)h * p.seqs + s) * p.tiles + t) * TILE + j % TILE;
     for (int w = share_at(at); w <= last; ++w) sum += part[(int64_t)w * TILE];
   }
-  if (p.base) sum += p.base[s * p.base_s + h * p.base_h + j];
-  p.out[s * p.out_s + h * p.out_h + j] = sum;
+  p.out[s * p.out_s + h * p.out_h + j] = p.base ? sum + prior : sum;
 }
 
 int64_t tiles_of(int64_t keys, int KT) { return (keys + tile_keys(KT) - 1) / tile_keys(KT); }
