@@ -80,7 +80,7 @@ __device__ __forceinline__ uint64_t bits(int lo, int hi, int base) {
 // E a thread (row e * NT + thread); 0 stands for a row that is protected or not
 // there (no weight ranks so low). The border, the rank of the last row kept, is
 // found 11, 11 and 10 bits at a time from histograms in LDS, of which the second
-// and third count few rows. What stays is then a bit a row, in words of 64 rows
+// and third count few rows, if they are needed at all. What stays is then a bit a row, in words of 64 rows
 // (a wave's ballots), and dropped slots and movers are numbered by words. Bound
 // by instructions (some 60 a row) and, where rows are few, by the barriers
 // between these steps; 8 bytes a row from and to memory.
@@ -127,6 +127,8 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
   };
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
+    // (all of the border's bin stay: its last bits do not matter)
+    if (pass > 0 && (none || want == equal)) continue;
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
     for (int i = tid; i < BINS; i += NT) hist[i] = 0;
     __syncthreads();
