@@ -315,7 +315,7 @@ int qx_copy_pages(void* pools, int64_t n_pools, int64_t pool_stride, int64_t pag
  * 0: bf16, 1: fp16, 2: fp32). The other columns are copied. turns: rotary_dim/2
  * doubles on the device. A row's heads lie D elements apart; the outputs are
  * the rows themselves or overlap none of them. No counterpart in the
- * reference, whose rotary module is vLLM's with its table of cos and sin.
+ * reference, whose rotary module reads a table of cos and sin.
  */
 int qx_rotary(const void* q, int64_t q_ld, const void* k, int64_t k_ld, void* q_out,
               int64_t qo_ld, void* k_out, int64_t ko_ld, const int64_t* positions,

@@ -92,7 +92,7 @@ def test_c_entry_refuses_what_the_kernels_do_not_take():
             ("D", 96, "head_dim"), ("HQ", 5, "heads"), ("HK", 0, "heads"), ("page", 32, "page"),
             ("max_used", 65, "columns"), ("max_used", -1, "rows"), ("rows", -1, "rows"), ("lse_ld", 59, "strides"),
             ("q_ld", 513, "strides"), ("q_ld", 1 << 19, "apart"), ("q", 8, "alignment"), ("k", 24, "alignment"), ("scale", float("nan"), "scale"),
-            ("scale", float("inf"), "scale"), ("q", None, "null"), ("lse", None, "null"), ("table", None, "null"),
+            ("scale", float("inf"), "scale"), ("scale", 3e38, "scale"), ("q", None, "null"), ("lse", None, "null"), ("table", None, "null"),
             ("out", None, "null"), ("cu_q", None, "null"), ("max_q", 1 << 30, "sequence of")]:
         with pytest.raises(_lib.QxError, match=match):
             _lib.call("qx_key_weights", *dict(ok, **{name: value}).values())
