@@ -377,6 +377,27 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
                  int64_t max_used, int64_t cols, int64_t keep, int64_t sinks, int64_t recent,
                  int* kept, float* out, hipStream_t stream);
 
+/*
+ * The same for sequences that are thinned over and over. A kept row that moves
+ * leaves the tokens' order, so that the last `recent` rows of qx_thin_rows are the
+ * newest tokens only where at least as many came since the last thinning. Here
+ * each row's token number goes with it, and the tokens numbered below `sinks` and
+ * the last `newest` of total[s] stay, as far as they are held, wherever their rows
+ * lie. tokens, layers, sequences and heads t_layer, t_seq and t_head apart, with
+ * cols columns: the number of the token that each row holds, negative for a row
+ * appended since, row i of which is token total[s] - used[s] + i (total[s] counts
+ * as at least used[s]). left, (layers, seqs, HK, cols): the slots' numbers, -1 past
+ * k. The rest is as above; whatever the numbers, k rows stay (of more than k
+ * protected ones the first). tokens and left overlap nothing.
+ */
+int qx_thin_rows_by_token(void* pools, int64_t pool_stride, int64_t element_bytes, void* scales,
+                          int64_t scale_stride, const float* weights, int64_t w_layer, int64_t w_seq,
+                          int64_t w_head, const int* tokens, int64_t t_layer, int64_t t_seq,
+                          int64_t t_head, const int* total, const int* used, const int* table,
+                          int64_t table_ld, int64_t layers, int64_t seqs, int64_t HK, int64_t D,
+                          int64_t page, int64_t max_used, int64_t cols, int64_t keep, int64_t sinks,
+                          int64_t newest, int* kept, float* out, int* left, hipStream_t stream);
+
 /* out[i] = table[ids[i]] (bf16 rows). Replaces vLLM embed_tokens (qwen3.py:123). */
 int qx_embed(const void* table, int64_t t_ld, const int64_t* ids, void* out, int64_t o_ld,
              int64_t n, int64_t H, hipStream_t stream);

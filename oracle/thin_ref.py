@@ -24,6 +24,25 @@ def kept_slots(weights, used, keep, sinks, recent):
     return [i if i in stay else next(movers) for i in range(keep)]
 
 
+def kept_slots_by_token(weights, tokens, total, used, keep, sinks, newest):
+    """The same where the tokens numbered below `sinks` and the last `newest` of
+    `total` stay, and each row's number goes with it (negative: appended since
+    the last thinning, numbered on to the end): the slots' rows and their numbers."""
+    number = [total - used + i if tokens[i] < 0 else tokens[i] for i in range(used)]
+    slots = list(range(used))
+    if used > keep:
+        safe = {i for i, t in enumerate(number) if t < sinks or t >= total - newest}
+
+        def first_out_last(i):
+            w = weights[i]
+            return (0, 0.0, i) if i in safe else (1, 0.0, i) if math.isnan(w) else (2, -w, i)
+
+        stay = set(sorted(range(used), key=first_out_last)[:keep])
+        movers = iter(sorted(i for i in stay if i >= keep))
+        slots = [i if i in stay else next(movers) for i in range(keep)]
+    return slots, [number[i] for i in slots]
+
+
 def key_weights(q, lse, keys, first, count, causal, scale, hk):
     """Accumulated weights (hk, keys) of one sequence: rows [first, first +
     count) of q (n, hq, d) and lse (hq, n) over keys (keys, hk, d), float64,

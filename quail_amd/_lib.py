@@ -69,6 +69,8 @@ SIGNATURES = {
     "qx_key_weights": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p] + 9 * [_i64] + [
         _f32, _i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],
     "qx_thin_rows": [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p] + 11 * [_i64] + [_p, _p, _p],
+    "qx_thin_rows_by_token": [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p,
+                              _p] + 11 * [_i64] + [_p, _p, _p, _p],
     "qx_rotary": [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _f32, _i64, _i64, _i64, _i64, _i64,
                   _i32, _i32, _p],
     "qx_embed": [_p, _i64, _p, _p, _i64, _i64, _i64, _p],

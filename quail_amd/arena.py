@@ -18,7 +18,9 @@ bytes a token takes and a reader moves): each pool holds e4m3 codes, and
 KV head), (num_layers, num_pages, num_kv_heads, 2).
 """
 
+import warnings
 from array import array
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
@@ -40,6 +42,20 @@ class _Claim:
         self.holds = 0
         self.reads = 0
         self.free_asked = False
+
+
+@dataclass(frozen=True)
+class _Thinned:
+    """A key whose rows are no longer its first tokens: its id in the accounting
+    (a key of the same name that comes later has another), the rows it held
+    after the last thinning, the tokens dropped until then, and the number of
+    the token that each of those rows holds, int32 (layers, KV heads, rows) or
+    None where they were not kept."""
+
+    ident: int
+    held: int
+    dropped: int
+    numbers: torch.Tensor | None
 
 
 class KVArena:
@@ -93,9 +109,7 @@ class KVArena:
             self._pointers = [(k.data_ptr(), v.data_ptr(), s.data_ptr())
                               for k, v, s in zip(self.k, self.v, self._layer_scales)]
         self._claims = {}
-        # keys whose rows are no longer their first tokens, and their ids in the
-        # accounting (a key of the same name that comes later has another)
-        self._thinned = {}
+        self._thinned = {}      # key -> _Thinned
 
     # ---- sizes -------------------------------------------------------------
 
@@ -316,7 +330,8 @@ class KVArena:
         if rest and children:
             self.copy_pages([table[full]] * len(children), [own[0] for own in pages])
         if self.is_thinned(key):
-            self._thinned.update((child, acct.key_id(child)) for child in children)
+            self._thinned.update((child, replace(self._thinned[key], ident=acct.key_id(child)))
+                                 for child in children)
         return pages
 
     def compact(self) -> int:
@@ -362,7 +377,7 @@ class KVArena:
 
     # ---- thinning ------------------------------------------------------------------
 
-    def thin_rows(self, tables, weights, keep, *, sinks=0, recent=0):
+    def thin_rows(self, tables, weights, keep, *, sinks=0, recent=0, newest=None, tokens=None):
         """Keep the heaviest rows of sequences that a caller lays out: of every
         (layer, sequence, KV head) the first `sinks` rows, the last `recent`
         and the heaviest of the others by `weights`, min(used, keep) in all
@@ -371,6 +386,18 @@ class KVArena:
         row past them (current stream), and rows from `keep` on stay as they
         were: the caller reads min(used, keep) rows afterwards. Keys keep the
         rotation they were written with.
+
+        `sinks` and `recent` count places. A kept row that moves leaves the
+        tokens' order, so of a sequence that was thinned before the last
+        `recent` rows are its newest tokens only if it grew by as many since.
+        Sequences that are thinned over and over take `newest` and `tokens`
+        instead of `recent`: then the tokens numbered below `sinks` and the
+        last `newest` ones stay, as far as they are held, wherever their rows
+        lie. tokens: int32 in the shape of `weights`, the number of the token
+        that each row holds (from 0, no two rows of a head alike), negative for
+        rows appended since the last call, which hold the last tokens in order
+        (at first every row is one); tables["tokens"], int32, one per sequence:
+        the tokens it has had so far, dropped ones among them.
 
         tables: used (int32, one per sequence), table (int32 rows of pages) and
         max_used, a bound of used, as a plan or read_pages' tables have them;
@@ -381,7 +408,8 @@ class KVArena:
         Returns (kept, weights): int32 (layers, sequences, KV heads, min(keep,
         columns)), the row that each slot holds as it was numbered before, -1
         past min(used, keep); and the slots' weights in the shape of `weights`,
-        0 past them."""
+        0 past them. With `tokens` also the slots' numbers in that shape, -1
+        past them: the next call's `tokens`."""
         from quail_amd.engine import _launch
         used, table = tables["used"], tables["table"]
         heads, dim = self.kv_shape
@@ -404,40 +432,67 @@ class KVArena:
         if tables.get("pages", 0) > self.num_pages:
             raise ValueError(f"page {tables['pages'] - 1} in the plan's table, {self.num_pages} in the "
                              "arena")
-        if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
-            raise ValueError(f"{sinks} first and {recent} last rows of {keep} that stay")
+        by_token = newest is not None
+        if by_token != (tokens is not None) or (by_token and recent):
+            raise ValueError("newest goes with the rows' tokens, and not with recent")
+        last = newest if by_token else recent
+        if keep < 0 or sinks < 0 or last < 0 or sinks + last > keep:
+            raise ValueError(f"{sinks} first and {last} last rows of {keep} that stay")
+        if by_token:
+            if tokens.dtype != torch.int32 or tokens.shape != weights.shape or (cols > 1 and tokens.stride(3) != 1):
+                raise ValueError(f"tokens: int32 {tuple(weights.shape)}, columns contiguous, not "
+                                 f"{tuple(tokens.shape)} {tokens.dtype}")
+            total = tables.get("tokens")
+            if total is None or total.dtype != torch.int32 or total.shape != (seqs,) or \
+                    (seqs > 1 and total.stride(0) != 1):
+                raise ValueError(f"the tables' tokens: int32, one for each of {seqs} sequences")
         if self.eight_bit and keep % self.page_tokens:
             raise ValueError(f"8-bit pages are kept whole: {keep} rows are not a multiple of "
                              f"{self.page_tokens}")
         device = self.storage.get_device()
         if device < 0:
             raise ValueError("rows are thinned on the GPU; this arena is on the CPU")
-        if not used.get_device() == table.get_device() == weights.get_device() == device:
+        if not used.get_device() == table.get_device() == weights.get_device() == device or \
+                by_token and not tokens.get_device() == total.get_device() == device:
             raise ValueError(f"tables and weights on the arena's GPU {device}")
         shape = (self.num_layers, seqs, heads)
         kept = torch.empty(*shape, min(keep, cols), dtype=torch.int32, device=weights.device)
         out = torch.empty_like(weights, memory_format=torch.contiguous_format)
         scales = (None, 0) if self.scales is None else (self.scales.data_ptr(), self.scales.stride(0))
         pool = self.num_pages * self.page_tokens * heads * dim * self.storage.element_size()
-        args = (self.storage.data_ptr(), pool, self.storage.element_size(), *scales,
-                weights.data_ptr(), *weights.stride()[:3], used.data_ptr(), table.data_ptr(),
-                table.stride(0), *shape, dim, self.page_tokens, max_used, cols, keep, sinks, recent,
-                kept.data_ptr(), out.data_ptr())
+        pages = (self.storage.data_ptr(), pool, self.storage.element_size(), *scales,
+                 weights.data_ptr(), *weights.stride()[:3])
+        rows = (used.data_ptr(), table.data_ptr(), table.stride(0), *shape, dim, self.page_tokens,
+                max_used, cols, keep, sinks, last, kept.data_ptr(), out.data_ptr())
         try:
-            _launch(device, "qx_thin_rows", *args)
+            if by_token:
+                left = torch.empty_like(out, dtype=torch.int32)
+                _launch(device, "qx_thin_rows_by_token", *pages, tokens.data_ptr(), *tokens.stride()[:3],
+                        total.data_ptr(), *rows, left.data_ptr())
+                return kept, out, left
+            _launch(device, "qx_thin_rows", *pages, *rows)
         except _lib.QxError as err:
             if "hipError" in str(err):
                 raise
             raise ValueError(str(err)) from err
         return kept, out
 
-    def thin(self, keys, weights, keep, *, sinks=0, recent=0):
+    def thin(self, keys, weights, keep, *, sinks=0, recent=0, newest=None):
         """thin_rows of resident keys, whose pages past `keep` rows go free.
         `weights` has a row per key, in the keys' order. A thinned key's rows
         are no longer its first tokens: it is read and continued by a caller
         (read_pages, append_rows, fork of all it holds), not lent, packed or
         activated again. ValueError where a key lends or borrows pages, is held
-        or is being read, or is named twice."""
+        or is being read, or is named twice.
+
+        A key that is thinned again as it grows takes `newest`, from the first
+        time on: its first `sinks` and last `newest` tokens stay wherever their
+        rows lie (the arena keeps the tokens' numbers). `recent` protects the
+        last places, whose rows are its newest tokens only where it grew by as
+        many since it was thinned: RuntimeWarning where it did not. ValueError
+        for `newest` of a key that was thinned without.
+
+        Returns (kept, weights) as thin_rows does."""
         acct = self.accounting
         keys = list(keys)
         if len(set(keys)) != len(keys):
@@ -452,22 +507,45 @@ class KVArena:
         for other in acct.resident_keys():
             if not pages.isdisjoint(acct.borrowed_pages(other)):
                 raise ValueError(f"{other!r} borrows pages of the keys")
-        if not keys:
-            return self.thin_rows(dict(used=torch.zeros(0, dtype=torch.int32, device=weights.device),
-                                       table=torch.zeros(0, 0, dtype=torch.int32,
-                                                         device=weights.device), max_used=0),
-                                  weights, keep, sinks=sinks, recent=recent)
-        table, used = self.block_table(keys)
+        found = [self._thinned[key] if self.is_thinned(key) else None for key in keys]
+        if newest is not None and any(f is not None and f.numbers is None for f in found):
+            raise ValueError("a key was thinned without newest: the tokens that its rows hold are not known")
+        if keys:
+            table, used = self.block_table(keys)
+        else:
+            table, used = np.zeros((0, 0), dtype=np.int32), np.zeros(0, dtype=np.int32)
         if any(len(acct.table_pages(key)) < acct.pages_needed(n) for key, n in zip(keys, used.tolist())):
             raise ValueError("a key's leading pages were dropped")
-        tables = dict(used=torch.from_numpy(used).to(self.storage.device),
-                      table=torch.from_numpy(table).to(self.storage.device), max_used=int(used.max()))
-        found = self.thin_rows(tables, weights, keep, sinks=sinks, recent=recent)
-        for key, n in zip(keys, used.tolist()):
+        device = self.storage.device if keys else weights.device
+        tables = dict(used=torch.from_numpy(used).to(device), table=torch.from_numpy(table).to(device),
+                      max_used=max([0, *used.tolist()]))
+        by_token = {}
+        if newest is None:
+            for key, n, f in zip(keys, used.tolist(), found):
+                if f is not None and keep < n < f.held + recent:
+                    warnings.warn(f"{key!r} grew by {n - f.held} rows since it was thinned: its last {recent} "
+                                  "places are not its newest tokens (newest protects those)",
+                                  RuntimeWarning, stacklevel=2)
+        else:
+            total = [n + (0 if f is None else f.dropped) for n, f in zip(used.tolist(), found)]
+            tables["tokens"] = torch.tensor(total, dtype=torch.int32).to(device)
+            cols = max([*weights.shape[-1:], tables["max_used"]])
+            tokens = torch.full((self.num_layers, len(keys), self.kv_shape[0], cols), -1, dtype=torch.int32,
+                                device=device)
+            for s, f in enumerate(found):
+                if f is not None:
+                    tokens[:, s, :, :f.held] = f.numbers
+                    if f.numbers.is_cuda:      # made on the stream of the thinning before
+                        f.numbers.record_stream(torch.cuda.current_stream(f.numbers.device))
+            by_token = dict(newest=newest, tokens=tokens)
+        result = self.thin_rows(tables, weights, keep, sinks=sinks, recent=recent, **by_token)
+        for s, (key, n, f) in enumerate(zip(keys, used.tolist(), found)):
             if n > keep:
                 acct.rewind(key, keep)
-                self._thinned[key] = acct.key_id(key)
-        return found
+                numbers = None if newest is None else result[2][:, s, :, :keep].clone()
+                self._thinned[key] = _Thinned(acct.key_id(key), keep, n - keep + (0 if f is None else f.dropped),
+                                              numbers)
+        return result if newest is None else result[:2]
 
     def append_rows(self, key, count: int):
         """Room for `count` more rows of a resident key: their pool rows (host
@@ -485,8 +563,8 @@ class KVArena:
 
     def is_thinned(self, key) -> bool:
         """Whether a resident key's rows are no longer its first tokens."""
-        ident = self._thinned.get(key)
-        return ident is not None and self.is_resident(key) and self.accounting.key_id(key) == ident
+        found = self._thinned.get(key)
+        return found is not None and self.is_resident(key) and self.accounting.key_id(key) == found.ident
 
     def check_whole(self, key) -> None:
         """ValueError for a thinned key."""

@@ -3,7 +3,11 @@
 //
 // With u = used rows and k = min(u, keep), the first `sinks` rows, the last
 // `recent` and the heaviest of the others stay, k in all (ties: the lowest row;
-// a NaN is heavier than every number). Kept rows below k stay where they are;
+// a NaN is heavier than every number). A row that moves leaves the order of the
+// tokens, so the last rows of a sequence that was thinned before are its newest
+// tokens only if it grew by as many since: by token, each row's number goes with
+// it, and the tokens below `sinks` and the newest stay instead, wherever their
+// rows lie. Kept rows below k stay where they are;
 // the j-th dropped slot below k takes the j-th kept row at or past k. So every
 // row that is read for a move lies at or past k and every one that is written
 // below it: the moves need no order among them, and only what has to move
@@ -30,6 +34,13 @@ struct ThinArgs {
   int seqs, HK, bound, cols, keep, slots, sinks, recent;
   int* kept;   // (layers, seqs, HK, slots)
   float* out;  // (layers, seqs, HK, cols)
+  // by token: each row's number (negative: appended since the last thinning), the
+  // tokens so far of a sequence, and the numbers left, (layers, seqs, HK, cols);
+  // `recent` counts the newest tokens then
+  const int* tokens;
+  int64_t t_layer, t_seq, t_head;
+  const int* total;
+  int* left;
 };
 
 // A float's rank as an unsigned number; -0 ranks as 0, NaN above all
@@ -78,13 +89,15 @@ __device__ __forceinline__ uint64_t bits(int lo, int hi, int base) {
 
 // One (layer, sequence, head) per workgroup, its weights' ranks in registers,
 // E a thread (row e * NT + thread); 0 stands for a row that is protected or not
-// there (no weight ranks so low). The border, the rank of the last row kept, is
+// there (no weight ranks so low). BY_TOKEN protects rows anywhere: they rank above
+// all others instead (a NaN just below them) and count among the k, so that k rows
+// stay whatever numbers a caller gives. The border, the rank of the last row kept, is
 // found 11, 11 and 10 bits at a time from histograms in LDS, of which the second
 // and third count few rows, if they are needed at all. What stays is then a bit a row, in words of 64 rows
 // (a wave's ballots), and dropped slots and movers are numbered by words. Bound
 // by instructions (some 60 a row) and, where rows are few, by the barriers
-// between these steps; 8 bytes a row from and to memory.
-template <int NT, int E>
+// between these steps; 8 bytes a row from and to memory, 16 by token.
+template <int NT, int E, bool BY_TOKEN>
 __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(ThinArgs p) {
   constexpr int W = NT / 64, WORDS = E * W, BINS = 2048, PER = BINS / NT;
   __shared__ int hist[BINS];
@@ -103,13 +116,29 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
   int* kept = p.kept + row * p.slots;
   float* out = p.out + row * p.cols;
   const int used = min(max(p.used[s], 0), p.bound);
+  const int* tokens = nullptr;
+  int* left = nullptr;
+  int newer = 0;                // the number of row i is i + newer where none is given
+  int first_token = 0, fresh = 0;  // tokens [first_token, fresh) may leave
+  if constexpr (BY_TOKEN) {
+    tokens = p.tokens + ls / p.seqs * p.t_layer + s * p.t_seq + h * p.t_head;
+    left = p.left + row * p.cols;
+    const int total = max(p.total[s], used);
+    newer = total - used;
+    first_token = p.sinks;
+    fresh = total - p.recent;
+  }
+  auto number_at = [&](int i, int given) { return given < 0 ? i + newer : given; };
   if (used <= p.keep) {
     for (int i = tid; i < p.cols; i += NT) out[i] = i < used ? w[i] : 0.f;
     for (int i = tid; i < p.slots; i += NT) kept[i] = i < used ? i : -1;
+    if constexpr (BY_TOKEN)
+      for (int i = tid; i < p.cols; i += NT) left[i] = i < used ? number_at(i, tokens[i]) : -1;
     return;
   }
-  const int k = p.keep, late = used - p.recent;
-  int want = k - p.sinks - p.recent;  // of the rows [sinks, late), which are more
+  const int k = p.keep;
+  const int early = BY_TOKEN ? 0 : p.sinks, late = BY_TOKEN ? used : used - p.recent;
+  int want = BY_TOKEN ? k : k - p.sinks - p.recent;  // of the rows [early, late), which are more
   const bool none = want == 0;
   uint32_t rank[E];
   uint32_t border = 0;
@@ -137,17 +166,26 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
 #pragma unroll
       for (int e0 = 0; e0 < E; e0 += AT_ONCE) {
         const int t = opaque(tid);
+        int given[BY_TOKEN ? AT_ONCE : 1];
 #pragma unroll
-        for (int e = e0; e < e0 + AT_ONCE; ++e) rank[e] = __float_as_uint(w[min(e * NT + t, used - 1)]);
+        for (int e = e0; e < e0 + AT_ONCE; ++e) {
+          rank[e] = __float_as_uint(w[min(e * NT + t, used - 1)]);
+          if constexpr (BY_TOKEN) given[e - e0] = tokens[min(e * NT + t, used - 1)];
+        }
 #pragma unroll
         for (int e = e0; e < e0 + AT_ONCE; ++e) {
           const int first = e * NT + wave * 64;
           rank[e] = rank_of(__uint_as_float(rank[e]));
-          if (first >= p.sinks && first + 64 <= late) {
+          if constexpr (BY_TOKEN) {
+            const int token = number_at(e * NT + t, given[e - e0]);
+            const bool stays = token < first_token || token >= fresh;
+            rank[e] = stays ? 0xffffffffu : min(rank[e], 0xfffffffeu);
+          }
+          if (first >= early && first + 64 <= late) {
             count(rank[e] >> 21);
           } else {
             const int i = e * NT + t;
-            if (i >= p.sinks && i < late) count(rank[e] >> 21); else rank[e] = 0;
+            if (i >= early && i < late) count(rank[e] >> 21); else rank[e] = 0;
           }
         }
       }
@@ -212,7 +250,8 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
       m |= __ballot((same >> lane & 1) && before[c] + lanes_before(same) < want);
     }
     if (none) m = 0;
-    if (64 * c < p.sinks || 64 * c + 64 > late) m |= bits(0, p.sinks, 64 * c) | bits(late, used, 64 * c);
+    if constexpr (!BY_TOKEN)
+      if (64 * c < early || 64 * c + 64 > late) m |= bits(0, early, 64 * c) | bits(late, used, 64 * c);
     if (lane == 0) stays[c] = m;
   }
   __syncthreads();
@@ -243,7 +282,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
   }
   __syncthreads();
   for (int c0 = 0; c0 * 64 < k; c0 += AT_ONCE * W) {
-    int src[AT_ONCE];
+    int src[AT_ONCE], given[BY_TOKEN ? AT_ONCE : 1];
     float f[AT_ONCE];
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
@@ -251,17 +290,24 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(Thi
       src[j] = n < 0 ? c * 64 + lane : n < holes ? movers[n] : 0;  // (0: past k)
     }
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) f[j] = w[min(src[j], used - 1)];
+    for (int j = 0; j < AT_ONCE; ++j) {
+      f[j] = w[min(src[j], used - 1)];
+      if constexpr (BY_TOKEN) given[j] = tokens[min(src[j], used - 1)];
+    }
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
       const int i = (c0 + j * W + wave) * 64 + lane;
       if (i < k) {
         kept[i] = src[j];
         out[i] = f[j];
+        if constexpr (BY_TOKEN) left[i] = number_at(src[j], given[j]);
       }
     }
   }
-  for (int i = k + tid; i < p.cols; i += NT) out[i] = 0.f;
+  for (int i = k + tid; i < p.cols; i += NT) {
+    out[i] = 0.f;
+    if constexpr (BY_TOKEN) left[i] = -1;
+  }
 }
 
 // The moves of a wave: 64 slots of a (layer, sequence, head), one a lane. Those
@@ -425,19 +471,19 @@ __global__ __launch_bounds__(256) void thin_move8_kernel(ThinArgs p, int64_t wav
   }
 }
 
-}  // namespace
-}  // namespace qx
+struct ByToken {
+  const int* tokens;
+  int64_t layer, seq, head;
+  const int* total;
+  int* left;
+};
 
-using namespace qx;
-
-extern "C" {
-
-int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* scales,
-                 int64_t scale_stride, const float* weights, int64_t w_layer, int64_t w_seq,
-                 int64_t w_head, const int* used, const int* table, int64_t table_ld,
-                 int64_t layers, int64_t seqs, int64_t HK, int64_t D, int64_t page,
-                 int64_t max_used, int64_t cols, int64_t keep, int64_t sinks, int64_t recent,
-                 int* kept, float* out, hipStream_t stream) {
+int thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* scales,
+              int64_t scale_stride, const float* weights, int64_t w_layer, int64_t w_seq,
+              int64_t w_head, const ByToken* by, const int* used, const int* table, int64_t table_ld,
+              int64_t layers, int64_t seqs, int64_t HK, int64_t D, int64_t page, int64_t max_used,
+              int64_t cols, int64_t keep, int64_t sinks, int64_t recent, int* kept, float* out,
+              hipStream_t stream) {
   QX_CHECK(D == 64 || D == 128, "thin_rows: head_dim %lld (64 or 128)", (long long)D);
   QX_CHECK(page == kPage, "thin_rows: page of %lld tokens (16)", (long long)page);
   QX_CHECK(element_bytes == 2 || (element_bytes == 1 && scales),
@@ -459,6 +505,7 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   const int64_t slots = keep < cols ? keep : cols;
   QX_CHECK(pools && weights && used && out && (kept || slots == 0) && (table || max_used == 0),
            "thin_rows: null pointer");
+  QX_CHECK(!by || (by->tokens && by->total && by->left), "thin_rows: null pointer");
   QX_CHECK(rows < (1LL << 21), "thin_rows: %lld heads exceed one launch", (long long)rows);
   const int parts = (int)((slots + 63) / 64);
   const int64_t waves = rows * parts;
@@ -466,23 +513,41 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
            (long long)slots, (long long)rows);
   ThinArgs a{(uint8_t*)pools, pool_stride, (uint8_t*)scales, scale_stride, weights, w_layer, w_seq,
              w_head, used, table, table_ld, (int)seqs, (int)HK, (int)max_used, (int)cols,
-             (int)(keep < kMaxKeys ? keep : kMaxKeys), (int)slots, (int)sinks, (int)recent, kept, out};
+             (int)(keep < kMaxKeys ? keep : kMaxKeys), (int)slots, (int)sinks, (int)recent, kept, out,
+             nullptr, 0, 0, 0, nullptr, nullptr};
+  if (by) {
+    a.tokens = by->tokens;
+    a.t_layer = by->layer, a.t_seq = by->seq, a.t_head = by->head;
+    a.total = by->total;
+    a.left = by->left;
+  }
   // A thread's rows as few as the bound allows (each step is done for all E), in
   // as few waves as hold them in registers, since barriers among many cost more:
   // of 2304 heads 1088 rows 26.5 us, by 16 waves 51; 4000 rows 49.5 and 65, 8000
   // rows 80 and 93 (by 4 waves 49.5 and 82.5). 288 heads leave CUs to spare: 4000
   // rows 16.8 and 17.1, 8000 rows 24.0 and 23.7 (by 4 waves 18.5 and 29). Of 20,000
   // rows 24 a thread 46, 40 56.
+#define QX_SELECT(NT, E, B) \
+  hipLaunchKernelGGL((thin_select_kernel<NT, E, B>), dim3((unsigned)rows), dim3(NT), 0, stream, a)
 #define QX_THIN(NT, E) \
-  hipLaunchKernelGGL((thin_select_kernel<NT, E>), dim3((unsigned)rows), dim3(NT), 0, stream, a)
-  if (max_used <= 1024) QX_THIN(256, 4);
-  else if (max_used <= 2048) QX_THIN(256, 8);
-  else if (max_used <= 4096) QX_THIN(512, 8);
-  else if (max_used <= 8192) QX_THIN(512, 16);
-  else if (max_used <= 16384) QX_THIN(1024, 16);
-  else if (max_used <= 24576) QX_THIN(1024, 24);
-  else QX_THIN(1024, 40);
+  if (by) QX_SELECT(NT, E, true); else QX_SELECT(NT, E, false)
+  if (max_used <= 1024) {
+    QX_THIN(256, 4);
+  } else if (max_used <= 2048) {
+    QX_THIN(256, 8);
+  } else if (max_used <= 4096) {
+    QX_THIN(512, 8);
+  } else if (max_used <= 8192) {
+    QX_THIN(512, 16);
+  } else if (max_used <= 16384) {
+    QX_THIN(1024, 16);
+  } else if (max_used <= 24576) {
+    QX_THIN(1024, 24);
+  } else {
+    QX_THIN(1024, 40);
+  }
 #undef QX_THIN
+#undef QX_SELECT
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (max_used <= keep) return QX_OK;  // no row moves
@@ -497,6 +562,37 @@ int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* 
   }
 #undef QX_MOVE
   QX_LAUNCH_STATUS();
+}
+
+}  // namespace
+}  // namespace qx
+
+using namespace qx;
+
+extern "C" {
+
+int qx_thin_rows(void* pools, int64_t pool_stride, int64_t element_bytes, void* scales,
+                 int64_t scale_stride, const float* weights, int64_t w_layer, int64_t w_seq,
+                 int64_t w_head, const int* used, const int* table, int64_t table_ld,
+                 int64_t layers, int64_t seqs, int64_t HK, int64_t D, int64_t page,
+                 int64_t max_used, int64_t cols, int64_t keep, int64_t sinks, int64_t recent,
+                 int* kept, float* out, hipStream_t stream) {
+  return thin_rows(pools, pool_stride, element_bytes, scales, scale_stride, weights, w_layer, w_seq,
+                   w_head, nullptr, used, table, table_ld, layers, seqs, HK, D, page, max_used, cols,
+                   keep, sinks, recent, kept, out, stream);
+}
+
+int qx_thin_rows_by_token(void* pools, int64_t pool_stride, int64_t element_bytes, void* scales,
+                          int64_t scale_stride, const float* weights, int64_t w_layer, int64_t w_seq,
+                          int64_t w_head, const int* tokens, int64_t t_layer, int64_t t_seq,
+                          int64_t t_head, const int* total, const int* used, const int* table,
+                          int64_t table_ld, int64_t layers, int64_t seqs, int64_t HK, int64_t D,
+                          int64_t page, int64_t max_used, int64_t cols, int64_t keep, int64_t sinks,
+                          int64_t newest, int* kept, float* out, int* left, hipStream_t stream) {
+  const ByToken by{tokens, t_layer, t_seq, t_head, total, left};
+  return thin_rows(pools, pool_stride, element_bytes, scales, scale_stride, weights, w_layer, w_seq,
+                   w_head, &by, used, table, table_ld, layers, seqs, HK, D, page, max_used, cols,
+                   keep, sinks, newest, kept, out, stream);
 }
 
 }  // extern "C"
