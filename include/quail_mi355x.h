@@ -668,6 +668,8 @@ int qx_prefix_tree(const int64_t* tokens, const int64_t* offsets, int64_t n,
  * qx_pages_keys: the resident keys in allocation order.
  * qx_pages_free_key / drop_leading / rewind / grow (pages.py:100-154):
  *   *out = pages freed (grow: pages added, or -1 when short).
+ * qx_pages_holders: the most keys that hold any one of pages [first, last) of
+ *   the key's table (not in the reference).
  * qx_pages_pin / retain / pop_victim (pages.py:168-250): retained keys are
  *   evicted lowest priority first, ties in retention order; the default
  *   priority is tokens per page the key alone holds. victim = {found, key,
@@ -691,6 +693,7 @@ int qx_pages_free_key(void* pool, int64_t key, int64_t* freed);
 int qx_pages_drop_leading(void* pool, int64_t key, int64_t pages, int64_t* freed);
 int qx_pages_rewind(void* pool, int64_t key, int64_t tokens, int64_t* freed);
 int qx_pages_grow(void* pool, int64_t key, int64_t capacity_tokens, int64_t* added);
+int qx_pages_holders(void* pool, int64_t key, int64_t first, int64_t last, int64_t* most);
 int qx_pages_set_tokens(void* pool, int64_t key, int64_t tokens);
 int qx_pages_pin(void* pool, int64_t key);
 int qx_pages_retain(void* pool, int64_t key, int has_priority, double priority);

@@ -103,6 +103,7 @@ SIGNATURES = {
     "qx_pages_drop_leading": [_p, _i64, _i64, _p],
     "qx_pages_rewind": [_p, _i64, _i64, _p],
     "qx_pages_grow": [_p, _i64, _i64, _p],
+    "qx_pages_holders": [_p, _i64, _i64, _i64, _p],
     "qx_pages_set_tokens": [_p, _i64, _i64],
     "qx_pages_pin": [_p, _i64],
     "qx_pages_retain": [_p, _i64, _i32, ctypes.c_double],

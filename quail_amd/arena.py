@@ -549,13 +549,18 @@ class KVArena:
 
     def append_rows(self, key, count: int):
         """Room for `count` more rows of a resident key: their pool rows (host
-        int64), or None with nothing changed when the free list is short."""
+        int64), or None with nothing changed when the free list is short.
+        ValueError where one of them lies in a page that another key reads (a
+        key that was rewound into a page it had lent, or holds fewer tokens
+        than it borrows): a fork of it has that page of its own."""
         acct = self.accounting
         tokens = acct.key_tokens(key)
         if count < 0:
             raise ValueError(f"{count} more rows")
         if len(acct.table_pages(key)) < acct.pages_needed(tokens):
             raise ValueError(f"{key!r}: leading pages were dropped")
+        if count and acct.holders(key, tokens // self.page_tokens, acct.pages_needed(tokens + count)) > 1:
+            raise ValueError(f"{key!r}: another key reads the page of row {tokens} or one after it")
         if acct.grow(key, tokens + count) is None:
             return None
         acct.set_tokens(key, tokens + count)

@@ -361,6 +361,20 @@ int qx_pages_grow(void* pool, int64_t key, int64_t capacity_tokens, int64_t* add
   return QX_OK;
 }
 
+// most = the most keys that hold any one of the key's pages [first, last) of
+// its table (0 of none)
+int qx_pages_holders(void* pool, int64_t key, int64_t first, int64_t last, int64_t* most) {
+  PagePool* p = pool_of(pool);
+  QX_CHECK(p && most, "pages_holders: null pointer");
+  Key* k = p->find(key);
+  if (!k) QX_FAIL(QX_ENOKEY, "key %lld is not resident", (long long)key);
+  const int64_t nb = (int64_t)k->borrowed.size(), no = (int64_t)k->owned.size();
+  *most = 0;
+  for (int64_t i = std::max<int64_t>(first, 0); i < std::min(last, nb + no); ++i)
+    *most = std::max<int64_t>(*most, p->holds[i < nb ? k->borrowed[i] : k->owned[i - nb]]);
+  return QX_OK;
+}
+
 int qx_pages_set_tokens(void* pool, int64_t key, int64_t tokens) {
   PagePool* p = pool_of(pool);
   QX_CHECK(p, "pages_set_tokens: null pointer");

@@ -244,6 +244,13 @@ class PageArena:
                     ctypes.byref(self._out))
         return None if self._out.value < 0 else self._out.value
 
+    def holders(self, key, first: int, last: int) -> int:
+        """The most keys that hold any one of pages [first, last) of the key's
+        table (0 of none)."""
+        _pages_call("qx_pages_holders", self.handle, self.key_id(key), first, last,
+                    ctypes.byref(self._out))
+        return self._out.value
+
     def row_indices(self, key, tokens=None):
         """Flat pool rows of the key's tokens: page p holds rows p*T .. p*T+T-1."""
         left = self.key_tokens(key) if tokens is None else tokens
