@@ -483,7 +483,8 @@ class KVArena:
         are no longer its first tokens: it is read and continued by a caller
         (read_pages, append_rows, fork of all it holds), not lent, packed or
         activated again. ValueError where a key lends or borrows pages, is held
-        or is being read, or is named twice.
+        or is being read, is retained (pin it first: an eviction may take it, and
+        fewer tokens would be retained with another priority) or is named twice.
 
         A key that is thinned again as it grows takes `newest`, from the first
         time on: its first `sinks` and last `newest` tokens stay wherever their
@@ -501,6 +502,8 @@ class KVArena:
         for key in keys:
             if key in self._claims:
                 raise ValueError(f"{key!r} is held for borrowers or being read")
+            if acct.is_retained(key):
+                raise ValueError(f"{key!r} is retained, so that an eviction may take it: pin it first")
             if acct.borrowed_pages(key):
                 raise ValueError(f"{key!r} borrows pages")
             pages.update(acct.owned_pages(key))
@@ -552,13 +555,17 @@ class KVArena:
         int64), or None with nothing changed when the free list is short.
         ValueError where one of them lies in a page that another key reads (a
         key that was rewound into a page it had lent, or holds fewer tokens
-        than it borrows): a fork of it has that page of its own."""
+        than it borrows): a fork of it has that page of its own. ValueError for
+        a retained key, which an eviction may take with the rows just handed
+        out: pin it first."""
         acct = self.accounting
         tokens = acct.key_tokens(key)
         if count < 0:
             raise ValueError(f"{count} more rows")
         if len(acct.table_pages(key)) < acct.pages_needed(tokens):
             raise ValueError(f"{key!r}: leading pages were dropped")
+        if acct.is_retained(key):
+            raise ValueError(f"{key!r} is retained, so that an eviction may take it: pin it first")
         if count and acct.holders(key, tokens // self.page_tokens, acct.pages_needed(tokens + count)) > 1:
             raise ValueError(f"{key!r}: another key reads the page of row {tokens} or one after it")
         if acct.grow(key, tokens + count) is None:

@@ -155,6 +155,9 @@ class PageArena:
     def key_tokens(self, key) -> int:
         return self._table(key)[0]
 
+    def is_retained(self, key) -> bool:
+        return self._table(key)[4]
+
     def set_tokens(self, key, tokens: int) -> None:
         _pages_call("qx_pages_set_tokens", self.handle, self.key_id(key), tokens)
 

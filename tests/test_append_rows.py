@@ -1,6 +1,7 @@
 """Rows appended to resident keys: the page accounting, on the CPU."""
 
 import pytest
+import torch
 
 from quail_amd.arena import KVArena
 
@@ -74,3 +75,39 @@ def test_holders_of_pages():
     assert acct.holders("b", 0, 2) == 3 and acct.holders("b", 2, 4) == 1
     with pytest.raises(KeyError):
         acct.holders("nobody", 0, 1)
+
+
+def test_retained_keys_are_pinned_before_they_are_continued():
+    """Their pages counted as retained, and the victims' sizes, stay true."""
+    arena = cpu_arena(8)
+    arena.activate("a", 64)
+    arena.retain("a", priority=7.0)
+    before = state(arena)
+    with pytest.raises(ValueError, match="pin it first"):
+        arena.append_rows("a", 10)
+    with pytest.raises(ValueError, match="pin it first"):
+        arena.thin(["a"], torch.zeros(2, 1, 2, 64), 16)
+    assert state(arena) == before and arena.retained_pages == 4 and not arena.is_thinned("a")
+    arena.pin("a")
+    assert len(arena.append_rows("a", 50)) == 50 and arena.retained_pages == 0
+    assert arena.activate("b", 64) is None and arena.is_resident("a")     # nothing to evict
+    arena.retain("a")
+    assert arena.retained_pages == 8
+    assert arena.activate("b", 64) is not None and not arena.is_resident("a")
+    assert (arena.evicted_pages, arena.evicted_prefix_tokens) == (8, 114)
+
+
+def test_the_priority_of_a_key_that_was_thinned_is_the_one_it_is_retained_with(monkeypatch):
+    monkeypatch.setattr(KVArena, "thin_rows", lambda self, tables, weights, keep, **kw: tables)
+    arena = cpu_arena(8)
+    for key in "ab":
+        arena.activate(key, 64)
+    arena.retain("a", priority=9.0)
+    arena.retain("b", priority=5.0)
+    arena.pin("a")
+    arena.thin(["a"], torch.zeros(2, 1, 2, 64), 32)
+    arena.append_rows("a", 16)
+    arena.retain("a", priority=9.0)
+    assert arena.retained_pages == 7
+    assert arena.activate("c", 48) is not None
+    assert arena.is_resident("a") and not arena.is_resident("b")
