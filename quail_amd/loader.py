@@ -23,16 +23,17 @@ from types import SimpleNamespace
 import torch
 
 from quail_amd.model import (BLOCK, Embedding, Qwen3Config, _linear, _norm, rope_cache)
-from quail_amd.rotary import RotaryEmbedding
+from quail_amd.rotary import RotaryEmbedding, scaling_type
 
 INDEX = "model.safetensors.index.json"
 
 
 def _scaled_rope(config: dict) -> dict | None:
-    """The rope scaling a config.json asks for, or None."""
+    """The rope scaling a config.json asks for, or None. ValueError for one
+    that names no type."""
     for name in ("rope_scaling", "rope_parameters"):
         rope = config.get(name) or {}
-        if rope.get("rope_type", rope.get("type", "default")) != "default":
+        if scaling_type(rope) != "default":
             return dict(rope)
     return None
 
@@ -60,7 +61,7 @@ def config_from_json(config: dict, name: str = "checkpoint", scaled_rope: bool =
     # transformers 5 writes the rotary settings as rope_parameters
     # {"rope_type", "rope_theta", ...} instead of a top-level rope_theta
     rope = config.get("rope_parameters") or {}
-    if rope.get("rope_type", "default") != "default" and not scaled_rope:
+    if scaling_type(rope) != "default" and not scaled_rope:
         raise ValueError(f"{name}: rope_parameters {rope} is not supported (only default rope)")
     theta = config.get("rope_theta", rope.get("rope_theta"))
     if config.get("use_sliding_window"):

@@ -29,15 +29,28 @@ _KNOWN = {"default": set(), "linear": {"factor"},
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+def scaling_type(scaling):
+    """The type that a checkpoint's rope_scaling (or rope_parameters) names;
+    "default" for none. ValueError where one that says how to scale names none."""
+    scaling = scaling or {}
+    kind = scaling.get("rope_type") or scaling.get("type")
+    if kind:
+        return kind
+    left = sorted(k for k, v in scaling.items() if v is not None and k not in ("rope_type", "type", "rope_theta"))
+    if left:
+        raise ValueError(f"a rope scaling with {left} and no rope_type")
+    return "default"
+
+
 def frequencies(rotary_dim, base, scaling=None, max_positions=None):
     """(angle per position of each pair, float64 on the CPU; factor of cos and
     sin) for `scaling` as a checkpoint's rope_scaling names it."""
     i = torch.arange(rotary_dim // 2, dtype=torch.float64)
     inv = float(base) ** (-2 * i / rotary_dim)
     scaling = dict(scaling or {})
-    kind = scaling.pop("rope_type", scaling.pop("type", "default"))
-    scaling.pop("type", None)
-    scaling.pop("rope_theta", None)
+    kind = scaling_type(scaling)
+    for name in ("rope_type", "type", "rope_theta"):
+        scaling.pop(name, None)
     if kind not in _KNOWN:
         raise ValueError(f"rope_type {kind!r}: one of {sorted(_KNOWN)}")
     if kind == "default":
