@@ -310,8 +310,10 @@ int qx_copy_pages(void* pools, int64_t n_pools, int64_t pool_stride, int64_t pag
  * 0): for each pair (a, b) of the first rotary_dim columns of a head,
  * (i, i + rotary_dim/2) or with interleaved (2i, 2i + 1),
  *   (a cos t - b sin t, b cos t + a sin t),  t = 2 pi positions[row] turns[i],
- * cos and sin times `factor`, t's whole turns dropped in 64 bits (any
- * position), products and sums in fp32, one rounding to the rows' type (type
+ * cos and sin times `factor`, t's whole turns dropped in 64 bits (any position
+ * is taken; t is off by up to 2^-53 of itself beside what turns is, less than
+ * fp32's rounding to positions of about 2^29), products and sums in fp32, one
+ * rounding to the rows' type (type
  * 0: bf16, 1: fp16, 2: fp32). The other columns are copied. turns: rotary_dim/2
  * doubles on the device. A row's heads lie D elements apart; the outputs are
  * the rows themselves or overlap none of them. No counterpart in the

@@ -62,8 +62,11 @@ __device__ __forceinline__ Pack<T, N> rounded(const float (&v)[N], const T*) {
 // y_a = a cos t - b sin t, y_b = b cos t + a sin t for each pair (a, b) of a
 // head, t = position * frequency of the pair, cos and sin times `factor`.
 // The position's turns are formed in 64 bits and their whole part dropped
-// there, so that cos and sin are those of any position to fp32's rounding;
-// a row of them serves every head of q and k.
+// there. The frequency in turns and the product are rounded, so the angle is off by
+// at most 3 2^-53 of itself: below what fp32 does to cos and sin (2^-22 of their
+// pair) up to positions of some 2^29, and growing with the position past that
+// (2^-12 at 2^40); past 2^53 the position itself is rounded. A row of cos and sin
+// serves every head of q and k.
 // A wave per row: its lanes compute the row's cos and sin into LDS, then take
 // units of N pairs' elements (16 bytes; N = 1: rows whose strides, alignment or
 // pairs do not allow that). Reads and writes each row once and is bound by HBM:

@@ -3,9 +3,10 @@ interleaved pairs, all of a head or its first part.
 
 A `RotaryEmbedding` is a model's rotary module. Called, it rotates rows of q
 and k by their positions (qx_rotary: angles from the positions themselves, so
-no table bounds them). Its `cos_sin_cache` is the table that the engine's own
-passes read (`Engine(rotary=...)`, a layer's `rotary_emb`), where the head is
-rotated whole in half pairs, as Qwen3's is.
+no table bounds them; they are off by up to 3 2^-53 of themselves, less than
+fp32 does to cos and sin at positions up to about 2^29). Its `cos_sin_cache` is
+the table that the engine's own passes read (`Engine(rotary=...)`, a layer's
+`rotary_emb`), where the head is rotated whole in half pairs, as Qwen3's is.
 
 Frequencies are base^(-2i / rotary_dim), or `inv_freq`, and with `scaling`:
   linear  all divided by `factor`;
