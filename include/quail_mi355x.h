@@ -367,7 +367,9 @@ int qx_key_weights(const void* q, int64_t q_ld, const float* lse, int64_t lse_ld
  * values of element_bytes 2, or e4m3 codes (1) with scales as qx_kv8_write lays
  * them out, layers scale_stride bytes apart: a page that a row moves into then
  * takes the largest scale its rows come with, codes of others move by the power
- * of two between (exactly unless they become subnormal), and keep is whole
+ * of two between (exactly unless they become subnormal: over many calls a value is
+ * off by less than 2^-9 of its scale, which is never larger than what some row of
+ * its head was written with, and never falls), and keep is whole
  * pages. No page may be in two of the call's tables. max_used bounds `used`
  * (larger entries count as max_used), at most qx_paged_attention_max_keys and
  * cols. sinks + recent <= keep. weights, kept and out overlap nowhere.

@@ -403,6 +403,10 @@ __device__ __forceinline__ v4i shifted16(v4i c, int shift) {
 // scale of those its rows come with (its own among them, where a row stays);
 // the codes of the others are shifted down to it, those of rows that stay too.
 // `keep` is whole pages, so no page is both read for a move and written.
+// A scale outlives the large row that it was for and goes with the page's other
+// rows, but never passes the largest that a row of the head was written with; over
+// any number of thinnings a value is off by less than 2^-9 of the scale it has then
+// (half a subnormal step each time the scale rises, by a factor of 2 or more).
 template <int D>
 __global__ __launch_bounds__(256) void thin_move8_kernel(ThinArgs p, int64_t waves, int parts) {
   constexpr int LPR = D / 16, RPP = 64 / LPR, kBatch = 4;
