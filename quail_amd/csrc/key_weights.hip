@@ -290,6 +290,7 @@ __device__ __forceinline__ float item_sums(const WeightsArgs& p, const Seq& x, i
     return (uint32_t)(at_col[t] >> 16) < (uint32_t)left && (at_col[t] & 0xffff) + g0 < p.G;
   };
   const float* all_lse = reinterpret_cast<const float*>(lds + 3 * kStage);
+  // (rounded once, at the size of the log-sum-exp: 2^-24 of it of a weight)
   auto bias_of = [&](int t, int step, bool live) {
     const float v = all_lse[step % 3 * kCols + t * 32 + col] * -kLog2e;
     return live ? v : -__builtin_inff();

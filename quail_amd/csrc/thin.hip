@@ -96,7 +96,8 @@ __device__ __forceinline__ uint64_t bits(int lo, int hi, int base) {
 // and third count few rows, if they are needed at all. What stays is then a bit a row, in words of 64 rows
 // (a wave's ballots), and dropped slots and movers are numbered by words. Bound
 // by instructions (some 60 a row) and, where rows are few, by the barriers
-// between these steps; 8 bytes a row from and to memory, 16 by token.
+// between these steps; 8 bytes a row from and to memory, 16 by token (2304 heads of
+// 1088 rows 23 us either way, 288 of 8003 rows 16.0 and 18.1, of 39,990 50 and 59).
 template <int NT, int E, bool BY_TOKEN>
 __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 4) void thin_select_kernel(ThinArgs p) {
   constexpr int W = NT / 64, WORDS = E * W, BINS = 2048, PER = BINS / NT;
