@@ -443,7 +443,7 @@ class KVArena:
                 raise ValueError(f"tokens: int32 {tuple(weights.shape)}, columns contiguous, not "
                                  f"{tuple(tokens.shape)} {tokens.dtype}")
             total = tables.get("tokens")
-            if total is None or total.dtype != torch.int32 or total.shape != (seqs,) or \
+            if not torch.is_tensor(total) or total.dtype != torch.int32 or total.shape != (seqs,) or \
                     (seqs > 1 and total.stride(0) != 1):
                 raise ValueError(f"the tables' tokens: int32, one for each of {seqs} sequences")
         if self.eight_bit and keep % self.page_tokens:

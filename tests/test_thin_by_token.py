@@ -180,7 +180,7 @@ def call(**kw):
     (dict(newest=-1), "stay"), (dict(newest=10, sinks=7), "stay"),
     (dict(tokens=torch.zeros(2, 2, 2, 32)), "tokens"), (dict(tokens=torch.zeros(2, 2, 2, 31).int()), "tokens"),
     (dict(tokens=torch.zeros(2, 2, 2, 64).int()[..., ::2]), "tokens"),
-    (dict(tables=dict(tokens=None)), "one for each"), (dict(tables=dict(tokens=torch.zeros(2))), "one for each"),
+    (dict(tables=dict(tokens=None)), "one for each"), (dict(tables=dict(tokens=30)), "one for each"), (dict(tables=dict(tokens=torch.zeros(2))), "one for each"),
     (dict(tables=dict(tokens=torch.zeros(3).int())), "one for each"),
     (dict(tables=dict(tokens=torch.zeros(4).int()[::2])), "one for each"), (dict(), "on the CPU")])
 def test_calls_that_are_refused(kw, match):
